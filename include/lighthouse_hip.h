@@ -371,6 +371,96 @@ int lh_hip_nanogpt_forward(float* logits, const float* x, const lh_nanogpt_block
                            int64_t T, int64_t C, int64_t n_head, int64_t vocab, float eps, int32_t dtype,
                            const lh_nanogpt_block_opts* opts, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------ generation over a paged cache ---- */
+
+/*
+ * A key / value cache in pages.  No counterpart in the reference, whose generation recomputes the whole
+ * context for every token (examples/xegpu/nanoGPT.py:225-297).  `k` and `v` are [n_pages, n_kv_heads,
+ * page_size, d] with element strides z (page), h (head), t (slot) and unit stride along d; position t of sequence b lies on page
+ * block_table[b * table_stride + t / page_size], slot t % page_size.  A page id outside 0 .. n_pages - 1
+ * holds nothing: it is neither read nor written, so unused entries of the table may hold anything.
+ * dtype is F32, BF16, F16 or F8E4M3; an e4m3 code stands for code * k_scale (or v_scale); the scales are 1 for
+ * the other types.  1 <= d <= 256; max_pages * page_size < 2^31 - 65536.
+ */
+typedef struct lh_paged_cache {
+  void* k;
+  void* v;
+  const int32_t* block_table; /* [B, max_pages] on the device */
+  int64_t table_stride;
+  lh_strides3 sk;
+  lh_strides3 sv;
+  int64_t n_pages;
+  int64_t max_pages;
+  int64_t page_size;
+  int64_t n_kv_heads;
+  int64_t d;
+  int32_t dtype;
+  float k_scale;
+  float v_scale;
+} lh_paged_cache;
+
+/*
+ * Keys and values of new tokens into the cache: k, v [B, n_kv_heads, T, d] (strides z: batch, h: head, t: token)
+ * in the cache's dtype, or F32, BF16 or F16 for a cache of e4m3, which holds e4m3(clamp(x / scale, +-448)), rounded to
+ * nearest even.  Token t of sequence b goes to position positions[b] + t if t < counts[b] (counts may be NULL: all of
+ * them do); a position outside the table or on a page that holds nothing is dropped.  Two tokens for one slot leave either.
+ */
+int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, lh_strides3 sk, lh_strides3 sv,
+                     const int32_t* positions, const int32_t* counts, int64_t B, int64_t T, int32_t dtype, void* stream);
+
+/*
+ * Attention of one new token of every sequence over its cache: q, out [B, H, d] (strides z: batch, h: head; t is
+ * not used), H a multiple of n_kv_heads, head h reads key / value head h / (H / n_kv_heads):
+ *   out[b, h] = sum_t p_t v_t,  p = softmax over t < lengths[b] of scale q . k_t,
+ * positions on pages that hold nothing left out; 0 where nothing is left.  `lengths` counts the new token if it has been
+ * appended and is clamped to 0 .. max_pages * page_size.  Scores, softmax and sums are f32.  dtype (of q and out) is the
+ * cache's, or BF16 or F16 for a cache of e4m3.  With `weights` ([B, n_kv_heads, >= max_pages * page_size] f32, element strides
+ * weights_stride_b, weights_stride_h), weights[b, g, t] grows by the sum of p_t over the H / n_kv_heads heads of group g.
+ * `workspace`, 256-byte aligned, of lh_hip_paged_attention_workspace_bytes(...): the call allocates nothing, and two calls
+ * that overlap in time need a workspace each.  It needs no clearing.
+ */
+size_t lh_hip_paged_attention_workspace_bytes(const lh_paged_cache* cache, int64_t B, int64_t H, int32_t with_weights);
+int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q, lh_strides3 so, lh_strides3 sq,
+                           const int32_t* lengths, float* weights, int64_t weights_stride_b, int64_t weights_stride_h,
+                           int64_t B, int64_t H, float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/*
+ * Positions that got least attention leave the cache.  For every sequence longer than `budget` and every key / value head:
+ * the last `recent` positions stay, and of the others the budget - recent with the largest weight (equal weights: the
+ * lowest positions; a NaN is below every number).  Rows of keys, values and weights that stay move up, in order, to the positions
+ * 0 .. budget - 1; weights behind them up to the old length become 0; rows behind them stay as they were.
+ * new_lengths[b] = min(lengths[b], budget); it may be `lengths`.  Every position below the length must
+ * lie on a page of its own that holds something (rows on others do not move).  1 <= budget, 0 <= recent <= budget.
+ */
+size_t lh_hip_kv_evict_workspace_bytes(int64_t B, int64_t n_kv_heads, int64_t budget);
+int lh_hip_kv_evict(const lh_paged_cache* cache, float* weights, int64_t weights_stride_b, int64_t weights_stride_h,
+                    const int32_t* lengths, int32_t* new_lengths, int64_t B, int64_t budget, int64_t recent,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The next token of every row of logits [B, V] (dtype F32, BF16 or F16, row stride ld): with w_i = exp((x_i - max x) / T)
+ * in 64 bits and the words in falling order of x (equal ones: lowest index first), the first top_k words stay; of those the shortest
+ * beginning that holds top_p of their mass (a word stays while the mass before it is below); of those the ones with
+ * w_i >= min_p.  The first always stays.  tokens[b] is the lowest index whose running sum of w over the words that
+ * stayed, in the order of the indices, exceeds u = uniform[b] times their sum (u below 0 counts as 0, u at or above 1, or NaN,
+ * takes the last word that stayed with w > 0).  T <= 0 or NaN: the largest logit, lowest index.  top_k <= 0, top_p not below 1 and
+ * min_p not above 0 keep everything.  A logit that is NaN or -inf is no word; a +inf leaves only those; a row without words gives -1.
+ * Each setting is one value for all rows or, where the pointer is not NULL, a device vector [B].
+ */
+typedef struct lh_sample_opts {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all;
+  float min_p_all;
+} lh_sample_opts;
+int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int64_t B, int64_t V, int64_t ld, int32_t dtype,
+                  const lh_sample_opts* opts, void* stream);
+
 /* ------------------------------------------------- packed-argument payloads ---- */
 
 /*

@@ -115,6 +115,19 @@ class GptFusedAttrs(ctypes.Structure):
                 ("causal", ctypes.c_int32), ("eps", ctypes.c_float)]
 
 
+class PagedCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("sk", Strides3), ("sv", Strides3), ("n_pages", ctypes.c_int64), ("max_pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("n_kv_heads", ctypes.c_int64), ("d", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
+
+
+class SampleOpts(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p),
+                ("temperature_all", ctypes.c_float), ("top_k_all", ctypes.c_int32), ("top_p_all", ctypes.c_float),
+                ("min_p_all", ctypes.c_float)]
+
+
 _vp, _i64, _i32, _u32, _f32, _sz = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32,
                                     ctypes.c_float, ctypes.c_size_t)
 
@@ -157,6 +170,13 @@ PROTOTYPES = {
     "lh_hip_nanogpt_forward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32, ctypes.POINTER(NanoGPTBlockOpts)]),
     "lh_hip_nanogpt_forward": (_i32, [_vp, _vp, ctypes.POINTER(NanoGPTBlockParams), _i64, _vp, _vp, _vp, _vp, _i64, _i64,
                                       _i64, _i64, _i64, _f32, _i32, ctypes.POINTER(NanoGPTBlockOpts), _vp, _sz, _vp]),
+    "lh_hip_kv_append": (_i32, [ctypes.POINTER(PagedCache), _vp, _vp, Strides3, Strides3, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "lh_hip_paged_attention_workspace_bytes": (_sz, [ctypes.POINTER(PagedCache), _i64, _i64, _i32]),
+    "lh_hip_paged_attention": (_i32, [ctypes.POINTER(PagedCache), _vp, _vp, Strides3, Strides3, _vp, _vp, _i64, _i64, _i64, _i64,
+                                      _f32, _i32, _vp, _sz, _vp]),
+    "lh_hip_kv_evict_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "lh_hip_kv_evict": (_i32, [ctypes.POINTER(PagedCache), _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "lh_hip_sample": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, ctypes.POINTER(SampleOpts), _vp]),
     "lh_hip_payload_matmul": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MatmulAttrs)]),
     "lh_hip_payload_matmul_fp8": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MatmulFp8Attrs)]),
     "lh_hip_payload_mlp": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MlpAttrs)]),

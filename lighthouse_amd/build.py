@@ -19,7 +19,8 @@ LIB_DIR = ROOT / "lighthouse_amd" / "lib"
 LIB_PATH = LIB_DIR / "liblighthouse_hip.so"
 PROBE_LIB = LIB_DIR / "liblighthouse_probe.so"  # bench.py's MFMA-rate probe, not part of the product library
 
-HIP_SOURCES = ["runtime.hip", "gemm16.hip", "gemm16_direct.hip", "gemm32.hip", "gemm8.hip", "gemm_small.hip", "gemm_small_norm.hip", "attention.hip", "attention_small.hip", "rowwise.hip", "api.hip"]
+HIP_SOURCES = ["runtime.hip", "gemm16.hip", "gemm16_direct.hip", "gemm32.hip", "gemm8.hip", "gemm_small.hip", "gemm_small_norm.hip", "attention.hip", "attention_small.hip", "rowwise.hip", "kv_cache.hip", "paged_attention.hip", "sample.hip",
+               "api.hip"]
 
 # A lone workgroup's main loop fetches a line more of instructions a turn where it starts at the end of one: the same loop 4 bytes
 # before a multiple of 64 and on it, 2923 x 768 x 5824 bf16 41.7 and 40.6 us.

@@ -1,0 +1,581 @@
+// Attention of one new token of every sequence over its paged key / value cache.
+//
+// Per sequence and key / value head: S = scale Q K^T for the G query heads that share it, a softmax over the positions
+// in one pass (running maximum and sum), O = P V.  Every key and value is read once and used for G heads: the work is
+// bound by memory, 1 to 2 operations a byte and head.  So the kernel is built around its loads:
+//
+//  * The G queries (up to 16) are the columns of 16-wide matrix instructions, whatever G is: the matrix cores have an order of
+//    magnitude to spare here, and the vector ALUs, which a dot product per head would fill, stay free.
+//  * Keys and values go from memory into registers in the layout that the matrix instructions take, without LDS and without
+//    barriers: S^T = K Q^T wants a key's row in pieces of 8 along d, which is how it lies in memory.  O^T = V^T P^T
+//    wants 8 keys of one column in a lane.  A lane loads the same piece of a row for 8 keys, 16 lanes a whole row, and turns the 8 x 8
+//    block in its registers, one v_perm_b32 per register: row m of fragment i is column m CE + i (CE = DP / 16 columns a lane).
+//  * The accumulators of S^T leave a lane with keys 4 g .. 4 g + 3 of both 16-key tiles of a step of one query, which, in that
+//    order of the keys, is the second operand of O^T (the lane loads the values of exactly those keys).
+//  * The waves of a workgroup take the steps of its share of the positions in turn, each on its own; their results are brought to
+//    the common maximum and added through LDS at the end.  A long cache is shared out between `splits` workgroups,
+//    each leaving (maximum, sum, sum of p v), which a second launch joins.
+//
+// 16-bit types: P is split into a value of the type and the value of the type nearest to what that leaves, two matrix
+// instructions instead of one (they cost nothing here): P alone rounded once to bf16 would add an error as large as the
+// rounding of the result.  f32 runs on v_mfma_f32_16x16x4_f32 with one 16-key tile a step.  e4m3 codes are converted to the queries' type, in
+// which every code has an exact value.
+#include "paged.h"
+
+namespace lh {
+
+struct PagedAttnArgs {
+  Paged c;
+  void* out;
+  const void* q;
+  int64_t so_z, so_h, sq_z, sq_h;
+  const int32_t* lengths;
+  int32_t B, H, G, rows, groups;  // rows = min(G, 16) queries a workgroup, groups = ceil(G / 16) of them
+  int32_t splits, min_share;      // of the positions: at least min_share each
+  float scale_log2e;
+  float* part_o;   // [B heads groups][splits][rows][DP]
+  float2* part_ml; // [B heads groups][splits][rows]
+  float* scores;   // [B H][cap_pad], scaled, times log2(e); or null
+  float* lse;      // [B H]: log2 of the sum of exp2(scores)
+  int32_t cap_pad;
+};
+
+// How many positions a workgroup takes of a sequence of n: as many for each of the splits, in whole rounds of its waves.
+__device__ __forceinline__ int paged_share(const PagedAttnArgs& a, int n) {
+  const int even = (n + a.splits - 1) / a.splits;
+  return (max(even, a.min_share) + a.min_share - 1) / a.min_share * a.min_share;
+}
+
+template <int DT>
+__device__ __forceinline__ f32x4 paged_mma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == LH_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Two e4m3 codes (the lower or upper two of a word) as two values of the 16-bit type DT: exact.
+template <int DT, bool HI>
+__device__ __forceinline__ uint32_t paged_e4m3(uint32_t w) {
+  if constexpr (DT == LH_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+}
+
+// BYTES from p, of which `left` lie inside the row (elements of ES bytes at their own alignment); the others are 0.
+template <int BYTES, int ES>
+__device__ __forceinline__ void load_row_piece(uint32_t* out, const uint8_t* p, int left) {
+  if (left >= BYTES) {
+    if constexpr (BYTES >= 16) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) {
+        const typename Chunk<ES>::type w = reinterpret_cast<const typename Chunk<ES>::type*>(p)[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[4 * i + e] = w[e];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < BYTES / 4; ++i) __builtin_memcpy(&out[i], p + 4 * i, 4);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < BYTES / 4; ++i) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4 / ES; ++e)
+      if (4 * i + ES * e < left) {
+        if constexpr (ES == 1) w |= (uint32_t)p[4 * i + e] << (8 * e);
+        else if constexpr (ES == 2) w |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[2 * i + e] << (16 * e);
+        else w = reinterpret_cast<const uint32_t*>(p)[i];
+      }
+    out[i] = w;
+  }
+}
+
+template <int BYTES>
+__device__ __forceinline__ void load_buffer(uint32_t* out, __amdgpu_buffer_rsrc_t r, int offset) {
+  if constexpr (BYTES == 4) {
+    out[0] = __builtin_amdgcn_raw_buffer_load_b32(r, offset, 0, 0);
+  } else if constexpr (BYTES == 8) {
+    const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(r, offset, 0, 0);
+    out[0] = w[0], out[1] = w[1];
+  } else {
+    const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = w[e];
+  }
+}
+
+// CDT: the cache's type, QDT: the queries' (the cache's, or a 16-bit type with e4m3).  DP: width that d is padded to.
+// TILES: the pages are multiples of 16 positions and rows 16-byte aligned, so that a tile of 16 keys has one base and its rows
+// are loaded through a buffer resource whose size is that of the rows that exist: what lies behind comes back as 0 without a
+// test.  Otherwise every lane finds the page of every row it loads.
+template <int CDT, int QDT, int DP, int NW, bool TILES>
+__global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs a) {
+  constexpr bool F32 = CDT == LH_F32;
+  constexpr int ES = CDT == LH_F8E4M3 ? 1 : F32 ? 4 : 2;
+  constexpr int KT = F32 ? 1 : 2;            // 16-key tiles a step
+  constexpr int KEYS = 16 * KT;
+  constexpr int KS = F32 ? DP / 16 : DP / 32;  // pieces of a key's row a lane takes
+  constexpr int KE = F32 ? 4 : 8;              // elements of such a piece
+  constexpr int KB = KE * ES;                  // its bytes
+  constexpr int CE = DP / 16;                  // columns of a value's row a lane takes
+  constexpr int VB = CE * ES;
+  constexpr int VP = VB > 16 ? VB / 16 : 1;    // loads for them
+  constexpr int VPB = VB / VP;
+  constexpr int kOutside = 0x40000000;         // an offset behind every buffer
+  __shared__ __attribute__((aligned(16))) f32x4 sums[NW / 2][CE][64];
+  __shared__ float2 stats[NW][16];
+
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int split = blockIdx.x % a.splits;
+  const int item = blockIdx.x / a.splits;  // (sequence, key / value head, group of queries)
+  const int group = item % a.groups, bh = item / a.groups;
+  const int hk = bh % a.c.heads, b = bh / a.c.heads;
+  const int n = min(max(a.lengths[b], 0), a.c.capacity());
+  const int share = paged_share(a, n);
+  const int k0 = split * share;
+  if (k0 >= n && split > 0) return;
+  const int k1 = min(n, k0 + share);
+  const int q_row = group * 16 + l16;           // of the G queries
+  const bool q_live = q_row < a.G;
+  const int head = hk * a.G + min(q_row, a.G - 1);
+
+  // The queries, in the layout of the second operand.
+  uint32_t qf[KS][4];
+  {
+    constexpr int QES = F32 ? 4 : 2;
+    const uint8_t* q = static_cast<const uint8_t*>(a.q) + (b * a.sq_z + head * a.sq_h) * QES;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d0 = s * (4 * KE) + g4 * KE;
+      load_row_piece<16, QES>(qf[s], q + d0 * QES, q_live ? (a.c.d - d0) * QES : 0);
+    }
+  }
+
+  f32x4 acc[CE];
+#pragma unroll
+  for (int i = 0; i < CE; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  const int32_t* table = a.c.table + b * a.c.table_stride;
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k);
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v);
+  const int row_bytes = a.c.d * ES;
+  uint32_t kr[KT][KS][KB / 4], vr[KT * 4][VB / 4];
+  int pages[KT];       // TILES: of the step whose keys are requested next
+  int held[KT];        // TILES: how many rows of its tiles exist
+  uint32_t live = 0;   // otherwise: which of the lane's KT * 4 keys do
+
+  int koff[KS], voff[4][VP];
+  if constexpr (TILES) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d0 = s * (4 * KE) + g4 * KE;
+      koff[s] = d0 < a.c.d ? l16 * (int)a.c.sk.t * ES + d0 * ES : kOutside;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int p = 0; p < VP; ++p) {
+        const int col = l16 * VB + p * VPB;
+        voff[r][p] = col < row_bytes ? (g4 * 4 + r) * (int)a.c.sv.t * ES + col : kOutside;
+      }
+  }
+  auto find_pages = [&](int step) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const int key = k0 + step * KEYS + 16 * t;
+      pages[t] = -1;
+      if (key < k1) {
+        const int p = table[a.c.by_size.div((uint32_t)key)];
+        if ((uint32_t)p < (uint32_t)a.c.pages) pages[t] = p;
+      }
+    }
+  };
+  auto request_tile = [&](int step, int t, const uint8_t* base, const lh_strides3& st, int page) {
+    const int key = k0 + step * KEYS + 16 * t;
+    const int slot = key - (int)a.c.by_size.div((uint32_t)key) * a.c.size;
+    const int rows = page < 0 ? 0 : min(16, k1 - key);
+    const int64_t at = page < 0 ? 0 : (page * st.z + hk * st.h + slot * st.t) * ES;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + at), 0, rows * (int)st.t * ES, 0x00020000);
+  };
+  auto request_keys = [&](int step) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      if constexpr (TILES) {
+        const __amdgpu_buffer_rsrc_t r = request_tile(step, t, kb, a.c.sk, pages[t]);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) load_buffer<KB>(kr[t][s], r, koff[s]);
+      } else {
+        const int key = k0 + step * KEYS + 16 * t + l16;
+        int slot = 0;
+        const int page = key < k1 ? a.c.page_of(b, key, &slot) : -1;
+        const uint8_t* row = kb + (max(page, 0) * a.c.sk.z + hk * a.c.sk.h + slot * a.c.sk.t) * ES;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int d0 = s * (4 * KE) + g4 * KE;
+          load_row_piece<KB, ES>(kr[t][s], row + d0 * ES, page < 0 ? 0 : (a.c.d - d0) * ES);
+        }
+      }
+    }
+  };
+  auto request_values = [&](int step) {
+    live = 0;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      if constexpr (TILES) {
+        const int key = k0 + step * KEYS + 16 * t;
+        held[t] = pages[t] < 0 ? 0 : min(16, k1 - key);
+        const __amdgpu_buffer_rsrc_t rs = request_tile(step, t, vb, a.c.sv, pages[t]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int p = 0; p < VP; ++p) load_buffer<VPB>(vr[t * 4 + r] + p * (VPB / 4), rs, voff[r][p]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = k0 + step * KEYS + 16 * t + 4 * g4 + r;
+          int slot = 0;
+          const int page = key < k1 ? a.c.page_of(b, key, &slot) : -1;
+          const uint8_t* row = vb + (max(page, 0) * a.c.sv.z + hk * a.c.sv.h + slot * a.c.sv.t) * ES;
+          load_row_piece<VB, ES>(vr[t * 4 + r], row + l16 * VB, page < 0 ? 0 : row_bytes - l16 * VB);
+          live |= (page >= 0 ? 1u : 0u) << (t * 4 + r);
+        }
+      }
+    }
+  };
+
+  const int steps = (k1 - k0 + KEYS - 1) / KEYS;
+  if (wave < steps) {
+    if constexpr (TILES) find_pages(wave);
+    request_keys(wave);
+    request_values(wave);
+  }
+#pragma unroll 1
+  for (int step = wave; step < steps; step += NW) {
+    const int next = step + NW;
+    if constexpr (TILES) find_pages(next);
+    // S^T: s[t][r] = S[query l16][key 16 t + 4 g4 + r]
+    f32x4 s[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[t][i][e]), __builtin_bit_cast(float, qf[i][e]), s[t], 0, 0, 0);
+        } else {
+          u32x4 kf;
+          if constexpr (CDT == LH_F8E4M3) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) kf[2 * e] = paged_e4m3<QDT, false>(kr[t][i][e]), kf[2 * e + 1] = paged_e4m3<QDT, true>(kr[t][i][e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) kf[e] = kr[t][i][e];
+          }
+          s[t] = paged_mma<QDT>(kf, u32x4{qf[i][0], qf[i][1], qf[i][2], qf[i][3]}, s[t]);
+        }
+      }
+    }
+    if (next < steps) request_keys(next);  // (the registers of the keys are free again)
+
+    // Softmax: x = s scale log2(e); a position that is not there has -inf.
+    f32x4 x[KT];
+    bool whole = true;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      x[t] = s[t] * a.scale_log2e;
+      if constexpr (TILES) whole = whole && held[t] == 16;
+    }
+    if (!TILES || !whole) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          bool there;
+          if constexpr (TILES) there = 4 * g4 + r < held[t];
+          else there = live >> (t * 4 + r) & 1;
+          if (!there) x[t][r] = s[t][r] = -INFINITY;
+        }
+    }
+    float mx = x[0][0];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, x[t][r]);
+    if (a.scores != nullptr && q_live) {
+      float* to = a.scores + ((int64_t)b * a.H + head) * a.cap_pad + k0 + step * KEYS + 4 * g4;
+#pragma unroll
+      for (int t = 0; t < KT; ++t) *reinterpret_cast<f32x4*>(to + 16 * t) = x[t];
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__any(mx > m_run)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int i = 0; i < CE; ++i) acc[i] *= alpha;
+    }
+    const float off = m_run == -INFINITY ? 0.0f : m_run;  // (nothing there yet: every p is exp2(-inf))
+    float p[KT * 4];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        // (one rounding of s scale - maximum; where s is -inf the product may be a NaN only for a scale of 0)
+        p[t * 4 + r] = x[t][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.scale_log2e, -off));
+        l_run += p[t * 4 + r];
+      }
+
+    if constexpr (F32) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < CE; ++i)
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[r][i]), p[r], acc[i], 0, 0, 0);
+    } else {
+      u32x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        hi[e] = pack2<QDT>(p[2 * e], p[2 * e + 1]);
+        lo[e] = pack2<QDT>(p[2 * e] - unpack_lo<QDT>(hi[e]), p[2 * e + 1] - unpack_hi<QDT>(hi[e]));
+      }
+      uint32_t vw[8][CE / 2];  // [key][pair of columns]
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < CE / 2; ++e) {
+          if constexpr (CDT == LH_F8E4M3) vw[j][e] = e % 2 ? paged_e4m3<QDT, true>(vr[j][e / 2]) : paged_e4m3<QDT, false>(vr[j][e / 2]);
+          else vw[j][e] = vr[j][e];
+        }
+#pragma unroll
+      for (int e = 0; e < CE / 2; ++e) {
+        u32x4 even, odd;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          even[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e], vw[2 * j][e], 0x05040100u);
+          odd[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e], vw[2 * j][e], 0x07060302u);
+        }
+        acc[2 * e] = paged_mma<QDT>(even, hi, acc[2 * e]);
+        acc[2 * e] = paged_mma<QDT>(even, lo, acc[2 * e]);
+        acc[2 * e + 1] = paged_mma<QDT>(odd, hi, acc[2 * e + 1]);
+        acc[2 * e + 1] = paged_mma<QDT>(odd, lo, acc[2 * e + 1]);
+      }
+    }
+    if (next < steps) request_values(next);
+  }
+
+  // acc[i][r] = sum p v of query l16, column (4 g4 + r) CE + i, over this wave's positions and relative to its maximum.
+  l_run += __shfl_xor(l_run, 16);
+  l_run += __shfl_xor(l_run, 32);
+  if (g4 == 0) stats[wave][l16] = make_float2(m_run, l_run);
+  __syncthreads();
+  float m_all = -INFINITY, l_all = 0.0f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) m_all = fmaxf(m_all, stats[w][l16].x);
+  const float m_safe = m_all == -INFINITY ? 0.0f : m_all;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) l_all += stats[w][l16].y * __builtin_amdgcn_exp2f(stats[w][l16].x - m_safe);
+  const float own = __builtin_amdgcn_exp2f(m_run - m_safe);
+#pragma unroll
+  for (int i = 0; i < CE; ++i) acc[i] *= own;
+#pragma unroll
+  for (int half = NW / 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half)
+#pragma unroll
+      for (int i = 0; i < CE; ++i) sums[wave - half][i][lane] = acc[i];
+    __syncthreads();
+    if (wave < half)
+#pragma unroll
+      for (int i = 0; i < CE; ++i) acc[i] += sums[wave][i][lane];
+    if (half > 1) __syncthreads();
+  }
+  if (wave != 0 || !q_live) return;
+  if (a.splits > 1) {
+    const int64_t part = ((int64_t)item * a.splits + split) * a.rows + l16;
+    if (g4 == 0) a.part_ml[part] = make_float2(m_all, l_all);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < CE; i += 4)
+        *reinterpret_cast<f32x4*>(a.part_o + part * DP + (4 * g4 + r) * CE + i) = f32x4{acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+    return;
+  }
+  if (a.lse != nullptr && g4 == 0) a.lse[(int64_t)b * a.H + head] = m_all + __builtin_amdgcn_logf(l_all);
+  const float inv = l_all == 0.0f ? 0.0f : a.c.v_scale / l_all;  // (no position there: 0)
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int i = 0; i < CE; ++i) {
+      const int col = (4 * g4 + r) * CE + i;
+      if (col < a.c.d) store_from_f32<QDT>(a.out, b * a.so_z + head * a.so_h + col, acc[i][r] * inv);
+    }
+}
+
+// Joins the parts of one query: brings them to the common maximum and adds them, in the order of the positions.
+template <int QDT, int DP>
+__global__ void __launch_bounds__(256) paged_attention_merge(PagedAttnArgs a) {
+  constexpr int GROUPS = 256 / DP;
+  __shared__ float sums[GROUPS][DP];
+  const int bh = blockIdx.x, b = bh / a.H, head = bh % a.H;
+  const int hk = head / a.G, q_row = head % a.G;
+  const int item = (b * a.c.heads + hk) * a.groups + q_row / 16;
+  const int tid = threadIdx.x, col = tid % DP, first = tid / DP;
+  const int n = min(max(a.lengths[b], 0), a.c.capacity());
+  const int parts = n == 0 ? 0 : (n + paged_share(a, n) - 1) / paged_share(a, n);
+  const int64_t at = (int64_t)item * a.splits * a.rows + q_row % 16;
+  float m = -INFINITY, l = 0.0f;
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[at + (int64_t)p * a.rows].x);
+  const float m_safe = m == -INFINITY ? 0.0f : m;
+  for (int p = 0; p < parts; ++p) {
+    const float2 ml = a.part_ml[at + (int64_t)p * a.rows];
+    l += ml.y * __builtin_amdgcn_exp2f(ml.x - m_safe);
+  }
+  float o = 0.0f;
+  for (int p = first; p < parts; p += GROUPS)
+    o += a.part_o[(at + (int64_t)p * a.rows) * DP + col] * __builtin_amdgcn_exp2f(a.part_ml[at + (int64_t)p * a.rows].x - m_safe);
+  if (GROUPS > 1) {
+    sums[first][col] = o;
+    __syncthreads();
+    if (first > 0) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) o += sums[g][col];
+  }
+  if (a.lse != nullptr && tid == 0) a.lse[bh] = m_safe + __builtin_amdgcn_logf(l);
+  if (col < a.c.d) store_from_f32<QDT>(a.out, b * a.so_z + head * a.so_h + col, l == 0.0f ? 0.0f : o * (a.c.v_scale / l));
+}
+
+// weights[b, g, t] += sum over the heads of the group of exp2(score - lse), heads in order.
+__global__ void __launch_bounds__(256) paged_attention_weights(PagedAttnArgs a, float* weights, int64_t sw_b, int64_t sw_h) {
+  const int per_head = (a.c.capacity() + 255) / 256, bh = blockIdx.x / per_head;
+  const int b = bh / a.c.heads, hk = bh % a.c.heads;
+  const int t = (blockIdx.x - bh * per_head) * 256 + threadIdx.x;
+  if (t >= min(max(a.lengths[b], 0), a.c.capacity())) return;
+  const int64_t first = (int64_t)b * a.H + hk * a.G;
+  float sum = 0.0f;
+  for (int g = 0; g < a.G; ++g) {
+    const float x = a.scores[(first + g) * a.cap_pad + t];
+    sum += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - a.lse[first + g]);
+  }
+  weights[b * sw_b + hk * sw_h + t] += sum;
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+
+constexpr int kPagedWaves = 4;
+
+struct PagedPlan {
+  int rows, groups, splits, min_share, dp, cap_pad;
+  size_t o_bytes, ml_bytes, score_bytes, lse_bytes;
+  size_t total() const { return o_bytes + ml_bytes + score_bytes + lse_bytes; }
+};
+
+static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
+
+static PagedPlan paged_plan(const Paged& c, int64_t B, int64_t H, bool with_weights) {
+  PagedPlan p = {};
+  const int G = (int)(H / c.heads);
+  p.rows = G < 16 ? G : 16, p.groups = (G + 15) / 16;
+  p.dp = c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
+  p.min_share = 32 * kPagedWaves;
+  const int64_t items = B * c.heads * p.groups, want = 6 * (int64_t)num_cus();
+  int64_t splits = (want + items - 1) / items;
+  const int64_t most = (c.capacity() + 2 * p.min_share - 1) / (2 * p.min_share);
+  if (splits > most) splits = most;
+  p.splits = splits < 1 ? 1 : (int)splits;
+  if (p.splits > 1) {
+    p.o_bytes = granules((size_t)items * p.splits * p.rows * p.dp * 4);
+    p.ml_bytes = granules((size_t)items * p.splits * p.rows * 8);
+  }
+  if (with_weights) {
+    p.cap_pad = (c.capacity() + 31) / 32 * 32;
+    p.score_bytes = granules((size_t)B * H * p.cap_pad * 4);
+    p.lse_bytes = granules((size_t)B * H * 4);
+  }
+  return p;
+}
+
+template <int CDT, int QDT, int DP>
+static int launch_paged(const PagedAttnArgs& a, bool tiles, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.B * a.c.heads * a.groups * a.splits)), block(kPagedWaves * 64);
+  if (tiles) LH_LAUNCH((paged_attention_kernel<CDT, QDT, DP, kPagedWaves, true>), grid, block, 0, s, a);
+  else LH_LAUNCH((paged_attention_kernel<CDT, QDT, DP, kPagedWaves, false>), grid, block, 0, s, a);
+  if (const int rc = check_launch("paged_attention")) return rc;
+  if (a.splits == 1) return LH_OK;
+  LH_LAUNCH((paged_attention_merge<QDT, DP>), dim3((unsigned)(a.B * a.H)), dim3(256), 0, s, a);
+  return check_launch("paged_attention_merge");
+}
+
+template <int CDT, int QDT>
+static int launch_paged_dp(const PagedAttnArgs& a, int dp, bool tiles, hipStream_t s) {
+  if (dp == 64) return launch_paged<CDT, QDT, 64>(a, tiles, s);
+  if (dp == 128) return launch_paged<CDT, QDT, 128>(a, tiles, s);
+  return launch_paged<CDT, QDT, 256>(a, tiles, s);
+}
+
+static bool paged_in_tiles(const Paged& c, int es) {
+  const int per = es == 4 ? 4 : 8, chunk = es == 1 ? 8 : 16;  // elements of a key's piece, bytes
+  // (a lane's piece of a value's row: 16 codes of a row of more than 128)
+  bool ok = c.size % 16 == 0 && c.d % per == 0 && (es != 1 || c.d <= 128 || c.d % 16 == 0);
+  for (const lh_strides3* s : {&c.sk, &c.sv}) ok = ok && (s->z * es) % chunk == 0 && (s->h * es) % chunk == 0 && (s->t * es) % chunk == 0 && 16 * s->t * es < 0x40000000 && s->t >= c.d;
+  return ok && reinterpret_cast<uintptr_t>(c.k) % chunk == 0 && reinterpret_cast<uintptr_t>(c.v) % chunk == 0;
+}
+
+}  // namespace lh
+
+using namespace lh;
+
+extern "C" {
+
+size_t lh_hip_paged_attention_workspace_bytes(const lh_paged_cache* cache, int64_t B, int64_t H, int32_t with_weights) {
+  Paged c;
+  if (paged_cache(cache, "lh_hip_paged_attention_workspace_bytes", &c) != LH_OK) return 0;
+  if (B <= 0 || H <= 0 || H % c.heads != 0) return 0;
+  return paged_plan(c, B, H, with_weights != 0).total();
+}
+
+int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q, lh_strides3 so, lh_strides3 sq,
+                           const int32_t* lengths, float* weights, int64_t weights_stride_b, int64_t weights_stride_h,
+                           int64_t B, int64_t H, float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  PagedAttnArgs a = {};
+  if (const int rc = paged_cache(cache, "lh_hip_paged_attention", &a.c)) return rc;
+  if (B == 0) return LH_OK;
+  LH_REQUIRE(out && q && lengths, "lh_hip_paged_attention: null pointer");
+  LH_REQUIRE(B >= 0 && H > 0 && H % a.c.heads == 0, "lh_hip_paged_attention: %lld heads are no multiple of %d key / value heads", (long long)H, a.c.heads);
+  LH_REQUIRE(B * H < (1ll << 20), "lh_hip_paged_attention: bad batch (fewer than 2^20 heads of sequences)");
+  LH_REQUIRE(dtype == cache->dtype || (cache->dtype == LH_F8E4M3 && (dtype == LH_BF16 || dtype == LH_F16)),
+             "lh_hip_paged_attention: queries must have the cache's dtype (bf16 or f16 for a cache of e4m3)");
+  LH_REQUIRE(weights == nullptr || ((a.c.heads == 1 || weights_stride_h >= a.c.capacity()) && (B <= 1 || weights_stride_b >= a.c.capacity())),
+             "lh_hip_paged_attention: rows of the weights overlap");
+  LH_REQUIRE(weights == nullptr || (a.c.capacity() + 255) / 256 * B * a.c.heads < (1ll << 24), "lh_hip_paged_attention: too many weights (fewer than 2^32)");
+  const PagedPlan p = paged_plan(a.c, B, H, weights != nullptr);
+  LH_REQUIRE(p.total() == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= p.total()),
+             "lh_hip_paged_attention: workspace too small or not 256-byte aligned: %zu of %zu bytes", workspace_bytes, p.total());
+  a.out = out, a.q = q, a.so_z = so.z, a.so_h = so.h, a.sq_z = sq.z, a.sq_h = sq.h, a.lengths = lengths;
+  a.B = (int32_t)B, a.H = (int32_t)H, a.G = (int32_t)(H / a.c.heads);
+  a.rows = p.rows, a.groups = p.groups, a.splits = p.splits, a.min_share = p.min_share, a.cap_pad = p.cap_pad;
+  a.scale_log2e = (float)((double)scale * a.c.k_scale * 1.4426950408889634);
+  char* ws = static_cast<char*>(workspace);
+  if (p.splits > 1) a.part_o = reinterpret_cast<float*>(ws), a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
+  if (weights) a.scores = reinterpret_cast<float*>(ws + p.o_bytes + p.ml_bytes), a.lse = reinterpret_cast<float*>(ws + p.o_bytes + p.ml_bytes + p.score_bytes);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const bool tiles = paged_in_tiles(a.c, (int)dtype_size(cache->dtype));
+  int rc = LH_ERR_UNSUPPORTED;
+  if (cache->dtype == LH_F8E4M3) rc = dtype == LH_BF16 ? launch_paged_dp<LH_F8E4M3, LH_BF16>(a, p.dp, tiles, s) : launch_paged_dp<LH_F8E4M3, LH_F16>(a, p.dp, tiles, s);
+  else if (dtype == LH_BF16) rc = launch_paged_dp<LH_BF16, LH_BF16>(a, p.dp, tiles, s);
+  else if (dtype == LH_F16) rc = launch_paged_dp<LH_F16, LH_F16>(a, p.dp, tiles, s);
+  else rc = launch_paged_dp<LH_F32, LH_F32>(a, p.dp, tiles, s);
+  if (rc != LH_OK || weights == nullptr) return rc;
+  LH_LAUNCH(paged_attention_weights, dim3((unsigned)((a.c.capacity() + 255) / 256 * B * a.c.heads)), dim3(256), 0, s, a, weights,
+            weights_stride_b, weights_stride_h);
+  return check_launch("paged_attention_weights");
+}
+
+}  // extern "C"

@@ -529,6 +529,236 @@ def nanogpt_forward(x, layers: list, lnf_g, lnf_b, lm_w, lm_b, n_head: int, *, e
     return out
 
 
+# ---- generation over a paged key / value cache ------------------------------------------------------------------------
+_CACHE_DTYPES = (torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn)
+
+
+def _on_current_device(*tensors) -> None:
+    """Launches go to the current device's stream: tensors of another device would be read there through the wrong one."""
+    _need_cuda(*tensors)
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.device.index != device:
+            raise ValueError(f"expected tensors on the current device (cuda:{device}), got {t.device}")
+
+
+def _is_index(t, shape, what: str) -> None:
+    if t.dtype != torch.int32 or t.shape != shape or (t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{what} must be an int32 tensor of shape {list(shape)} with innermost stride 1, got {tuple(t.shape)} {t.dtype}")
+
+
+def _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale) -> _lib.PagedCache:
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have the same shape [pages, kv heads, page size, d]")
+    if k_cache.dtype not in _CACHE_DTYPES or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must have one dtype (float32, bfloat16, float16 or float8_e4m3fn)")
+    pages, heads, size, d = k_cache.shape
+    if not (1 <= d <= 256 and pages and heads and size):
+        raise ValueError(f"the cache must hold something, with a head dimension of 1 to 256, got {tuple(k_cache.shape)}")
+    for t in (k_cache, v_cache):
+        st = t.stride()
+        if st[3] != 1 and d != 1:
+            raise ValueError("k_cache and v_cache: innermost stride must be 1")
+        if any(n > 1 and step < d for n, step in zip(t.shape[:3], st)):
+            raise ValueError("k_cache and v_cache: rows overlap")
+    if block_table.dim() != 2 or block_table.shape[1] < 1:
+        raise ValueError("block_table must have shape [B, pages of a sequence]")
+    _is_index(block_table, (B, block_table.shape[1]), "block_table")
+    if B > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("rows of block_table overlap")
+    if block_table.shape[1] * size >= 2**31 - 65536:
+        raise ValueError("the block table must hold fewer than 2^31 - 65536 positions")
+    if k_cache.dtype != torch.float8_e4m3fn and not (k_scale == 1.0 and v_scale == 1.0):
+        raise ValueError("k_scale and v_scale belong to a cache of float8_e4m3fn")
+    if not (0.0 < k_scale < math.inf and 0.0 < v_scale < math.inf):
+        raise ValueError("k_scale and v_scale must be positive numbers")
+    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                           max(block_table.stride(0), block_table.shape[1]), _strides3(k_cache),
+                           _strides3(v_cache), pages, block_table.shape[1], size, heads, d, lh_dtype(k_cache.dtype), k_scale, v_scale)
+
+
+def _cache_weights(weights, B, heads, capacity):
+    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[:2] != (B, heads) or weights.shape[2] < capacity:
+        raise ValueError(f"weights must be a float32 tensor of shape [{B}, {heads}, {capacity} or more], got {tuple(weights.shape)} {weights.dtype}")
+    st = weights.stride()
+    if (st[2] != 1 and weights.shape[2] != 1) or (heads > 1 and st[1] < capacity) or (B > 1 and st[0] < capacity):
+        raise ValueError("weights: innermost stride must be 1, and rows must not overlap")
+
+
+def kv_append(k, v, k_cache, v_cache, block_table, positions, *, counts=None, k_scale=1.0, v_scale=1.0):
+    """Writes the keys and values of new tokens into a paged cache and returns (k_cache, v_cache).
+
+    k, v: [B, kv heads, T, d] (any strides with unit stride along d, so a projection's output can be passed as a view) in the cache's
+    dtype; for a cache of float8_e4m3fn in float32, bfloat16 or float16, of which it holds e4m3(x / scale), clamped to +-448.
+    k_cache, v_cache: [pages, kv heads, page size, d], any strides with unit stride along d.  block_table int32 [B, P]: position t of
+    sequence b lies on page block_table[b, t // size], slot t % size.  Token t goes to position positions[b] + t (int32 [B]) if
+    t < counts[b] (int32 [B]; None: all do).  Positions outside the table, and pages outside the cache (-1 for an entry not in use), are left out.
+    Every token needs a slot of its own."""
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k and v must have the same shape [B, kv heads, T, d] and dtype")
+    B, heads, T, d = k.shape
+    cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
+    if (heads, d) != (k_cache.shape[1], k_cache.shape[3]):
+        raise ValueError(f"k and v have {heads} heads of {d}, the cache {k_cache.shape[1]} of {k_cache.shape[3]}")
+    if k.dtype not in _FLOATS or (k.dtype != k_cache.dtype and k_cache.dtype != torch.float8_e4m3fn):
+        raise ValueError("k and v must have the cache's dtype (float32, bfloat16 or float16 for a cache of float8_e4m3fn)")
+    if d != 1 and (k.stride(3) != 1 or v.stride(3) != 1):
+        raise ValueError("innermost stride must be 1")
+    _is_index(positions, (B,), "positions")
+    if counts is not None:
+        _is_index(counts, (B,), "counts")
+    _on_current_device(k, v, k_cache, v_cache, block_table, positions, counts)
+    if k.numel() == 0:
+        return k_cache, v_cache
+    _lib.check(_lib.load().lh_hip_kv_append(
+        ctypes.byref(cache), k.data_ptr(), v.data_ptr(), *_strides3_of(k, v), positions.data_ptr(),
+        counts.data_ptr() if counts is not None else None, B, T, lh_dtype(k.dtype), _stream()), "kv_append")
+    return k_cache, v_cache
+
+
+def _vector_workspace(workspace, need, like):
+    """The caller's workspace, or one from torch's allocator, which a captured graph keeps for itself."""
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=like.device) if need else None
+    _on_current_device(workspace)
+    if not (workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous() and workspace.numel() >= need
+            and workspace.data_ptr() % 256 == 0):
+        raise ValueError(f"workspace must be a contiguous uint8 vector of at least {need} bytes, 256-byte aligned")
+    return workspace
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, out=None, weights=None, k_scale=1.0, v_scale=1.0,
+                    workspace=None):
+    """Attention of one new token of every sequence over its paged cache (laid out as for kv_append): out[b, h] =
+    softmax(scale q[b, h] . k_t over t < lengths[b]) v_t, 0 where nothing is there.
+
+    q, out: [B, H, d] (unit stride along d) in the cache's dtype, or bfloat16 / float16 for a cache of float8_e4m3fn, whose codes stand for
+    code * k_scale and code * v_scale.  H is a multiple of the cache's heads; head h reads head h // (H // kv heads).  lengths int32 [B]
+    counts the new token once it has been appended.  scale: 1 / sqrt(d) if None.  `weights`, float32 [B, kv heads, N] with N at least the
+    positions of the block table: weights[b, g, t] grows by the probabilities of position t, added over the heads of group g
+    (what kv_evict goes by).  `workspace` (uint8, see paged_attention_workspace_bytes): temporary memory, otherwise
+    torch's allocator is asked; two calls that overlap in time need one each."""
+    if q.dim() != 3:
+        raise ValueError("paged_attention expects q of shape [B, H, d]")
+    B, H, d = q.shape
+    cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
+    if d != k_cache.shape[3]:
+        raise ValueError(f"q has a head dimension of {d}, the cache of {k_cache.shape[3]}")
+    if H == 0 or H % k_cache.shape[1]:
+        raise ValueError(f"{H} heads are no multiple of the cache's {k_cache.shape[1]}")
+    if q.dtype != k_cache.dtype and not (k_cache.dtype == torch.float8_e4m3fn and q.dtype in (torch.bfloat16, torch.float16)):
+        raise ValueError("q must have the cache's dtype (bfloat16 or float16 for a cache of float8_e4m3fn)")
+    if q.dtype not in _FLOATS:
+        raise ValueError(f"unsupported dtype {q.dtype}")
+    if out is None:
+        out = torch.empty((B, H, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have the shape and dtype of q")
+    so, sq = out.stride(), q.stride()
+    if d != 1 and (so[2] != 1 or sq[2] != 1):
+        raise ValueError("innermost stride must be 1")
+    if (H > 1 and so[1] < d) or (B > 1 and so[0] < d):
+        raise ValueError("rows of out overlap")
+    _is_index(lengths, (B,), "lengths")
+    capacity = cache.max_pages * cache.page_size
+    if weights is not None:
+        _cache_weights(weights, B, cache.n_kv_heads, capacity)
+    _on_current_device(q, k_cache, v_cache, block_table, lengths, out, weights)
+    if B == 0:
+        return out
+    lib = _lib.load()
+    workspace = _vector_workspace(workspace, lib.lh_hip_paged_attention_workspace_bytes(ctypes.byref(cache), B, H, weights is not None), q)
+    _lib.check(lib.lh_hip_paged_attention(
+        ctypes.byref(cache), out.data_ptr(), q.data_ptr(), _lib.Strides3(so[0], so[1], 0), _lib.Strides3(sq[0], sq[1], 0),
+        lengths.data_ptr(), weights.data_ptr() if weights is not None else None,
+        weights.stride(0) if weights is not None else 0, weights.stride(1) if weights is not None else 0, B, H,
+        float(scale) if scale is not None else 1.0 / math.sqrt(d), lh_dtype(q.dtype),
+        workspace.data_ptr() if workspace is not None else None, workspace.numel() if workspace is not None else 0, _stream()),
+        "paged_attention")
+    return out
+
+
+def paged_attention_workspace_bytes(q, k_cache, v_cache, block_table, *, weights=False) -> int:
+    """Bytes of temporary memory that paged_attention takes for these tensors (only their shapes and strides matter);
+    `weights`: whether the call passes any."""
+    cache = _paged_cache(k_cache, v_cache, block_table, q.shape[0], 1.0, 1.0)
+    return int(_lib.load().lh_hip_paged_attention_workspace_bytes(ctypes.byref(cache), q.shape[0], q.shape[1], 1 if weights else 0))
+
+
+def kv_evict(k_cache, v_cache, weights, block_table, lengths, budget, *, recent=0, out=None, workspace=None):
+    """Shrinks every sequence longer than `budget` to it and returns the new lengths (int32 [B]; written to `out` if given, which may be
+    `lengths`).  Of each kv head the last `recent` positions stay, and of the others the budget - recent with the largest weight
+    (ties: the lowest positions; NaN is below every number).  Keys, values and weights of what stays move up, in order; weights behind
+    them up to the old length become 0.  Every position below the length must lie on a page of its own.
+    Cache, block table and weights are those of kv_append and paged_attention; `workspace` as there (kv_evict_workspace_bytes)."""
+    B = lengths.shape[0] if lengths.dim() == 1 else -1
+    _is_index(lengths, (B,), "lengths")
+    cache = _paged_cache(k_cache, v_cache, block_table, B, 1.0, 1.0)
+    _cache_weights(weights, B, cache.n_kv_heads, cache.max_pages * cache.page_size)
+    budget, recent = int(budget), int(recent)
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"budget must be at least 1 and recent between 0 and the budget, got {budget} and {recent}")
+    if out is None:
+        out = torch.empty(B, dtype=torch.int32, device=lengths.device)
+    _is_index(out, (B,), "out")
+    _on_current_device(k_cache, v_cache, weights, block_table, lengths, out)
+    if B == 0:
+        return out
+    lib = _lib.load()
+    need = lib.lh_hip_kv_evict_workspace_bytes(B, cache.n_kv_heads, min(budget, cache.max_pages * cache.page_size))
+    workspace = _vector_workspace(workspace, need, lengths)
+    _lib.check(lib.lh_hip_kv_evict(
+        ctypes.byref(cache), weights.data_ptr(), weights.stride(0), weights.stride(1), lengths.data_ptr(), out.data_ptr(), B,
+        budget, recent, workspace.data_ptr() if workspace is not None else None, need, _stream()), "kv_evict")
+    return out
+
+
+def kv_evict_workspace_bytes(k_cache, block_table, budget) -> int:
+    """Bytes of temporary memory that kv_evict takes for this cache and block table."""
+    capacity = block_table.shape[1] * k_cache.shape[2]
+    return int(_lib.load().lh_hip_kv_evict_workspace_bytes(block_table.shape[0], k_cache.shape[1], min(int(budget), capacity)))
+
+
+def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """The next token of every row of logits [B, V] (float32, bfloat16 or float16, rows of any stride): int64 [B].
+
+    With w = exp((x - max) / temperature) in 64 bits and the words in falling order of x (equal ones: lowest index first): the first
+    top_k words stay, of those the shortest beginning with at least top_p of their mass, of those the ones with w >= min_p;
+    the first always does.  The token is the lowest index whose running sum of w over what stayed, by index, exceeds uniform[b] (float32
+    [B], in [0, 1)) times their sum.  temperature <= 0: the largest logit.  top_k <= 0, top_p >= 1 and min_p <= 0 keep everything.
+    NaN and -inf are no words, a +inf leaves only those, a row without words gives -1.
+    Each setting is a number or a tensor [B] on the GPU (int32 for top_k, float32 for the others)."""
+    if logits.dim() != 2 or logits.dtype not in _FLOATS or logits.shape[1] < 1:
+        raise ValueError("sample expects logits of shape [B, V] in float32, bfloat16 or float16")
+    B, V = logits.shape
+    if logits.stride(1) != 1 and V != 1:
+        raise ValueError("innermost stride must be 1")
+    if B > 1 and logits.stride(0) < V:
+        raise ValueError("rows of logits overlap")
+    _is_vector(uniform, B, torch.float32, "uniform")
+    opts = _lib.SampleOpts()
+    vectors = []
+    for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                               ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(value, torch.Tensor):
+            _is_vector(value, B, dtype, name)
+            vectors.append(value)
+            setattr(opts, name, value.data_ptr())
+        elif name == "top_k":
+            opts.top_k_all = max(0, min(int(value), 2**31 - 1))
+        else:
+            setattr(opts, name + "_all", float(value))
+    if out is None:
+        out = torch.empty(B, dtype=torch.int64, device=logits.device)
+    _is_vector(out, B, torch.int64, "out")
+    _on_current_device(logits, uniform, out, *vectors)
+    if B == 0:
+        return out
+    _lib.check(_lib.load().lh_hip_sample(out.data_ptr(), logits.data_ptr(), uniform.data_ptr(), B, V, max(logits.stride(0), V),
+                                         lh_dtype(logits.dtype), ctypes.byref(opts), _stream()), "sample")
+    return out
+
+
 def release_scratch() -> None:
     """Free the library's pool of temporary buffers on the current device (waits for the device)."""
     _lib.check(_lib.load().lh_hip_release_scratch(), "release_scratch")

@@ -1,0 +1,132 @@
+"""Sampling against the 64-bit statement of it: the token has to be the same one."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from lighthouse_amd import ops
+from tests import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+bf16, f16, f32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def check(logits, uniform, **options):
+    x = logits.cuda()
+    u = torch.as_tensor(uniform, dtype=f32)
+    row = lambda v, b: v[b].item() if isinstance(v, torch.Tensor) else v  # noqa: E731
+    got = ops.sample(x, u.cuda(), **{k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in options.items()}).tolist()
+    rows = logits.double().numpy()
+    want = [ref.sample(rows[b], u[b].item(), **{k: row(v, b) for k, v in options.items()}) for b in range(len(rows))]
+    assert got == want
+
+
+FILTERS = [{}, {"top_k": 1}, {"top_k": 50}, {"top_p": 0.9}, {"min_p": 0.05}, {"top_k": 40, "top_p": 0.8}, {"top_k": 300, "top_p": 0.95, "min_p": 0.01},
+           {"temperature": 0.0}, {"temperature": -1.0}, {"temperature": 0.05, "top_p": 0.9}, {"temperature": 5.0, "top_p": 0.99},
+           {"top_p": 0.0}, {"top_p": 1e-6}, {"min_p": 2.0}, {"top_k": 10**6, "top_p": 0.5}, {"temperature": math.inf, "top_k": 9}]
+
+
+@pytest.mark.parametrize("options", FILTERS, ids=lambda o: "-".join(f"{k}{v}" for k, v in o.items()) or "plain")
+@pytest.mark.parametrize("dtype,V", [(f32, 5000), (bf16, 5000), (f16, 1237)])
+def test_filters(options, dtype, V):
+    g = torch.Generator().manual_seed(V)
+    logits = (2.5 * torch.randn(24, V, generator=g) + 30).to(dtype)
+    check(logits, torch.rand(24, generator=g), **options)
+
+
+@pytest.mark.parametrize("V", [1, 2, 3, 63, 64, 65, 255, 256, 257, 1023, 1025, 4096, 8191, 16385, 50257])
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_sizes(V, dtype):
+    g = torch.Generator().manual_seed(V)
+    logits = (3 * torch.randn(6, V, generator=g)).to(dtype)
+    u = torch.rand(6, generator=g)
+    for options in ({}, {"top_k": 5}, {"top_p": 0.7}):
+        check(logits, u, **options)
+
+
+def test_a_large_vocabulary_with_settings_for_every_row():
+    g = torch.Generator().manual_seed(1)
+    logits = (2.5 * torch.randn(8, 131072, generator=g)).to(bf16)
+    check(logits, torch.rand(8, generator=g), temperature=torch.tensor([0.7, 1.0, 1.3, 0.0, 0.9, 1.0, 2.0, 1.0]),
+          top_k=torch.tensor([0, 50, 3000, 7, 0, 0, 20000, 0], dtype=torch.int32),
+          top_p=torch.tensor([0.9, 0.95, 1.0, 0.5, 0.99, 1.0, 0.9, 0.3]), min_p=torch.tensor([0.0, 0.0, 0.1, 0.0, 0.02, 0.0, 0.0, 0.5]))
+
+
+@pytest.mark.parametrize("dtype", [f32, bf16, f16])
+def test_ties(dtype):
+    """Few values, thousands of words each: the cut falls among words of one value, the lowest indices stay."""
+    g = torch.Generator().manual_seed(2)
+    logits = torch.randint(0, 3, (12, 6000), generator=g).to(dtype)
+    u = torch.tensor([0.0, 0.1, 0.25, 0.5, 0.75, 0.9, 0.99, 0.999, 0.9999, 0.33, 0.66, 0.5])
+    for options in ({}, {"top_k": 777}, {"top_k": 2500}, {"top_p": 0.3}, {"top_p": 0.8}, {"top_k": 1999, "top_p": 0.5}, {"temperature": 0.0}, {"top_k": 1}):
+        check(logits, u, **options)
+    same = torch.full((4, 4096), -3.5, dtype=dtype)
+    check(same, [0.0, 0.25, 0.5, 0.75])
+    check(same, [0.0, 0.25, 0.5, 0.75], top_p=0.5)
+    check(same, [0.0, 0.25, 0.5, 0.75], top_k=1024)
+
+
+@pytest.mark.parametrize("u", [0.0, -1.0, 1.0, 2.0, math.inf, math.nan, float(np.nextafter(np.float32(1), np.float32(0)))])
+def test_numbers_at_the_ends(u):
+    g = torch.Generator().manual_seed(3)
+    logits = 4 * torch.randn(3, 900, generator=g)
+    for options in ({}, {"top_k": 20}, {"top_p": 0.6}):
+        check(logits, [u] * 3, **options)
+
+
+def test_masked_words():
+    """-inf and NaN are no words, the type's lowest value is one; rows of none and of one, infinite ones."""
+    g = torch.Generator().manual_seed(4)
+    x = 2 * torch.randn(10, 2000, generator=g)
+    x[0, ::2] = -math.inf
+    x[1, 5:] = -math.inf
+    x[2] = -math.inf
+    x[3, 1999] = 1.0
+    x[3, :1999] = -math.inf
+    x[4, ::3] = math.nan
+    x[5] = math.nan
+    x[6, ::2] = torch.finfo(f32).min
+    x[7] = torch.finfo(f32).min
+    x[8, [7, 100, 1500]] = math.inf
+    x[9, ::2] = -1e9
+    u = torch.rand(10, generator=g)
+    for options in ({}, {"top_k": 30}, {"top_k": 2}, {"top_k": 1500}, {"top_p": 0.9}, {"top_p": 0.5, "top_k": 1500}, {"min_p": 0.1}, {"temperature": 0.0}, {"temperature": 1e-30}):
+        check(x, u, **options)
+    check(x.to(bf16), u, top_p=0.9)
+    check(torch.full((2, 1), -math.inf), [0.5, 0.5])
+
+
+def test_values_close_together_and_far_apart():
+    """Differences of the last bit, of denormals and of the whole range of f32 all end in the right cut."""
+    g = torch.Generator().manual_seed(5)
+    near = (torch.full((4, 3000), 1.0).view(torch.int32) + torch.randint(0, 50, (4, 3000), generator=g).int()).view(f32)
+    tiny = torch.randint(0, 90, (4, 3000), generator=g).int().view(f32)
+    far = torch.randn(4, 3000, generator=g) * 10.0 ** torch.randint(-44, 38, (4, 3000), generator=g).double().float()
+    u = torch.rand(4, generator=g)
+    for x in (near, tiny, far):
+        for options in ({}, {"top_k": 700}, {"top_k": 2999}, {"top_p": 0.4}, {"top_p": 0.95, "temperature": 1e30}, {"top_k": 1000, "temperature": 1e-20}):
+            check(x, u, **options)
+
+
+def test_rows_of_any_stride_and_alignment():
+    g = torch.Generator().manual_seed(6)
+    for dtype in (f32, bf16):
+        store = torch.randn(5, 1003, generator=g).to(dtype).cuda()
+        x = store[:, 1:778]
+        u = torch.rand(5, generator=g)
+        got = ops.sample(x, u.cuda(), top_p=0.8).tolist()
+        assert got == [ref.sample(x[b].double().cpu().numpy(), u[b].item(), top_p=0.8) for b in range(5)]
+
+
+def test_draws_follow_the_probabilities():
+    """4096 draws from one row at evenly spaced numbers: each word as often as its share, to the one draw that its ends decide."""
+    x = torch.tensor([0.3, -1.0, 2.0, 1.2, -math.inf, 0.0, 1.9])
+    n = 4096
+    u = (torch.arange(n, dtype=torch.float64) / n).float()
+    got = ops.sample(x.repeat(n, 1).cuda(), u.cuda(), temperature=0.7)
+    p = torch.softmax(x.double() / 0.7, 0)
+    assert ((torch.bincount(got.cpu(), minlength=7) - n * p).abs() <= 1).all()
+    assert (got.diff() >= 0).all()
