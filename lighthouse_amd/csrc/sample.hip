@@ -2,16 +2,18 @@
 //
 // With w_i = exp((x_i - max) / T) and the words in falling order of (x, then rising index), each filter keeps a beginning of
 // that order: the first k; the words before which less than top_p of the mass lies; the words with w >= min_p.  So what stays
-// is described by its last word (cut_x, cut_i), and no row is ever sorted: the last word is found in a histogram of the distance
-// max - x, by counts (top-k) or masses (top-p), and then among the few words of the bin it lies in.  The draw is
-// a search in the running sum over the indices.
+// is described by its last word, and no row is ever sorted.  The draw is a search in the running sum over the indices.
 //
-// Masses are whole numbers, w in units of 2^-kBits with w from a 64-bit exponential: sums of them are exact in any order, so
-// neither the atomics of the histogram nor the split over lanes and waves can change a token, and a sum over
-// 131072 words is off by about 1e-12 of the whole: as good as a sum in 64-bit floating point.  (In 32 bits a row of 5000 likely words would
-// get another token about once in 10^4 rows.)
+// Masses are whole numbers, w in units of 2^-bits with w from a 64-bit exponential: sums of them are exact in any order, so
+// neither atomics nor the split over lanes and waves can change a token, and a sum over 131072 words is off by about 1e-12
+// of the whole: as good as a sum in 64-bit floating point.  (In 32 bits a row of 5000 likely words would get another token about
+// once in 10^4 rows.)
 //
-// One workgroup of 16 waves takes a row; a wave takes a contiguous share of it.
+// One workgroup of 16 waves takes a row; a wave takes a contiguous share of it.  Where few words can stay (top-k, or a top-p
+// or min-p that a few hundred words reach), they are listed: of the largest word of each of the 1024 threads the K-th is at
+// most the K-th of the row, so the words that reach it are K or a few more; the list is sorted in LDS and everything else
+// happens on it, two passes over the row in all.  Otherwise the last word is found in a histogram of the distance max - x, by
+// counts (top-k) or masses (top-p), and then among the words of the bin it lies in.
 #include "common.h"
 
 namespace lh {
@@ -28,46 +30,65 @@ struct SampleArgs {
 
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
 constexpr int kSampleBins = 2048;
-constexpr int kSampleList = 512;
-constexpr int kSampleBatch = 4;  // pieces of a row that a lane has in flight
+constexpr int kSampleList = 2048;   // words: two a thread
+constexpr int kSampleTopK = 512;    // up to here top-k is tried on a list; also how many words a list for top-p aims at
 
 // (By value: a bit cast of a vector's element itself reads its first one.)
 __device__ __forceinline__ float sample_bits(uint32_t u) { return __builtin_bit_cast(float, u); }
 
 template <int DT>
 struct SampleRow {
-  static constexpr int E = DT == LH_F32 ? 4 : 8;
+  static constexpr int E = DT == LH_F32 ? 4 : 8;  // words of a piece
+  static constexpr int kBatch = DT == LH_F32 ? 6 : 4;  // pieces that a lane has in flight
   const uint8_t* base;
   int V, begin, end, lane;  // of this wave
 
-  __device__ __forceinline__ void load(float* x, int i0) const {
+  __device__ __forceinline__ u32x4 load(int i0) const {
     constexpr int ES = DT == LH_F32 ? 4 : 2;
     if (i0 + E <= V) {
       const typename Chunk<ES>::type w = *reinterpret_cast<const typename Chunk<ES>::type*>(base + (int64_t)i0 * ES);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (DT == LH_F32) x[e] = sample_bits(w[e]);
-        else x[2 * e] = unpack_lo<DT>(w[e]), x[2 * e + 1] = unpack_hi<DT>(w[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = i0 + e < V ? load_as_f32<DT>(base, i0 + e) : -INFINITY;
+      return u32x4{w[0], w[1], w[2], w[3]};
     }
-    // No word: NaN, like -inf.
+    u32x4 w;
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = x[e] != x[e] ? -INFINITY : x[e];
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (DT == LH_F32) {
+        w[e] = i0 + e < V ? reinterpret_cast<const uint32_t*>(base)[i0 + e] : 0xff800000u;
+      } else {
+        constexpr uint32_t none = DT == LH_BF16 ? 0xff80u : 0xfc00u;  // -inf
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(base);
+        const uint32_t lo = i0 + 2 * e < V ? p[i0 + 2 * e] : none, hi = i0 + 2 * e + 1 < V ? p[i0 + 2 * e + 1] : none;
+        w[e] = lo | hi << 16;
+      }
+    }
+    return w;
+  }
+  // Words as numbers; what is no word (NaN) is -inf, -0 is 0.
+  __device__ __forceinline__ static void unpack(u32x4 w, float* x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (DT == LH_F32) x[e] = sample_bits(w[e]);
+      else x[2 * e] = unpack_lo<DT>(w[e]), x[2 * e + 1] = unpack_hi<DT>(w[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = x[e] >= -INFINITY ? x[e] + 0.0f : -INFINITY;
   }
   // f(x, first index) for every piece of the wave's share, in order.
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll 1
-    for (int i = begin; i < end; i += 64 * E * kSampleBatch) {
-      float x[kSampleBatch][E];
+    for (int i = begin; i < end; i += 64 * E * kBatch) {
+      u32x4 w[kBatch];
 #pragma unroll
-      for (int p = 0; p < kSampleBatch; ++p) load(x[p], i + p * 64 * E < end ? i + p * 64 * E + lane * E : V);
+      for (int p = 0; p < kBatch; ++p)
+        if (i + p * 64 * E < end) w[p] = load(i + p * 64 * E + lane * E);
 #pragma unroll
-      for (int p = 0; p < kSampleBatch; ++p)
-        if (i + p * 64 * E < end) f(x[p], i + p * 64 * E + lane * E);
+      for (int p = 0; p < kBatch; ++p)
+        if (i + p * 64 * E < end) {
+          float x[E];
+          unpack(w[p], x);
+          f(x, i + p * 64 * E + lane * E);
+        }
     }
   }
 };
@@ -77,13 +98,26 @@ __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor((unsigned long long)v, o);
   return v;
 }
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t v, int lane) {  // sum over the lanes up to this one
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t up = __shfl_up((unsigned long long)v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+
+// Numbers in the order of floats (no NaN, no -0), and back.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float of_order(uint32_t k) { return sample_bits(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 struct SampleShared {
-  unsigned long long mass[kSampleBins];
+  unsigned long long mass[kSampleBins];  // of a bin; of a word of the list
+  unsigned long long list[kSampleList];  // order of x, then falling index, of a word
   uint32_t count[kSampleBins];
-  float list_x[kSampleList];
-  int32_t list_i[kSampleList];
-  unsigned long long list_w[kSampleList];
   unsigned long long wave_mass[kSampleWaves];
   uint32_t wave_count[kSampleWaves];
   float wave_lo[kSampleWaves], wave_hi[kSampleWaves];
@@ -91,8 +125,7 @@ struct SampleShared {
   int32_t bin, listed;
   float cut_x;
   int32_t cut_i;
-  unsigned long long above_mass;
-  uint32_t above_count, in_bin;
+  unsigned long long above;
 };
 
 template <int DT>
@@ -102,19 +135,89 @@ struct Sampler {
   SampleRow<DT> row;
   int tid, lane, wave;
   float top;       // the largest logit
-  double inv_t, unit;
+  double c;        // log2(e) / T
+  double inv_t;
+  int bits;
   float cut_x;     // words below (cut_x, cut_i) have been dropped
   int32_t cut_i;
 
-  __device__ __forceinline__ double weight(float x) const { return x == top ? 1.0 : exp(((double)x - (double)top) * inv_t); }
-  __device__ __forceinline__ uint64_t mass(float x) const { return (uint64_t)(weight(x) * unit + 0.5); }
+  // 2^((x - top) c + shift): n + f = (x - top) c with |f| <= 1/2, 2^f = 1 + f p(f) with p of degree 7 through the values at the
+  // Chebyshev nodes of the interval (relative error 2.2e-12, at top exactly 1).
+  __device__ __forceinline__ double power(float x, int shift) const {
+    const double t = ((double)x - (double)top) * c, n = __builtin_rint(t), f = t - n;
+    double p = 1.325080551750225e-06;
+    p = __builtin_fma(p, f, 1.5303700711365693e-05);
+    p = __builtin_fma(p, f, 0.00015403475186530786);
+    p = __builtin_fma(p, f, 0.0013333478473685416);
+    p = __builtin_fma(p, f, 0.00961812913523614);
+    p = __builtin_fma(p, f, 0.055504109063258665);
+    p = __builtin_fma(p, f, 0.24022650695888503);
+    p = __builtin_fma(p, f, 0.6931471805568324);
+    p = __builtin_fma(p, f, 1.0);
+    return __builtin_ldexp(p, (int)fmax(n, -2000.0) + shift);
+  }
+  __device__ __forceinline__ double weight(float x) const { return x == top ? 1.0 : power(x, 0); }
+  // (A number below 2^52 plus 2^52 has its nearest whole number in the lower bits.)
+  __device__ __forceinline__ uint64_t mass(float x) const {
+    const uint64_t m = __builtin_bit_cast(uint64_t, power(x, bits) + 4503599627370496.0) & ((1ull << 52) - 1);
+    return x == top ? 1ull << bits : x > -INFINITY ? m : 0;
+  }
   __device__ __forceinline__ bool stays(float x, int i) const { return x > cut_x || (x == cut_x && i <= cut_i); }
+  __device__ __forceinline__ static unsigned long long entry(float x, int i) { return (unsigned long long)order_of(x) << 32 | (uint32_t)~i; }
+  __device__ __forceinline__ static float entry_x(unsigned long long e) { return of_order((uint32_t)(e >> 32)); }
+  __device__ __forceinline__ static int entry_i(unsigned long long e) { return (int)~(uint32_t)e; }
+
+  // Sum over the workgroup of all threads before this one; `total` of all.
+  __device__ __forceinline__ uint64_t block_before(uint64_t v, uint64_t* total) {
+    const uint64_t run = wave_scan64(v, lane);
+    __syncthreads();
+    if (lane == 63) s.wave_mass[wave] = run;
+    __syncthreads();
+    uint64_t before = run - v, all = 0;
+    for (int w = 0; w < kSampleWaves; ++w) {
+      if (w < wave) before += s.wave_mass[w];
+      all += s.wave_mass[w];
+    }
+    *total = all;
+    return before;
+  }
+
+  // The list in falling order; `n` words of it, the rest up to a power of two becomes 0.
+  __device__ __forceinline__ void sort(int n) {
+    int size = 64;
+    while (size < n) size <<= 1;
+    for (int i = n + tid; i < size; i += kSampleThreads) s.list[i] = 0;
+    __syncthreads();
+    if (size == 64) {  // one wave, in registers
+      if (wave == 0) {
+        unsigned long long v = s.list[lane];
+        for (int k = 2; k <= 64; k <<= 1)
+          for (int j = k >> 1; j > 0; j >>= 1) {
+            const unsigned long long o = __shfl_xor(v, j);
+            const bool larger = ((lane & k) == 0) == ((lane & j) == 0);  // this lane keeps the larger of the two
+            v = (v > o) == larger ? v : o;
+          }
+        s.list[lane] = v;
+      }
+      __syncthreads();
+      return;
+    }
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        const int i = 2 * tid - (tid & (j - 1));  // the lower of the thread's pair
+        if (i < size) {
+          const unsigned long long a = s.list[i], b = s.list[i + j];
+          if ((a < b) == ((i & k) == 0)) s.list[i] = b, s.list[i + j] = a;
+        }
+        __syncthreads();
+      }
+  }
 
   // Finds the last word that stays and makes it the cut: the first `k` words (BY_MASS false), or those before which less than top_p of
   // the mass of what is left lies.
   template <bool BY_MASS>
   __device__ __forceinline__ void cut(uint32_t k, double top_p, float lowest) {
-    float hi = top, lo = fmaxf(lowest, BY_MASS ? top - (float)(40.0 / inv_t) : top - 32.0f);
+    float hi = top, lo = fmaxf(lowest, BY_MASS ? top - (float)(20.0 / inv_t) : top - 32.0f);
     float below = INFINITY;          // words of this interval are at most this (and at least `from` after the first level)
     float from = -INFINITY;
     uint64_t above = 0, goal = 0;    // mass, or count, in front of the interval; what the last word brings it to, at least
@@ -122,56 +225,60 @@ struct Sampler {
 #pragma unroll 1
     for (int level = 0;; ++level) {
       const double width = (double)hi - (double)lo;
-      const float inv32 = (float)(kSampleBins / (width > 0 ? width : 1.0));
       const double inv64 = kSampleBins / (width > 0 ? width : 1.0);
+      const float inv32 = (float)inv64;
       // Falls with x: the same expression finds a word's bin when it is counted and when it is listed.
       auto bin_of = [&](float x) -> int {
         if (level == 0) return (int)fminf((hi - x) * inv32, (float)(kSampleBins - 1));
         return (int)fmin(((double)hi - (double)x) * inv64, (double)(kSampleBins - 1));
       };
       auto inside = [&](float x, int i) { return x <= below && x >= from && x > -INFINITY && stays(x, i); };
-      for (int i = tid; i < kSampleBins; i += kSampleThreads) s.mass[i] = 0, s.count[i] = 0;
+      for (int i = tid; i < kSampleBins; i += kSampleThreads) {
+        if (BY_MASS) s.mass[i] = 0;
+        else s.count[i] = 0;
+      }
       if (tid == 0) s.listed = 0;
       __syncthreads();
+      uint64_t rest = 0;  // of the last bin: what does not come by an atomic
       row.each([&](const float* x, int i0) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (inside(x[e], i0 + e)) {
+        for (int e = 0; e < E; ++e) {
+          if constexpr (BY_MASS) {
+            const uint64_t m = mass(x[e]);
+            if (inside(x[e], i0 + e)) {
+              const int at = bin_of(x[e]);
+              if (at == kSampleBins - 1) rest += m;
+              else atomicAdd(&s.mass[at], (unsigned long long)m);
+            }
+          } else if (inside(x[e], i0 + e)) {
             const int at = bin_of(x[e]);
-            atomicAdd(&s.count[at], 1u);
-            if (BY_MASS) atomicAdd(&s.mass[at], (unsigned long long)mass(x[e]));
+            if (at == kSampleBins - 1) ++rest;
+            else atomicAdd(&s.count[at], 1u);
           }
+        }
       });
+      rest = wave_sum64(rest);
+      if (lane == 0 && rest != 0) {
+        if (BY_MASS) atomicAdd(&s.mass[kSampleBins - 1], (unsigned long long)rest);
+        else atomicAdd(&s.count[kSampleBins - 1], (uint32_t)rest);
+      }
       __syncthreads();
       // Running sums over the bins, two a thread, from above.
-      const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
-      const uint64_t v0 = BY_MASS ? s.mass[2 * tid] : c0, v1 = BY_MASS ? s.mass[2 * tid + 1] : c1;
-      uint64_t run = v0 + v1;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t up = __shfl_up((unsigned long long)run, o);
-        if (lane >= o) run += up;
-      }
-      if (lane == 63) s.wave_mass[wave] = run;
-      __syncthreads();
-      uint64_t before = above + run - v0 - v1, total = above;
-      for (int w = 0; w < kSampleWaves; ++w) {
-        if (w < wave) before += s.wave_mass[w];
-        total += s.wave_mass[w];
-      }
+      const uint64_t v0 = BY_MASS ? s.mass[2 * tid] : s.count[2 * tid], v1 = BY_MASS ? s.mass[2 * tid + 1] : s.count[2 * tid + 1];
+      uint64_t total;
+      const uint64_t before = above + block_before(v0 + v1, &total);
       if (BY_MASS && level == 0) {
         // "less than top_p of the mass before it" in whole numbers: before < ceil(top_p * mass).
         goal = (uint64_t)ceil(top_p * (double)total);
         if (goal < 1) goal = 1;
         if (goal > total) goal = total;
       }
-      if (goal > total) return;  // (fewer than k words are left: infinite ones)
-      if (before < goal && goal <= before + v0) s.bin = 2 * tid, s.above_mass = before, s.in_bin = c0;
-      else if (before + v0 < goal && goal <= before + v0 + v1) s.bin = 2 * tid + 1, s.above_mass = before + v0, s.in_bin = c1;
+      if (goal > above + total) return;  // (fewer than k words are left: infinite ones)
+      if (before < goal && goal <= before + v0) s.bin = 2 * tid, s.above = before;
+      else if (before + v0 < goal && goal <= before + v0 + v1) s.bin = 2 * tid + 1, s.above = before + v0;
       __syncthreads();
       const int at = s.bin;
-      const uint32_t members = s.in_bin;
-      above = s.above_mass;
+      above = s.above;
       // The members of the bin: listed if they are few, and their lowest and highest value.
       float low = INFINITY, high = -INFINITY;
       row.each([&](const float* x, int i0) {
@@ -179,11 +286,8 @@ struct Sampler {
         for (int e = 0; e < E; ++e)
           if (inside(x[e], i0 + e) && bin_of(x[e]) == at) {
             low = fminf(low, x[e]), high = fmaxf(high, x[e]);
-            if (members <= kSampleList) {
-              const int j = atomicAdd(&s.listed, 1);
-              s.list_x[j] = x[e], s.list_i[j] = i0 + e;
-              if (BY_MASS) s.list_w[j] = mass(x[e]);
-            }
+            const int j = atomicAdd(&s.listed, 1);
+            if (j < kSampleList) s.list[j] = entry(x[e], i0 + e);
           }
       });
 #pragma unroll
@@ -191,18 +295,16 @@ struct Sampler {
       if (lane == 0) s.wave_lo[wave] = low, s.wave_hi[wave] = high;
       __syncthreads();
       for (int w = 0; w < kSampleWaves; ++w) low = fminf(low, s.wave_lo[w]), high = fmaxf(high, s.wave_hi[w]);
+      const int members = s.listed;
       if (members <= kSampleList) {
-        if (tid < (int)members) {  // what lies before this member, in the order
-          const float x = s.list_x[tid];
-          const int i = s.list_i[tid];
-          const uint64_t own = BY_MASS ? s.list_w[tid] : 1;
-          uint64_t front = above;
-          for (int j = 0; j < (int)members; ++j) {
-            const float y = s.list_x[j];
-            if (y > x || (y == x && s.list_i[j] < i)) front += BY_MASS ? s.list_w[j] : 1;
-          }
-          if (front < goal && goal <= front + own) s.cut_x = x, s.cut_i = i;
-        }
+        sort(members);
+        const int j0 = 2 * tid, j1 = j0 + 1;
+        const unsigned long long e0 = j0 < members ? s.list[j0] : 0, e1 = j1 < members ? s.list[j1] : 0;
+        const uint64_t m0 = j0 >= members ? 0 : BY_MASS ? mass(entry_x(e0)) : 1, m1 = j1 >= members ? 0 : BY_MASS ? mass(entry_x(e1)) : 1;
+        uint64_t all;
+        const uint64_t front = above + block_before(m0 + m1, &all);
+        if (front < goal && goal <= front + m0) s.cut_x = entry_x(e0), s.cut_i = entry_i(e0);
+        else if (front + m0 < goal && goal <= front + m0 + m1) s.cut_x = entry_x(e1), s.cut_i = entry_i(e1);
         __syncthreads();
         cut_x = s.cut_x, cut_i = s.cut_i;
         return;
@@ -255,6 +357,97 @@ struct Sampler {
     __syncthreads();
     return s.cut_i;
   }
+
+  // u * all as the whole number that the running sum has to exceed.
+  __device__ __forceinline__ static uint64_t goal_of(double u, uint64_t all) {
+    uint64_t goal = all - 1;
+    if (u < 1.0) goal = u > 0.0 ? (uint64_t)(u * (double)all) : 0;
+    return goal > all - 1 ? all - 1 : goal;
+  }
+
+  // Everything on a list of the largest words, if they are enough: whether they were (to every thread alike).  `mine`: this thread's
+  // largest word.  top_k: 0 or at most kSampleTopK.
+  __device__ __forceinline__ bool by_list(float mine, uint32_t words, uint32_t top_k, float top_p, double least, double u, int64_t* token) {
+    const uint32_t aim = top_k > 0 ? top_k : kSampleTopK;
+    // The value that `aim` threads reach: the lower end of its bin among the threads' largest.
+    const float lo = top - (float)(32.0 / (top_k > 0 ? 1.0 : inv_t));
+    const float inv = (float)kSampleBins / (top - lo);
+    for (int i = tid; i < kSampleBins; i += kSampleThreads) s.count[i] = 0;
+    if (tid == 0) s.listed = 0, s.bin = -1;
+    __syncthreads();
+    // (a width that is 0 or infinite sends all of them to one bin: still the lower end of a bin)
+    const int bin = mine > -INFINITY ? (int)fminf((top - mine) * inv, (float)(kSampleBins - 1)) : kSampleBins;
+    if (bin < kSampleBins) atomicAdd(&s.count[bin], 1u);
+    __syncthreads();
+    const uint64_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+    uint64_t threads;
+    const uint64_t before = block_before(c0 + c1, &threads);
+    if (before < aim && aim <= before + c0) s.bin = 2 * tid;
+    else if (before + c0 < aim && aim <= before + c0 + c1) s.bin = 2 * tid + 1;
+    __syncthreads();
+    float least_x = INFINITY;
+    if (s.bin < 0) {
+      least_x = -INFINITY;  // fewer threads have words: all of them
+    } else {
+      if (bin <= s.bin) least_x = mine;
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) least_x = fminf(least_x, __shfl_xor(least_x, o));
+      if (lane == 0) s.wave_lo[wave] = least_x;
+      __syncthreads();
+      for (int w = 0; w < kSampleWaves; ++w) least_x = fminf(least_x, s.wave_lo[w]);
+    }
+    const bool weigh = top_k == 0 && top_p < 1.0f;
+    uint64_t all_mass = 0;
+    row.each([&](const float* x, int i0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (weigh) all_mass += mass(x[e]);
+        if (x[e] >= least_x && x[e] > -INFINITY) {
+          const int j = atomicAdd(&s.listed, 1);
+          if (j < kSampleList) s.list[j] = entry(x[e], i0 + e);
+        }
+      }
+    });
+    __syncthreads();
+    const int n = s.listed;
+    if (n > kSampleList) return false;
+    uint64_t total = 0;
+    if (weigh) block_before(all_mass, &total);
+    sort(n);
+    const int j0 = 2 * tid, j1 = j0 + 1;
+    const int first = top_k > 0 ? min((int)top_k, n) : n;  // of the list
+    const unsigned long long e0 = j0 < first ? s.list[j0] : 0, e1 = j1 < first ? s.list[j1] : 0;
+    const uint64_t m0 = j0 < first ? mass(entry_x(e0)) : 0, m1 = j1 < first ? mass(entry_x(e1)) : 0;
+    uint64_t of_list;
+    uint64_t front = block_before(m0 + m1, &of_list);
+    if (!weigh) total = of_list;
+    uint64_t goal = ~0ull;
+    if (top_p < 1.0f) {
+      goal = (uint64_t)ceil((double)top_p * (double)total);
+      goal = goal < 1 ? 1 : goal > total ? total : goal;
+    }
+    uint64_t kept;
+    block_before((uint64_t)(j0 < first && (j0 == 0 || (front < goal && weight(entry_x(e0)) >= least))) +
+                     (j1 < first && front + m0 < goal && weight(entry_x(e1)) >= least), &kept);
+    const bool in0 = j0 < (int)kept, in1 = j1 < (int)kept;
+    // All of the list stays, and words that are not on it might: it was too short.
+    if (kept == (uint64_t)n && (uint32_t)n < words && !(top_k > 0 && (int)top_k <= n) && of_list < goal) return false;
+    uint64_t all;
+    block_before((in0 ? m0 : 0) + (in1 ? m1 : 0), &all);
+    const uint64_t aim_mass = goal_of(u, all);
+    // In the order of the indices.
+    __syncthreads();
+    if (in0) s.list[j0] = (unsigned long long)(uint32_t)~entry_i(e0) << 32 | (uint32_t)j0, s.mass[j0] = m0;
+    if (in1) s.list[j1] = (unsigned long long)(uint32_t)~entry_i(e1) << 32 | (uint32_t)j1, s.mass[j1] = m1;
+    __syncthreads();
+    sort((int)kept);
+    const unsigned long long f0 = j0 < (int)kept ? s.list[j0] : 0, f1 = j1 < (int)kept ? s.list[j1] : 0;
+    const uint64_t g0 = j0 < (int)kept ? s.mass[(uint32_t)f0] : 0, g1 = j1 < (int)kept ? s.mass[(uint32_t)f1] : 0;
+    front = block_before(g0 + g1, &all);
+    if (front <= aim_mass && aim_mass < front + g0) *token = (int)~(uint32_t)(f0 >> 32);
+    else if (front + g0 <= aim_mass && aim_mass < front + g0 + g1) *token = (int)~(uint32_t)(f1 >> 32);
+    return true;
+  }
 };
 
 template <int DT>
@@ -284,6 +477,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
       if (x[e] > -INFINITY) lowest = fminf(lowest, x[e]), ++words;
     }
   });
+  const float mine = top;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
     const float x = __shfl_xor(top, o);
@@ -307,9 +501,15 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
     return;
   }
 
-  Sampler<DT> f = {s, row, tid, lane, wave, top, 1.0 / (double)temperature, (double)(1ull << a.bits), -INFINITY, -1};
+  const double inv_t = 1.0 / (double)temperature;
+  Sampler<DT> f = {s, row, tid, lane, wave, top, inv_t * 1.4426950408889634, inv_t, a.bits, -INFINITY, -1};
+  const double least = min_p > 0.0f ? (double)min_p : 0.0;
+  const bool few = top_k > 0 && (uint32_t)top_k < words;
+  if (top < INFINITY && (few ? top_k <= kSampleTopK : top_p < 1.0f || least > 0.0))
+    if (f.by_list(mine, words, few ? top_k : 0, top_p, least, u, a.tokens + b)) return;
+  __syncthreads();
   if (top == INFINITY) f.cut_x = INFINITY, f.cut_i = 0x7fffffff, lowest = top;  // only those
-  if (top_k > 0 && (uint32_t)top_k < words) f.template cut<false>((uint32_t)top_k, 0.0, lowest);
+  if (few) f.template cut<false>((uint32_t)top_k, 0.0, lowest);
   if (top_p < 1.0f) {
     __syncthreads();
     f.template cut<true>(0, (double)top_p, lowest);
@@ -317,11 +517,10 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   __syncthreads();
 
   // What stays: its mass by waves, and within a wave by up to 64 groups of pieces, lane g has group g's.
-  const double least = min_p > 0.0f ? (double)min_p : 0.0;
   auto left = [&](float x, int i) -> uint64_t {
+    const uint64_t m = f.mass(x);
     if (!(x > -INFINITY) || !f.stays(x, i)) return 0;
-    const double w = f.weight(x);
-    return w >= least || i == top_i ? (uint64_t)(w * f.unit + 0.5) : 0;
+    return least == 0.0 || f.weight(x) >= least || i == top_i ? m : 0;
   };
   const int group = ((share / (64 * E) + 63) / 64) * 64 * E;  // words
   uint64_t of_group = 0, total = 0;
@@ -342,32 +541,19 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
     if (w < wave) before += s.wave_mass[w];
     all += s.wave_mass[w];
   }
-  // The word whose running sum is the first above u * all: above `goal`, a whole number below `all`.
-  uint64_t goal = all - 1;
-  if (u < 1.0) goal = u > 0.0 ? (uint64_t)(u * (double)all) : 0;
-  if (goal > all - 1) goal = all - 1;
+  const uint64_t goal = f.goal_of(u, all);
   if (!(before <= goal && goal < before + total)) return;
-  uint64_t run = of_group;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t up = __shfl_up((unsigned long long)run, o);
-    if (lane >= o) run += up;
-  }
+  const uint64_t run = wave_scan64(of_group, lane);
   const int g = __popcll(__ballot(before + run <= goal));  // groups that end at or before it
   before += g == 0 ? 0 : __shfl((unsigned long long)run, g - 1);
   for (int i = begin + g * group; i < end; i += 64 * E) {
     const int i0 = i + lane * E;
     float x[E];
-    row.load(x, i0);
+    row.unpack(row.load(i0), x);
     uint64_t m[E], own = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) own += m[e] = left(x[e], i0 + e);
-    uint64_t sum = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t up = __shfl_up((unsigned long long)sum, o);
-      if (lane >= o) sum += up;
-    }
+    const uint64_t sum = wave_scan64(own, lane);
     uint64_t at = before + sum - own;
     if (at <= goal && goal < at + own) {
 #pragma unroll
@@ -392,9 +578,8 @@ extern "C" int lh_hip_sample(int64_t* tokens, const void* logits, const float* u
   LH_REQUIRE(B <= 1 || ld >= V, "lh_hip_sample: rows overlap");
   LH_REQUIRE(dtype == LH_F32 || dtype == LH_BF16 || dtype == LH_F16, "lh_hip_sample: unsupported dtype %d", dtype);
   if (B == 0) return LH_OK;
-  SampleArgs a = {tokens, logits, uniform, ld, (int32_t)V, 62, *opts};
+  SampleArgs a = {tokens, logits, uniform, ld, (int32_t)V, 50, *opts};
   while ((V >> (62 - a.bits)) != 0) --a.bits;
-  if (a.bits > 52) a.bits = 52;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)B), block(kSampleThreads);
   if (dtype == LH_F32) LH_LAUNCH(sample_kernel<LH_F32>, grid, block, 0, s, a);
