@@ -400,17 +400,18 @@ typedef struct lh_paged_cache {
 } lh_paged_cache;
 
 /*
- * Keys and values of new tokens into the cache: k, v [B, n_kv_heads, T, d] (strides z: batch, h: head, t: token)
- * in the cache's dtype, or F32, BF16 or F16 for a cache of e4m3, which holds e4m3(clamp(x / scale, +-448)), rounded to
+ * Keys and values of new tokens into the cache: k, v [B, n_kv_heads, T, d] (element strides of batch,
+ * head and token, unit stride along d) in the cache's dtype, or F32, BF16 or F16 for a cache of e4m3, which holds e4m3(clamp(x / scale, +-448)), rounded to
  * nearest even.  Token t of sequence b goes to position positions[b] + t if t < counts[b] (counts may be NULL: all of
  * them do); a position outside the table or on a page that holds nothing is dropped.  Two tokens for one slot leave either.
  */
-int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, lh_strides3 sk, lh_strides3 sv,
-                     const int32_t* positions, const int32_t* counts, int64_t B, int64_t T, int32_t dtype, void* stream);
+int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, int64_t k_stride_b, int64_t k_stride_h,
+                     int64_t k_stride_t, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, const int32_t* positions,
+                     const int32_t* counts, int64_t B, int64_t T, int32_t dtype, void* stream);
 
 /*
- * Attention of one new token of every sequence over its cache: q, out [B, H, d] (strides z: batch, h: head; t is
- * not used), H a multiple of n_kv_heads, head h reads key / value head h / (H / n_kv_heads):
+ * Attention of one new token of every sequence over its cache: q, out [B, H, d] (element strides of batch and head, unit
+ * stride along d), H a multiple of n_kv_heads, head h reads key / value head h / (H / n_kv_heads):
  *   out[b, h] = sum_t p_t v_t,  p = softmax over t < lengths[b] of scale q . k_t,
  * positions on pages that hold nothing left out; 0 where nothing is left.  `lengths` counts the new token if it has been
  * appended and is clamped to 0 .. max_pages * page_size.  Scores, softmax and sums are f32.  dtype (of q and out) is the
@@ -420,8 +421,8 @@ int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, 
  * that overlap in time need a workspace each.  It needs no clearing.
  */
 size_t lh_hip_paged_attention_workspace_bytes(const lh_paged_cache* cache, int64_t B, int64_t H, int32_t with_weights);
-int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q, lh_strides3 so, lh_strides3 sq,
-                           const int32_t* lengths, float* weights, int64_t weights_stride_b, int64_t weights_stride_h,
+int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q, int64_t out_stride_b, int64_t out_stride_h,
+                           int64_t q_stride_b, int64_t q_stride_h, const int32_t* lengths, float* weights, int64_t weights_stride_b, int64_t weights_stride_h,
                            int64_t B, int64_t H, float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
                            void* stream);
 

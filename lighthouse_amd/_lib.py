@@ -122,6 +122,11 @@ class PagedCache(ctypes.Structure):
                 ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
 
 
+# These two for struct.pack, a fifth of the time: the entry points take their bytes.
+PAGED_CACHE_FORMAT = "@PPPq3q3q5qi2f4x"
+SAMPLE_OPTS_FORMAT = "@4Pfi2f"
+
+
 class SampleOpts(ctypes.Structure):
     _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p),
                 ("temperature_all", ctypes.c_float), ("top_k_all", ctypes.c_int32), ("top_p_all", ctypes.c_float),
@@ -170,13 +175,12 @@ PROTOTYPES = {
     "lh_hip_nanogpt_forward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32, ctypes.POINTER(NanoGPTBlockOpts)]),
     "lh_hip_nanogpt_forward": (_i32, [_vp, _vp, ctypes.POINTER(NanoGPTBlockParams), _i64, _vp, _vp, _vp, _vp, _i64, _i64,
                                       _i64, _i64, _i64, _f32, _i32, ctypes.POINTER(NanoGPTBlockOpts), _vp, _sz, _vp]),
-    "lh_hip_kv_append": (_i32, [ctypes.POINTER(PagedCache), _vp, _vp, Strides3, Strides3, _vp, _vp, _i64, _i64, _i32, _vp]),
-    "lh_hip_paged_attention_workspace_bytes": (_sz, [ctypes.POINTER(PagedCache), _i64, _i64, _i32]),
-    "lh_hip_paged_attention": (_i32, [ctypes.POINTER(PagedCache), _vp, _vp, Strides3, Strides3, _vp, _vp, _i64, _i64, _i64, _i64,
-                                      _f32, _i32, _vp, _sz, _vp]),
+    "lh_hip_kv_append": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "lh_hip_paged_attention_workspace_bytes": (_sz, [_vp, _i64, _i64, _i32]),
+    "lh_hip_paged_attention": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _i32, _vp, _sz, _vp]),
     "lh_hip_kv_evict_workspace_bytes": (_sz, [_i64, _i64, _i64]),
-    "lh_hip_kv_evict": (_i32, [ctypes.POINTER(PagedCache), _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
-    "lh_hip_sample": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, ctypes.POINTER(SampleOpts), _vp]),
+    "lh_hip_kv_evict": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "lh_hip_sample": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp]),
     "lh_hip_payload_matmul": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MatmulAttrs)]),
     "lh_hip_payload_matmul_fp8": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MatmulFp8Attrs)]),
     "lh_hip_payload_mlp": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MlpAttrs)]),

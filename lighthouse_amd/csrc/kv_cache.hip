@@ -324,8 +324,9 @@ using namespace lh;
 
 extern "C" {
 
-int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, lh_strides3 sk, lh_strides3 sv,
-                     const int32_t* positions, const int32_t* counts, int64_t B, int64_t T, int32_t dtype, void* stream) {
+int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, int64_t k_stride_b, int64_t k_stride_h,
+                     int64_t k_stride_t, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, const int32_t* positions,
+                     const int32_t* counts, int64_t B, int64_t T, int32_t dtype, void* stream) {
   AppendArgs a = {};
   if (const int rc = paged_cache(cache, "lh_hip_kv_append", &a.c)) return rc;
   LH_REQUIRE(k && v && positions, "lh_hip_kv_append: null pointer");
@@ -334,7 +335,7 @@ int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, 
   LH_REQUIRE(dtype == cache->dtype || cache->dtype == LH_F8E4M3,
              "lh_hip_kv_append: keys and values must have the cache's dtype (any of 16 or 32 bits for a cache of e4m3)");
   if (B == 0 || T == 0) return LH_OK;
-  a.k = k, a.v = v, a.sk = sk, a.sv = sv, a.positions = positions, a.counts = counts;
+  a.k = k, a.v = v, a.sk = {k_stride_b, k_stride_h, k_stride_t}, a.sv = {v_stride_b, v_stride_h, v_stride_t}, a.positions = positions, a.counts = counts;
   a.B = (int32_t)B, a.T = (int32_t)T;
   const int e = dtype == LH_F32 && cache->dtype == LH_F32 ? 4 : 8, chunks = (a.c.d + e - 1) / e;
   a.per_token = 2 * a.c.heads * chunks;

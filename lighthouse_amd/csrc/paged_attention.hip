@@ -31,7 +31,7 @@ struct PagedAttnArgs {
   int64_t so_z, so_h, sq_z, sq_h;
   const int32_t* lengths;
   int32_t B, H, G, rows, groups;  // rows = min(G, 16) queries a workgroup, groups = ceil(G / 16) of them
-  int32_t splits, min_share;      // of the positions: at least min_share each
+  int32_t share, splits;          // positions a workgroup takes of a sequence, workgroups for the positions of the table
   float scale_log2e;
   float* part_o;   // [B heads groups][splits][rows][DP]
   float2* part_ml; // [B heads groups][splits][rows]
@@ -40,11 +40,10 @@ struct PagedAttnArgs {
   int32_t cap_pad;
 };
 
-// How many positions a workgroup takes of a sequence of n: as many for each of the splits, in whole rounds of its waves.
-__device__ __forceinline__ int paged_share(const PagedAttnArgs& a, int n) {
-  const int even = (n + a.splits - 1) / a.splits;
-  return (max(even, a.min_share) + a.min_share - 1) / a.min_share * a.min_share;
-}
+constexpr int kPagedWaves = 4;
+constexpr int kPagedShare = 32 * kPagedWaves;  // positions a share is a multiple of
+
+__device__ __forceinline__ int paged_length(const PagedAttnArgs& a, int b) { return min(max(a.lengths[b], 0), a.c.capacity()); }
 
 template <int DT>
 __device__ __forceinline__ f32x4 paged_mma(u32x4 a, u32x4 b, f32x4 c) {
@@ -110,15 +109,19 @@ __device__ __forceinline__ void load_buffer(uint32_t* out, __amdgpu_buffer_rsrc_
 // TILES: the pages are multiples of 16 positions and rows 16-byte aligned, so that a tile of 16 keys has one base and its rows
 // are loaded through a buffer resource whose size is that of the rows that exist: what lies behind comes back as 0 without a
 // test.  Otherwise every lane finds the page of every row it loads.
+// Waves of a SIMD that the registers have to suffice for: as many as they do without scratch memory.
+constexpr int paged_occupancy(int cdt, int dp, bool tiles) {
+  return dp == 64 ? 4 : dp == 256 ? 1 : tiles && cdt != LH_F32 ? 3 : 2;
+}
 template <int CDT, int QDT, int DP, int NW, bool TILES>
-__global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) paged_attention_kernel(PagedAttnArgs a) {
   constexpr bool F32 = CDT == LH_F32;
   constexpr int ES = CDT == LH_F8E4M3 ? 1 : F32 ? 4 : 2;
   constexpr int KT = F32 ? 1 : 2;            // 16-key tiles a step
   constexpr int KEYS = 16 * KT;
-  constexpr int KS = F32 ? DP / 16 : DP / 32;  // pieces of a key's row a lane takes
-  constexpr int KE = F32 ? 4 : 8;              // elements of such a piece
-  constexpr int KB = KE * ES;                  // its bytes
+  constexpr int KB = 16;                       // bytes of a piece of a key's row
+  constexpr int KE = KB / ES;                  // its elements
+  constexpr int KS = DP / 4 / KE;              // pieces a lane takes: columns s 4 KE + g4 KE and on of piece s
   constexpr int CE = DP / 16;                  // columns of a value's row a lane takes
   constexpr int VB = CE * ES;
   constexpr int VP = VB > 16 ? VB / 16 : 1;    // loads for them
@@ -129,29 +132,43 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = blockIdx.x % a.splits;
-  const int item = blockIdx.x / a.splits;  // (sequence, key / value head, group of queries)
-  const int group = item % a.groups, bh = item / a.groups;
-  const int hk = bh % a.c.heads, b = bh / a.c.heads;
-  const int n = min(max(a.lengths[b], 0), a.c.capacity());
-  const int share = paged_share(a, n);
-  const int k0 = split * share;
-  if (k0 >= n && split > 0) return;
-  const int k1 = min(n, k0 + share);
+  // An item is a (sequence, key / value head, group of queries).  The first shares of all items come first.  Workgroups whose ids
+  // agree modulo 8 run on one XCD: an item's shares go round them, else those of the long sequences could meet on a few.
+  const int items = a.B * a.c.heads * a.groups, split = blockIdx.x / items;
+  const int item = (int)((blockIdx.x - (unsigned)split * items + split) % (unsigned)items);
+  const int group = item % a.groups, rest = item / a.groups;
+  const int hk = rest % a.c.heads, b = rest / a.c.heads;
+  const int k0 = split * a.share, table_end = min(a.c.capacity(), k0 + a.share);
+  const int32_t* table = a.c.table + b * a.c.table_stride;
+  int ahead[KT];       // what the table says for a later step
+  auto find_pages = [&](int step, int* found) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const int key = k0 + step * KEYS + 16 * t + (TILES ? 0 : l16);
+      found[t] = key < table_end ? table[a.c.by_size.div((uint32_t)key)] : -1;
+    }
+  };
+  // (The share is the host's choice, so that the table is asked without waiting for the length.)
+  int head_start[KT];
+  find_pages(wave, head_start);
+  find_pages(wave + NW, ahead);
+  const int n = paged_length(a, b);
   const int q_row = group * 16 + l16;           // of the G queries
   const bool q_live = q_row < a.G;
   const int head = hk * a.G + min(q_row, a.G - 1);
 
   // The queries, in the layout of the second operand.
-  uint32_t qf[KS][4];
+  constexpr int QES = F32 ? 4 : 2, QP = KE * QES / 16;  // 16-byte pieces of a query that go with a piece of a key
+  uint32_t qf[KS * QP][4];
   {
-    constexpr int QES = F32 ? 4 : 2;
     const uint8_t* q = static_cast<const uint8_t*>(a.q) + (b * a.sq_z + head * a.sq_h) * QES;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d0 = s * (4 * KE) + g4 * KE;
-      load_row_piece<16, QES>(qf[s], q + d0 * QES, q_live ? (a.c.d - d0) * QES : 0);
-    }
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < QP; ++i) {
+        const int d0 = s * (4 * KE) + g4 * KE + i * (16 / QES);
+        load_row_piece<16, QES>(qf[s * QP + i], q + d0 * QES, q_live ? (a.c.d - d0) * QES : 0);
+      }
   }
 
   f32x4 acc[CE];
@@ -159,12 +176,13 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
   for (int i = 0; i < CE; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m_run = -INFINITY, l_run = 0.0f;
 
-  const int32_t* table = a.c.table + b * a.c.table_stride;
+  if (k0 >= n && split > 0) return;
+  const int k1 = min(n, k0 + a.share);
   const uint8_t* kb = static_cast<const uint8_t*>(a.c.k);
   const uint8_t* vb = static_cast<const uint8_t*>(a.c.v);
   const int row_bytes = a.c.d * ES;
   uint32_t kr[KT][KS][KB / 4], vr[KT * 4][VB / 4];
-  int pages[KT];       // TILES: of the step whose keys are requested next
+  int pages[KT];       // of the step that is requested next: of its tiles, or of the key 16 t + l16 that is the lane's
   int held[KT];        // TILES: how many rows of its tiles exist
   uint32_t live = 0;   // otherwise: which of the lane's KT * 4 keys do
 
@@ -183,35 +201,32 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
         voff[r][p] = col < row_bytes ? (g4 * 4 + r) * (int)a.c.sv.t * ES + col : kOutside;
       }
   }
-  auto find_pages = [&](int step) {
+  // TILES: where the rows of a tile of the next step begin (keys and values are laid out alike), and how many bytes there are.
+  int64_t tile_at[KT];
+  int tile_bytes[KT];
+  auto next_pages = [&](int step, const int* found) {
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      const int key = k0 + step * KEYS + 16 * t;
-      pages[t] = -1;
-      if (key < k1) {
-        const int p = table[a.c.by_size.div((uint32_t)key)];
-        if ((uint32_t)p < (uint32_t)a.c.pages) pages[t] = p;
+      const int key = k0 + step * KEYS + 16 * t + (TILES ? 0 : l16);
+      pages[t] = (uint32_t)found[t] < (uint32_t)a.c.pages && key < k1 ? found[t] : -1;
+      if constexpr (TILES) {
+        const int slot = key - (int)a.c.by_size.div((uint32_t)key) * a.c.size;
+        const int rows = pages[t] < 0 ? 0 : min(16, k1 - key);
+        tile_at[t] = rows == 0 ? 0 : (pages[t] * a.c.sk.z + hk * a.c.sk.h + slot * a.c.sk.t) * ES;
+        tile_bytes[t] = rows * (int)a.c.sk.t * ES;
       }
     }
-  };
-  auto request_tile = [&](int step, int t, const uint8_t* base, const lh_strides3& st, int page) {
-    const int key = k0 + step * KEYS + 16 * t;
-    const int slot = key - (int)a.c.by_size.div((uint32_t)key) * a.c.size;
-    const int rows = page < 0 ? 0 : min(16, k1 - key);
-    const int64_t at = page < 0 ? 0 : (page * st.z + hk * st.h + slot * st.t) * ES;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + at), 0, rows * (int)st.t * ES, 0x00020000);
   };
   auto request_keys = [&](int step) {
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       if constexpr (TILES) {
-        const __amdgpu_buffer_rsrc_t r = request_tile(step, t, kb, a.c.sk, pages[t]);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kb + tile_at[t]), 0, tile_bytes[t], 0x00020000);
 #pragma unroll
         for (int s = 0; s < KS; ++s) load_buffer<KB>(kr[t][s], r, koff[s]);
       } else {
-        const int key = k0 + step * KEYS + 16 * t + l16;
-        int slot = 0;
-        const int page = key < k1 ? a.c.page_of(b, key, &slot) : -1;
+        const int key = k0 + step * KEYS + 16 * t + l16, page = pages[t];
+        const int slot = key - (int)a.c.by_size.div((uint32_t)key) * a.c.size;
         const uint8_t* row = kb + (max(page, 0) * a.c.sk.z + hk * a.c.sk.h + slot * a.c.sk.t) * ES;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -228,7 +243,7 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
       if constexpr (TILES) {
         const int key = k0 + step * KEYS + 16 * t;
         held[t] = pages[t] < 0 ? 0 : min(16, k1 - key);
-        const __amdgpu_buffer_rsrc_t rs = request_tile(step, t, vb, a.c.sv, pages[t]);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vb + tile_at[t]), 0, tile_bytes[t], 0x00020000);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -236,9 +251,8 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int key = k0 + step * KEYS + 16 * t + 4 * g4 + r;
-          int slot = 0;
-          const int page = key < k1 ? a.c.page_of(b, key, &slot) : -1;
+          const int key = k0 + step * KEYS + 16 * t + 4 * g4 + r, page = __shfl(pages[t], 4 * g4 + r);
+          const int slot = key - (int)a.c.by_size.div((uint32_t)key) * a.c.size;
           const uint8_t* row = vb + (max(page, 0) * a.c.sv.z + hk * a.c.sv.h + slot * a.c.sv.t) * ES;
           load_row_piece<VB, ES>(vr[t * 4 + r], row + l16 * VB, page < 0 ? 0 : row_bytes - l16 * VB);
           live |= (page >= 0 ? 1u : 0u) << (t * 4 + r);
@@ -249,14 +263,15 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
 
   const int steps = (k1 - k0 + KEYS - 1) / KEYS;
   if (wave < steps) {
-    if constexpr (TILES) find_pages(wave);
+    next_pages(wave, head_start);
     request_keys(wave);
     request_values(wave);
   }
 #pragma unroll 1
   for (int step = wave; step < steps; step += NW) {
     const int next = step + NW;
-    if constexpr (TILES) find_pages(next);
+    next_pages(next, ahead);
+    find_pages(next + NW, ahead);
     // S^T: s[t][r] = S[query l16][key 16 t + 4 g4 + r]
     f32x4 s[KT];
 #pragma unroll
@@ -269,15 +284,22 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
           for (int e = 0; e < 4; ++e)
             s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kr[t][i][e]), __builtin_bit_cast(float, qf[i][e]), s[t], 0, 0, 0);
         } else {
-          u32x4 kf;
-          if constexpr (CDT == LH_F8E4M3) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) kf[2 * e] = paged_e4m3<QDT, false>(kr[t][i][e]), kf[2 * e + 1] = paged_e4m3<QDT, true>(kr[t][i][e]);
-          } else {
+          for (int j = 0; j < QP; ++j) {
+            u32x4 kf;
+            if constexpr (CDT == LH_F8E4M3) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) kf[e] = kr[t][i][e];
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t codes = kr[t][i][2 * j + e];
+                kf[2 * e] = paged_e4m3<QDT, false>(codes), kf[2 * e + 1] = paged_e4m3<QDT, true>(codes);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) kf[e] = kr[t][i][e];
+            }
+            const uint32_t(&qq)[4] = qf[i * QP + j];
+            s[t] = paged_mma<QDT>(kf, u32x4{qq[0], qq[1], qq[2], qq[3]}, s[t]);
           }
-          s[t] = paged_mma<QDT>(kf, u32x4{qf[i][0], qf[i][1], qf[i][2], qf[i][3]}, s[t]);
         }
       }
     }
@@ -312,9 +334,11 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
 #pragma unroll
       for (int t = 0; t < KT; ++t) *reinterpret_cast<f32x4*>(to + 16 * t) = x[t];
     }
-    mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
-    if (__any(mx > m_run)) {
+    // The maximum that p is relative to follows the true one with a delay: nothing is done until a score is 2^10 above it (a p of
+    // 2^10 is as accurate as one of 1), and then by all lanes together.
+    if (__any(mx > m_run + 10.0f)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float m_new = fmaxf(m_run, mx);
       const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
@@ -335,10 +359,10 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
 
     if constexpr (F32) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int j = 0; j < KT * 4; ++j)
 #pragma unroll
         for (int i = 0; i < CE; ++i)
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[r][i]), p[r], acc[i], 0, 0, 0);
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[j][i]), p[j], acc[i], 0, 0, 0);
     } else {
       u32x4 hi, lo;
 #pragma unroll
@@ -363,8 +387,8 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
           odd[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e], vw[2 * j][e], 0x07060302u);
         }
         acc[2 * e] = paged_mma<QDT>(even, hi, acc[2 * e]);
-        acc[2 * e] = paged_mma<QDT>(even, lo, acc[2 * e]);
         acc[2 * e + 1] = paged_mma<QDT>(odd, hi, acc[2 * e + 1]);
+        acc[2 * e] = paged_mma<QDT>(even, lo, acc[2 * e]);
         acc[2 * e + 1] = paged_mma<QDT>(odd, lo, acc[2 * e + 1]);
       }
     }
@@ -397,7 +421,7 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
     if (half > 1) __syncthreads();
   }
   if (wave != 0 || !q_live) return;
-  if (a.splits > 1) {
+  if (n > a.share) {
     const int64_t part = ((int64_t)item * a.splits + split) * a.rows + l16;
     if (g4 == 0) a.part_ml[part] = make_float2(m_all, l_all);
 #pragma unroll
@@ -418,77 +442,136 @@ __global__ void __launch_bounds__(NW * 64) paged_attention_kernel(PagedAttnArgs 
     }
 }
 
-// Joins the parts of one query: brings them to the common maximum and adds them, in the order of the positions.
-template <int QDT, int DP>
-__global__ void __launch_bounds__(256) paged_attention_merge(PagedAttnArgs a) {
-  constexpr int GROUPS = 256 / DP;
-  __shared__ float sums[GROUPS][DP];
-  const int bh = blockIdx.x, b = bh / a.H, head = bh % a.H;
-  const int hk = head / a.G, q_row = head % a.G;
-  const int item = (b * a.c.heads + hk) * a.groups + q_row / 16;
-  const int tid = threadIdx.x, col = tid % DP, first = tid / DP;
-  const int n = min(max(a.lengths[b], 0), a.c.capacity());
-  const int parts = n == 0 ? 0 : (n + paged_share(a, n) - 1) / paged_share(a, n);
-  const int64_t at = (int64_t)item * a.splits * a.rows + q_row % 16;
+// (maximum, sum) of one query over its parts, to every lane of the wave: the lanes take the parts in turn, the lanes' values are
+// brought together in a fixed order.
+__device__ __forceinline__ float2 paged_join(const float2* ml, int parts, int rows, int lane) {
   float m = -INFINITY, l = 0.0f;
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[at + (int64_t)p * a.rows].x);
-  const float m_safe = m == -INFINITY ? 0.0f : m;
-  for (int p = 0; p < parts; ++p) {
-    const float2 ml = a.part_ml[at + (int64_t)p * a.rows];
-    l += ml.y * __builtin_amdgcn_exp2f(ml.x - m_safe);
+  for (int p = lane; p < parts; p += 64) {
+    const float2 x = ml[(int64_t)p * rows];
+    const float to = fmaxf(m, x.x), safe = to == -INFINITY ? 0.0f : to;
+    l = l * __builtin_amdgcn_exp2f(m - safe) + x.y * __builtin_amdgcn_exp2f(x.x - safe);
+    m = to;
   }
-  float o = 0.0f;
-  for (int p = first; p < parts; p += GROUPS)
-    o += a.part_o[(at + (int64_t)p * a.rows) * DP + col] * __builtin_amdgcn_exp2f(a.part_ml[at + (int64_t)p * a.rows].x - m_safe);
-  if (GROUPS > 1) {
-    sums[first][col] = o;
-    __syncthreads();
-    if (first > 0) return;
+  float all = m;
 #pragma unroll
-    for (int g = 1; g < GROUPS; ++g) o += sums[g][col];
-  }
-  if (a.lse != nullptr && tid == 0) a.lse[bh] = m_safe + __builtin_amdgcn_logf(l);
-  if (col < a.c.d) store_from_f32<QDT>(a.out, b * a.so_z + head * a.so_h + col, l == 0.0f ? 0.0f : o * (a.c.v_scale / l));
+  for (int o = 32; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
+  const float safe = all == -INFINITY ? 0.0f : all;
+  l *= __builtin_amdgcn_exp2f(m - safe);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o);
+  return make_float2(safe, l);
 }
 
-// weights[b, g, t] += sum over the heads of the group of exp2(score - lse), heads in order.
-__global__ void __launch_bounds__(256) paged_attention_weights(PagedAttnArgs a, float* weights, int64_t sw_b, int64_t sw_h) {
-  const int per_head = (a.c.capacity() + 255) / 256, bh = blockIdx.x / per_head;
+// The first B H workgroups join the parts of a query each: they bring them to the common maximum and add them in the order of the
+// positions.  The others, where weights are asked for, take 256 positions of a head of a sequence: weights[b, g, t] += sum over the
+// heads of the group of exp2(score - log2 of the head's sum), heads in order; they find that sum for themselves.
+template <int QDT, int DP>
+__global__ void __launch_bounds__(256) paged_attention_finish(PagedAttnArgs a, int joins, float* weights, int64_t sw_b, int64_t sw_h) {
+  constexpr int GROUPS = 256 / DP;
+  __shared__ float sums[GROUPS][DP];
+  __shared__ float lse[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if ((int)blockIdx.x < joins) {
+    const int bh = blockIdx.x, b = bh / a.H, head = bh % a.H;
+    const int n = paged_length(a, b), parts = (n + a.share - 1) / a.share;
+    if (parts <= 1) return;  // (written at once)
+    const int hk = head / a.G, q_row = head % a.G, col = tid % DP, first = tid / DP;
+    const int64_t at = ((int64_t)(b * a.c.heads + hk) * a.groups + q_row / 16) * a.splits * a.rows + q_row % 16;
+    // (the first of a thread's parts are requested before the maximum is known)
+    constexpr int EARLY = 8;
+    float early[EARLY], scale[EARLY];
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) {
+      const int64_t p = at + (int64_t)min(first + i * GROUPS, parts - 1) * a.rows;
+      early[i] = a.part_o[p * DP + col], scale[i] = a.part_ml[p].x;
+    }
+    const float2 ml = paged_join(a.part_ml + at, parts, a.rows, lane);
+    float o = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i)
+      if (first + i * GROUPS < parts) o += early[i] * __builtin_amdgcn_exp2f(scale[i] - ml.x);
+#pragma unroll 4
+    for (int p = first + EARLY * GROUPS; p < parts; p += GROUPS)
+      o += a.part_o[(at + (int64_t)p * a.rows) * DP + col] * __builtin_amdgcn_exp2f(a.part_ml[at + (int64_t)p * a.rows].x - ml.x);
+    if (GROUPS > 1) {
+      sums[first][col] = o;
+      __syncthreads();
+      if (first > 0) return;
+#pragma unroll
+      for (int g = 1; g < GROUPS; ++g) o += sums[g][col];
+    }
+    if (col < a.c.d) store_from_f32<QDT>(a.out, b * a.so_z + head * a.so_h + col, ml.y == 0.0f ? 0.0f : o * (a.c.v_scale / ml.y));
+    return;
+  }
+  const int per_head = (a.c.capacity() + 255) / 256, bh = (blockIdx.x - joins) / per_head;
   const int b = bh / a.c.heads, hk = bh % a.c.heads;
-  const int t = (blockIdx.x - bh * per_head) * 256 + threadIdx.x;
-  if (t >= min(max(a.lengths[b], 0), a.c.capacity())) return;
+  const int t0 = (blockIdx.x - joins - bh * per_head) * 256, t = t0 + tid;
+  const int n = paged_length(a, b);
+  if (t0 >= n) return;
+  const int parts = (n + a.share - 1) / a.share;
   const int64_t first = (int64_t)b * a.H + hk * a.G;
   float sum = 0.0f;
-  for (int g = 0; g < a.G; ++g) {
-    const float x = a.scores[(first + g) * a.cap_pad + t];
-    sum += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - a.lse[first + g]);
+  for (int g0 = 0; g0 < a.G; g0 += 256) {  // (up to 256 heads of a group at a time)
+    const int many = min(256, a.G - g0);
+    if (g0 > 0) __syncthreads();
+    if (parts == 1) {
+      if (tid < many) lse[tid] = a.lse[first + g0 + tid];
+    } else {
+      for (int g = wave; g < many; g += 4) {
+        const int64_t at = ((int64_t)bh * a.groups + (g0 + g) / 16) * a.splits * a.rows + (g0 + g) % 16;
+        const float2 ml = paged_join(a.part_ml + at, parts, a.rows, lane);
+        if (lane == 0) lse[g] = ml.x + __builtin_amdgcn_logf(ml.y);
+      }
+    }
+    __syncthreads();
+    if (t < n)
+      for (int g = 0; g < many; ++g) {
+        const float x = a.scores[(first + g0 + g) * a.cap_pad + t];
+        sum += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - lse[g]);
+      }
   }
-  weights[b * sw_b + hk * sw_h + t] += sum;
+  if (t < n) weights[b * sw_b + hk * sw_h + t] += sum;
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 
-constexpr int kPagedWaves = 4;
-
 struct PagedPlan {
-  int rows, groups, splits, min_share, dp, cap_pad;
+  int rows, groups, share, splits, dp, cap_pad;
+  bool tiles;
   size_t o_bytes, ml_bytes, score_bytes, lse_bytes;
   size_t total() const { return o_bytes + ml_bytes + score_bytes + lse_bytes; }
 };
 
 static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
 
-static PagedPlan paged_plan(const Paged& c, int64_t B, int64_t H, bool with_weights) {
+static bool paged_in_tiles(const Paged& c, int es) {
+  const lh_strides3& s = c.sk;
+  return c.size % 16 == 0 && c.d * es % 16 == 0 && s.z == c.sv.z && s.h == c.sv.h && s.t == c.sv.t && s.z * es % 16 == 0 && s.h * es % 16 == 0 &&
+         s.t * es % 16 == 0 && 16 * s.t * es < 0x40000000 && s.t >= c.d && aligned16(c.k) && aligned16(c.v);
+}
+
+// How many positions a workgroup takes of a sequence; `items` (sequence, head, group of queries), `per_cu` workgroups that a CU
+// holds at once, `row_bytes` of a position's key and value.
+static int paged_share(int64_t items, int capacity, int per_cu, int64_t row_bytes) {
+  const int64_t cus = num_cus();
+  int64_t splits = ((per_cu < 2 ? 1 : 2) * cus + items - 1) / items;
+  if (per_cu >= 3) {
+    const int64_t level = (8 * cus + items - 1) / items, most = capacity * row_bytes >> 19;
+    splits = splits > level ? splits : level < most ? level : splits > most ? splits : most;
+  }
+  const int64_t share = (capacity + splits - 1) / splits;
+  return (int)((share + kPagedShare - 1) / kPagedShare * kPagedShare);
+}
+
+static PagedPlan paged_plan(const Paged& c, int cache_dtype, int64_t B, int64_t H, bool with_weights) {
   PagedPlan p = {};
   const int G = (int)(H / c.heads);
   p.rows = G < 16 ? G : 16, p.groups = (G + 15) / 16;
   p.dp = c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
-  p.min_share = 32 * kPagedWaves;
-  const int64_t items = B * c.heads * p.groups, want = 6 * (int64_t)num_cus();
-  int64_t splits = (want + items - 1) / items;
-  const int64_t most = (c.capacity() + 2 * p.min_share - 1) / (2 * p.min_share);
-  if (splits > most) splits = most;
-  p.splits = splits < 1 ? 1 : (int)splits;
+  p.tiles = paged_in_tiles(c, (int)dtype_size(cache_dtype));
+  const int64_t items = B * c.heads * p.groups;
+  p.share = paged_share(items, c.capacity(), paged_occupancy(cache_dtype, p.dp, p.tiles), 2 * (int64_t)c.d * (int64_t)dtype_size(cache_dtype));
+  p.splits = (c.capacity() + p.share - 1) / p.share;
   if (p.splits > 1) {
     p.o_bytes = granules((size_t)items * p.splits * p.rows * p.dp * 4);
     p.ml_bytes = granules((size_t)items * p.splits * p.rows * 8);
@@ -502,29 +585,23 @@ static PagedPlan paged_plan(const Paged& c, int64_t B, int64_t H, bool with_weig
 }
 
 template <int CDT, int QDT, int DP>
-static int launch_paged(const PagedAttnArgs& a, bool tiles, hipStream_t s) {
+static int launch_paged(const PagedAttnArgs& a, bool tiles, float* weights, int64_t sw_b, int64_t sw_h, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.B * a.c.heads * a.groups * a.splits)), block(kPagedWaves * 64);
   if (tiles) LH_LAUNCH((paged_attention_kernel<CDT, QDT, DP, kPagedWaves, true>), grid, block, 0, s, a);
   else LH_LAUNCH((paged_attention_kernel<CDT, QDT, DP, kPagedWaves, false>), grid, block, 0, s, a);
   if (const int rc = check_launch("paged_attention")) return rc;
-  if (a.splits == 1) return LH_OK;
-  LH_LAUNCH((paged_attention_merge<QDT, DP>), dim3((unsigned)(a.B * a.H)), dim3(256), 0, s, a);
-  return check_launch("paged_attention_merge");
+  const int joins = a.splits > 1 ? a.B * a.H : 0;
+  const unsigned blocks = joins + (weights ? (unsigned)((a.c.capacity() + 255) / 256 * (int64_t)a.B * a.c.heads) : 0u);
+  if (blocks == 0) return LH_OK;
+  LH_LAUNCH((paged_attention_finish<QDT, DP>), dim3(blocks), dim3(256), 0, s, a, joins, weights, sw_b, sw_h);
+  return check_launch("paged_attention_finish");
 }
 
 template <int CDT, int QDT>
-static int launch_paged_dp(const PagedAttnArgs& a, int dp, bool tiles, hipStream_t s) {
-  if (dp == 64) return launch_paged<CDT, QDT, 64>(a, tiles, s);
-  if (dp == 128) return launch_paged<CDT, QDT, 128>(a, tiles, s);
-  return launch_paged<CDT, QDT, 256>(a, tiles, s);
-}
-
-static bool paged_in_tiles(const Paged& c, int es) {
-  const int per = es == 4 ? 4 : 8, chunk = es == 1 ? 8 : 16;  // elements of a key's piece, bytes
-  // (a lane's piece of a value's row: 16 codes of a row of more than 128)
-  bool ok = c.size % 16 == 0 && c.d % per == 0 && (es != 1 || c.d <= 128 || c.d % 16 == 0);
-  for (const lh_strides3* s : {&c.sk, &c.sv}) ok = ok && (s->z * es) % chunk == 0 && (s->h * es) % chunk == 0 && (s->t * es) % chunk == 0 && 16 * s->t * es < 0x40000000 && s->t >= c.d;
-  return ok && reinterpret_cast<uintptr_t>(c.k) % chunk == 0 && reinterpret_cast<uintptr_t>(c.v) % chunk == 0;
+static int launch_paged_dp(const PagedAttnArgs& a, int dp, bool tiles, float* w, int64_t sw_b, int64_t sw_h, hipStream_t s) {
+  if (dp == 64) return launch_paged<CDT, QDT, 64>(a, tiles, w, sw_b, sw_h, s);
+  if (dp == 128) return launch_paged<CDT, QDT, 128>(a, tiles, w, sw_b, sw_h, s);
+  return launch_paged<CDT, QDT, 256>(a, tiles, w, sw_b, sw_h, s);
 }
 
 }  // namespace lh
@@ -537,11 +614,11 @@ size_t lh_hip_paged_attention_workspace_bytes(const lh_paged_cache* cache, int64
   Paged c;
   if (paged_cache(cache, "lh_hip_paged_attention_workspace_bytes", &c) != LH_OK) return 0;
   if (B <= 0 || H <= 0 || H % c.heads != 0) return 0;
-  return paged_plan(c, B, H, with_weights != 0).total();
+  return paged_plan(c, cache->dtype, B, H, with_weights != 0).total();
 }
 
-int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q, lh_strides3 so, lh_strides3 sq,
-                           const int32_t* lengths, float* weights, int64_t weights_stride_b, int64_t weights_stride_h,
+int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q, int64_t out_stride_b, int64_t out_stride_h,
+                           int64_t q_stride_b, int64_t q_stride_h, const int32_t* lengths, float* weights, int64_t weights_stride_b, int64_t weights_stride_h,
                            int64_t B, int64_t H, float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
                            void* stream) {
   PagedAttnArgs a = {};
@@ -555,27 +632,25 @@ int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q
   LH_REQUIRE(weights == nullptr || ((a.c.heads == 1 || weights_stride_h >= a.c.capacity()) && (B <= 1 || weights_stride_b >= a.c.capacity())),
              "lh_hip_paged_attention: rows of the weights overlap");
   LH_REQUIRE(weights == nullptr || (a.c.capacity() + 255) / 256 * B * a.c.heads < (1ll << 24), "lh_hip_paged_attention: too many weights (fewer than 2^32)");
-  const PagedPlan p = paged_plan(a.c, B, H, weights != nullptr);
+  const PagedPlan p = paged_plan(a.c, cache->dtype, B, H, weights != nullptr);
   LH_REQUIRE(p.total() == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= p.total()),
              "lh_hip_paged_attention: workspace too small or not 256-byte aligned: %zu of %zu bytes", workspace_bytes, p.total());
-  a.out = out, a.q = q, a.so_z = so.z, a.so_h = so.h, a.sq_z = sq.z, a.sq_h = sq.h, a.lengths = lengths;
+  a.out = out, a.q = q, a.so_z = out_stride_b, a.so_h = out_stride_h, a.sq_z = q_stride_b, a.sq_h = q_stride_h, a.lengths = lengths;
   a.B = (int32_t)B, a.H = (int32_t)H, a.G = (int32_t)(H / a.c.heads);
-  a.rows = p.rows, a.groups = p.groups, a.splits = p.splits, a.min_share = p.min_share, a.cap_pad = p.cap_pad;
+  a.rows = p.rows, a.groups = p.groups, a.share = p.share, a.splits = p.splits, a.cap_pad = p.cap_pad;
   a.scale_log2e = (float)((double)scale * a.c.k_scale * 1.4426950408889634);
   char* ws = static_cast<char*>(workspace);
   if (p.splits > 1) a.part_o = reinterpret_cast<float*>(ws), a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
   if (weights) a.scores = reinterpret_cast<float*>(ws + p.o_bytes + p.ml_bytes), a.lse = reinterpret_cast<float*>(ws + p.o_bytes + p.ml_bytes + p.score_bytes);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const bool tiles = paged_in_tiles(a.c, (int)dtype_size(cache->dtype));
-  int rc = LH_ERR_UNSUPPORTED;
-  if (cache->dtype == LH_F8E4M3) rc = dtype == LH_BF16 ? launch_paged_dp<LH_F8E4M3, LH_BF16>(a, p.dp, tiles, s) : launch_paged_dp<LH_F8E4M3, LH_F16>(a, p.dp, tiles, s);
-  else if (dtype == LH_BF16) rc = launch_paged_dp<LH_BF16, LH_BF16>(a, p.dp, tiles, s);
-  else if (dtype == LH_F16) rc = launch_paged_dp<LH_F16, LH_F16>(a, p.dp, tiles, s);
-  else rc = launch_paged_dp<LH_F32, LH_F32>(a, p.dp, tiles, s);
-  if (rc != LH_OK || weights == nullptr) return rc;
-  LH_LAUNCH(paged_attention_weights, dim3((unsigned)((a.c.capacity() + 255) / 256 * B * a.c.heads)), dim3(256), 0, s, a, weights,
-            weights_stride_b, weights_stride_h);
-  return check_launch("paged_attention_weights");
+  const bool tiles = p.tiles;
+  const int64_t sb = weights_stride_b, sh = weights_stride_h;
+  if (cache->dtype == LH_F8E4M3)
+    return dtype == LH_BF16 ? launch_paged_dp<LH_F8E4M3, LH_BF16>(a, p.dp, tiles, weights, sb, sh, s)
+                            : launch_paged_dp<LH_F8E4M3, LH_F16>(a, p.dp, tiles, weights, sb, sh, s);
+  if (dtype == LH_BF16) return launch_paged_dp<LH_BF16, LH_BF16>(a, p.dp, tiles, weights, sb, sh, s);
+  if (dtype == LH_F16) return launch_paged_dp<LH_F16, LH_F16>(a, p.dp, tiles, weights, sb, sh, s);
+  return launch_paged_dp<LH_F32, LH_F32>(a, p.dp, tiles, weights, sb, sh, s);
 }
 
 }  // extern "C"

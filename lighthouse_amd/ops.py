@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -531,58 +532,75 @@ def nanogpt_forward(x, layers: list, lnf_g, lnf_b, lm_w, lm_b, n_head: int, *, e
 
 # ---- generation over a paged key / value cache ------------------------------------------------------------------------
 _CACHE_DTYPES = (torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn)
+_SAMPLE_OPTIONS = ("temperature", "top_k", "top_p", "min_p")
+_PACK_SAMPLE = struct.Struct(_lib.SAMPLE_OPTS_FORMAT).pack
+_PACK_CACHE = struct.Struct(_lib.PAGED_CACHE_FORMAT).pack
 
 
 def _on_current_device(*tensors) -> None:
     """Launches go to the current device's stream: tensors of another device would be read there through the wrong one."""
-    _need_cuda(*tensors)
-    device = torch._C._cuda_getDevice()
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device.index != device:
-            raise ValueError(f"expected tensors on the current device (cuda:{device}), got {t.device}")
+        if t is not None and t.get_device() != device:
+            _need_cuda(*tensors)
+            raise ValueError(f"expected tensors on one device, got {tensors[0].device} and {t.device}")
+    if device < 0:
+        raise ValueError("expected tensors on the GPU")
+    if device != torch._C._cuda_getDevice():
+        raise ValueError(f"expected tensors on the current device (cuda:{torch._C._cuda_getDevice()}), got {tensors[0].device}")
 
 
-def _is_index(t, shape, what: str) -> None:
-    if t.dtype != torch.int32 or t.shape != shape or (t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{what} must be an int32 tensor of shape {list(shape)} with innermost stride 1, got {tuple(t.shape)} {t.dtype}")
+def _is_index(t, n, what: str) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what} must be a contiguous int32 vector of {n}, got {tuple(t.shape)} {t.dtype}")
 
 
-def _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale) -> _lib.PagedCache:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+def _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale):
+    """Checks a cache and its block table for B sequences: (lh_paged_cache as bytes, kv heads, d, positions of the table).
+    (Runs in front of launches of a few microseconds: plain conditions, the struct packed in one go.)"""
+    shape, dtype = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must have the same shape [pages, kv heads, page size, d]")
-    if k_cache.dtype not in _CACHE_DTYPES or v_cache.dtype != k_cache.dtype:
+    if dtype not in _CACHE_DTYPES or v_cache.dtype != dtype:
         raise ValueError("k_cache and v_cache must have one dtype (float32, bfloat16, float16 or float8_e4m3fn)")
-    pages, heads, size, d = k_cache.shape
+    pages, heads, size, d = shape
     if not (1 <= d <= 256 and pages and heads and size):
-        raise ValueError(f"the cache must hold something, with a head dimension of 1 to 256, got {tuple(k_cache.shape)}")
-    for t in (k_cache, v_cache):
-        st = t.stride()
+        raise ValueError(f"the cache must hold something, with a head dimension of 1 to 256, got {tuple(shape)}")
+    sk, sv = k_cache.stride(), v_cache.stride()
+    for st in (sk,) if sv == sk else (sk, sv):
         if st[3] != 1 and d != 1:
             raise ValueError("k_cache and v_cache: innermost stride must be 1")
-        if any(n > 1 and step < d for n, step in zip(t.shape[:3], st)):
+        if (st[0] < d and pages > 1) or (st[1] < d and heads > 1) or (st[2] < d and size > 1):
             raise ValueError("k_cache and v_cache: rows overlap")
-    if block_table.dim() != 2 or block_table.shape[1] < 1:
-        raise ValueError("block_table must have shape [B, pages of a sequence]")
-    _is_index(block_table, (B, block_table.shape[1]), "block_table")
-    if B > 1 and block_table.stride(0) < block_table.shape[1]:
-        raise ValueError("rows of block_table overlap")
-    if block_table.shape[1] * size >= 2**31 - 65536:
+    rows = block_table.shape
+    if len(rows) != 2 or rows[0] != B or rows[1] < 1 or block_table.dtype != torch.int32:
+        raise ValueError(f"block_table must be an int32 tensor of shape [{B}, pages of a sequence], got {tuple(rows)} {block_table.dtype}")
+    step, inner = block_table.stride()
+    if inner != 1 and rows[1] > 1:
+        raise ValueError("block_table: innermost stride must be 1")
+    if step < rows[1]:
+        if B > 1:
+            raise ValueError("rows of block_table overlap")
+        step = rows[1]
+    if rows[1] * size >= 2**31 - 65536:
         raise ValueError("the block table must hold fewer than 2^31 - 65536 positions")
-    if k_cache.dtype != torch.float8_e4m3fn and not (k_scale == 1.0 and v_scale == 1.0):
-        raise ValueError("k_scale and v_scale belong to a cache of float8_e4m3fn")
-    if not (0.0 < k_scale < math.inf and 0.0 < v_scale < math.inf):
-        raise ValueError("k_scale and v_scale must be positive numbers")
-    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-                           max(block_table.stride(0), block_table.shape[1]), _strides3(k_cache),
-                           _strides3(v_cache), pages, block_table.shape[1], size, heads, d, lh_dtype(k_cache.dtype), k_scale, v_scale)
+    if not (k_scale == 1.0 and v_scale == 1.0):
+        if dtype != torch.float8_e4m3fn:
+            raise ValueError("k_scale and v_scale belong to a cache of float8_e4m3fn")
+        if not (0.0 < k_scale < math.inf and 0.0 < v_scale < math.inf):
+            raise ValueError("k_scale and v_scale must be positive numbers")
+    return (_PACK_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), step, *sk[:3], *sv[:3], pages, rows[1], size,
+                        heads, d, lh_dtype(dtype), k_scale, v_scale), heads, d, rows[1] * size)
 
 
 def _cache_weights(weights, B, heads, capacity):
-    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[:2] != (B, heads) or weights.shape[2] < capacity:
-        raise ValueError(f"weights must be a float32 tensor of shape [{B}, {heads}, {capacity} or more], got {tuple(weights.shape)} {weights.dtype}")
+    shape = weights.shape
+    if weights.dtype != torch.float32 or len(shape) != 3 or shape[0] != B or shape[1] != heads or shape[2] < capacity:
+        raise ValueError(f"weights must be a float32 tensor of shape [{B}, {heads}, {capacity} or more], got {tuple(shape)} {weights.dtype}")
     st = weights.stride()
-    if (st[2] != 1 and weights.shape[2] != 1) or (heads > 1 and st[1] < capacity) or (B > 1 and st[0] < capacity):
+    if (st[2] != 1 and shape[2] != 1) or (heads > 1 and st[1] < capacity) or (B > 1 and st[0] < capacity):
         raise ValueError("weights: innermost stride must be 1, and rows must not overlap")
+    return st
 
 
 def kv_append(k, v, k_cache, v_cache, block_table, positions, *, counts=None, k_scale=1.0, v_scale=1.0):
@@ -594,37 +612,39 @@ def kv_append(k, v, k_cache, v_cache, block_table, positions, *, counts=None, k_
     sequence b lies on page block_table[b, t // size], slot t % size.  Token t goes to position positions[b] + t (int32 [B]) if
     t < counts[b] (int32 [B]; None: all do).  Positions outside the table, and pages outside the cache (-1 for an entry not in use), are left out.
     Every token needs a slot of its own."""
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 4 or v.shape != shape or v.dtype != dtype:
         raise ValueError("k and v must have the same shape [B, kv heads, T, d] and dtype")
-    B, heads, T, d = k.shape
-    cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
-    if (heads, d) != (k_cache.shape[1], k_cache.shape[3]):
-        raise ValueError(f"k and v have {heads} heads of {d}, the cache {k_cache.shape[1]} of {k_cache.shape[3]}")
-    if k.dtype not in _FLOATS or (k.dtype != k_cache.dtype and k_cache.dtype != torch.float8_e4m3fn):
+    B, heads, T, d = shape
+    cache, cache_heads, cache_d, _ = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
+    if heads != cache_heads or d != cache_d:
+        raise ValueError(f"k and v have {heads} heads of {d}, the cache {cache_heads} of {cache_d}")
+    if dtype not in _FLOATS or (dtype != k_cache.dtype and k_cache.dtype != torch.float8_e4m3fn):
         raise ValueError("k and v must have the cache's dtype (float32, bfloat16 or float16 for a cache of float8_e4m3fn)")
-    if d != 1 and (k.stride(3) != 1 or v.stride(3) != 1):
+    sk, sv = k.stride(), v.stride()
+    if d != 1 and (sk[3] != 1 or sv[3] != 1):
         raise ValueError("innermost stride must be 1")
-    _is_index(positions, (B,), "positions")
+    _is_index(positions, B, "positions")
     if counts is not None:
-        _is_index(counts, (B,), "counts")
+        _is_index(counts, B, "counts")
     _on_current_device(k, v, k_cache, v_cache, block_table, positions, counts)
-    if k.numel() == 0:
-        return k_cache, v_cache
-    _lib.check(_lib.load().lh_hip_kv_append(
-        ctypes.byref(cache), k.data_ptr(), v.data_ptr(), *_strides3_of(k, v), positions.data_ptr(),
-        counts.data_ptr() if counts is not None else None, B, T, lh_dtype(k.dtype), _stream()), "kv_append")
+    if B and T:
+        _lib.check(_lib.load().lh_hip_kv_append(
+            cache, k.data_ptr(), v.data_ptr(), *sk[:3], *sv[:3], positions.data_ptr(),
+            counts.data_ptr() if counts is not None else None, B, T, lh_dtype(dtype), _stream()), "kv_append")
     return k_cache, v_cache
 
 
 def _vector_workspace(workspace, need, like):
-    """The caller's workspace, or one from torch's allocator, which a captured graph keeps for itself."""
+    """(address, bytes) of the caller's workspace, or of one from torch's allocator, which hands out its memory again only to work
+    that follows on this stream, and which a captured graph keeps for itself."""
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=like.device) if need else None
+        return (torch.empty(need, dtype=torch.uint8, device=like.device).data_ptr(), need) if need else (None, 0)
     _on_current_device(workspace)
     if not (workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous() and workspace.numel() >= need
             and workspace.data_ptr() % 256 == 0):
         raise ValueError(f"workspace must be a contiguous uint8 vector of at least {need} bytes, 256-byte aligned")
-    return workspace
+    return workspace.data_ptr(), workspace.numel()
 
 
 def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, out=None, weights=None, k_scale=1.0, v_scale=1.0,
@@ -638,51 +658,48 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, ou
     positions of the block table: weights[b, g, t] grows by the probabilities of position t, added over the heads of group g
     (what kv_evict goes by).  `workspace` (uint8, see paged_attention_workspace_bytes): temporary memory, otherwise
     torch's allocator is asked; two calls that overlap in time need one each."""
-    if q.dim() != 3:
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3:
         raise ValueError("paged_attention expects q of shape [B, H, d]")
-    B, H, d = q.shape
-    cache = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
-    if d != k_cache.shape[3]:
-        raise ValueError(f"q has a head dimension of {d}, the cache of {k_cache.shape[3]}")
-    if H == 0 or H % k_cache.shape[1]:
-        raise ValueError(f"{H} heads are no multiple of the cache's {k_cache.shape[1]}")
-    if q.dtype != k_cache.dtype and not (k_cache.dtype == torch.float8_e4m3fn and q.dtype in (torch.bfloat16, torch.float16)):
+    B, H, d = shape
+    cache, heads, cache_d, capacity = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
+    if d != cache_d:
+        raise ValueError(f"q has a head dimension of {d}, the cache of {cache_d}")
+    if H == 0 or H % heads:
+        raise ValueError(f"{H} heads are no multiple of the cache's {heads}")
+    if dtype not in _FLOATS or (dtype != k_cache.dtype and (k_cache.dtype != torch.float8_e4m3fn or dtype == torch.float32)):
         raise ValueError("q must have the cache's dtype (bfloat16 or float16 for a cache of float8_e4m3fn)")
-    if q.dtype not in _FLOATS:
-        raise ValueError(f"unsupported dtype {q.dtype}")
+    sq = q.stride()
     if out is None:
-        out = torch.empty((B, H, d), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.shape != shape or out.dtype != dtype:
         raise ValueError("out must have the shape and dtype of q")
-    so, sq = out.stride(), q.stride()
+    so = out.stride()
     if d != 1 and (so[2] != 1 or sq[2] != 1):
         raise ValueError("innermost stride must be 1")
     if (H > 1 and so[1] < d) or (B > 1 and so[0] < d):
         raise ValueError("rows of out overlap")
-    _is_index(lengths, (B,), "lengths")
-    capacity = cache.max_pages * cache.page_size
+    _is_index(lengths, B, "lengths")
+    w_ptr, w_b, w_h = None, 0, 0
     if weights is not None:
-        _cache_weights(weights, B, cache.n_kv_heads, capacity)
+        w_b, w_h, _ = _cache_weights(weights, B, heads, capacity)
+        w_ptr = weights.data_ptr()
     _on_current_device(q, k_cache, v_cache, block_table, lengths, out, weights)
     if B == 0:
         return out
     lib = _lib.load()
-    workspace = _vector_workspace(workspace, lib.lh_hip_paged_attention_workspace_bytes(ctypes.byref(cache), B, H, weights is not None), q)
+    ws_ptr, ws_bytes = _vector_workspace(workspace, lib.lh_hip_paged_attention_workspace_bytes(cache, B, H, w_ptr is not None), q)
     _lib.check(lib.lh_hip_paged_attention(
-        ctypes.byref(cache), out.data_ptr(), q.data_ptr(), _lib.Strides3(so[0], so[1], 0), _lib.Strides3(sq[0], sq[1], 0),
-        lengths.data_ptr(), weights.data_ptr() if weights is not None else None,
-        weights.stride(0) if weights is not None else 0, weights.stride(1) if weights is not None else 0, B, H,
-        float(scale) if scale is not None else 1.0 / math.sqrt(d), lh_dtype(q.dtype),
-        workspace.data_ptr() if workspace is not None else None, workspace.numel() if workspace is not None else 0, _stream()),
-        "paged_attention")
+        cache, out.data_ptr(), q.data_ptr(), so[0], so[1], sq[0], sq[1], lengths.data_ptr(), w_ptr, w_b, w_h, B, H,
+        1.0 / math.sqrt(d) if scale is None else scale, lh_dtype(dtype), ws_ptr, ws_bytes, _stream()), "paged_attention")
     return out
 
 
 def paged_attention_workspace_bytes(q, k_cache, v_cache, block_table, *, weights=False) -> int:
     """Bytes of temporary memory that paged_attention takes for these tensors (only their shapes and strides matter);
     `weights`: whether the call passes any."""
-    cache = _paged_cache(k_cache, v_cache, block_table, q.shape[0], 1.0, 1.0)
-    return int(_lib.load().lh_hip_paged_attention_workspace_bytes(ctypes.byref(cache), q.shape[0], q.shape[1], 1 if weights else 0))
+    cache = _paged_cache(k_cache, v_cache, block_table, q.shape[0], 1.0, 1.0)[0]
+    return int(_lib.load().lh_hip_paged_attention_workspace_bytes(cache, q.shape[0], q.shape[1], 1 if weights else 0))
 
 
 def kv_evict(k_cache, v_cache, weights, block_table, lengths, budget, *, recent=0, out=None, workspace=None):
@@ -692,24 +709,22 @@ def kv_evict(k_cache, v_cache, weights, block_table, lengths, budget, *, recent=
     them up to the old length become 0.  Every position below the length must lie on a page of its own.
     Cache, block table and weights are those of kv_append and paged_attention; `workspace` as there (kv_evict_workspace_bytes)."""
     B = lengths.shape[0] if lengths.dim() == 1 else -1
-    _is_index(lengths, (B,), "lengths")
-    cache = _paged_cache(k_cache, v_cache, block_table, B, 1.0, 1.0)
-    _cache_weights(weights, B, cache.n_kv_heads, cache.max_pages * cache.page_size)
+    _is_index(lengths, B, "lengths")
+    cache, heads, _, capacity = _paged_cache(k_cache, v_cache, block_table, B, 1.0, 1.0)
+    w_b, w_h, _ = _cache_weights(weights, B, heads, capacity)
     budget, recent = int(budget), int(recent)
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"budget must be at least 1 and recent between 0 and the budget, got {budget} and {recent}")
     if out is None:
         out = torch.empty(B, dtype=torch.int32, device=lengths.device)
-    _is_index(out, (B,), "out")
+    _is_index(out, B, "out")
     _on_current_device(k_cache, v_cache, weights, block_table, lengths, out)
     if B == 0:
         return out
     lib = _lib.load()
-    need = lib.lh_hip_kv_evict_workspace_bytes(B, cache.n_kv_heads, min(budget, cache.max_pages * cache.page_size))
-    workspace = _vector_workspace(workspace, need, lengths)
-    _lib.check(lib.lh_hip_kv_evict(
-        ctypes.byref(cache), weights.data_ptr(), weights.stride(0), weights.stride(1), lengths.data_ptr(), out.data_ptr(), B,
-        budget, recent, workspace.data_ptr() if workspace is not None else None, need, _stream()), "kv_evict")
+    ws_ptr, ws_bytes = _vector_workspace(workspace, lib.lh_hip_kv_evict_workspace_bytes(B, heads, min(budget, capacity)), lengths)
+    _lib.check(lib.lh_hip_kv_evict(cache, weights.data_ptr(), w_b, w_h, lengths.data_ptr(), out.data_ptr(), B, min(budget, capacity),
+                                   min(recent, capacity), ws_ptr, ws_bytes, _stream()), "kv_evict")
     return out
 
 
@@ -736,26 +751,22 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, o
     if B > 1 and logits.stride(0) < V:
         raise ValueError("rows of logits overlap")
     _is_vector(uniform, B, torch.float32, "uniform")
-    opts = _lib.SampleOpts()
-    vectors = []
-    for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                               ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+    pointers, numbers, vectors = [0, 0, 0, 0], [1.0, 0, 1.0, 0.0], []
+    for i, value in enumerate((temperature, top_k, top_p, min_p)):
         if isinstance(value, torch.Tensor):
-            _is_vector(value, B, dtype, name)
+            _is_vector(value, B, torch.int32 if i == 1 else torch.float32, _SAMPLE_OPTIONS[i])
+            pointers[i] = value.data_ptr()
             vectors.append(value)
-            setattr(opts, name, value.data_ptr())
-        elif name == "top_k":
-            opts.top_k_all = max(0, min(int(value), 2**31 - 1))
         else:
-            setattr(opts, name + "_all", float(value))
+            numbers[i] = max(0, min(int(value), 2**31 - 1)) if i == 1 else value
     if out is None:
         out = torch.empty(B, dtype=torch.int64, device=logits.device)
     _is_vector(out, B, torch.int64, "out")
     _on_current_device(logits, uniform, out, *vectors)
-    if B == 0:
-        return out
-    _lib.check(_lib.load().lh_hip_sample(out.data_ptr(), logits.data_ptr(), uniform.data_ptr(), B, V, max(logits.stride(0), V),
-                                         lh_dtype(logits.dtype), ctypes.byref(opts), _stream()), "sample")
+    if B:
+        _lib.check(_lib.load().lh_hip_sample(
+            out.data_ptr(), logits.data_ptr(), uniform.data_ptr(), B, V, max(logits.stride(0), V), lh_dtype(logits.dtype),
+            _PACK_SAMPLE(*pointers, *numbers), _stream()), "sample")
     return out
 
 

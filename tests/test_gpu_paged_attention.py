@@ -87,7 +87,8 @@ def test_weights_grow_by_the_probabilities(dtype, G, size):
 def test_long_caches_are_split_and_joined(lengths, heads):
     c = ref.Cache(lengths, heads, 64, 128, bf16, seed=7)
     q = (3.0 * torch.randn(len(lengths), 4 * heads, 128, generator=torch.Generator().manual_seed(7))).to(bf16).cuda()
-    assert ops.paged_attention_workspace_bytes(q, c.k_cache, c.v_cache, c.table) > 0
+    if max(lengths) > 1000:  # (partial results of several workgroups)
+        assert ops.paged_attention_workspace_bytes(q, c.k_cache, c.v_cache, c.table) > 0
     check(q, c, ops.paged_attention(q, c.k_cache, c.v_cache, c.table, c.device_lengths))
 
 

@@ -43,7 +43,7 @@ def test_a_cache_is_refused():
     refused("block_table", call, q, k, v, table[:2], n)
     refused("block_table", call, q, k, v, z(3, dtype=i32), n)
     refused("block_table", call, q, k, v, z(3, 0, dtype=i32), n)
-    refused("innermost stride 1", call, q, k, v, z(2, 3, dtype=i32).t(), n)
+    refused("innermost stride", call, q, k, v, z(2, 3, dtype=i32).t(), n)
     refused("rows of block_table overlap", call, q, k, v, z(1, 2, dtype=i32).expand(3, 2), n)
     long = z(1, 1, 2**20, 8, dtype=bf16)
     refused("positions", call, q[:, :1], long, long, z(3, 2**11, dtype=i32), n)
@@ -140,13 +140,13 @@ def test_the_c_entry_points_refuse_without_a_gpu():
         return ctypes.byref(c)
 
     def attention(c, q=4096, B=3, H=4, dtype=_lib.BF16, ws=None, size=0, weights=None):
-        return lib.lh_hip_paged_attention(c, 4096, q, st, st, 4096, weights, 16, 8, B, H, 1.0, dtype, ws, size, None)
+        return lib.lh_hip_paged_attention(c, 4096, q, 32, 8, 32, 8, 4096, weights, 16, 8, B, H, 1.0, dtype, ws, size, None)
 
     bad = {"k": None, "block_table": None, "n_pages": 0, "max_pages": 2**30, "page_size": 0, "n_kv_heads": 0, "d": 257, "dtype": _lib.I8,
            "table_stride": 1, "k_scale": 0.0, "v_scale": math.inf, "sk": _lib.Strides3(64, 32, 7)}
     for name, value in bad.items():
         assert attention(paged(**{name: value})) == _lib.LH_ERR_INVALID, name
-        assert lib.lh_hip_kv_append(paged(**{name: value}), 4096, 4096, st, st, 4096, None, 3, 5, _lib.BF16, None) == _lib.LH_ERR_INVALID
+        assert lib.lh_hip_kv_append(paged(**{name: value}), 4096, 4096, 64, 32, 8, 64, 32, 8, 4096, None, 3, 5, _lib.BF16, None) == _lib.LH_ERR_INVALID
         assert lib.lh_hip_kv_evict(paged(**{name: value}), 4096, 16, 8, 4096, 4096, 3, 4, 0, 4096, 1 << 20, None) == _lib.LH_ERR_INVALID
         assert lib.lh_hip_paged_attention_workspace_bytes(paged(**{name: value}), 3, 4, 1) == 0
     assert attention(None) == _lib.LH_ERR_INVALID and attention(paged(), q=None) == _lib.LH_ERR_INVALID
@@ -157,8 +157,8 @@ def test_the_c_entry_points_refuse_without_a_gpu():
     assert need > 0 and need % 256 == 0
     assert attention(paged(), weights=4096, ws=4096, size=need - 1) == _lib.LH_ERR_INVALID
     assert attention(paged(), weights=4096, ws=4096 + 16, size=need) == _lib.LH_ERR_INVALID
-    assert lib.lh_hip_kv_append(paged(), None, 4096, st, st, 4096, None, 3, 5, _lib.BF16, None) == _lib.LH_ERR_INVALID
-    assert lib.lh_hip_kv_append(paged(), 4096, 4096, st, st, 4096, None, 2**20, 2**20, _lib.BF16, None) == _lib.LH_ERR_INVALID
+    assert lib.lh_hip_kv_append(paged(), None, 4096, 64, 32, 8, 64, 32, 8, 4096, None, 3, 5, _lib.BF16, None) == _lib.LH_ERR_INVALID
+    assert lib.lh_hip_kv_append(paged(), 4096, 4096, 64, 32, 8, 64, 32, 8, 4096, None, 2**20, 2**20, _lib.BF16, None) == _lib.LH_ERR_INVALID
     assert lib.lh_hip_kv_evict(paged(), 4096, 16, 8, 4096, 4096, 3, 4, 5, 4096, 1 << 20, None) == _lib.LH_ERR_INVALID
     assert lib.lh_hip_kv_evict(paged(), 4096, 16, 7, 4096, 4096, 3, 4, 0, 4096, 1 << 20, None) == _lib.LH_ERR_INVALID
     assert lib.lh_hip_kv_evict(paged(), 4096, 16, 8, 4096, 4096, 3, 4, 0, 4096, 16, None) == _lib.LH_ERR_INVALID
@@ -167,3 +167,18 @@ def test_the_c_entry_points_refuse_without_a_gpu():
                  (4096, 4096, 4096, 3, 50, 50, _lib.F8E4M3), (4096, 4096, 4096, -1, 50, 50, _lib.F32)):
         assert lib.lh_hip_sample(*args, ctypes.byref(opts), None) == _lib.LH_ERR_INVALID
     assert lib.lh_hip_sample(4096, 4096, 4096, 3, 50, 50, _lib.F32, None, None) == _lib.LH_ERR_INVALID
+
+
+def test_packed_structs_are_laid_out_like_the_c_ones():
+    import struct
+
+    values = list(range(1, 18))
+    packed = struct.pack(_lib.PAGED_CACHE_FORMAT, *values[:15], 2, 3.5, 4.5)
+    c = _lib.PagedCache.from_buffer_copy(packed)
+    assert len(packed) == ctypes.sizeof(c)
+    assert [c.k, c.v, c.block_table, c.table_stride, c.sk.z, c.sk.h, c.sk.t, c.sv.z, c.sv.h, c.sv.t, c.n_pages, c.max_pages,
+            c.page_size, c.n_kv_heads, c.d, c.dtype, c.k_scale, c.v_scale] == [*values[:15], 2, 3.5, 4.5]
+    packed = struct.pack(_lib.SAMPLE_OPTS_FORMAT, 1, 2, 3, 4, 0.5, 6, 0.25, 0.125)
+    o = _lib.SampleOpts.from_buffer_copy(packed)
+    assert len(packed) == ctypes.sizeof(o)
+    assert [o.temperature, o.top_k, o.top_p, o.min_p, o.temperature_all, o.top_k_all, o.top_p_all, o.min_p_all] == [1, 2, 3, 4, 0.5, 6, 0.25, 0.125]
