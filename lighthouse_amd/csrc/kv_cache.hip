@@ -1,6 +1,9 @@
 // Filling a paged key / value cache and dropping from it the positions that got least attention.  Both move bytes: what
 // bounds them is memory, or, for a step of one token per sequence, the launch.
+#include <cstring>
+
 #include "paged.h"
+#include "wave_scan.h"
 
 namespace lh {
 
@@ -39,85 +42,120 @@ struct AppendArgs {
   lh_strides3 sk, sv;  // batch, head, token
   const int32_t* positions;
   const int32_t* counts;  // or null: every token counts
-  int32_t B, T;
-  int32_t per_token;        // chunks of a token's keys and values
-  int32_t tokens_per_block;
-  FastDiv by_token, by_T, by_chunks, by_heads;
+  int32_t T;
+  int32_t per_token;      // chunks of a token's keys and values
+  int32_t parts;          // workgroups that share them
+  int32_t tokens;         // of a sequence that a workgroup takes
+  int32_t token_blocks;   // workgroups for T tokens
+  FastDiv by_chunks;
+  float k_inv, v_inv;     // 1 / scale, rounded, or 0 where the short division does not apply
 };
 
-// Two floats -> two e4m3 codes in the low half of a word: clamped to the largest finite value, rounded to nearest even;
-// a NaN stays one (a comparison keeps it, fmin and fmax would not).
+// Two floats, no larger than 448, -> two e4m3 codes in the low half of a word, rounded to nearest even; a NaN stays one.
+__device__ __forceinline__ uint32_t e4m3_pack2(float a, float b) { return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu; }
+// (Comparisons keep a NaN, fmin and fmax would not.)
 __device__ __forceinline__ float e4m3_clamp(float x) {
   x = x > 448.0f ? 448.0f : x;
   return x < -448.0f ? -448.0f : x;
 }
-__device__ __forceinline__ uint32_t e4m3_pack2(float a, float b) {
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(a), e4m3_clamp(b), 0, false) & 0xffffu;
+// Eight numbers x -> x / scale, clamped to +-448: the quotient that a division rounds, so that the codes are those of the formula and
+// not of a rounded reciprocal.  With inv = 1 / scale rounded, q = x inv and r = q scale - x (exact), q - r inv is that quotient
+// (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990), but for a
+// scale whose mantissa is all ones, and where x or r leaves the normal range: the host passes inv = 0 for scales
+// that are not between 2^-60 and 2^60, whose quotients that are not 0 in e4m3 are far from it, and numbers that are not finite
+// or far above 448 take the division.  (3 instructions instead of 11: 8 prompts of 1024 tokens, 12 heads of 64, 15.9 -> 11.4 us.)
+__device__ __forceinline__ void e4m3_divide(float* x, float scale, float inv) {
+  float size = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) size += fabsf(x[e]);
+  if (inv != 0.0f && size <= 4096.0f * scale) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float q = x[e] * inv, r = __builtin_fmaf(q, scale, -x[e]);
+      x[e] = __builtin_amdgcn_fmed3f(__builtin_fmaf(-r, inv, q), -448.0f, 448.0f);
+    }
+  } else {
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) x[e] = e4m3_clamp(x[e] / scale);
+  }
 }
 
-// A thread takes one chunk (16 bytes of the source; 8 elements for a cache of 8 bits) of one head's key or value of one
-// token; a token's chunks are neighbours, so that both sides are read and written in whole lines whatever the
-// layout of heads and tokens.  Any strides and alignment: gfx9 global memory takes 16 bytes at element alignment, the end of
-// a row that is no whole chunk goes element by element.
+// A thread takes one chunk (16 bytes of the source; 8 elements for a cache of 8 bits) of one head's key or value, of several
+// tokens of a sequence one after the other, four at a time; a token's chunks are neighbours, so that both sides are read and
+// written in whole lines whatever the layout of heads and tokens.  The slot of a token is the same for the workgroup: the scalar
+// unit finds it.  (With a token per workgroup and the slot found by every thread, eight prompts of up to 1024 tokens into
+// a cache of 8 bits took 13.4 us.)  Any strides and alignment: gfx9 global memory takes 16 bytes at element alignment, the end of a row that
+// is no whole chunk goes element by element.
 template <int SDT, int CDT>
 __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
   constexpr int E = SDT == LH_F32 && CDT == LH_F32 ? 4 : 8;
   constexpr int SES = SDT == LH_F32 ? 4 : 2, CES = CDT == LH_F32 ? 4 : CDT == LH_F8E4M3 ? 1 : 2;
+  constexpr int LOADS = E * SES / 16, BATCH = 4;
   typedef typename Chunk<SES>::type src16;
-  const int items = a.per_token * a.tokens_per_block;
-  for (int i = threadIdx.x; i < items; i += 256) {
-    const int in_block = (int)a.by_token.div(i);
-    const int64_t token = (int64_t)blockIdx.x * a.tokens_per_block + in_block;
-    if (token >= (int64_t)a.B * a.T) return;
-    const int b = (int)a.by_T.div((uint32_t)token), t = (int)token - b * a.T;
-    if (a.counts != nullptr && t >= a.counts[b]) continue;
-    const int64_t at = (int64_t)a.positions[b] + t;
-    if (at < 0 || at >= a.c.capacity()) continue;
-    int slot;
-    const int page = a.c.page_of(b, (int)at, &slot);
-    if (page < 0) continue;
-    const int rest = i - in_block * a.per_token;  // [k or v][head][chunk]
-    const int row = (int)a.by_chunks.div(rest), col = (rest - row * (int)a.by_chunks.d) * E;
-    const bool is_v = row >= a.c.heads;
-    const int h = row - (is_v ? a.c.heads : 0);
-    const lh_strides3 ss = is_v ? a.sv : a.sk, cs = is_v ? a.c.sv : a.c.sk;
-    const uint8_t* src = static_cast<const uint8_t*>(is_v ? a.v : a.k) + (b * ss.z + h * ss.h + t * ss.t + col) * SES;
-    uint8_t* dst = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + (page * cs.z + h * cs.h + slot * cs.t + col) * CES;
-    const int n = min(E, a.c.d - col);
-    if constexpr (CDT != LH_F8E4M3) {
-      if (n == E) {
-        *reinterpret_cast<src16*>(dst) = *reinterpret_cast<const src16*>(src);
-      } else {
-        for (int e = 0; e < n; ++e) {
-          if constexpr (SES == 4) reinterpret_cast<uint32_t*>(dst)[e] = reinterpret_cast<const uint32_t*>(src)[e];
-          else reinterpret_cast<uint16_t*>(dst)[e] = reinterpret_cast<const uint16_t*>(src)[e];
+  const int part = blockIdx.x % a.parts, rest = blockIdx.x / a.parts;
+  const int b = rest / a.token_blocks, t0 = (rest - b * a.token_blocks) * a.tokens;
+  const int i = part * blockDim.x + threadIdx.x;
+  if (i >= a.per_token) return;
+  const int row = (int)a.by_chunks.div(i), col = (i - row * (int)a.by_chunks.d) * E;
+  const bool is_v = row >= a.c.heads;
+  const int h = row - (is_v ? a.c.heads : 0);
+  const lh_strides3 ss = is_v ? a.sv : a.sk, cs = is_v ? a.c.sv : a.c.sk;
+  const uint8_t* src = static_cast<const uint8_t*>(is_v ? a.v : a.k) + (b * ss.z + h * ss.h + col) * SES;
+  uint8_t* dst = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + (h * cs.h + col) * CES;
+  const int n = min(E, a.c.d - col);
+  const float scale = is_v ? a.c.v_scale : a.c.k_scale, inv = is_v ? a.v_inv : a.k_inv;
+  const int t_end = min(t0 + a.tokens, a.counts == nullptr ? a.T : min(a.T, a.counts[b]));
+  const int64_t position = a.positions[b];
+#pragma unroll 1
+  for (int t1 = t0; t1 < t_end; t1 += BATCH) {
+    int page[BATCH], slot[BATCH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int64_t at = position + t1 + u;
+      page[u] = -1, slot[u] = 0;
+      if (t1 + u < t_end && at >= 0 && at < a.c.capacity()) page[u] = a.c.page_of(b, (int)at, &slot[u]);
+    }
+    if (n == E) {
+      src16 w[BATCH][LOADS];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u)
+        if (page[u] >= 0)
+#pragma unroll
+          for (int l = 0; l < LOADS; ++l) w[u][l] = reinterpret_cast<const src16*>(src + (int64_t)(t1 + u) * ss.t * SES)[l];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        if (page[u] < 0) continue;
+        uint8_t* to = dst + (page[u] * cs.z + slot[u] * cs.t) * CES;
+        if constexpr (CDT != LH_F8E4M3) {
+          *reinterpret_cast<src16*>(to) = w[u][0];
+        } else {
+          float x[E];
+#pragma unroll
+          for (int l = 0; l < LOADS; ++l)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (SES == 2) x[2 * e] = unpack_lo<SDT>(w[u][l][e]), x[2 * e + 1] = unpack_hi<SDT>(w[u][l][e]);
+              else x[4 * l + e] = bits_to_f32(w[u][l][e]);
+            }
+          typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+          e4m3_divide(x, scale, inv);
+          u32x2_any o;
+#pragma unroll
+          for (int p = 0; p < 2; ++p) o[p] = e4m3_pack2(x[4 * p], x[4 * p + 1]) | e4m3_pack2(x[4 * p + 2], x[4 * p + 3]) << 16;
+          *reinterpret_cast<u32x2_any*>(to) = o;
         }
       }
     } else {
-      // x / scale in f32 (a true division: the codes are those of the formula, not of a rounded reciprocal).
-      const float scale = is_v ? a.c.v_scale : a.c.k_scale;
-      float x[E];
-      if (n == E) {
-        if constexpr (SES == 2) {
-          const src16 w = *reinterpret_cast<const src16*>(src);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[2 * e] = unpack_lo<SDT>(w[e]), x[2 * e + 1] = unpack_hi<SDT>(w[e]);
-        } else {
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const src16 w = reinterpret_cast<const src16*>(src)[p];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * p + e] = bits_to_f32(w[e]);
-          }
+#pragma unroll 1
+      for (int u = 0; u < BATCH; ++u) {
+        if (page[u] < 0) continue;
+        const uint8_t* from = src + (int64_t)(t1 + u) * ss.t * SES;
+        uint8_t* to = dst + (page[u] * cs.z + slot[u] * cs.t) * CES;
+        for (int e = 0; e < n; ++e) {
+          if constexpr (CDT == LH_F8E4M3) to[e] = (uint8_t)e4m3_pack2(e4m3_clamp(load_as_f32<SDT>(from, e) / scale), 0.0f);
+          else if constexpr (SES == 4) reinterpret_cast<uint32_t*>(to)[e] = reinterpret_cast<const uint32_t*>(from)[e];
+          else reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(from)[e];
         }
-        typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
-        u32x2_any o;
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-          o[p] = e4m3_pack2(x[4 * p] / scale, x[4 * p + 1] / scale) | e4m3_pack2(x[4 * p + 2] / scale, x[4 * p + 3] / scale) << 16;
-        *reinterpret_cast<u32x2_any*>(dst) = o;
-      } else {
-        for (int e = 0; e < n; ++e) dst[e] = (uint8_t)e4m3_pack2(load_as_f32<SDT>(src, e) / scale, 0.0f);
       }
     }
   }
@@ -140,92 +178,186 @@ struct EvictArgs {
 
 __device__ __forceinline__ int evict_length(const EvictArgs& a, int b) { return min(max(a.lengths[b], 0), a.c.capacity()); }
 
-// An order of the weights as unsigned numbers: larger weight, larger number; -0 and 0 alike, a NaN below everything.
+// An order of the weights as unsigned numbers: larger weight, larger number; -0 and 0 alike, a NaN below everything.  Positions that
+// stay in any case are above all of them, positions that are not there below.
+constexpr uint32_t kKeyAbsent = 0, kKeyNaN = 1, kKeyRecent = 0xffffffffu;
 __device__ __forceinline__ uint32_t evict_key(float w) {
-  if (w != w) return 0;
-  const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f), sign = (uint32_t)((int32_t)u >> 31);
+  return w != w ? kKeyNaN : u ^ (sign | 0x80000000u);
 }
 
-constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
 constexpr int kEvictBins = 2048;  // 11 bits of the key a pass
 
 // Which positions of one head of one sequence stay, in order.  The (budget - recent)-th largest key among the positions that
-// are not recent is found by its digits, 11, 11 and 10 bits, from counts in LDS; of the positions that share it the lowest stay.
-// Then each wave goes through a contiguous share of the positions: it knows from the shares before it how many
-// stay in front, and counts on by ballots.
-__global__ void __launch_bounds__(kEvictThreads) kv_evict_select(EvictArgs a) {
-  __shared__ uint32_t bins[kEvictBins];
-  __shared__ uint32_t wave_sum[kEvictWaves], wave_ties[kEvictWaves];
-  __shared__ uint32_t found[2];  // digit, how many of the digit's keys stay
-  const int b = blockIdx.x / a.c.heads, h = blockIdx.x % a.c.heads;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = evict_length(a, b);
-  if (tid == 0) a.held[blockIdx.x] = n;
-  if (n <= a.budget) return;
-  const float* w = a.weights + b * a.sw_b + h * a.sw_h;
+// are not recent is found by its digits, 11, 11 and 10 bits, from counts in LDS, until so few keys share the digits that
+// they are ranked against each other; of the positions that share it the lowest stay.  A thread has up to 16 neighbouring
+// positions, whose place among those that stay comes from one running sum over the workgroup.  4 waves for tables of up to 4096
+// positions, 16 for longer ones; up to 16384 positions the keys stay in registers, a longer sequence reads its weights (which the L2 holds) in
+// every pass, 16384 at a time.  What bounds it is the chain of passes: 16384 positions of 32 heads 13 us, 1024 of 192 heads 7.5.
+constexpr int kEvictKeys = 16;   // of a thread
+constexpr int kEvictRank = 128;  // keys that are ranked
+template <int THREADS>
+struct EvictShared {
+  // (Weights share a few exponents, so a wave's lanes meet in a few bins: four counts a bin, lanes take turns.)
+  // A thread adds up kEvictBins / THREADS neighbours: one element more behind them keeps lanes off each other's banks.
+  u32x4 bins[kEvictBins + THREADS];
+  unsigned long long wave_sum[THREADS / 64];
+  uint32_t found[3];  // digit, how many of the digit's keys stay, how many there are
+  uint32_t ranked;
+  u32x4 rank[kEvictRank / 4];
+};
+// The sum over the threads before this one.
+template <int THREADS, typename T>
+__device__ __forceinline__ T evict_before(EvictShared<THREADS>& s, T mine, T* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const T run = wave_scan(mine);
+  if (lane == 63) s.wave_sum[wave] = run;
+  __syncthreads();
+  T before = run - mine, total = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) {
+    const T x = (T)s.wave_sum[i];
+    before += i < wave ? x : 0;
+    total += x;
+  }
+  *all = total;
+  return before;
+}
+
+template <int THREADS>
+__device__ __forceinline__ void evict_select(const EvictArgs& a, int n, const float* w, EvictShared<THREADS>& s) {
+  constexpr int BINS = kEvictBins / THREADS;  // bins a thread adds up
+  const int tid = threadIdx.x, lane = tid & 63;
   const int old = n - a.recent;             // positions that compete
   uint32_t want = a.budget - a.recent;      // of them stay; below `old`
-  uint32_t prefix = 0, threshold = 0xffffffffu;
+  const int mine = n <= THREADS * kEvictKeys ? ((n + THREADS - 1) / THREADS + 3) / 4 * 4 : kEvictKeys;  // positions of a thread
+  const int chunks = (n + THREADS * mine - 1) / (THREADS * mine);
+  uint32_t keys[kEvictKeys];
+  auto load = [&](int chunk) {
+    const int t0 = (chunk * THREADS + tid) * mine;
+#pragma unroll
+    for (int q = 0; q < kEvictKeys; q += 4) {
+      if (q >= mine) break;
+      if (t0 + q + 4 <= old) {
+        const Chunk<4>::type v = *reinterpret_cast<const Chunk<4>::type*>(w + t0 + q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) keys[q + e] = evict_key(bits_to_f32(v[e]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = t0 + q + e;
+          keys[q + e] = t < old ? evict_key(w[t]) : t < n ? kKeyRecent : kKeyAbsent;
+        }
+      }
+    }
+  };
+  // f(position, key) for the thread's positions among `chunk`.
+  auto each = [&](int chunk, auto f) {
+    const int t0 = (chunk * THREADS + tid) * mine;
+#pragma unroll
+    for (int q = 0; q < kEvictKeys; q += 4) {
+      if (q >= mine) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(t0 + q + e, keys[q + e]);
+    }
+  };
+  uint32_t threshold = kKeyRecent - 1;  // (no weight's key)
+  load(0);
   if (want > 0) {
+    uint32_t prefix = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kEvictBins; i += kEvictThreads) bins[i] = 0;
-      __syncthreads();
-      for (int t = tid; t < old; t += kEvictThreads) {
-        const uint32_t key = evict_key(w[t]);
-        if (pass == 0 || key >> (shift + bits) == prefix) atomicAdd(&bins[(key >> shift) & ((1u << bits) - 1)], 1u);
-      }
-      __syncthreads();
-      // The digit in which the want-th key from above lies: thread i has the bins 2 i and 2 i + 1 of the order from above.
-      const uint32_t c0 = bins[kEvictBins - 1 - 2 * tid], c1 = bins[kEvictBins - 2 - 2 * tid];
-      uint32_t s = c0 + c1;
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t up = __shfl_up(s, o);
-        if (lane >= o) s += up;
+      for (int i = 0; i < BINS; ++i) s.bins[tid * (BINS + 1) + i] = u32x4{0, 0, 0, 0};
+      if (tid == 0) s.ranked = 0;
+      if (tid < kEvictRank / 4) s.rank[tid] = u32x4{kKeyAbsent, kKeyAbsent, kKeyAbsent, kKeyAbsent};
+      __syncthreads();
+      uint32_t* const counts = reinterpret_cast<uint32_t*>(s.bins) + (lane & 3);
+      for (int chunk = 0; chunk < chunks; ++chunk) {
+        if (chunks > 1) load(chunk);
+        each(chunk, [&](int t, uint32_t key) {
+          const uint32_t bin = (key >> shift) & ((1u << bits) - 1);
+          if ((key - 1u < kKeyRecent - 1u) & ((pass == 0) | (key >> (shift + bits) % 32 == prefix))) {
+            // The lanes that share the first one's bin add up first: weights that are all 0 would come one by one.
+            const uint64_t same = __ballot(bin == (uint32_t)__builtin_amdgcn_readfirstlane(bin));
+            const uint32_t number = same >> lane & 1 ? __popcll(same) : 1u;
+            if (number == 1u || __ffsll((unsigned long long)same) - 1 == lane) atomicAdd(&counts[4 * (bin + bin / BINS)], number);
+          }
+        });
       }
-      if (lane == 63) wave_sum[wave] = s;
       __syncthreads();
-      uint32_t before = s - c0 - c1;
-      for (int i = 0; i < wave; ++i) before += wave_sum[i];
-      if (before < want && want <= before + c0) found[0] = kEvictBins - 1 - 2 * tid, found[1] = want - before;
-      else if (before + c0 < want && want <= before + c0 + c1) found[0] = kEvictBins - 2 - 2 * tid, found[1] = want - before - c0;
+      // The digit in which the want-th key from above lies: thread i has the bins BINS i and on in the order from above.
+      uint32_t c[BINS], sum = 0;
+#pragma unroll
+      for (int i = 0; i < BINS; ++i) {
+        const u32x4 x = s.bins[(THREADS - 1 - tid) * (BINS + 1) + BINS - 1 - i];
+        sum += c[i] = x[0] + x[1] + x[2] + x[3];
+      }
+      uint32_t all, before = evict_before<THREADS>(s, sum, &all);
+#pragma unroll
+      for (int i = 0; i < BINS; ++i) {
+        if (before < want && want <= before + c[i]) s.found[0] = kEvictBins - 1 - BINS * tid - i, s.found[1] = want - before, s.found[2] = c[i];
+        before += c[i];
+      }
       __syncthreads();
-      prefix = prefix << bits | found[0];
-      want = found[1];
-      __syncthreads();
+      prefix = prefix << bits | s.found[0];
+      want = s.found[1];
+      const uint32_t left = s.found[2];
+      if (pass < 2 && left <= kEvictRank) {
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+          if (chunks > 1) load(chunk);
+          each(chunk, [&](int t, uint32_t key) {
+            if ((key - 1u < kKeyRecent - 1u) & (key >> shift == prefix)) reinterpret_cast<uint32_t*>(s.rank)[atomicAdd(&s.ranked, 1u)] = key;
+          });
+        }
+        __syncthreads();
+        if (tid < (int)left) {
+          const uint32_t key = reinterpret_cast<const uint32_t*>(s.rank)[tid];
+          uint32_t above = 0, same = 0;
+#pragma unroll 8
+          for (uint32_t j = 0; j < (left + 3) / 4; ++j) {
+            const u32x4 x = s.rank[j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) above += x[e] > key, same += x[e] == key;
+          }
+          if (above < want && want <= above + same) s.found[0] = key, s.found[1] = want - above;
+        }
+        __syncthreads();
+        prefix = s.found[0], want = s.found[1];
+        break;
+      }
     }
     threshold = prefix;  // the want lowest positions of those with this key stay
   }
-  // Shares of the positions, whole multiples of 64.
-  const int share = ((n + 63) / 64 + kEvictWaves - 1) / kEvictWaves * 64;
-  const int begin = wave * share, end = min(begin + share, n);
-  uint32_t above = 0, ties = 0;
-  for (int t0 = begin; t0 < end; t0 += 64) {
-    const int t = t0 + lane;
-    const uint32_t key = t < old ? evict_key(w[t]) : 0;
-    above += __popcll(__ballot(t < n && (t >= old || (want > 0 && key > threshold))));
-    ties += __popcll(__ballot(t < old && want > 0 && key == threshold));
-  }
-  if (lane == 0) wave_sum[wave] = above, wave_ties[wave] = ties;
-  __syncthreads();
-  uint32_t at = 0, tied = 0;
-  for (int i = 0; i < wave; ++i) at += wave_sum[i], tied += wave_ties[i];
-  at += min(tied, want);
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
-  const uint64_t below = (1ull << lane) - 1;
-  for (int t0 = begin; t0 < end; t0 += 64) {
-    const int t = t0 + lane;
-    const uint32_t key = t < old ? evict_key(w[t]) : 0;
-    const uint64_t tie = __ballot(t < old && want > 0 && key == threshold);
-    const bool stays = t < n && (t >= old || (want > 0 && (key > threshold || (key == threshold && tied + __popcll(tie & below) < want))));
-    const uint64_t stay = __ballot(stays);
-    if (stays) kept[at + __popcll(stay & below)] = t;
-    at += __popcll(stay);
-    tied += __popcll(tie);
+  uint32_t base = 0, base_ties = 0;  // of the chunks before: above the threshold, at it
+  for (int chunk = 0; chunk < chunks; ++chunk) {
+    if (chunks > 1) load(chunk);
+    uint32_t above = 0, ties = 0;
+    each(chunk, [&](int, uint32_t key) { above += key > threshold, ties += key == threshold; });
+    uint64_t all;
+    __syncthreads();
+    const uint64_t before = evict_before<THREADS>(s, (uint64_t)ties << 32 | above, &all);
+    uint32_t tied = base_ties + (uint32_t)(before >> 32), at = base + (uint32_t)before + min(tied, want);
+    each(chunk, [&](int t, uint32_t key) {
+      const bool tie = key == threshold;
+      if ((key > threshold) | (tie & (tied < want))) kept[at++] = t;
+      tied += tie;
+    });
+    base += (uint32_t)all, base_ties += (uint32_t)(all >> 32);
   }
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_evict_select(EvictArgs a) {
+  __shared__ EvictShared<THREADS> s;
+  const int b = blockIdx.x / a.c.heads, h = blockIdx.x % a.c.heads;
+  const int n = evict_length(a, b);
+  if (threadIdx.x == 0) a.held[blockIdx.x] = n;
+  if (n <= a.budget) return;
+  const float* w = a.weights + b * a.sw_b + h * a.sw_h;
+  evict_select<THREADS>(a, n, w, s);
 }
 
 // Rows move up, row kept[j] to row j: kept[j] >= j, so what a block of rows j .. j + R - 1 overwrites no later block reads,
@@ -313,8 +445,8 @@ __global__ void __launch_bounds__(kMoveThreads) kv_evict_move(EvictArgs a) {
 }
 
 template <int SDT, int CDT>
-static int append_launch(const AppendArgs& a, unsigned blocks, hipStream_t s) {
-  LH_LAUNCH((kv_append_kernel<SDT, CDT>), dim3(blocks), dim3(256), 0, s, a);
+static int append_launch(const AppendArgs& a, unsigned blocks, unsigned threads, hipStream_t s) {
+  LH_LAUNCH((kv_append_kernel<SDT, CDT>), dim3(blocks), dim3(threads), 0, s, a);
   return check_launch("kv_append");
 }
 
@@ -336,20 +468,31 @@ int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, 
              "lh_hip_kv_append: keys and values must have the cache's dtype (any of 16 or 32 bits for a cache of e4m3)");
   if (B == 0 || T == 0) return LH_OK;
   a.k = k, a.v = v, a.sk = {k_stride_b, k_stride_h, k_stride_t}, a.sv = {v_stride_b, v_stride_h, v_stride_t}, a.positions = positions, a.counts = counts;
-  a.B = (int32_t)B, a.T = (int32_t)T;
+  a.T = (int32_t)T;
   const int e = dtype == LH_F32 && cache->dtype == LH_F32 ? 4 : 8, chunks = (a.c.d + e - 1) / e;
-  a.per_token = 2 * a.c.heads * chunks;
-  a.tokens_per_block = a.per_token < 256 ? 256 / a.per_token : 1;
-  a.by_token = FastDiv((uint32_t)a.per_token), a.by_T = FastDiv((uint32_t)T), a.by_chunks = FastDiv((uint32_t)chunks);
-  const unsigned blocks = (unsigned)((B * T + a.tokens_per_block - 1) / a.tokens_per_block);
+  a.per_token = 2 * a.c.heads * chunks, a.by_chunks = FastDiv((uint32_t)chunks);
+  const unsigned threads = a.per_token >= 256 ? 256 : (unsigned)(a.per_token + 63) / 64 * 64;
+  a.parts = (a.per_token + (int)threads - 1) / (int)threads;
+  // As many tokens a workgroup as leave about 8 workgroups per CU, 16 at most.
+  const int64_t tokens = B * T * a.parts / (8 * num_cus());
+  a.tokens = tokens < 1 ? 1 : tokens > 16 ? 16 : (int32_t)tokens;
+  a.token_blocks = (int32_t)((T + a.tokens - 1) / a.tokens);
+  LH_REQUIRE(B * a.token_blocks * a.parts < (1ll << 24), "lh_hip_kv_append: too many tokens");
+  const unsigned blocks = (unsigned)(B * a.token_blocks * a.parts);
+  auto short_division = [](float scale) {
+    uint32_t bits;
+    std::memcpy(&bits, &scale, 4);
+    return scale >= 0x1p-60f && scale <= 0x1p60f && (bits & 0x7fffffu) != 0x7fffffu ? 1.0f / scale : 0.0f;
+  };
+  a.k_inv = short_division(a.c.k_scale), a.v_inv = short_division(a.c.v_scale);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (cache->dtype == LH_F8E4M3) {
-    if (dtype == LH_BF16) return append_launch<LH_BF16, LH_F8E4M3>(a, blocks, s);
-    if (dtype == LH_F16) return append_launch<LH_F16, LH_F8E4M3>(a, blocks, s);
-    return append_launch<LH_F32, LH_F8E4M3>(a, blocks, s);
+    if (dtype == LH_BF16) return append_launch<LH_BF16, LH_F8E4M3>(a, blocks, threads, s);
+    if (dtype == LH_F16) return append_launch<LH_F16, LH_F8E4M3>(a, blocks, threads, s);
+    return append_launch<LH_F32, LH_F8E4M3>(a, blocks, threads, s);
   }
-  if (dtype == LH_F32) return append_launch<LH_F32, LH_F32>(a, blocks, s);
-  return append_launch<LH_BF16, LH_BF16>(a, blocks, s);  // (16 bits either way: they are only moved)
+  if (dtype == LH_F32) return append_launch<LH_F32, LH_F32>(a, blocks, threads, s);
+  return append_launch<LH_BF16, LH_BF16>(a, blocks, threads, s);  // (16 bits either way: they are only moved)
 }
 
 size_t lh_hip_kv_evict_workspace_bytes(int64_t B, int64_t n_kv_heads, int64_t budget) {
@@ -379,7 +522,9 @@ int lh_hip_kv_evict(const lh_paged_cache* cache, float* weights, int64_t weights
   a.elem_bytes = (int32_t)dtype_size(cache->dtype);
   a.slices = (a.c.d * a.elem_bytes + 127) / 128;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  LH_LAUNCH(kv_evict_select, dim3((unsigned)(B * a.c.heads)), dim3(kEvictThreads), 0, s, a);
+  const dim3 heads((unsigned)(B * a.c.heads));
+  if (a.c.capacity() <= 256 * kEvictKeys) LH_LAUNCH(kv_evict_select<256>, heads, dim3(256), 0, s, a);
+  else LH_LAUNCH(kv_evict_select<1024>, heads, dim3(1024), 0, s, a);
   if (const int rc = check_launch("kv_evict_select")) return rc;
   LH_LAUNCH(kv_evict_move, dim3((unsigned)(B * a.c.heads * (1 + 2 * a.slices))), dim3(kMoveThreads), 0, s, a);
   return check_launch("kv_evict_move");

@@ -636,15 +636,15 @@ def kv_append(k, v, k_cache, v_cache, block_table, positions, *, counts=None, k_
 
 
 def _vector_workspace(workspace, need, like):
-    """(address, bytes) of the caller's workspace, or of one from torch's allocator, which hands out its memory again only to work
-    that follows on this stream, and which a captured graph keeps for itself."""
+    """The caller's workspace or, from torch's allocator, one that a captured graph keeps for itself.  To be held until the launch is
+    enqueued: from then on the allocator hands the memory out again only to work that follows on this stream."""
     if workspace is None:
-        return (torch.empty(need, dtype=torch.uint8, device=like.device).data_ptr(), need) if need else (None, 0)
+        return like.new_empty(need, dtype=torch.uint8)
     _on_current_device(workspace)
     if not (workspace.dtype == torch.uint8 and workspace.dim() == 1 and workspace.is_contiguous() and workspace.numel() >= need
             and workspace.data_ptr() % 256 == 0):
         raise ValueError(f"workspace must be a contiguous uint8 vector of at least {need} bytes, 256-byte aligned")
-    return workspace.data_ptr(), workspace.numel()
+    return workspace
 
 
 def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, out=None, weights=None, k_scale=1.0, v_scale=1.0,
@@ -671,7 +671,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, ou
         raise ValueError("q must have the cache's dtype (bfloat16 or float16 for a cache of float8_e4m3fn)")
     sq = q.stride()
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype:
         raise ValueError("out must have the shape and dtype of q")
     so = out.stride()
@@ -688,10 +688,13 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, ou
     if B == 0:
         return out
     lib = _lib.load()
-    ws_ptr, ws_bytes = _vector_workspace(workspace, lib.lh_hip_paged_attention_workspace_bytes(cache, B, H, w_ptr is not None), q)
+    need = lib.lh_hip_paged_attention_workspace_bytes(cache, B, H, w_ptr is not None)
+    if need:
+        workspace = _vector_workspace(workspace, need, q)
     _lib.check(lib.lh_hip_paged_attention(
         cache, out.data_ptr(), q.data_ptr(), so[0], so[1], sq[0], sq[1], lengths.data_ptr(), w_ptr, w_b, w_h, B, H,
-        1.0 / math.sqrt(d) if scale is None else scale, lh_dtype(dtype), ws_ptr, ws_bytes, _stream()), "paged_attention")
+        1.0 / math.sqrt(d) if scale is None else scale, lh_dtype(dtype),
+        workspace.data_ptr() if need else None, need, _stream()), "paged_attention")
     return out
 
 
@@ -716,15 +719,16 @@ def kv_evict(k_cache, v_cache, weights, block_table, lengths, budget, *, recent=
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"budget must be at least 1 and recent between 0 and the budget, got {budget} and {recent}")
     if out is None:
-        out = torch.empty(B, dtype=torch.int32, device=lengths.device)
+        out = lengths.new_empty(B)
     _is_index(out, B, "out")
     _on_current_device(k_cache, v_cache, weights, block_table, lengths, out)
     if B == 0:
         return out
     lib = _lib.load()
-    ws_ptr, ws_bytes = _vector_workspace(workspace, lib.lh_hip_kv_evict_workspace_bytes(B, heads, min(budget, capacity)), lengths)
+    need = lib.lh_hip_kv_evict_workspace_bytes(B, heads, min(budget, capacity))
+    workspace = _vector_workspace(workspace, need, lengths)
     _lib.check(lib.lh_hip_kv_evict(cache, weights.data_ptr(), w_b, w_h, lengths.data_ptr(), out.data_ptr(), B, min(budget, capacity),
-                                   min(recent, capacity), ws_ptr, ws_bytes, _stream()), "kv_evict")
+                                   min(recent, capacity), workspace.data_ptr(), need, _stream()), "kv_evict")
     return out
 
 
@@ -760,7 +764,7 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, o
         else:
             numbers[i] = max(0, min(int(value), 2**31 - 1)) if i == 1 else value
     if out is None:
-        out = torch.empty(B, dtype=torch.int64, device=logits.device)
+        out = logits.new_empty(B, dtype=torch.int64)
     _is_vector(out, B, torch.int64, "out")
     _on_current_device(logits, uniform, out, *vectors)
     if B:
