@@ -459,8 +459,11 @@ typedef struct lh_sample_opts {
   float top_p_all;
   float min_p_all;
 } lh_sample_opts;
+/* `workspace`, 256-byte aligned, of lh_hip_sample_workspace_bytes(B, V) (0 up to 8192 words); it needs no clearing, and two calls that
+ * overlap in time need one each. */
+size_t lh_hip_sample_workspace_bytes(int64_t B, int64_t V);
 int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int64_t B, int64_t V, int64_t ld, int32_t dtype,
-                  const lh_sample_opts* opts, void* stream);
+                  const lh_sample_opts* opts, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------- packed-argument payloads ---- */
 

@@ -180,7 +180,8 @@ PROTOTYPES = {
     "lh_hip_paged_attention": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _i32, _vp, _sz, _vp]),
     "lh_hip_kv_evict_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "lh_hip_kv_evict": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
-    "lh_hip_sample": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp]),
+    "lh_hip_sample_workspace_bytes": (_sz, [_i64, _i64]),
+    "lh_hip_sample": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _sz, _vp]),
     "lh_hip_payload_matmul": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MatmulAttrs)]),
     "lh_hip_payload_matmul_fp8": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MatmulFp8Attrs)]),
     "lh_hip_payload_mlp": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MlpAttrs)]),

@@ -9,14 +9,44 @@
 // of the whole: as good as a sum in 64-bit floating point.  (In 32 bits a row of 5000 likely words would get another token about
 // once in 10^4 rows.)
 //
-// One workgroup of 16 waves takes a row; a wave takes a contiguous share of it.  Where few words can stay (top-k, or a top-p
-// or min-p that a few hundred words reach), they are listed: of the largest word of each of the 1024 threads the K-th is at
-// most the K-th of the row, so the words that reach it are K or a few more; the list is sorted in LDS and everything else
-// happens on it, two passes over the row in all.  Otherwise the last word is found in a histogram of the distance max - x, by
-// counts (top-k) or masses (top-p), and then among the words of the bin it lies in.
+// A row of more than 8192 words is digested first, 8192 words a workgroup: for top-k (up to 512) a chunk lists its own largest words, otherwise
+// it adds up its masses, in units of a power of two near its largest word's, and, where a filter will ask for it, by sixteenths of an octave
+// of w below it.  Whole powers and a grid that starts at them let another workgroup put the chunks of a row together
+// exactly.  That one then has the candidates of top-k to sort, or finds in the sums the bin that the last word lies in, collects the words
+// of that bin, and evaluates one chunk, the one that the draw falls into.
+//
+// Rows of one chunk, and what a digest does not settle (top-k above 512, thousands of words in the bin of the cut, infinite logits), take
+// one workgroup of 16 waves from the start.  Where few words can stay, they are listed: of the largest word of each of the 1024 threads the K-th
+// is at most the K-th of the row, so the words that reach it are K or a few more; the list is sorted in LDS.  Otherwise the last
+// word is found in a histogram of the distance max - x, by counts (top-k) or masses (top-p), and then among the words of the bin it
+// lies in.
 #include "common.h"
+#include "wave_scan.h"
 
 namespace lh {
+
+constexpr int kChunkWords = 8192, kChunkBins = 512, kChunkList = 1024, kChunks = 64;  // words of a chunk, ..., most chunks of a row
+constexpr int kDigestThreads = 256;
+
+enum SampleMode {  // what a chunk holds: the same for all of a row
+  kDigestNone = 0,    // nothing
+  kDigestTop = 1,     // its largest word
+  kDigestList = 2,    // its largest words, top_k of them or more, or all
+  kDigestTotal = 3,   // its mass
+  kDigestBins = 4     // and by bins
+};
+struct SampleChunk {
+  double power;               // masses are in units of 2^(power - bits); bins count sixteenths of an octave down from 2^power
+  unsigned long long total;
+  float top;                  // -inf: no words
+  int32_t top_i;
+  int32_t listed;             // or -1: the chunk settles nothing
+  int32_t mode;
+  union {
+    unsigned long long bins[kChunkBins];   // the last one holds what lies below, too
+    unsigned long long list[kChunkList];
+  };
+};
 
 struct SampleArgs {
   int64_t* tokens;
@@ -26,6 +56,8 @@ struct SampleArgs {
   int32_t V;
   int32_t bits;  // of a mass behind the point: V words of weight 1 stay below 2^62
   lh_sample_opts o;
+  SampleChunk* chunks;  // [B][n_chunks], or null
+  int32_t n_chunks;
 };
 
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
@@ -93,18 +125,22 @@ struct SampleRow {
   }
 };
 
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor((unsigned long long)v, o);
-  return v;
-}
-__device__ __forceinline__ uint64_t wave_scan64(uint64_t v, int lane) {  // sum over the lanes up to this one
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t up = __shfl_up((unsigned long long)v, o);
-    if (lane >= o) v += up;
+// all * f, rounded down, or up, for 0 < f < 1 and all < 2^63: f is a whole number of up to 24 bits times a power of two.
+__device__ __forceinline__ uint64_t part_of(uint64_t all, float f, bool up) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, f), e = u >> 23;
+  const uint64_t m = e ? (u & 0x7fffffu) | 0x800000u : u;
+  const int shift = 150 - (e ? (int)e : 1);  // at least 24
+  const uint64_t hi = __umul64hi(all, m), lo = all * m;
+  uint64_t whole, rest;
+  if (shift < 64) {
+    whole = hi << (64 - shift) | lo >> shift;
+    rest = lo & ((1ull << shift) - 1);
+  } else {
+    const int more = shift - 64;
+    whole = more < 64 ? hi >> more : 0;
+    rest = lo | (more < 64 ? hi & ((1ull << more) - 1) : hi);
   }
-  return v;
+  return whole + (up && rest != 0);
 }
 
 // Numbers in the order of floats (no NaN, no -0), and back.
@@ -126,6 +162,10 @@ struct SampleShared {
   float cut_x;
   int32_t cut_i;
   unsigned long long above;
+  double chunk_power[kChunks];
+  int32_t chunk_shift[kChunks];
+  unsigned long long chunk_kept[kChunks];
+  uint32_t wave_chunk[kChunks];
 };
 
 template <int DT>
@@ -141,10 +181,10 @@ struct Sampler {
   float cut_x;     // words below (cut_x, cut_i) have been dropped
   int32_t cut_i;
 
-  // 2^((x - top) c + shift): n + f = (x - top) c with |f| <= 1/2, 2^f = 1 + f p(f) with p of degree 7 through the values at the
+  // 2^(t + shift): n + f = t with |f| <= 1/2, 2^f = 1 + f p(f) with p of degree 7 through the values at the
   // Chebyshev nodes of the interval (relative error 2.2e-12, at top exactly 1).
-  __device__ __forceinline__ double power(float x, int shift) const {
-    const double t = ((double)x - (double)top) * c, n = __builtin_rint(t), f = t - n;
+  __device__ __forceinline__ static double power(double t, int shift) {
+    const double n = __builtin_rint(t), f = t - n;
     double p = 1.325080551750225e-06;
     p = __builtin_fma(p, f, 1.5303700711365693e-05);
     p = __builtin_fma(p, f, 0.00015403475186530786);
@@ -156,11 +196,21 @@ struct Sampler {
     p = __builtin_fma(p, f, 1.0);
     return __builtin_ldexp(p, (int)fmax(n, -2000.0) + shift);
   }
-  __device__ __forceinline__ double weight(float x) const { return x == top ? 1.0 : power(x, 0); }
+  __device__ __forceinline__ double weight(float x) const { return x == top ? 1.0 : power(((double)x - (double)top) * c, 0); }
   // (A number below 2^52 plus 2^52 has its nearest whole number in the lower bits.)
   __device__ __forceinline__ uint64_t mass(float x) const {
-    const uint64_t m = __builtin_bit_cast(uint64_t, power(x, bits) + 4503599627370496.0) & ((1ull << 52) - 1);
+    const uint64_t m = whole(power(((double)x - (double)top) * c, bits));
     return x == top ? 1ull << bits : x > -INFINITY ? m : 0;
+  }
+  __device__ __forceinline__ static uint64_t whole(double w) { return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & ((1ull << 52) - 1); }
+  // The same in the units of a chunk.  (x c - power is exact but for the last rounding, so words of all chunks keep their ratios.)
+  __device__ __forceinline__ static double chunk_exponent(float x, double c, double chunk_power) { return __builtin_fma((double)x, c, -chunk_power); }
+  __device__ __forceinline__ static uint64_t chunk_mass(float x, double c, double chunk_power, int bits) {
+    const uint64_t m = whole(power(chunk_exponent(x, c, chunk_power), bits));
+    return x > -INFINITY ? m : 0;
+  }
+  __device__ __forceinline__ static int chunk_bin(float x, double c, double chunk_power) {
+    return (int)fmin(-16.0 * chunk_exponent(x, c, chunk_power), (double)(kChunkBins - 1));
   }
   __device__ __forceinline__ bool stays(float x, int i) const { return x > cut_x || (x == cut_x && i <= cut_i); }
   __device__ __forceinline__ static unsigned long long entry(float x, int i) { return (unsigned long long)order_of(x) << 32 | (uint32_t)~i; }
@@ -169,7 +219,7 @@ struct Sampler {
 
   // Sum over the workgroup of all threads before this one; `total` of all.
   __device__ __forceinline__ uint64_t block_before(uint64_t v, uint64_t* total) {
-    const uint64_t run = wave_scan64(v, lane);
+    const uint64_t run = wave_scan(v);
     __syncthreads();
     if (lane == 63) s.wave_mass[wave] = run;
     __syncthreads();
@@ -216,7 +266,7 @@ struct Sampler {
   // Finds the last word that stays and makes it the cut: the first `k` words (BY_MASS false), or those before which less than top_p of
   // the mass of what is left lies.
   template <bool BY_MASS>
-  __device__ __forceinline__ void cut(uint32_t k, double top_p, float lowest) {
+  __device__ __forceinline__ void cut(uint32_t k, float top_p, float lowest) {
     float hi = top, lo = fmaxf(lowest, BY_MASS ? top - (float)(20.0 / inv_t) : top - 32.0f);
     float below = INFINITY;          // words of this interval are at most this (and at least `from` after the first level)
     float from = -INFINITY;
@@ -257,7 +307,7 @@ struct Sampler {
           }
         }
       });
-      rest = wave_sum64(rest);
+      rest = wave_total(rest);
       if (lane == 0 && rest != 0) {
         if (BY_MASS) atomicAdd(&s.mass[kSampleBins - 1], (unsigned long long)rest);
         else atomicAdd(&s.count[kSampleBins - 1], (uint32_t)rest);
@@ -269,9 +319,7 @@ struct Sampler {
       const uint64_t before = above + block_before(v0 + v1, &total);
       if (BY_MASS && level == 0) {
         // "less than top_p of the mass before it" in whole numbers: before < ceil(top_p * mass).
-        goal = (uint64_t)ceil(top_p * (double)total);
-        if (goal < 1) goal = 1;
-        if (goal > total) goal = total;
+        goal = top_goal(top_p, total);
       }
       if (goal > above + total) return;  // (fewer than k words are left: infinite ones)
       if (before < goal && goal <= before + v0) s.bin = 2 * tid, s.above = before;
@@ -322,6 +370,183 @@ struct Sampler {
     }
   }
 
+  // The draw from the digests of a row's chunks, if they settle it (to every thread alike).
+  __device__ __forceinline__ bool by_chunks(const SampleChunk* chunks, int n_chunks, int mode, int top_i, uint32_t top_k, float top_p, double least,
+                                            float u, int64_t* token) {
+    const SampleChunk& mine = chunks[min(lane, n_chunks - 1)];
+    const int own = lane < n_chunks ? mine.listed : 0;
+    if (__any(own < 0)) return false;
+    if (mode == kDigestList) {
+      const uint32_t end = wave_scan((uint32_t)own), all = wave_last(end);
+      if (wave == 0 && lane < n_chunks) s.wave_chunk[lane] = end - own;
+      if (tid == 0) s.listed = 0;
+      __syncthreads();
+      const int chunks_wave = (n_chunks + kSampleWaves - 1) / kSampleWaves;
+      int n = (int)all;
+      if (n <= kSampleList) {
+        for (int q = 0; q < chunks_wave; ++q) {
+          const int k = q * kSampleWaves + wave;
+          if (k >= n_chunks) break;
+          const int many = chunks[k].listed, at = (int)s.wave_chunk[k];
+          for (int j = lane; j < many; j += 64) s.list[at + j] = chunks[k].list[j];
+        }
+      } else {
+        // Too many for the list: those that the largest top_k of them reach, by the bins of their distance.
+        const float inv = (float)kSampleBins / 32.0f;
+        for (int i = tid; i < kSampleBins; i += kSampleThreads) s.count[i] = 0;
+        __syncthreads();
+        auto bin_of = [&](unsigned long long e) { return (int)fminf((top - entry_x(e)) * inv, (float)(kSampleBins - 1)); };
+        for (int k = wave; k < n_chunks; k += kSampleWaves)
+          for (int j = lane; j < chunks[k].listed; j += 64) atomicAdd(&s.count[bin_of(chunks[k].list[j])], 1u);
+        __syncthreads();
+        const uint64_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+        uint64_t total;
+        const uint64_t before = block_before(c0 + c1, &total);
+        if (before < top_k && top_k <= before + c0) s.bin = 2 * tid;
+        else if (before + c0 < top_k && top_k <= before + c0 + c1) s.bin = 2 * tid + 1;
+        __syncthreads();
+        const int last = s.bin;
+        for (int k = wave; k < n_chunks; k += kSampleWaves)
+          for (int j = lane; j < chunks[k].listed; j += 64) {
+            const unsigned long long e = chunks[k].list[j];
+            if (bin_of(e) <= last) {
+              const int at = atomicAdd(&s.listed, 1);
+              if (at < kSampleList) s.list[at] = e;
+            }
+          }
+        __syncthreads();
+        n = s.listed;
+        if (n > kSampleList) return false;
+      }
+      __syncthreads();
+      return on_list(n, (int)top_k >= n, top_k, top_p, least, u, 0, token);
+    }
+
+    // Every wave has the chunks in its lanes: the row's unit is that of the largest power.
+    const bool words = lane < n_chunks && mine.total != 0;
+    const double own_power = words ? mine.power : -INFINITY;
+    double power_of_row = own_power;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) power_of_row = fmax(power_of_row, __shfl_xor(power_of_row, o));
+    const int shift = words ? (int)fmin(power_of_row - own_power, 63.0) : 63;
+    const uint64_t total = words ? mine.total : 0;
+    if (wave == 0) s.chunk_power[lane] = mine.power, s.chunk_shift[lane] = shift, s.chunk_kept[lane] = total;
+    int last = kChunkBins;                   // words of bins before it stay, and those of it down to the cut
+    if (mode == kDigestBins) {
+      const uint64_t all = wave_total(total >> shift);
+      const uint64_t goal = top_p < 1.0f ? top_goal(top_p, all) : ~0ull;
+      // The row's bins, two threads each.
+      const int bin = tid & (kChunkBins - 1);
+      __syncthreads();
+      uint64_t v = 0;
+      if (bin < kChunkBins - 1)
+        for (int k = tid >> 9; k < n_chunks; k += 2) {
+          const int at = bin - 16 * s.chunk_shift[k];
+          if (at >= 0 && s.chunk_kept[k] != 0) v += chunks[k].bins[at] >> s.chunk_shift[k];
+        }
+      s.mass[tid] = v;
+      if (tid == 0) s.bin = kChunkBins - 1, s.listed = 0, s.cut_x = INFINITY, s.cut_i = -1;
+      __syncthreads();
+      v = tid < kChunkBins ? s.mass[tid] + s.mass[tid + kChunkBins] : 0;
+      uint64_t sum;
+      const uint64_t before = block_before(v, &sum);
+      if (tid < kChunkBins - 1 && before < goal && goal <= before + v) s.bin = tid;
+      __syncthreads();
+      last = s.bin;
+      if (least > 0.0) {  // the bin of the least weight, but none before the largest word's, which stays (least may be above 1)
+        const double t = power_of_row - ((double)top * c + log2(least));
+        const int of_least = t < 0.0 ? 0 : (int)fmin(16.0 * t, (double)(kChunkBins - 1));
+        last = min(last, max(of_least, chunk_bin(top, c, power_of_row)));
+      }
+      if (last == kChunkBins - 1) return false;
+      if (tid == last) s.above = before;
+      // What a chunk has in the bins before it.
+      for (int k = wave; k < n_chunks; k += kSampleWaves) {
+        const int bins = s.chunk_kept[k] == 0 ? 0 : last - 16 * s.chunk_shift[k];
+        uint64_t m = 0;
+        for (int i = lane; i < bins; i += 64) m += chunks[k].bins[i];
+        m = wave_total(m);
+        if (lane == 0) s.mass[k] = m;
+      }
+      // The words of the bin.  (First by a range of x, a little too wide.)
+      const double wide = 1e-6 * (fabs(power_of_row) + 32.0);
+      const float x_hi = (float)((power_of_row - last / 16.0 + wide) / c), x_lo = (float)((power_of_row - (last + 1) / 16.0 - wide) / c);
+      row.each([&](const float* x, int i0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (x[e] >= x_lo && x[e] <= x_hi && x[e] > -INFINITY) {
+            const int k = (i0 + e) / kChunkWords;
+            if (chunk_bin(x[e], c, s.chunk_power[k]) + 16 * s.chunk_shift[k] == last) {
+              const int j = atomicAdd(&s.listed, 1);
+              if (j < kSampleList) s.list[j] = entry(x[e], i0 + e);
+            }
+          }
+      });
+      __syncthreads();
+      const int n = s.listed;
+      const uint64_t above = s.above;
+      if (n > kSampleList) return false;
+      if (wave == 0 && lane < n_chunks) s.chunk_kept[lane] = s.mass[lane];
+      sort(n);
+      const int j0 = 2 * tid, j1 = j0 + 1;
+      const unsigned long long e0 = j0 < n ? s.list[j0] : 0, e1 = j1 < n ? s.list[j1] : 0;
+      const int k0 = j0 < n ? entry_i(e0) / kChunkWords : 0, k1 = j1 < n ? entry_i(e1) / kChunkWords : 0;
+      const uint64_t m0 = j0 < n ? chunk_mass(entry_x(e0), c, s.chunk_power[k0], bits) : 0;
+      const uint64_t m1 = j1 < n ? chunk_mass(entry_x(e1), c, s.chunk_power[k1], bits) : 0;
+      const uint64_t r0 = m0 >> s.chunk_shift[k0], r1 = m1 >> s.chunk_shift[k1];
+      uint64_t of_list, kept;
+      const uint64_t front = above + block_before(r0 + r1, &of_list);
+      block_before((uint64_t)(j0 < n && front < goal && (weight(entry_x(e0)) >= least || entry_i(e0) == top_i)) +
+                       (j1 < n && front + r0 < goal && (weight(entry_x(e1)) >= least || entry_i(e1) == top_i)), &kept);
+      if (j0 < (int)kept) atomicAdd(&s.chunk_kept[k0], (unsigned long long)m0);
+      if (j1 < (int)kept) atomicAdd(&s.chunk_kept[k1], (unsigned long long)m1);
+      if (j0 == (int)kept - 1) s.cut_x = entry_x(e0), s.cut_i = entry_i(e0);
+      if (j1 == (int)kept - 1) s.cut_x = entry_x(e1), s.cut_i = entry_i(e1);
+    }
+    __syncthreads();
+    // The chunk that the draw falls into.
+    const uint64_t kept = lane < n_chunks ? s.chunk_kept[lane] : 0, units = kept >> shift;
+    const uint64_t run = wave_scan(units), all = wave_last(run);
+    if (all == 0) return false;  // (the largest word stays: this does not happen, and without it there would be no chunk to find)
+    int k;
+    uint64_t goal;
+    if (u < 1.0f) {
+      const uint64_t of_row = goal_of(u, all);
+      k = __ffsll((unsigned long long)__ballot(of_row < run)) - 1;
+      goal = (of_row - __shfl((unsigned long long)(run - units), k)) << s.chunk_shift[k];
+    } else {
+      k = 63 - __clzll((unsigned long long)__ballot(kept != 0));
+      goal = s.chunk_kept[k] - 1;
+    }
+    k = __builtin_amdgcn_readfirstlane(k);
+    const double power_of_chunk = s.chunk_power[k];
+    const int bin_shift = 16 * s.chunk_shift[k];
+    cut_x = s.cut_x, cut_i = s.cut_i;
+    constexpr int EACH = kChunkWords / kSampleThreads;  // neighbouring words of a thread
+    const int i0 = k * kChunkWords + tid * EACH;
+    float x[EACH];
+#pragma unroll
+    for (int p = 0; p < EACH; p += E) row.unpack(row.load(i0 + p), x + p);
+    uint64_t m[EACH], sum = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      bool in = x[e] > -INFINITY;
+      if (last < kChunkBins) {
+        const int bin = chunk_bin(x[e], c, power_of_chunk) + bin_shift;
+        in = in && (bin < last || (bin == last && stays(x[e], i0 + e)));
+      }
+      m[e] = in ? chunk_mass(x[e], c, power_of_chunk, bits) : 0;
+      sum += m[e];
+    }
+    uint64_t of_chunk, at = block_before(sum, &of_chunk);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (at <= goal && goal < at + m[e]) *token = i0 + e;
+      at += m[e];
+    }
+    return true;
+  }
+
   // The index of the n-th word (from 1) of those of this value that stay.
   __device__ __forceinline__ int nth(float value, uint32_t n) {
     uint32_t mine = 0;
@@ -359,15 +584,17 @@ struct Sampler {
   }
 
   // u * all as the whole number that the running sum has to exceed.
-  __device__ __forceinline__ static uint64_t goal_of(double u, uint64_t all) {
-    uint64_t goal = all - 1;
-    if (u < 1.0) goal = u > 0.0 ? (uint64_t)(u * (double)all) : 0;
-    return goal > all - 1 ? all - 1 : goal;
+  __device__ __forceinline__ static uint64_t goal_of(float u, uint64_t all) {
+    return u < 1.0f ? u > 0.0f ? part_of(all, u, false) : 0 : all - 1;
+  }
+  __device__ __forceinline__ static uint64_t top_goal(float top_p, uint64_t all) {
+    const uint64_t goal = top_p > 0.0f ? part_of(all, top_p, true) : 1;
+    return goal < 1 ? 1 : goal;
   }
 
   // Everything on a list of the largest words, if they are enough: whether they were (to every thread alike).  `mine`: this thread's
   // largest word.  top_k: 0 or at most kSampleTopK.
-  __device__ __forceinline__ bool by_list(float mine, uint32_t words, uint32_t top_k, float top_p, double least, double u, int64_t* token) {
+  __device__ __forceinline__ bool by_list(float mine, uint32_t words, uint32_t top_k, float top_p, double least, float u, int64_t* token) {
     const uint32_t aim = top_k > 0 ? top_k : kSampleTopK;
     // The value that `aim` threads reach: the lower end of its bin among the threads' largest.
     const float lo = top - (float)(32.0 / (top_k > 0 ? 1.0 : inv_t));
@@ -413,6 +640,12 @@ struct Sampler {
     if (n > kSampleList) return false;
     uint64_t total = 0;
     if (weigh) block_before(all_mass, &total);
+    return on_list(n, (uint32_t)n == words, top_k, top_p, least, u, weigh ? total : 0, token);
+  }
+
+  // The draw from a list of the n largest words.  `complete`: there are no others; `total`: the mass of all words, or 0: that of the first
+  // top_k counts.  Returns whether the list was long enough.
+  __device__ __forceinline__ bool on_list(int n, bool complete, uint32_t top_k, float top_p, double least, float u, uint64_t total, int64_t* token) {
     sort(n);
     const int j0 = 2 * tid, j1 = j0 + 1;
     const int first = top_k > 0 ? min((int)top_k, n) : n;  // of the list
@@ -420,18 +653,14 @@ struct Sampler {
     const uint64_t m0 = j0 < first ? mass(entry_x(e0)) : 0, m1 = j1 < first ? mass(entry_x(e1)) : 0;
     uint64_t of_list;
     uint64_t front = block_before(m0 + m1, &of_list);
-    if (!weigh) total = of_list;
-    uint64_t goal = ~0ull;
-    if (top_p < 1.0f) {
-      goal = (uint64_t)ceil((double)top_p * (double)total);
-      goal = goal < 1 ? 1 : goal > total ? total : goal;
-    }
+    if (total == 0) total = of_list;
+    const uint64_t goal = top_p < 1.0f ? top_goal(top_p, total) : ~0ull;
     uint64_t kept;
     block_before((uint64_t)(j0 < first && (j0 == 0 || (front < goal && weight(entry_x(e0)) >= least))) +
                      (j1 < first && front + m0 < goal && weight(entry_x(e1)) >= least), &kept);
     const bool in0 = j0 < (int)kept, in1 = j1 < (int)kept;
     // All of the list stays, and words that are not on it might: it was too short.
-    if (kept == (uint64_t)n && (uint32_t)n < words && !(top_k > 0 && (int)top_k <= n) && of_list < goal) return false;
+    if (kept == (uint64_t)n && !complete && !(top_k > 0 && (int)top_k <= n) && of_list < goal) return false;
     uint64_t all;
     block_before((in0 ? m0 : 0) + (in1 ? m1 : 0), &all);
     const uint64_t aim_mass = goal_of(u, all);
@@ -450,6 +679,122 @@ struct Sampler {
   }
 };
 
+// A chunk's words in registers, and what the row's settings will ask of it.
+template <int DT>
+__global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
+  typedef Sampler<DT> S;
+  constexpr int E = SampleRow<DT>::E, ES = DT == LH_F32 ? 4 : 2, PIECES = kChunkWords / (kDigestThreads * E), WAVES = kDigestThreads / 64;
+  __shared__ unsigned long long bins[kChunkBins];
+  __shared__ unsigned long long wave_mass[WAVES];
+  __shared__ float wave_top[WAVES];
+  __shared__ int32_t wave_i[WAVES];
+  __shared__ int32_t last_bin, listed;
+  const int b = blockIdx.x / a.n_chunks, chunk = blockIdx.x % a.n_chunks, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int first = chunk * kChunkWords;
+  const SampleRow<DT> row = {static_cast<const uint8_t*>(a.logits) + b * a.ld * ES, a.V, 0, 0, lane};
+  u32x4 raw[PIECES];
+#pragma unroll
+  for (int p = 0; p < PIECES; ++p) raw[p] = row.load(first + (p * kDigestThreads + tid) * E);
+  const float temperature = a.o.temperature ? a.o.temperature[b] : a.o.temperature_all;
+  const int top_k = a.o.top_k ? a.o.top_k[b] : a.o.top_k_all;
+  const float top_p = a.o.top_p ? a.o.top_p[b] : a.o.top_p_all;
+  const float min_p = a.o.min_p ? a.o.min_p[b] : a.o.min_p_all;
+  SampleChunk& out = a.chunks[blockIdx.x];
+
+  float top = -INFINITY;
+  // f(x, index) for every word of the thread.
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      float x[E];
+      row.unpack(raw[p], x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f(x[e], first + (p * kDigestThreads + tid) * E + e);
+    }
+  };
+  each([&](float x, int) { top = fmaxf(top, x); });
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane == 0) wave_top[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, wave_top[w]);
+  int top_i = 0x7fffffff;
+  each([&](float x, int i) { top_i = x == top && i < top_i ? i : top_i; });
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) top_i = min(top_i, __shfl_xor(top_i, o));
+  if (lane == 0) wave_i[wave] = top_i;
+
+  int mode = kDigestTotal;
+  if (!(temperature > 0.0f) || top_k == 1) mode = kDigestTop;
+  else if (top_k > 0 && top_k < a.V) mode = top_k <= kSampleTopK ? kDigestList : kDigestNone;
+  else if (top_p < 1.0f || min_p > 0.0f) mode = kDigestBins;
+  // (The settings and the chunk's largest word are the same for the workgroup: all branches below are uniform.)
+  // Left to the row's workgroup: an infinite word, and exponents so large that x c has no places behind the point.
+  const double c = 1.0 / (double)temperature * 1.4426950408889634, exponent = (double)top * c;
+  const bool some = top > -INFINITY, words = some && fabs(exponent) <= 0x1p40;
+  const double power = words ? ceil(exponent) : 0.0;
+  unsigned long long total = 0;
+  int in_list = 0;
+  if (words && mode == kDigestTotal) {
+    each([&](float x, int) { total += S::chunk_mass(x, c, power, a.bits); });
+  } else if (words && mode == kDigestBins) {
+    for (int i = tid; i < kChunkBins; i += kDigestThreads) bins[i] = 0;
+    __syncthreads();
+    unsigned long long below = 0;
+    each([&](float x, int) {
+      const uint64_t m = S::chunk_mass(x, c, power, a.bits);
+      const int bin = S::chunk_bin(x, c, power);
+      total += m;
+      if (bin == kChunkBins - 1) below += m;
+      else if (x > -INFINITY) atomicAdd(&bins[bin], (unsigned long long)m);
+    });
+    __syncthreads();
+    for (int i = tid; i < kChunkBins - 1; i += kDigestThreads) out.bins[i] = bins[i];
+    (void)below;  // (total tells it)
+  } else if (words && mode == kDigestList) {
+    uint32_t* const counts = reinterpret_cast<uint32_t*>(bins);
+    for (int i = tid; i < kChunkBins; i += kDigestThreads) counts[i] = 0;
+    if (tid == 0) listed = 0, last_bin = kChunkBins - 1;  // fewer than top_k words: all of them
+    __syncthreads();
+    each([&](float x, int) {
+      const int bin = S::chunk_bin(x, c, power);
+      if (bin < kChunkBins - 1 && x > -INFINITY) atomicAdd(&counts[bin], 1u);
+    });
+    __syncthreads();
+    const uint32_t c0 = counts[2 * tid], c1 = counts[2 * tid + 1], run = wave_scan(c0 + c1);
+    if (lane == 63) wave_mass[wave] = run;
+    __syncthreads();
+    uint32_t before = run - c0 - c1;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) before += w < wave ? (uint32_t)wave_mass[w] : 0;
+    const uint32_t k = (uint32_t)top_k;
+    if (before < k && k <= before + c0) last_bin = 2 * tid;
+    else if (before + c0 < k && k <= before + c0 + c1) last_bin = 2 * tid + 1;
+    __syncthreads();
+    const int last = last_bin;
+    each([&](float x, int i) {
+      if (x > -INFINITY && S::chunk_bin(x, c, power) <= last) {
+        const int j = atomicAdd(&listed, 1);
+        if (j < kChunkList) out.list[j] = S::entry(x, i);
+      }
+    });
+    __syncthreads();
+    in_list = listed;
+  }
+  total = wave_total((uint64_t)total);
+  __syncthreads();
+  if (lane == 0) wave_mass[wave] = total;
+  __syncthreads();
+  if (tid == 0) {
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) total += wave_mass[w], top_i = min(top_i, wave_i[w]);
+    out.power = power, out.total = total, out.top = top, out.top_i = top_i, out.mode = mode;
+    out.listed = in_list > kChunkList || (some && !words) ? -1 : in_list;
+  }
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   __shared__ SampleShared s;
@@ -460,11 +805,34 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   const int top_k = a.o.top_k ? a.o.top_k[b] : a.o.top_k_all;
   const float top_p = a.o.top_p ? a.o.top_p[b] : a.o.top_p_all;
   const float min_p = a.o.min_p ? a.o.min_p[b] : a.o.min_p_all;
-  const double u = (double)a.uniform[b];
+  const float u = a.uniform[b];
 
   const int pieces = (a.V + 64 * E - 1) / (64 * E), share = (pieces + kSampleWaves - 1) / kSampleWaves * (64 * E);
   const int begin = min(wave * (int64_t)share, (int64_t)a.V), end = min(begin + (int64_t)share, (int64_t)a.V);
   const SampleRow<DT> row = {static_cast<const uint8_t*>(a.logits) + b * a.ld * ES, a.V, begin, end, lane};
+
+  const double inv_t = 1.0 / (double)temperature;
+  const double least = min_p > 0.0f ? (double)min_p : 0.0;
+  if (a.chunks != nullptr) {
+    const SampleChunk* chunks = a.chunks + (int64_t)b * a.n_chunks;
+    const SampleChunk& mine = chunks[min(lane, a.n_chunks - 1)];
+    float top = mine.top;
+    int top_i = mine.top_i;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const float x = __shfl_xor(top, o);
+      const int i = __shfl_xor(top_i, o);
+      if (x > top || (x == top && i < top_i)) top = x, top_i = i;
+    }
+    const int mode = __builtin_amdgcn_readfirstlane(mine.mode);
+    if (top == -INFINITY || mode == kDigestTop) {
+      if (tid == 0) a.tokens[b] = top == -INFINITY ? -1 : top_i;
+      return;
+    }
+    Sampler<DT> f = {s, row, tid, lane, wave, top, inv_t * 1.4426950408889634, inv_t, a.bits, -INFINITY, -1};
+    if (mode != kDigestNone && top < INFINITY && f.by_chunks(chunks, a.n_chunks, mode, top_i, (uint32_t)top_k, top_p, least, u, a.tokens + b)) return;
+    __syncthreads();
+  }
 
   // Largest logit, its lowest index, the smallest, how many words.
   float top = -INFINITY, lowest = INFINITY;
@@ -501,18 +869,16 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
     return;
   }
 
-  const double inv_t = 1.0 / (double)temperature;
   Sampler<DT> f = {s, row, tid, lane, wave, top, inv_t * 1.4426950408889634, inv_t, a.bits, -INFINITY, -1};
-  const double least = min_p > 0.0f ? (double)min_p : 0.0;
   const bool few = top_k > 0 && (uint32_t)top_k < words;
   if (top < INFINITY && (few ? top_k <= kSampleTopK : top_p < 1.0f || least > 0.0))
     if (f.by_list(mine, words, few ? top_k : 0, top_p, least, u, a.tokens + b)) return;
   __syncthreads();
   if (top == INFINITY) f.cut_x = INFINITY, f.cut_i = 0x7fffffff, lowest = top;  // only those
-  if (few) f.template cut<false>((uint32_t)top_k, 0.0, lowest);
+  if (few) f.template cut<false>((uint32_t)top_k, 0.0f, lowest);
   if (top_p < 1.0f) {
     __syncthreads();
-    f.template cut<true>(0, (double)top_p, lowest);
+    f.template cut<true>(0, top_p, lowest);
   }
   __syncthreads();
 
@@ -529,7 +895,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) m += left(x[e], i0 + e);
     if (__any(m != 0)) {
-      m = wave_sum64(m);
+      m = wave_total(m);
       if (lane == (i0 - lane * E - begin) / group) of_group += m;
       total += m;
     }
@@ -543,7 +909,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   }
   const uint64_t goal = f.goal_of(u, all);
   if (!(before <= goal && goal < before + total)) return;
-  const uint64_t run = wave_scan64(of_group, lane);
+  const uint64_t run = wave_scan(of_group);
   const int g = __popcll(__ballot(before + run <= goal));  // groups that end at or before it
   before += g == 0 ? 0 : __shfl((unsigned long long)run, g - 1);
   for (int i = begin + g * group; i < end; i += 64 * E) {
@@ -553,7 +919,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
     uint64_t m[E], own = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) own += m[e] = left(x[e], i0 + e);
-    const uint64_t sum = wave_scan64(own, lane);
+    const uint64_t sum = wave_scan(own);
     uint64_t at = before + sum - own;
     if (at <= goal && goal < at + own) {
 #pragma unroll
@@ -571,19 +937,43 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
 
 using namespace lh;
 
-extern "C" int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int64_t B, int64_t V, int64_t ld,
-                             int32_t dtype, const lh_sample_opts* opts, void* stream) {
-  LH_REQUIRE(tokens && logits && uniform && opts, "lh_hip_sample: null pointer");
-  LH_REQUIRE(B >= 0 && B < (1ll << 22) && V >= 1 && V < (1ll << 30), "lh_hip_sample: bad shape %lld x %lld", (long long)B, (long long)V);
-  LH_REQUIRE(B <= 1 || ld >= V, "lh_hip_sample: rows overlap");
-  LH_REQUIRE(dtype == LH_F32 || dtype == LH_BF16 || dtype == LH_F16, "lh_hip_sample: unsupported dtype %d", dtype);
-  if (B == 0) return LH_OK;
-  SampleArgs a = {tokens, logits, uniform, ld, (int32_t)V, 50, *opts};
-  while ((V >> (62 - a.bits)) != 0) --a.bits;
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)B), block(kSampleThreads);
-  if (dtype == LH_F32) LH_LAUNCH(sample_kernel<LH_F32>, grid, block, 0, s, a);
-  else if (dtype == LH_BF16) LH_LAUNCH(sample_kernel<LH_BF16>, grid, block, 0, s, a);
-  else LH_LAUNCH(sample_kernel<LH_F16>, grid, block, 0, s, a);
+static int sample_chunks(int64_t V) {
+  const int64_t n = (V + kChunkWords - 1) / kChunkWords;
+  return n < 2 || n > kChunks ? 0 : (int)n;
+}
+
+template <int DT>
+static int launch_sample(const SampleArgs& a, int64_t B, hipStream_t s) {
+  if (a.chunks) {
+    LH_LAUNCH(sample_digest<DT>, dim3((unsigned)(B * a.n_chunks)), dim3(kDigestThreads), 0, s, a);
+    if (const int rc = check_launch("sample_digest")) return rc;
+  }
+  LH_LAUNCH(sample_kernel<DT>, dim3((unsigned)B), dim3(kSampleThreads), 0, s, a);
   return check_launch("sample");
 }
+
+extern "C" {
+
+size_t lh_hip_sample_workspace_bytes(int64_t B, int64_t V) {
+  return B <= 0 || V <= 0 ? 0 : ((size_t)B * sample_chunks(V) * sizeof(SampleChunk) + 255) / 256 * 256;
+}
+
+int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int64_t B, int64_t V, int64_t ld, int32_t dtype,
+                  const lh_sample_opts* opts, void* workspace, size_t workspace_bytes, void* stream) {
+  LH_REQUIRE(B >= 0 && B < (1ll << 18) && V >= 1 && V < (1ll << 30), "lh_hip_sample: bad shape %lld x %lld (fewer than 2^18 rows)", (long long)B, (long long)V);
+  if (B == 0) return LH_OK;
+  LH_REQUIRE(tokens && logits && uniform && opts, "lh_hip_sample: null pointer");
+  LH_REQUIRE(B == 1 || ld >= V, "lh_hip_sample: rows overlap");
+  LH_REQUIRE(dtype == LH_F32 || dtype == LH_BF16 || dtype == LH_F16, "lh_hip_sample: unsupported dtype %d", dtype);
+  const size_t need = lh_hip_sample_workspace_bytes(B, V);
+  LH_REQUIRE(need == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= need),
+             "lh_hip_sample: workspace too small or not 256-byte aligned: %zu of %zu bytes", workspace_bytes, need);
+  SampleArgs a = {tokens, logits, uniform, ld, (int32_t)V, 50, *opts, need ? static_cast<SampleChunk*>(workspace) : nullptr, sample_chunks(V)};
+  while ((V >> (62 - a.bits)) != 0) --a.bits;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == LH_F32) return launch_sample<LH_F32>(a, B, s);
+  if (dtype == LH_BF16) return launch_sample<LH_BF16>(a, B, s);
+  return launch_sample<LH_F16>(a, B, s);
+}
+
+}  // extern "C"

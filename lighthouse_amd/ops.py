@@ -738,7 +738,7 @@ def kv_evict_workspace_bytes(k_cache, block_table, budget) -> int:
     return int(_lib.load().lh_hip_kv_evict_workspace_bytes(block_table.shape[0], k_cache.shape[1], min(int(budget), capacity)))
 
 
-def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, workspace=None):
     """The next token of every row of logits [B, V] (float32, bfloat16 or float16, rows of any stride): int64 [B].
 
     With w = exp((x - max) / temperature) in 64 bits and the words in falling order of x (equal ones: lowest index first): the first
@@ -746,7 +746,8 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, o
     the first always does.  The token is the lowest index whose running sum of w over what stayed, by index, exceeds uniform[b] (float32
     [B], in [0, 1)) times their sum.  temperature <= 0: the largest logit.  top_k <= 0, top_p >= 1 and min_p <= 0 keep everything.
     NaN and -inf are no words, a +inf leaves only those, a row without words gives -1.
-    Each setting is a number or a tensor [B] on the GPU (int32 for top_k, float32 for the others)."""
+    Each setting is a number or a tensor [B] on the GPU (int32 for top_k, float32 for the others).  `workspace` as for paged_attention
+    (sample_workspace_bytes; rows of up to 8192 words need none)."""
     if logits.dim() != 2 or logits.dtype not in _FLOATS or logits.shape[1] < 1:
         raise ValueError("sample expects logits of shape [B, V] in float32, bfloat16 or float16")
     B, V = logits.shape
@@ -767,11 +768,21 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, o
         out = logits.new_empty(B, dtype=torch.int64)
     _is_vector(out, B, torch.int64, "out")
     _on_current_device(logits, uniform, out, *vectors)
-    if B:
-        _lib.check(_lib.load().lh_hip_sample(
-            out.data_ptr(), logits.data_ptr(), uniform.data_ptr(), B, V, max(logits.stride(0), V), lh_dtype(logits.dtype),
-            _PACK_SAMPLE(*pointers, *numbers), _stream()), "sample")
+    if B == 0:
+        return out
+    lib = _lib.load()
+    need = lib.lh_hip_sample_workspace_bytes(B, V)
+    if need:
+        workspace = _vector_workspace(workspace, need, logits)
+    _lib.check(lib.lh_hip_sample(
+        out.data_ptr(), logits.data_ptr(), uniform.data_ptr(), B, V, max(logits.stride(0), V), lh_dtype(logits.dtype),
+        _PACK_SAMPLE(*pointers, *numbers), workspace.data_ptr() if need else None, need, _stream()), "sample")
     return out
+
+
+def sample_workspace_bytes(B, V) -> int:
+    """Bytes of temporary memory that sample takes for B rows of V words."""
+    return int(_lib.load().lh_hip_sample_workspace_bytes(B, V))
 
 
 def release_scratch() -> None:

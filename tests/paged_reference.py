@@ -107,45 +107,33 @@ def evict(weights, n, budget, recent):
     return sorted(order[:budget - recent]) + list(range(n - recent, n))
 
 
-def kept_words(x, temperature, top_k, top_p, min_p):
-    """(words that stay, by index; their weights) of one row, in 64 bits."""
-    x = np.asarray(x, np.float64)
-    words = [i for i in range(len(x)) if not np.isnan(x[i]) and x[i] > -np.inf]
-    if any(np.isinf(x[i]) for i in words):
-        words = [i for i in words if np.isinf(x[i])]
-    order = sorted(words, key=lambda i: (-x[i], i))
-    if not order:
-        return [], []
-    top = x[order[0]]
-    w = {i: 1.0 if x[i] == top else float(np.exp((x[i] - top) / np.float64(np.float32(temperature)))) for i in order}
-    if top_k > 0:
-        order = order[:top_k]
-    if np.float32(top_p) < 1:
-        goal, mass, n = float(np.float32(top_p)) * math.fsum(w[i] for i in order), 0.0, 0
-        while n < len(order) and (n == 0 or mass < goal):
-            mass = math.fsum((mass, w[order[n]]))
-            n += 1
-        order = order[:n]
-    if min_p > 0:
-        order = order[:1] + [i for i in order[1:] if w[i] >= float(np.float32(min_p))]
-    order = sorted(order)
-    return order, [w[i] for i in order]
-
-
 def sample(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The token of one row: the words in falling order, the beginning that every filter leaves, the draw by index; sums in the
+    widest floating point there is."""
     x = np.asarray(x, np.float64)
-    if not temperature > 0:
-        words = [i for i in range(len(x)) if not np.isnan(x[i]) and x[i] > -np.inf]
-        return min(words, key=lambda i: (-x[i], i)) if words else -1
-    kept, w = kept_words(x, temperature, top_k, top_p, min_p)
-    if not kept:
+    words = np.flatnonzero(x > -np.inf)  # (NaN is not)
+    if np.isposinf(x[words]).any():
+        words = words[np.isposinf(x[words])]
+    if not len(words):
         return -1
-    live = [i for i, m in zip(kept, w) if m > 0]
+    order = words[np.lexsort((words, -x[words]))]
+    top = x[order[0]]
+    if not temperature > 0:
+        return int(order[0])
+    with np.errstate(invalid="ignore", over="ignore"):
+        w = np.where(x[order] == top, 1.0, np.exp((x[order] - top) / np.float64(np.float32(temperature)))).astype(np.longdouble)
+    n = len(order)
+    if top_k > 0:
+        n = min(n, top_k)
+    if np.float32(top_p) < 1:
+        before = np.concatenate([[0], np.cumsum(w[:n])[:-1]])
+        n = max(1, int(np.count_nonzero(before < np.longdouble(np.float32(top_p)) * w[:n].sum())))
+    if min_p > 0:
+        n = max(1, int(np.count_nonzero(w[:n] >= np.float64(np.float32(min_p)))))
+    by_index = np.argsort(order[:n])
+    kept, w = order[:n][by_index], w[:n][by_index]
     if not u < 1:
-        return live[-1]
-    goal, run = max(float(np.float32(u)), 0.0) * math.fsum(w), 0.0
-    for i, m in zip(kept, w):
-        run += m
-        if run > goal:
-            return i
-    return live[-1]
+        return int(kept[w > 0][-1])
+    run = np.cumsum(w)
+    above = np.flatnonzero(run > max(np.longdouble(np.float32(u)), 0) * run[-1])
+    return int(kept[above[0]]) if len(above) else int(kept[w > 0][-1])

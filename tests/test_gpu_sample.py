@@ -130,3 +130,55 @@ def test_draws_follow_the_probabilities():
     p = torch.softmax(x.double() / 0.7, 0)
     assert ((torch.bincount(got.cpu(), minlength=7) - n * p).abs() <= 1).all()
     assert (got.diff() >= 0).all()
+
+
+@pytest.mark.parametrize("V", [8192, 8193, 16384, 20011, 131072, 524288, 524289])
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_rows_of_several_chunks(V, dtype):
+    """From 8193 words on a row is digested in chunks, up to 524288."""
+    g = torch.Generator().manual_seed(V)
+    logits = (2.5 * torch.randn(3, V, generator=g)).to(dtype)
+    logits[1] += torch.linspace(-30, 30, V).to(dtype)  # chunks whose largest words are far apart
+    u = torch.rand(3, generator=g)
+    for options in ({}, {"top_k": 40}, {"top_k": 512, "top_p": 0.9}, {"top_k": 513}, {"top_p": 0.9}, {"top_p": 0.2, "min_p": 0.01},
+                    {"min_p": 0.001}, {"temperature": 0.0}, {"temperature": 0.1, "top_p": 0.95}):
+        check(logits, u, **options)
+
+
+def test_chunks_that_differ():
+    """Empty chunks, one word, all of one value, infinite ones, values far from 0, ties at a chunk's border."""
+    V = 40000
+    g = torch.Generator().manual_seed(7)
+    x = 2 * torch.randn(12, V, generator=g)
+    x[0, 8192:24576] = -math.inf
+    x[1] = -math.inf
+    x[1, 30000] = 2.0
+    x[2] = 0.5
+    x[3, 5] = math.inf
+    x[3, 39999] = math.inf
+    x[4] += 1e6
+    x[5] -= 1e30
+    x[6] = torch.randint(0, 2, (V,), generator=g).float() * 60  # two values, far apart
+    x[7] = math.nan
+    x[8, 8000:8400] = 9.0
+    x[9] *= 1e-30
+    x[10] = -math.inf
+    x[11, ::2] = torch.finfo(f32).min
+    u = torch.tensor([0.1, 0.5, 0.5, 0.7, 0.3, 0.25, 0.5, 0.1, 0.6, 0.9, 0.3, 0.99])
+    for options in ({}, {"top_k": 100}, {"top_k": 2}, {"top_p": 0.5}, {"top_p": 0.999}, {"min_p": 0.3}, {"min_p": 5.0}, {"temperature": 0.0},
+                    {"top_k": 300, "top_p": 0.3}, {"temperature": 1e-20, "top_p": 0.5}, {"temperature": 1e20, "top_p": 0.5}, {"temperature": math.inf}):
+        check(x, u, **options)
+    same = torch.full((4, 32768), -3.5)
+    check(same, [0.0, 0.25, 0.5, 0.75])
+    check(same, [0.0, 0.25, 0.5, 0.75], top_p=0.5)
+
+
+def test_workspace_of_the_caller():
+    g = torch.Generator().manual_seed(8)
+    x, u = torch.randn(2, 20000, generator=g).cuda(), torch.rand(2, generator=g).cuda()
+    need = ops.sample_workspace_bytes(2, 20000)
+    assert need > 0 and ops.sample_workspace_bytes(2, 8192) == 0
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    assert torch.equal(ops.sample(x, u, top_p=0.9, workspace=ws), ops.sample(x, u, top_p=0.9))
+    with pytest.raises(ValueError, match="workspace"):
+        ops.sample(x, u, workspace=ws[: need - 256])

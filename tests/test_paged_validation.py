@@ -165,8 +165,13 @@ def test_the_c_entry_points_refuse_without_a_gpu():
     opts = _lib.SampleOpts(temperature_all=1.0, top_p_all=1.0)
     for args in ((None, 4096, 4096, 3, 50, 50, _lib.F32), (4096, 4096, 4096, 3, 0, 50, _lib.F32), (4096, 4096, 4096, 3, 50, 49, _lib.F32),
                  (4096, 4096, 4096, 3, 50, 50, _lib.F8E4M3), (4096, 4096, 4096, -1, 50, 50, _lib.F32)):
-        assert lib.lh_hip_sample(*args, ctypes.byref(opts), None) == _lib.LH_ERR_INVALID
-    assert lib.lh_hip_sample(4096, 4096, 4096, 3, 50, 50, _lib.F32, None, None) == _lib.LH_ERR_INVALID
+        assert lib.lh_hip_sample(*args, ctypes.byref(opts), None, 0, None) == _lib.LH_ERR_INVALID
+    assert lib.lh_hip_sample(4096, 4096, 4096, 3, 50, 50, _lib.F32, None, None, 0, None) == _lib.LH_ERR_INVALID
+    assert lib.lh_hip_sample_workspace_bytes(3, 8192) == 0
+    need = lib.lh_hip_sample_workspace_bytes(3, 8193)
+    for ws, size in ((None, need), (4096, need - 1), (4096 + 16, need)):
+        assert lib.lh_hip_sample(4096, 4096, 4096, 3, 8193, 8193, _lib.F32, ctypes.byref(opts), ws, size, None) == _lib.LH_ERR_INVALID
+        assert b"workspace" in lib.lh_hip_last_error()
 
 
 def test_packed_structs_are_laid_out_like_the_c_ones():
