@@ -26,7 +26,7 @@
 namespace lh {
 
 constexpr int kChunkWords = 8192, kChunkBins = 512, kChunkList = 1024, kChunks = 64;  // words of a chunk, ..., most chunks of a row
-constexpr int kDigestThreads = 256;
+constexpr int kDigestThreads = 512;
 
 enum SampleMode {  // what a chunk holds: the same for all of a row
   kDigestNone = 0,    // nothing
@@ -63,6 +63,7 @@ struct SampleArgs {
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
 constexpr int kSampleBins = 2048;
 constexpr int kSampleList = 2048;   // words: two a thread
+constexpr int kSampleRank = 512;    // words: up to here they are ranked against each other
 constexpr int kSampleTopK = 512;    // up to here top-k is tried on a list; also how many words a list for top-p aims at
 
 // (By value: a bit cast of a vector's element itself reads its first one.)
@@ -97,16 +98,19 @@ struct SampleRow {
   }
   // Words as numbers; what is no word (NaN) is -inf, -0 is 0.
   __device__ __forceinline__ static void unpack(u32x4 w, float* x) {
+    numbers(w, x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = x[e] >= -INFINITY ? x[e] + 0.0f : -INFINITY;
+  }
+  __device__ __forceinline__ static void numbers(u32x4 w, float* x) {  // (a NaN as it is)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if constexpr (DT == LH_F32) x[e] = sample_bits(w[e]);
       else x[2 * e] = unpack_lo<DT>(w[e]), x[2 * e + 1] = unpack_hi<DT>(w[e]);
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = x[e] >= -INFINITY ? x[e] + 0.0f : -INFINITY;
   }
   // f(x, first index) for every piece of the wave's share, in order.
-  template <typename F>
+  template <bool AS_IT_IS = false, typename F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll 1
     for (int i = begin; i < end; i += 64 * E * kBatch) {
@@ -118,7 +122,8 @@ struct SampleRow {
       for (int p = 0; p < kBatch; ++p)
         if (i + p * 64 * E < end) {
           float x[E];
-          unpack(w[p], x);
+          if (AS_IT_IS) numbers(w[p], x);
+          else unpack(w[p], x);
           f(x, i + p * 64 * E + lane * E);
         }
     }
@@ -152,7 +157,7 @@ __device__ __forceinline__ float of_order(uint32_t k) { return sample_bits(k & 0
 
 struct SampleShared {
   unsigned long long mass[kSampleBins];  // of a bin; of a word of the list
-  unsigned long long list[kSampleList];  // order of x, then falling index, of a word
+  alignas(16) unsigned long long list[kSampleList];  // order of x, then falling index, of a word
   uint32_t count[kSampleBins];
   unsigned long long wave_mass[kSampleWaves];
   uint32_t wave_count[kSampleWaves];
@@ -232,26 +237,34 @@ struct Sampler {
     return before;
   }
 
-  // The list in falling order; `n` words of it, the rest up to a power of two becomes 0.
+  // The list in falling order; `n` words of it (no two alike), the rest up to a power of two becomes 0.  A few are put where the number of larger
+  // ones says; many go through a bitonic network, whose steps over less than a wave's 128 words need no barrier.
   __device__ __forceinline__ void sort(int n) {
-    int size = 64;
-    while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += kSampleThreads) s.list[i] = 0;
-    __syncthreads();
-    if (size == 64) {  // one wave, in registers
-      if (wave == 0) {
-        unsigned long long v = s.list[lane];
-        for (int k = 2; k <= 64; k <<= 1)
-          for (int j = k >> 1; j > 0; j >>= 1) {
-            const unsigned long long o = __shfl_xor(v, j);
-            const bool larger = ((lane & k) == 0) == ((lane & j) == 0);  // this lane keeps the larger of the two
-            v = (v > o) == larger ? v : o;
-          }
-        s.list[lane] = v;
+    if (n <= kSampleRank) {
+      __syncthreads();
+      unsigned long long own = 0;
+      int place = 0;
+      if (tid < n) {
+        own = s.list[tid];
+        if (tid == 0 && (n & 1)) s.list[n] = 0;
       }
+      __syncthreads();
+      if (tid < n) {
+#pragma unroll 8
+        for (int j = 0; j < (n + 1) / 2; ++j) {
+          const ulonglong2 o = reinterpret_cast<const ulonglong2*>(s.list)[j];
+          place += (o.x > own) + (o.y > own);
+        }
+      }
+      __syncthreads();
+      if (tid < n) s.list[place] = own;
       __syncthreads();
       return;
     }
+    int size = 2 * kSampleRank;  // (two of a wave's pairs of 128 words at least)
+    while (size < n) size <<= 1;
+    for (int i = n + tid; i < size; i += kSampleThreads) s.list[i] = 0;
+    __syncthreads();
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
         const int i = 2 * tid - (tid & (j - 1));  // the lower of the thread's pair
@@ -259,8 +272,10 @@ struct Sampler {
           const unsigned long long a = s.list[i], b = s.list[i + j];
           if ((a < b) == ((i & k) == 0)) s.list[i] = b, s.list[i + j] = a;
         }
-        __syncthreads();
+        if (j > 64 || (j == 1 && k >= 128)) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
       }
+    __syncthreads();
   }
 
   // Finds the last word that stays and makes it the cut: the first `k` words (BY_MASS false), or those before which less than top_p of
@@ -371,54 +386,59 @@ struct Sampler {
   }
 
   // The draw from the digests of a row's chunks, if they settle it (to every thread alike).
-  __device__ __forceinline__ bool by_chunks(const SampleChunk* chunks, int n_chunks, int mode, int top_i, uint32_t top_k, float top_p, double least,
+  // `early`: what the first 64 places of the wave's chunk's list hold.
+  __device__ __forceinline__ bool by_chunks(const SampleChunk* chunks, int n_chunks, unsigned long long early, int mode, int top_i, uint32_t top_k, float top_p, double least,
                                             float u, int64_t* token) {
     const SampleChunk& mine = chunks[min(lane, n_chunks - 1)];
     const int own = lane < n_chunks ? mine.listed : 0;
     if (__any(own < 0)) return false;
     if (mode == kDigestList) {
+      // The candidates, through LDS where all of them fit; those that the largest top_k reach go on the list, by the bins of their distance.
       const uint32_t end = wave_scan((uint32_t)own), all = wave_last(end);
-      if (wave == 0 && lane < n_chunks) s.wave_chunk[lane] = end - own;
-      if (tid == 0) s.listed = 0;
+      if (wave == 0) s.wave_chunk[lane] = end - own;
+      for (int i = tid; i < kSampleBins; i += kSampleThreads) s.count[i] = 0;
+      if (tid == 0) s.listed = 0, s.bin = kSampleBins;
       __syncthreads();
-      const int chunks_wave = (n_chunks + kSampleWaves - 1) / kSampleWaves;
-      int n = (int)all;
-      if (n <= kSampleList) {
-        for (int q = 0; q < chunks_wave; ++q) {
-          const int k = q * kSampleWaves + wave;
-          if (k >= n_chunks) break;
-          const int many = chunks[k].listed, at = (int)s.wave_chunk[k];
-          for (int j = lane; j < many; j += 64) s.list[at + j] = chunks[k].list[j];
+      const float inv = (float)(64.0 * c);  // (sixty-fourths of an octave of w)
+      auto bin_of = [&](unsigned long long e) { return (int)fminf((top - entry_x(e)) * inv, (float)(kSampleBins - 1)); };
+      const bool staged = all <= kSampleBins;
+      for (int k = wave; k < n_chunks; k += kSampleWaves) {
+        const int many = __shfl(own, k), at = (int)s.wave_chunk[k];
+        for (int j = lane; j < many; j += 64) {
+          const unsigned long long e = k == wave && j < 64 ? early : chunks[k].list[j];
+          if (staged) s.mass[at + j] = e;
+          atomicAdd(&s.count[bin_of(e)], 1u);
         }
-      } else {
-        // Too many for the list: those that the largest top_k of them reach, by the bins of their distance.
-        const float inv = (float)kSampleBins / 32.0f;
-        for (int i = tid; i < kSampleBins; i += kSampleThreads) s.count[i] = 0;
-        __syncthreads();
-        auto bin_of = [&](unsigned long long e) { return (int)fminf((top - entry_x(e)) * inv, (float)(kSampleBins - 1)); };
-        for (int k = wave; k < n_chunks; k += kSampleWaves)
-          for (int j = lane; j < chunks[k].listed; j += 64) atomicAdd(&s.count[bin_of(chunks[k].list[j])], 1u);
-        __syncthreads();
-        const uint64_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
-        uint64_t total;
-        const uint64_t before = block_before(c0 + c1, &total);
-        if (before < top_k && top_k <= before + c0) s.bin = 2 * tid;
-        else if (before + c0 < top_k && top_k <= before + c0 + c1) s.bin = 2 * tid + 1;
-        __syncthreads();
-        const int last = s.bin;
-        for (int k = wave; k < n_chunks; k += kSampleWaves)
-          for (int j = lane; j < chunks[k].listed; j += 64) {
-            const unsigned long long e = chunks[k].list[j];
-            if (bin_of(e) <= last) {
-              const int at = atomicAdd(&s.listed, 1);
-              if (at < kSampleList) s.list[at] = e;
-            }
-          }
-        __syncthreads();
-        n = s.listed;
-        if (n > kSampleList) return false;
       }
       __syncthreads();
+      const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+      uint64_t total;
+      const uint64_t before = block_before(c0 + c1, &total);
+      if (before < top_k && top_k <= before + c0) s.bin = 2 * tid;
+      else if (before + c0 < top_k && top_k <= before + c0 + c1) s.bin = 2 * tid + 1;
+      __syncthreads();
+      const int last = s.bin;  // (fewer than top_k: all of them)
+      auto put = [&](unsigned long long e) {
+        if (bin_of(e) <= last) {
+          const int at = atomicAdd(&s.listed, 1);
+          if (at < kSampleList) s.list[at] = e;
+        }
+      };
+      if (staged) {
+        for (int i = tid; i < (int)all; i += kSampleThreads) put(s.mass[i]);
+      } else {
+        for (int k = wave; k < n_chunks; k += kSampleWaves) {
+          const int many = __shfl(own, k);
+          for (int j = lane; j < many; j += 64) put(chunks[k].list[j]);
+        }
+      }
+      __syncthreads();
+      const int n = s.listed;
+      if (n > kSampleList) return false;
+      if (n <= 64) {
+        if (wave == 0) on_wave(n, top_k, top_p, least, u, token);
+        return true;
+      }
       return on_list(n, (int)top_k >= n, top_k, top_p, least, u, 0, token);
     }
 
@@ -471,21 +491,40 @@ struct Sampler {
       // The words of the bin.  (First by a range of x, a little too wide.)
       const double wide = 1e-6 * (fabs(power_of_row) + 32.0);
       const float x_hi = (float)((power_of_row - last / 16.0 + wide) / c), x_lo = (float)((power_of_row - (last + 1) / 16.0 - wide) / c);
-      row.each([&](const float* x, int i0) {
+      row.template each<true>([&](const float* x, int i0) {
+        bool any = false;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (x[e] >= x_lo && x[e] <= x_hi && x[e] > -INFINITY) {
-            const int k = (i0 + e) / kChunkWords;
-            if (chunk_bin(x[e], c, s.chunk_power[k]) + 16 * s.chunk_shift[k] == last) {
+        for (int e = 0; e < E; ++e) any |= (x[e] >= x_lo) & (x[e] <= x_hi);
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if ((x[e] >= x_lo) & (x[e] <= x_hi) & (x[e] > -INFINITY)) {
               const int j = atomicAdd(&s.listed, 1);
-              if (j < kSampleList) s.list[j] = entry(x[e], i0 + e);
+              if (j < kSampleList) s.list[j] = entry(x[e] + 0.0f, i0 + e);
             }
-          }
+        }
       });
+      __syncthreads();
+      // Of those the ones that lie in the bin.
+      const int range = s.listed;
+      if (range > kSampleList) return false;
+      unsigned long long member[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (tid + i * kSampleThreads < range) {
+          const unsigned long long e = s.list[tid + i * kSampleThreads];
+          const int k = entry_i(e) / kChunkWords;
+          if (chunk_bin(entry_x(e), c, s.chunk_power[k]) + 16 * s.chunk_shift[k] == last) member[i] = e;
+        }
+      __syncthreads();
+      if (tid == 0) s.listed = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (member[i] != 0) s.list[atomicAdd(&s.listed, 1)] = member[i];
       __syncthreads();
       const int n = s.listed;
       const uint64_t above = s.above;
-      if (n > kSampleList) return false;
       if (wave == 0 && lane < n_chunks) s.chunk_kept[lane] = s.mass[lane];
       sort(n);
       const int j0 = 2 * tid, j1 = j0 + 1;
@@ -643,6 +682,34 @@ struct Sampler {
     return on_list(n, (uint32_t)n == words, top_k, top_p, least, u, weigh ? total : 0, token);
   }
 
+  // The lanes' numbers in falling order (no two alike but 0): through LDS, where a lane finds how many are larger.
+  __device__ __forceinline__ unsigned long long wave_sort(unsigned long long own) {
+    s.list[lane] = own;
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    int place = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const ulonglong2 o = reinterpret_cast<const ulonglong2*>(s.list)[j];
+      place += (o.x > own || (o.x == own && 2 * j < lane)) + (o.y > own || (o.y == own && 2 * j + 1 < lane));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    s.list[place] = own;
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    return s.list[lane];
+  }
+  // on_list for a list of up to 64 words that is long enough, in one wave.
+  __device__ __forceinline__ void on_wave(int n, uint32_t top_k, float top_p, double least, float u, int64_t* token) {
+    const unsigned long long e = wave_sort(lane < n ? s.list[lane] : 0);
+    const bool first = lane < min((int)top_k, n);
+    const uint64_t m = first ? mass(entry_x(e)) : 0, run = wave_scan(m), of_list = wave_last(run);
+    const uint64_t goal = top_p < 1.0f ? top_goal(top_p, of_list) : ~0ull;
+    const int kept = __popcll(__ballot(lane == 0 || (first && run - m < goal && weight(entry_x(e)) >= least)));
+    const uint64_t own = lane < kept ? m : 0, aim = goal_of(u, wave_total(own));
+    const unsigned long long by_index = wave_sort(lane < kept ? (unsigned long long)(uint32_t)~entry_i(e) << 32 | (uint32_t)lane : 0);
+    const uint64_t here = lane < kept ? __shfl((unsigned long long)own, (int)(by_index & 63)) : 0, end = wave_scan(here);
+    if (end - here <= aim && aim < end) *token = (int)~(uint32_t)(by_index >> 32);
+  }
+
   // The draw from a list of the n largest words.  `complete`: there are no others; `total`: the mass of all words, or 0: that of the first
   // top_k counts.  Returns whether the list was long enough.
   __device__ __forceinline__ bool on_list(int n, bool complete, uint32_t top_k, float top_p, double least, float u, uint64_t total, int64_t* token) {
@@ -692,9 +759,14 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
   const int b = blockIdx.x / a.n_chunks, chunk = blockIdx.x % a.n_chunks, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int first = chunk * kChunkWords;
   const SampleRow<DT> row = {static_cast<const uint8_t*>(a.logits) + b * a.ld * ES, a.V, 0, 0, lane};
-  u32x4 raw[PIECES];
+  float x[PIECES][E];
+  {
+    u32x4 raw[PIECES];
 #pragma unroll
-  for (int p = 0; p < PIECES; ++p) raw[p] = row.load(first + (p * kDigestThreads + tid) * E);
+    for (int p = 0; p < PIECES; ++p) raw[p] = row.load(first + (p * kDigestThreads + tid) * E);
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) row.unpack(raw[p], x[p]);
+  }
   const float temperature = a.o.temperature ? a.o.temperature[b] : a.o.temperature_all;
   const int top_k = a.o.top_k ? a.o.top_k[b] : a.o.top_k_all;
   const float top_p = a.o.top_p ? a.o.top_p[b] : a.o.top_p_all;
@@ -705,12 +777,9 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
   // f(x, index) for every word of the thread.
   auto each = [&](auto f) {
 #pragma unroll
-    for (int p = 0; p < PIECES; ++p) {
-      float x[E];
-      row.unpack(raw[p], x);
+    for (int p = 0; p < PIECES; ++p)
 #pragma unroll
-      for (int e = 0; e < E; ++e) f(x[e], first + (p * kDigestThreads + tid) * E + e);
-    }
+      for (int e = 0; e < E; ++e) f(x[p][e], first + (p * kDigestThreads + tid) * E + e);
   };
   each([&](float x, int) { top = fmaxf(top, x); });
 #pragma unroll
@@ -719,16 +788,19 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) top = fmaxf(top, wave_top[w]);
-  int top_i = 0x7fffffff;
-  each([&](float x, int i) { top_i = x == top && i < top_i ? i : top_i; });
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) top_i = min(top_i, __shfl_xor(top_i, o));
-  if (lane == 0) wave_i[wave] = top_i;
-
   int mode = kDigestTotal;
   if (!(temperature > 0.0f) || top_k == 1) mode = kDigestTop;
   else if (top_k > 0 && top_k < a.V) mode = top_k <= kSampleTopK ? kDigestList : kDigestNone;
   else if (top_p < 1.0f || min_p > 0.0f) mode = kDigestBins;
+  int top_i = 0x7fffffff;
+  if (mode == kDigestTop || min_p > 1.0f) {  // (otherwise nobody asks which it is)
+    each([&](float x, int i) { top_i = x == top && i < top_i ? i : top_i; });
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top_i = min(top_i, __shfl_xor(top_i, o));
+    if (lane == 0) wave_i[wave] = top_i;
+  } else if (lane == 0) {
+    wave_i[wave] = top_i;
+  }
   // (The settings and the chunk's largest word are the same for the workgroup: all branches below are uniform.)
   // Left to the row's workgroup: an infinite word, and exponents so large that x c has no places behind the point.
   const double c = 1.0 / (double)temperature * 1.4426950408889634, exponent = (double)top * c;
@@ -757,24 +829,26 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
     for (int i = tid; i < kChunkBins; i += kDigestThreads) counts[i] = 0;
     if (tid == 0) listed = 0, last_bin = kChunkBins - 1;  // fewer than top_k words: all of them
     __syncthreads();
+    // (The chunk's own affair: the distance from its largest word in f32 will do, the same expression every time.)
+    const float inv = (float)(16.0 * c);
+    auto bin_of = [&](float x) { return (int)fminf((top - x) * inv, (float)(kChunkBins - 1)); };
     each([&](float x, int) {
-      const int bin = S::chunk_bin(x, c, power);
+      const int bin = bin_of(x);
       if (bin < kChunkBins - 1 && x > -INFINITY) atomicAdd(&counts[bin], 1u);
     });
     __syncthreads();
-    const uint32_t c0 = counts[2 * tid], c1 = counts[2 * tid + 1], run = wave_scan(c0 + c1);
+    static_assert(kDigestThreads >= kChunkBins, "a bin a thread");
+    const uint32_t own = tid < kChunkBins ? counts[tid] : 0, run = wave_scan(own);
     if (lane == 63) wave_mass[wave] = run;
     __syncthreads();
-    uint32_t before = run - c0 - c1;
+    uint32_t before = run - own;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) before += w < wave ? (uint32_t)wave_mass[w] : 0;
-    const uint32_t k = (uint32_t)top_k;
-    if (before < k && k <= before + c0) last_bin = 2 * tid;
-    else if (before + c0 < k && k <= before + c0 + c1) last_bin = 2 * tid + 1;
+    if (before < (uint32_t)top_k && (uint32_t)top_k <= before + own) last_bin = tid;
     __syncthreads();
     const int last = last_bin;
     each([&](float x, int i) {
-      if (x > -INFINITY && S::chunk_bin(x, c, power) <= last) {
+      if (x > -INFINITY && bin_of(x) <= last) {
         const int j = atomicAdd(&listed, 1);
         if (j < kChunkList) out.list[j] = S::entry(x, i);
       }
@@ -816,6 +890,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   if (a.chunks != nullptr) {
     const SampleChunk* chunks = a.chunks + (int64_t)b * a.n_chunks;
     const SampleChunk& mine = chunks[min(lane, a.n_chunks - 1)];
+    const unsigned long long early = chunks[min(wave, a.n_chunks - 1)].list[lane];  // (on the way before anything is known)
     float top = mine.top;
     int top_i = mine.top_i;
 #pragma unroll
@@ -830,7 +905,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
       return;
     }
     Sampler<DT> f = {s, row, tid, lane, wave, top, inv_t * 1.4426950408889634, inv_t, a.bits, -INFINITY, -1};
-    if (mode != kDigestNone && top < INFINITY && f.by_chunks(chunks, a.n_chunks, mode, top_i, (uint32_t)top_k, top_p, least, u, a.tokens + b)) return;
+    if (mode != kDigestNone && top < INFINITY && f.by_chunks(chunks, a.n_chunks, early, mode, top_i, (uint32_t)top_k, top_p, least, u, a.tokens + b)) return;
     __syncthreads();
   }
 
