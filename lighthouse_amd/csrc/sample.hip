@@ -148,6 +148,44 @@ __device__ __forceinline__ uint64_t part_of(uint64_t all, float f, bool up) {
   return whole + (up && rest != 0);
 }
 
+// w of a word of a chunk, in the units that the chunk counts in: sixteenths of an octave above 2^(power - bits), t = 16 (x c - power + bits).
+// With n the nearest whole number and f the rest, 2^(t / 16) = 2^(n / 16) 2^(f / 16): a table of sixteenths, and 1 + f p(f) with p of degree 3
+// through the values at the Chebyshev nodes (relative error 5.1e-12).  x c - power is rounded once, so words of all chunks keep
+// their ratios; what is no word (-inf) comes out as 0 and in the last bin.
+struct ChunkScale {
+  double c16, offset;
+  int top;  // n of the power itself
+  __device__ __forceinline__ ChunkScale(double c, double power, int bits) : c16(16.0 * c), offset(16.0 * ((double)bits - power)), top(16 * bits) {}
+  __device__ __forceinline__ double split(float x, int* n) const {
+    const double t = fmax(__builtin_fma((double)x, c16, offset), -32768.0), whole = __builtin_rint(t);
+    *n = (int)whole;
+    return t - whole;
+  }
+  __device__ __forceinline__ int bin_of(int n) const { return min(max(top - n, 0), kChunkBins - 1); }
+  __device__ __forceinline__ int bin(float x) const {
+    int n;
+    split(x, &n);
+    return bin_of(n);
+  }
+  __device__ __forceinline__ uint64_t mass(float x, const double* sixteenths, int* bin) const {
+    int n;
+    const double f = split(x, &n);
+    double p = 1.4676329855091502e-07;
+    p = __builtin_fma(p, f, 1.3551125679403628e-05);
+    p = __builtin_fma(p, f, 0.0009383847927372583);
+    p = __builtin_fma(p, f, 0.043321698775062194);
+    p = __builtin_fma(p, f, 1.0);
+    *bin = bin_of(n);
+    return whole_of(__builtin_ldexp(p * sixteenths[n & 15], n >> 4));
+  }
+  // (A number below 2^52 plus 2^52 has its nearest whole number in the lower bits.)
+  __device__ __forceinline__ static uint64_t whole_of(double w) { return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & ((1ull << 52) - 1); }
+};
+// 2^(i / 16), i < 16.
+__device__ __forceinline__ void fill_sixteenths(double* to) {
+  if (threadIdx.x < 16) to[threadIdx.x] = exp2((double)threadIdx.x * 0.0625);
+}
+
 // Numbers in the order of floats (no NaN, no -0), and back.
 __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
@@ -167,7 +205,7 @@ struct SampleShared {
   float cut_x;
   int32_t cut_i;
   unsigned long long above;
-  double chunk_power[kChunks];
+  double chunk_power[kChunks], sixteenths[16];
   int32_t chunk_shift[kChunks];
   unsigned long long chunk_kept[kChunks];
   uint32_t wave_chunk[kChunks];
@@ -202,21 +240,11 @@ struct Sampler {
     return __builtin_ldexp(p, (int)fmax(n, -2000.0) + shift);
   }
   __device__ __forceinline__ double weight(float x) const { return x == top ? 1.0 : power(((double)x - (double)top) * c, 0); }
-  // (A number below 2^52 plus 2^52 has its nearest whole number in the lower bits.)
   __device__ __forceinline__ uint64_t mass(float x) const {
-    const uint64_t m = whole(power(((double)x - (double)top) * c, bits));
+    const uint64_t m = ChunkScale::whole_of(power(((double)x - (double)top) * c, bits));
     return x == top ? 1ull << bits : x > -INFINITY ? m : 0;
   }
   __device__ __forceinline__ static uint64_t whole(double w) { return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & ((1ull << 52) - 1); }
-  // The same in the units of a chunk.  (x c - power is exact but for the last rounding, so words of all chunks keep their ratios.)
-  __device__ __forceinline__ static double chunk_exponent(float x, double c, double chunk_power) { return __builtin_fma((double)x, c, -chunk_power); }
-  __device__ __forceinline__ static uint64_t chunk_mass(float x, double c, double chunk_power, int bits) {
-    const uint64_t m = whole(power(chunk_exponent(x, c, chunk_power), bits));
-    return x > -INFINITY ? m : 0;
-  }
-  __device__ __forceinline__ static int chunk_bin(float x, double c, double chunk_power) {
-    return (int)fmin(-16.0 * chunk_exponent(x, c, chunk_power), (double)(kChunkBins - 1));
-  }
   __device__ __forceinline__ bool stays(float x, int i) const { return x > cut_x || (x == cut_x && i <= cut_i); }
   __device__ __forceinline__ static unsigned long long entry(float x, int i) { return (unsigned long long)order_of(x) << 32 | (uint32_t)~i; }
   __device__ __forceinline__ static float entry_x(unsigned long long e) { return of_order((uint32_t)(e >> 32)); }
@@ -448,6 +476,7 @@ struct Sampler {
     double power_of_row = own_power;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) power_of_row = fmax(power_of_row, __shfl_xor(power_of_row, o));
+    fill_sixteenths(s.sixteenths);
     const int shift = words ? (int)fmin(power_of_row - own_power, 63.0) : 63;
     const uint64_t total = words ? mine.total : 0;
     if (wave == 0) s.chunk_power[lane] = mine.power, s.chunk_shift[lane] = shift, s.chunk_kept[lane] = total;
@@ -456,12 +485,12 @@ struct Sampler {
       const uint64_t all = wave_total(total >> shift);
       const uint64_t goal = top_p < 1.0f ? top_goal(top_p, all) : ~0ull;
       // The row's bins, two threads each.
-      const int bin = tid & (kChunkBins - 1);
+      const int row_bin = tid & (kChunkBins - 1);
       __syncthreads();
       uint64_t v = 0;
-      if (bin < kChunkBins - 1)
+      if (row_bin < kChunkBins - 1)
         for (int k = tid >> 9; k < n_chunks; k += 2) {
-          const int at = bin - 16 * s.chunk_shift[k];
+          const int at = row_bin - 16 * s.chunk_shift[k];
           if (at >= 0 && s.chunk_kept[k] != 0) v += chunks[k].bins[at] >> s.chunk_shift[k];
         }
       s.mass[tid] = v;
@@ -475,8 +504,8 @@ struct Sampler {
       last = s.bin;
       if (least > 0.0) {  // the bin of the least weight, but none before the largest word's, which stays (least may be above 1)
         const double t = power_of_row - ((double)top * c + log2(least));
-        const int of_least = t < 0.0 ? 0 : (int)fmin(16.0 * t, (double)(kChunkBins - 1));
-        last = min(last, max(of_least, chunk_bin(top, c, power_of_row)));
+        const int of_least = t <= 0.0 ? 0 : (int)fmin(__builtin_rint(16.0 * t), (double)(kChunkBins - 1));
+        last = min(last, max(of_least, ChunkScale(c, power_of_row, bits).bin(top)));
       }
       if (last == kChunkBins - 1) return false;
       if (tid == last) s.above = before;
@@ -490,7 +519,7 @@ struct Sampler {
       }
       // The words of the bin.  (First by a range of x, a little too wide.)
       const double wide = 1e-6 * (fabs(power_of_row) + 32.0);
-      const float x_hi = (float)((power_of_row - last / 16.0 + wide) / c), x_lo = (float)((power_of_row - (last + 1) / 16.0 - wide) / c);
+      const float x_hi = (float)((power_of_row - (last - 0.5) / 16.0 + wide) / c), x_lo = (float)((power_of_row - (last + 0.5) / 16.0 - wide) / c);
       row.template each<true>([&](const float* x, int i0) {
         bool any = false;
 #pragma unroll
@@ -514,7 +543,7 @@ struct Sampler {
         if (tid + i * kSampleThreads < range) {
           const unsigned long long e = s.list[tid + i * kSampleThreads];
           const int k = entry_i(e) / kChunkWords;
-          if (chunk_bin(entry_x(e), c, s.chunk_power[k]) + 16 * s.chunk_shift[k] == last) member[i] = e;
+          if (ChunkScale(c, s.chunk_power[k], bits).bin(entry_x(e)) + 16 * s.chunk_shift[k] == last) member[i] = e;
         }
       __syncthreads();
       if (tid == 0) s.listed = 0;
@@ -530,8 +559,9 @@ struct Sampler {
       const int j0 = 2 * tid, j1 = j0 + 1;
       const unsigned long long e0 = j0 < n ? s.list[j0] : 0, e1 = j1 < n ? s.list[j1] : 0;
       const int k0 = j0 < n ? entry_i(e0) / kChunkWords : 0, k1 = j1 < n ? entry_i(e1) / kChunkWords : 0;
-      const uint64_t m0 = j0 < n ? chunk_mass(entry_x(e0), c, s.chunk_power[k0], bits) : 0;
-      const uint64_t m1 = j1 < n ? chunk_mass(entry_x(e1), c, s.chunk_power[k1], bits) : 0;
+      int bin;
+      const uint64_t m0 = j0 < n ? ChunkScale(c, s.chunk_power[k0], bits).mass(entry_x(e0), s.sixteenths, &bin) : 0;
+      const uint64_t m1 = j1 < n ? ChunkScale(c, s.chunk_power[k1], bits).mass(entry_x(e1), s.sixteenths, &bin) : 0;
       const uint64_t r0 = m0 >> s.chunk_shift[k0], r1 = m1 >> s.chunk_shift[k1];
       uint64_t of_list, kept;
       const uint64_t front = above + block_before(r0 + r1, &of_list);
@@ -558,7 +588,7 @@ struct Sampler {
       goal = s.chunk_kept[k] - 1;
     }
     k = __builtin_amdgcn_readfirstlane(k);
-    const double power_of_chunk = s.chunk_power[k];
+    const ChunkScale scale(c, s.chunk_power[k], bits);
     const int bin_shift = 16 * s.chunk_shift[k];
     cut_x = s.cut_x, cut_i = s.cut_i;
     constexpr int EACH = kChunkWords / kSampleThreads;  // neighbouring words of a thread
@@ -569,12 +599,10 @@ struct Sampler {
     uint64_t m[EACH], sum = 0;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      bool in = x[e] > -INFINITY;
-      if (last < kChunkBins) {
-        const int bin = chunk_bin(x[e], c, power_of_chunk) + bin_shift;
-        in = in && (bin < last || (bin == last && stays(x[e], i0 + e)));
-      }
-      m[e] = in ? chunk_mass(x[e], c, power_of_chunk, bits) : 0;
+      int bin;
+      m[e] = scale.mass(x[e], s.sixteenths, &bin);
+      bin += bin_shift;
+      if (last < kChunkBins && !(bin < last || (bin == last && stays(x[e], i0 + e)))) m[e] = 0;
       sum += m[e];
     }
     uint64_t of_chunk, at = block_before(sum, &of_chunk);
@@ -756,6 +784,7 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
   __shared__ float wave_top[WAVES];
   __shared__ int32_t wave_i[WAVES];
   __shared__ int32_t last_bin, listed;
+  __shared__ double sixteenths[16];
   const int b = blockIdx.x / a.n_chunks, chunk = blockIdx.x % a.n_chunks, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int first = chunk * kChunkWords;
   const SampleRow<DT> row = {static_cast<const uint8_t*>(a.logits) + b * a.ld * ES, a.V, 0, 0, lane};
@@ -781,6 +810,7 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) f(x[p][e], first + (p * kDigestThreads + tid) * E + e);
   };
+  fill_sixteenths(sixteenths);
   each([&](float x, int) { top = fmaxf(top, x); });
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -806,24 +836,25 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
   const double c = 1.0 / (double)temperature * 1.4426950408889634, exponent = (double)top * c;
   const bool some = top > -INFINITY, words = some && fabs(exponent) <= 0x1p40;
   const double power = words ? ceil(exponent) : 0.0;
+  const ChunkScale scale(c, power, a.bits);
   unsigned long long total = 0;
   int in_list = 0;
   if (words && mode == kDigestTotal) {
-    each([&](float x, int) { total += S::chunk_mass(x, c, power, a.bits); });
+    each([&](float x, int) {
+      int bin;
+      total += scale.mass(x, sixteenths, &bin);
+    });
   } else if (words && mode == kDigestBins) {
     for (int i = tid; i < kChunkBins; i += kDigestThreads) bins[i] = 0;
     __syncthreads();
-    unsigned long long below = 0;
     each([&](float x, int) {
-      const uint64_t m = S::chunk_mass(x, c, power, a.bits);
-      const int bin = S::chunk_bin(x, c, power);
+      int bin;
+      const uint64_t m = scale.mass(x, sixteenths, &bin);
       total += m;
-      if (bin == kChunkBins - 1) below += m;
-      else if (x > -INFINITY) atomicAdd(&bins[bin], (unsigned long long)m);
+      if (bin < kChunkBins - 1) atomicAdd(&bins[bin], (unsigned long long)m);
     });
     __syncthreads();
     for (int i = tid; i < kChunkBins - 1; i += kDigestThreads) out.bins[i] = bins[i];
-    (void)below;  // (total tells it)
   } else if (words && mode == kDigestList) {
     uint32_t* const counts = reinterpret_cast<uint32_t*>(bins);
     for (int i = tid; i < kChunkBins; i += kDigestThreads) counts[i] = 0;
