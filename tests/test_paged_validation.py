@@ -187,3 +187,19 @@ def test_packed_structs_are_laid_out_like_the_c_ones():
     o = _lib.SampleOpts.from_buffer_copy(packed)
     assert len(packed) == ctypes.sizeof(o)
     assert [o.temperature, o.top_k, o.top_p, o.min_p, o.temperature_all, o.top_k_all, o.top_p_all, o.min_p_all] == [1, 2, 3, 4, 0.5, 6, 0.25, 0.125]
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    class On:
+        def __init__(self, index):
+            self.index, self.is_cuda, self.device = index, index >= 0, f"cuda:{index}"
+
+        def get_device(self):
+            return self.index
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    ops._on_current_device(On(0), None, On(0))
+    refused("on one device", ops._on_current_device, On(0), On(1))
+    refused("current device", ops._on_current_device, On(1), None, On(1))
+    refused(ON_GPU, ops._on_current_device, On(-1), On(-1))
+    refused(ON_GPU, ops._on_current_device, On(0), On(-1))
