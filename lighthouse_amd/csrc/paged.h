@@ -28,11 +28,18 @@ struct Paged {
   float k_scale, v_scale;
   FastDiv by_size;
 
+  // Entry i of the table, through the address space of what no kernel writes while it runs: where i is the same for the wave, the
+  // scalar unit loads it.  (As a plain load, which the compiler has to keep in order with the kernel's stores, it went through
+  // the vector memory unit, and waiting for it meant waiting for every key and value on the way.)
+  __device__ __forceinline__ int entry(int64_t i) const {
+    typedef const int32_t __attribute__((address_space(4))) constant_i32;
+    return reinterpret_cast<constant_i32*>(reinterpret_cast<uintptr_t>(table))[i];
+  }
   // The page of position t < max_pages * size of sequence b, or -1.
   __device__ __forceinline__ int page_of(int b, int t, int* slot) const {
     const int i = (int)by_size.div((uint32_t)t);
     *slot = t - i * size;
-    const int p = table[b * table_stride + i];
+    const int p = entry(b * table_stride + i);
     return (uint32_t)p < (uint32_t)pages ? p : -1;
   }
   __host__ __device__ int capacity() const { return max_pages * size; }

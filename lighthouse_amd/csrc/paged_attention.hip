@@ -139,13 +139,13 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
   const int group = item % a.groups, rest = item / a.groups;
   const int hk = rest % a.c.heads, b = rest / a.c.heads;
   const int k0 = split * a.share, table_end = min(a.c.capacity(), k0 + a.share);
-  const int32_t* table = a.c.table + b * a.c.table_stride;
+  const int64_t table_row = b * a.c.table_stride;
   int ahead[KT];       // what the table says for a later step
   auto find_pages = [&](int step, int* found) {
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      const int key = k0 + step * KEYS + 16 * t + (TILES ? 0 : l16);
-      found[t] = key < table_end ? table[a.c.by_size.div((uint32_t)key)] : -1;
+      const int key = min(k0 + step * KEYS + 16 * t + (TILES ? 0 : l16), table_end - 1);
+      found[t] = a.c.entry(table_row + a.c.by_size.div((uint32_t)key));
     }
   };
   // (The share is the host's choice, so that the table is asked without waiting for the length.)
