@@ -334,12 +334,13 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
 #pragma unroll
       for (int t = 0; t < KT; ++t) *reinterpret_cast<f32x4*>(to + 16 * t) = x[t];
     }
-    // The maximum that p is relative to follows the true one with a delay: nothing is done until a score is 2^10 above it (a p of
-    // 2^10 is as accurate as one of 1), and then by all lanes together.
-    if (__any(mx > m_run + 10.0f)) {
+    // What p is relative to follows the true maximum with a delay: nothing is done until a p would be above 2^10 (which is as
+    // accurate as one of 1), or 2^14 in f16, and then by all lanes together.  In f16 it lies 2^12 below the maximum: thousands of positions
+    // with 2^-25 of the largest weight, which f16 has no numbers for, have their part in a long row.
+    if (__any(mx > m_run + (QDT == LH_F16 ? 14.0f : 10.0f))) {
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float m_new = fmaxf(m_run, mx);
+      const float m_new = fmaxf(m_run, QDT == LH_F16 ? mx - 12.0f : mx);
       const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
@@ -631,7 +632,7 @@ int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q
              "lh_hip_paged_attention: queries must have the cache's dtype (bf16 or f16 for a cache of e4m3)");
   LH_REQUIRE(weights == nullptr || ((a.c.heads == 1 || weights_stride_h >= a.c.capacity()) && (B <= 1 || weights_stride_b >= a.c.capacity())),
              "lh_hip_paged_attention: rows of the weights overlap");
-  LH_REQUIRE(weights == nullptr || (a.c.capacity() + 255) / 256 * B * a.c.heads < (1ll << 24), "lh_hip_paged_attention: too many weights (fewer than 2^32)");
+  LH_REQUIRE(weights == nullptr || (a.c.capacity() + 255) / 256 * B * a.c.heads < (1ll << 23), "lh_hip_paged_attention: too many weights (fewer than 2^31)");
   const PagedPlan p = paged_plan(a.c, cache->dtype, B, H, weights != nullptr);
   LH_REQUIRE(p.total() == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= p.total()),
              "lh_hip_paged_attention: workspace too small or not 256-byte aligned: %zu of %zu bytes", workspace_bytes, p.total());

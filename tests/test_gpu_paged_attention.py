@@ -149,6 +149,24 @@ def test_scales(factor):
     check(q, c, ops.paged_attention(q, c.k_cache, c.v_cache, c.table, c.device_lengths, scale=factor / 8), scale=factor / 8)
 
 
+def test_many_small_probabilities_in_f16():
+    """One position and, far below it, the 131071 others: each has a probability that f16 has no number for, together they are 0.4 %.
+    All of them lie on one page, so that 512 long rows fit in little memory."""
+    d, size, n, B, heads = 64, 16, 131072, 64, 8
+    k, v = torch.zeros(2, heads, size, d, dtype=f16), torch.ones(2, heads, size, d, dtype=f16)
+    k[0, :, 0, 0], v[0, :, 0] = 17.375, 0.0
+    table = torch.ones(B, n // size, dtype=torch.int32)
+    table[:, 0] = 0
+    q = torch.zeros(B, heads, d, dtype=f16)
+    q[:, :, 0] = 1.0
+    out = ops.paged_attention(q.cuda(), k.cuda(), v.cuda(), table.cuda(), torch.full((B,), n, dtype=torch.int32).cuda(), scale=1.0).cpu().double()
+    small = (n - 1) * math.exp(-17.375)
+    want = small / (1.0 + small)
+    # The result's rounding 2^-11.  The sum of a lane that starts with 1 does not see its 8 positions of at most 1024 steps: 8192 exp(-17.375)
+    # = 2^-12.07.  The accumulators: at most 1024 steps of two products, 2^-24 each, 2^-13.  exp2 of a score of 25: 2^-19.
+    assert ((out - want).abs() <= want * (2.0**-11 + 2.0**-12 + 2.0**-13 + 2.0**-16)).all(), float((out - want).abs().max() / want)
+
+
 def test_strided_queries_and_outputs():
     c = ref.Cache([100, 30], 4, 16, 64, bf16, seed=13)
     store = torch.randn(2, 3 * 512 + 8, generator=torch.Generator().manual_seed(13)).to(bf16).cuda()
