@@ -380,7 +380,7 @@ int lh_hip_nanogpt_forward(float* logits, const float* x, const lh_nanogpt_block
  * block_table[b * table_stride + t / page_size], slot t % page_size.  A page id outside 0 .. n_pages - 1
  * holds nothing: it is neither read nor written, so unused entries of the table may hold anything.
  * dtype is F32, BF16, F16 or F8E4M3; an e4m3 code stands for code * k_scale (or v_scale); the scales are 1 for
- * the other types.  1 <= d <= 256; max_pages * page_size < 2^31 - 65536.
+ * the other types.  1 <= d <= 256; n_kv_heads < 65536; max_pages * page_size < 2^31 - 65536.
  */
 typedef struct lh_paged_cache {
   void* k;
@@ -404,6 +404,7 @@ typedef struct lh_paged_cache {
  * head and token, unit stride along d) in the cache's dtype, or F32, BF16 or F16 for a cache of e4m3, which holds e4m3(clamp(x / scale, +-448)), rounded to
  * nearest even.  Token t of sequence b goes to position positions[b] + t if t < counts[b] (counts may be NULL: all of
  * them do); a position outside the table or on a page that holds nothing is dropped.  Two tokens for one slot leave either.
+ * B T ceil(n_kv_heads (d + 3) / 512) < 2^24 is always taken.
  */
 int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, int64_t k_stride_b, int64_t k_stride_h,
                      int64_t k_stride_t, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, const int32_t* positions,
@@ -417,6 +418,7 @@ int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, 
  * appended and is clamped to 0 .. max_pages * page_size.  Scores, softmax and sums are f32.  dtype (of q and out) is the
  * cache's, or BF16 or F16 for a cache of e4m3.  With `weights` ([B, n_kv_heads, >= max_pages * page_size] f32, element strides
  * weights_stride_b, weights_stride_h), weights[b, g, t] grows by the sum of p_t over the H / n_kv_heads heads of group g.
+ * B H < 2^20, and with weights B n_kv_heads ceil(max_pages * page_size / 256) < 2^23.
  * `workspace`, 256-byte aligned, of lh_hip_paged_attention_workspace_bytes(...): the call allocates nothing, and two calls
  * that overlap in time need a workspace each.  It needs no clearing.
  */
@@ -432,7 +434,8 @@ int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q
  * lowest positions; a NaN is below every number).  Rows of keys, values and weights that stay move up, in order, to the positions
  * 0 .. budget - 1; weights behind them up to the old length become 0; rows behind them stay as they were.
  * new_lengths[b] = min(lengths[b], budget); it may be `lengths`.  Every position below the length must
- * lie on a page of its own that holds something (rows on others do not move).  1 <= budget, 0 <= recent <= budget.
+ * lie on a page of its own that holds something (rows on others do not move).  1 <= budget, 0 <= recent <= budget,
+ * B n_kv_heads < 2^16.
  */
 size_t lh_hip_kv_evict_workspace_bytes(int64_t B, int64_t n_kv_heads, int64_t budget);
 int lh_hip_kv_evict(const lh_paged_cache* cache, float* weights, int64_t weights_stride_b, int64_t weights_stride_h,
@@ -447,7 +450,8 @@ int lh_hip_kv_evict(const lh_paged_cache* cache, float* weights, int64_t weights
  * stayed, in the order of the indices, exceeds u = uniform[b] times their sum (u below 0 counts as 0, u at or above 1, or NaN,
  * takes the last word that stayed with w > 0).  T <= 0 or NaN: the largest logit, lowest index.  top_k <= 0, top_p not below 1 and
  * min_p not above 0 keep everything.  A logit that is NaN or -inf is no word; a +inf leaves only those; a row without words gives -1.
- * Each setting is one value for all rows or, where the pointer is not NULL, a device vector [B].
+ * Each setting is one value for all rows or, where the pointer is not NULL, a device vector [B].  B < 2^18, V < 2^30, and fewer than
+ * 2^23 parts of 8192 words in rows of 8193 to 524288.
  */
 typedef struct lh_sample_opts {
   const float* temperature;

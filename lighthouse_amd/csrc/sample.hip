@@ -1066,7 +1066,8 @@ size_t lh_hip_sample_workspace_bytes(int64_t B, int64_t V) {
 
 int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int64_t B, int64_t V, int64_t ld, int32_t dtype,
                   const lh_sample_opts* opts, void* workspace, size_t workspace_bytes, void* stream) {
-  LH_REQUIRE(B >= 0 && B < (1ll << 18) && V >= 1 && V < (1ll << 30), "lh_hip_sample: bad shape %lld x %lld (fewer than 2^18 rows)", (long long)B, (long long)V);
+  LH_REQUIRE(B >= 0 && B < (1ll << 18) && V >= 1 && V < (1ll << 30) && B * sample_chunks(V) < (1ll << 23),
+             "lh_hip_sample: bad shape %lld x %lld (fewer than 2^18 rows, and 2^23 parts of 8192 words)", (long long)B, (long long)V);
   if (B == 0) return LH_OK;
   LH_REQUIRE(tokens && logits && uniform && opts, "lh_hip_sample: null pointer");
   LH_REQUIRE(B == 1 || ld >= V, "lh_hip_sample: rows overlap");

@@ -535,6 +535,7 @@ _CACHE_DTYPES = (torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3
 _SAMPLE_OPTIONS = ("temperature", "top_k", "top_p", "min_p")
 _PACK_SAMPLE = struct.Struct(_lib.SAMPLE_OPTS_FORMAT).pack
 _PACK_CACHE = struct.Struct(_lib.PAGED_CACHE_FORMAT).pack
+_F32_MAX = torch.finfo(torch.float32).max
 
 
 def _on_current_device(*tensors) -> None:
@@ -587,7 +588,7 @@ def _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale):
     if not (k_scale == 1.0 and v_scale == 1.0):
         if dtype != torch.float8_e4m3fn:
             raise ValueError("k_scale and v_scale belong to a cache of float8_e4m3fn")
-        if not (0.0 < k_scale < math.inf and 0.0 < v_scale < math.inf):
+        if not (0.0 < k_scale <= _F32_MAX and 0.0 < v_scale <= _F32_MAX):
             raise ValueError("k_scale and v_scale must be positive numbers")
     return (_PACK_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), step, *sk[:3], *sv[:3], pages, rows[1], size,
                         heads, d, lh_dtype(dtype), k_scale, v_scale), heads, d, rows[1] * size)
@@ -764,6 +765,10 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, o
             vectors.append(value)
         else:
             numbers[i] = max(0, min(int(value), 2**31 - 1)) if i == 1 else value
+    try:
+        options = _PACK_SAMPLE(*pointers, *numbers)
+    except (OverflowError, struct.error):  # more than a float holds is infinite
+        options = _PACK_SAMPLE(*pointers, *(x if i == 1 else ctypes.c_float(float(x)).value for i, x in enumerate(numbers)))
     if out is None:
         out = logits.new_empty(B, dtype=torch.int64)
     _is_vector(out, B, torch.int64, "out")
@@ -776,7 +781,7 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, o
         workspace = _vector_workspace(workspace, need, logits)
     _lib.check(lib.lh_hip_sample(
         out.data_ptr(), logits.data_ptr(), uniform.data_ptr(), B, V, max(logits.stride(0), V), lh_dtype(logits.dtype),
-        _PACK_SAMPLE(*pointers, *numbers), workspace.data_ptr() if need else None, need, _stream()), "sample")
+        options, workspace.data_ptr() if need else None, need, _stream()), "sample")
     return out
 
 

@@ -48,7 +48,7 @@ def test_a_cache_is_refused():
     long = z(1, 1, 2**20, 8, dtype=bf16)
     refused("positions", call, q[:, :1], long, long, z(3, 2**11, dtype=i32), n)
     refused("belong to a cache", call, q, k, v, table, n, k_scale=2.0)
-    for bad in (0.0, -1.0, math.inf, math.nan):
+    for bad in (0.0, -1.0, math.inf, math.nan, 1e39):
         refused("positive", call, q, k.to(e4m3), v.to(e4m3), table, n, v_scale=bad)
     refused(ON_GPU, call, q, k.to(e4m3), v.to(e4m3), table, n, k_scale=0.5, v_scale=2.0)
 
@@ -127,6 +127,9 @@ def test_sample_rejections():
     refused("top_p must have shape", ops.sample, x, u, top_p=z(2))
     refused("min_p must be contiguous", ops.sample, x, u, min_p=z(6)[::2])
     refused("out must be", ops.sample, x, u, out=z(3, dtype=i32))
+    for option in ("temperature", "top_p", "min_p"):
+        refused(ON_GPU, ops.sample, x, u, **{option: 1e39})  # (more than a float holds: infinite)
+        refused("could not convert", ops.sample, x, u, **{option: "much"})
 
 
 def test_the_c_entry_points_refuse_without_a_gpu():
@@ -153,6 +156,9 @@ def test_the_c_entry_points_refuse_without_a_gpu():
     assert attention(paged(), H=3) == _lib.LH_ERR_INVALID and b"no multiple" in lib.lh_hip_last_error()
     assert attention(paged(), dtype=_lib.F16) == _lib.LH_ERR_INVALID
     assert attention(paged(), weights=4096) == _lib.LH_ERR_INVALID and b"workspace" in lib.lh_hip_last_error()
+    long = paged(max_pages=2**20, table_stride=2**20)
+    assert lib.lh_hip_paged_attention(long, 4096, 4096, 32, 8, 32, 8, 4096, 4096, 2**23, 2**22, 256, 2, 1.0, _lib.BF16, None, 0, None) == _lib.LH_ERR_INVALID
+    assert b"too many weights" in lib.lh_hip_last_error()
     need = lib.lh_hip_paged_attention_workspace_bytes(paged(), 3, 4, 1)
     assert need > 0 and need % 256 == 0
     assert attention(paged(), weights=4096, ws=4096, size=need - 1) == _lib.LH_ERR_INVALID
@@ -167,6 +173,8 @@ def test_the_c_entry_points_refuse_without_a_gpu():
                  (4096, 4096, 4096, 3, 50, 50, _lib.F8E4M3), (4096, 4096, 4096, -1, 50, 50, _lib.F32)):
         assert lib.lh_hip_sample(*args, ctypes.byref(opts), None, 0, None) == _lib.LH_ERR_INVALID
     assert lib.lh_hip_sample(4096, 4096, 4096, 3, 50, 50, _lib.F32, None, None, 0, None) == _lib.LH_ERR_INVALID
+    assert lib.lh_hip_sample(4096, 4096, 4096, 2**17, 2**19, 2**19, _lib.F32, ctypes.byref(opts), 4096, 1 << 40, None) == _lib.LH_ERR_INVALID
+    assert b"bad shape" in lib.lh_hip_last_error()
     assert lib.lh_hip_sample_workspace_bytes(3, 8192) == 0
     need = lib.lh_hip_sample_workspace_bytes(3, 8193)
     for ws, size in ((None, need), (4096, need - 1), (4096 + 16, need)):
