@@ -13,7 +13,7 @@
 // it adds up its masses, in units of a power of two near its largest word's, and, where a filter will ask for it, by sixteenths of an octave
 // of w below it.  Whole powers and a grid that starts at them let another workgroup put the chunks of a row together
 // exactly.  That one then has the candidates of top-k to sort, or finds in the sums the bin that the last word lies in, collects the words
-// of that bin, and evaluates one chunk, the one that the draw falls into.
+// of that bin from the chunks that have any, and evaluates one chunk, the one that the draw falls into.
 //
 // Rows of one chunk, and what a digest does not settle (top-k above 512, thousands of words in the bin of the cut, infinite logits), take
 // one workgroup of 16 waves from the start.  Where few words can stay, they are listed: of the largest word of each of the 1024 threads the K-th
@@ -58,6 +58,7 @@ struct SampleArgs {
   lh_sample_opts o;
   SampleChunk* chunks;  // [B][n_chunks], or null
   int32_t n_chunks;
+  int32_t may_bin;      // whether a row's settings may ask for bins, as far as the host knows them
 };
 
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
@@ -110,7 +111,7 @@ struct SampleRow {
     }
   }
   // f(x, first index) for every piece of the wave's share, in order.
-  template <bool AS_IT_IS = false, typename F>
+  template <typename F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll 1
     for (int i = begin; i < end; i += 64 * E * kBatch) {
@@ -122,8 +123,7 @@ struct SampleRow {
       for (int p = 0; p < kBatch; ++p)
         if (i + p * 64 * E < end) {
           float x[E];
-          if (AS_IT_IS) numbers(w[p], x);
-          else unpack(w[p], x);
+          unpack(w[p], x);
           f(x, i + p * 64 * E + lane * E);
         }
     }
@@ -201,7 +201,7 @@ struct SampleShared {
   uint32_t wave_count[kSampleWaves];
   float wave_lo[kSampleWaves], wave_hi[kSampleWaves];
   int32_t wave_i[kSampleWaves];
-  int32_t bin, listed;
+  int32_t bin, listed, pieces, some;  // (`some`: chunks)
   float cut_x;
   int32_t cut_i;
   unsigned long long above;
@@ -414,8 +414,8 @@ struct Sampler {
   }
 
   // The draw from the digests of a row's chunks, if they settle it (to every thread alike).
-  // `early`: what the first 64 places of the wave's chunk's list hold.
-  __device__ __forceinline__ bool by_chunks(const SampleChunk* chunks, int n_chunks, unsigned long long early, int mode, int top_i, uint32_t top_k, float top_p, double least,
+  // `early`: what the wave's chunk's list, or bins, hold in the places 64 i + lane.
+  __device__ __forceinline__ bool by_chunks(const SampleChunk* chunks, int n_chunks, unsigned long long (&early)[kChunkBins / 64], int mode, int top_i, uint32_t top_k, float top_p, double least,
                                             float u, int64_t* token) {
     const SampleChunk& mine = chunks[min(lane, n_chunks - 1)];
     const int own = lane < n_chunks ? mine.listed : 0;
@@ -433,7 +433,7 @@ struct Sampler {
       for (int k = wave; k < n_chunks; k += kSampleWaves) {
         const int many = __shfl(own, k), at = (int)s.wave_chunk[k];
         for (int j = lane; j < many; j += 64) {
-          const unsigned long long e = k == wave && j < 64 ? early : chunks[k].list[j];
+          const unsigned long long e = k == wave && j < 64 ? early[0] : chunks[k].list[j];
           if (staged) s.mass[at + j] = e;
           atomicAdd(&s.count[bin_of(e)], 1u);
         }
@@ -484,19 +484,26 @@ struct Sampler {
     if (mode == kDigestBins) {
       const uint64_t all = wave_total(total >> shift);
       const uint64_t goal = top_p < 1.0f ? top_goal(top_p, all) : ~0ull;
-      // The row's bins, two threads each.
-      const int row_bin = tid & (kChunkBins - 1);
+      // The row's bins: a wave adds those of a chunk.
+      if (tid < kChunkBins) s.mass[tid] = 0;
+      if (tid == 0) s.bin = kChunkBins - 1, s.listed = 0, s.pieces = 0, s.some = 0, s.cut_x = INFINITY, s.cut_i = -1;
       __syncthreads();
-      uint64_t v = 0;
-      if (row_bin < kChunkBins - 1)
-        for (int k = tid >> 9; k < n_chunks; k += 2) {
-          const int at = row_bin - 16 * s.chunk_shift[k];
-          if (at >= 0 && s.chunk_kept[k] != 0) v += chunks[k].bins[at] >> s.chunk_shift[k];
+      auto fetch = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < kChunkBins / 64; ++i) early[i] = chunks[k].bins[64 * i + lane];
+      };
+      for (int k = wave; k < n_chunks; k += kSampleWaves) {
+        const int down = s.chunk_shift[k];
+        if (s.chunk_kept[k] == 0) continue;
+        if (k != wave) fetch(k);  // (those are there already)
+#pragma unroll
+        for (int i = 0; i < kChunkBins / 64; ++i) {
+          const int at = 64 * i + lane;  // (the last one is not in use)
+          if (at < kChunkBins - 1 && at + 16 * down < kChunkBins - 1) atomicAdd(&s.mass[at + 16 * down], early[i] >> down);
         }
-      s.mass[tid] = v;
-      if (tid == 0) s.bin = kChunkBins - 1, s.listed = 0, s.cut_x = INFINITY, s.cut_i = -1;
+      }
       __syncthreads();
-      v = tid < kChunkBins ? s.mass[tid] + s.mass[tid + kChunkBins] : 0;
+      const uint64_t v = tid < kChunkBins ? s.mass[tid] : 0;
       uint64_t sum;
       const uint64_t before = block_before(v, &sum);
       if (tid < kChunkBins - 1 && before < goal && goal <= before + v) s.bin = tid;
@@ -509,30 +516,63 @@ struct Sampler {
       }
       if (last == kChunkBins - 1) return false;
       if (tid == last) s.above = before;
-      // What a chunk has in the bins before it.
+      // What a chunk has in the bins before it, and which chunks have words of it.
       for (int k = wave; k < n_chunks; k += kSampleWaves) {
         const int bins = s.chunk_kept[k] == 0 ? 0 : last - 16 * s.chunk_shift[k];
         uint64_t m = 0;
-        for (int i = lane; i < bins; i += 64) m += chunks[k].bins[i];
+        if (n_chunks > kSampleWaves) fetch(k);
+#pragma unroll
+        for (int i = 0; i < kChunkBins / 64; ++i) m += 64 * i + lane < bins ? early[i] : 0;
         m = wave_total(m);
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < kChunkBins / 64; ++i) some |= bins >= 0 && 64 * i + lane == bins && s.chunk_kept[k] != 0 && early[i] != 0;
         if (lane == 0) s.mass[k] = m;
+        if (some) s.wave_chunk[atomicAdd(&s.some, 1)] = (uint32_t)k;
       }
-      // The words of the bin.  (First by a range of x, a little too wide.)
+      __syncthreads();
+      const int some = s.some;
+      // The words of the bin.  (First by a range of x, a little too wide, and first the pieces that have any: a few words of a wave's
+      // would keep all of it busy with each.  Without, 1000 of 131072 words took 4 us longer.)
       const double wide = 1e-6 * (fabs(power_of_row) + 32.0);
       const float x_hi = (float)((power_of_row - (last - 0.5) / 16.0 + wide) / c), x_lo = (float)((power_of_row - (last + 0.5) / 16.0 - wide) / c);
-      row.template each<true>([&](const float* x, int i0) {
-        bool any = false;
+      constexpr int PIECES = kChunkWords / (kSampleThreads * E), BATCH = 4 / PIECES;
+#pragma unroll 1
+      for (int c0 = 0; c0 < some; c0 += BATCH) {
+        u32x4 w[BATCH * PIECES];
+        int at[BATCH * PIECES];
 #pragma unroll
-        for (int e = 0; e < E; ++e) any |= (x[e] >= x_lo) & (x[e] <= x_hi);
-        if (any) {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if ((x[e] >= x_lo) & (x[e] <= x_hi) & (x[e] > -INFINITY)) {
-              const int j = atomicAdd(&s.listed, 1);
-              if (j < kSampleList) s.list[j] = entry(x[e] + 0.0f, i0 + e);
-            }
+        for (int p = 0; p < BATCH * PIECES; ++p) {
+          at[p] = (int)s.wave_chunk[min(c0 + p / PIECES, some - 1)] * kChunkWords + (p % PIECES * kSampleThreads + tid) * E;
+          w[p] = row.load(at[p]);
         }
-      });
+#pragma unroll
+        for (int p = 0; p < BATCH * PIECES; ++p) {
+          float x[E];
+          row.numbers(w[p], x);
+          bool any = false;
+#pragma unroll
+          for (int e = 0; e < E; ++e) any |= (x[e] >= x_lo) & (x[e] <= x_hi);
+          if (any && c0 + p / PIECES < some) {
+            const int j = atomicAdd(&s.pieces, 1);
+            if (j < kSampleBins) s.count[j] = (uint32_t)at[p];
+          }
+        }
+      }
+      __syncthreads();
+      const int pieces = s.pieces;
+      if (pieces > kSampleBins) return false;
+      for (int j = tid; j < pieces; j += kSampleThreads) {
+        const int i0 = (int)s.count[j];
+        float x[E];
+        row.numbers(row.load(i0), x);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if ((x[e] >= x_lo) & (x[e] <= x_hi) & (x[e] > -INFINITY)) {
+            const int at = atomicAdd(&s.listed, 1);
+            if (at < kSampleList) s.list[at] = entry(x[e] + 0.0f, i0 + e);
+          }
+      }
       __syncthreads();
       // Of those the ones that lie in the bin.
       const int range = s.listed;
@@ -921,7 +961,10 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   if (a.chunks != nullptr) {
     const SampleChunk* chunks = a.chunks + (int64_t)b * a.n_chunks;
     const SampleChunk& mine = chunks[min(lane, a.n_chunks - 1)];
-    const unsigned long long early = chunks[min(wave, a.n_chunks - 1)].list[lane];  // (on the way before anything is known)
+    unsigned long long early[kChunkBins / 64];  // (on the way before anything is known)
+#pragma unroll
+    for (int i = 0; i < kChunkBins / 64; ++i)
+      if (i == 0 || a.may_bin) early[i] = chunks[min(wave, a.n_chunks - 1)].list[64 * i + lane];
     float top = mine.top;
     int top_i = mine.top_i;
 #pragma unroll
@@ -1075,8 +1118,9 @@ int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int
   const size_t need = lh_hip_sample_workspace_bytes(B, V);
   LH_REQUIRE(need == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= need),
              "lh_hip_sample: workspace too small or not 256-byte aligned: %zu of %zu bytes", workspace_bytes, need);
-  SampleArgs a = {tokens, logits, uniform, ld, (int32_t)V, 50, *opts, need ? static_cast<SampleChunk*>(workspace) : nullptr, sample_chunks(V)};
+  SampleArgs a = {tokens, logits, uniform, ld, (int32_t)V, 50, *opts, need ? static_cast<SampleChunk*>(workspace) : nullptr, sample_chunks(V), 0};
   while ((V >> (62 - a.bits)) != 0) --a.bits;
+  a.may_bin = (opts->top_k || opts->top_k_all <= 0 || opts->top_k_all >= V) && (opts->top_p || opts->min_p || opts->top_p_all < 1.0f || opts->min_p_all > 0.0f);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == LH_F32) return launch_sample<LH_F32>(a, B, s);
   if (dtype == LH_BF16) return launch_sample<LH_BF16>(a, B, s);
