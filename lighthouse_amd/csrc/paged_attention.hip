@@ -15,6 +15,13 @@
 //  * The waves of a workgroup take the steps of its share of the positions in turn, each on its own; their results are brought to
 //    the common maximum and added through LDS at the end.  A long cache is shared out between `splits` workgroups,
 //    each leaving (maximum, sum, sum of p v), which a second launch joins.
+//  * The table is read two steps ahead by the scalar unit, so that no step waits for a lookup or drains the loads on the way.
+//
+// Measured, keys and values out of memory: 16 sequences of 8192 to 32768 in bf16, 8 heads of 128 with 4 queries each, 255 us (5.2 TB/s) and 5 for
+// the join; 64 sequences of 256 to 1024, 12 heads of 64, 29 us (4.3 TB/s); 32 sequences of 2048 to 8192 in e4m3, 4 heads of 128 with 8 queries
+// each, 38 us (4.4 TB/s) and 5.  Out of the caches the same take 131, 20 and 31: the longer ones are bound by memory, and by what one CU draws of it
+// (31 B/ns) where the sequences' lengths do not fill all CUs to the end.  One sequence of 1000, 12 heads of 64: 5.3 us and 3.2, the chain of table, keys, values
+// and join.
 //
 // 16-bit types: P is split into a value of the type and the value of the type nearest to what that leaves, two matrix
 // instructions instead of one (they cost nothing here): P alone rounded once to bf16 would add an error as large as the
@@ -552,7 +559,11 @@ static bool paged_in_tiles(const Paged& c, int es) {
 }
 
 // How many positions a workgroup takes of a sequence; `items` (sequence, head, group of queries), `per_cu` workgroups that a CU
-// holds at once, `row_bytes` of a position's key and value.
+// holds at once, `row_bytes` of a position's key and value.  There are to be two workgroups per CU (one, if no more fit): with few items the
+// shares are short.  (One sequence of 1000, 12 heads of 64: 7.9 us with 128 positions a share, 9.8 in one; one of 32768, 8 heads of 128: 35 with
+// 512, 57 with 4096, 362 in one; heads of 256, 16 sequences of 1024 to 4096: 73 with 2048, 94 with 512.)  With items enough for that, up to 8 per CU
+// even out sequences of unlike length, while a share has 512 KB of keys and values, which the join's launch costs nothing against.  (16
+// sequences of 8192 to 32768, 8 heads of 128: 255 with 2048, 263 with 512, 384 in one; 64 of 256 to 1024, 12 heads of 64, 30 in one, 33 with 512.)
 static int paged_share(int64_t items, int capacity, int per_cu, int64_t row_bytes) {
   const int64_t cus = num_cus();
   int64_t splits = ((per_cu < 2 ? 1 : 2) * cus + items - 1) / items;
