@@ -413,7 +413,7 @@ int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, 
 /*
  * Attention of one new token of every sequence over its cache: q, out [B, H, d] (element strides of batch and head, unit
  * stride along d), H a multiple of n_kv_heads, head h reads key / value head h / (H / n_kv_heads):
- *   out[b, h] = sum_t p_t v_t,  p = softmax over t < lengths[b] of scale q . k_t,
+ *   out[b, h] = sum_t p_t v_t,  p = softmax over t < lengths[b] of scale q . k_t  (an infinite v_t may give a NaN),
  * positions on pages that hold nothing left out; 0 where nothing is left.  `lengths` counts the new token if it has been
  * appended and is clamped to 0 .. max_pages * page_size.  Scores, softmax and sums are f32.  dtype (of q and out) is the
  * cache's, or BF16 or F16 for a cache of e4m3.  With `weights` ([B, n_kv_heads, >= max_pages * page_size] f32, element strides

@@ -497,7 +497,8 @@ int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, 
 }
 
 size_t lh_hip_kv_evict_workspace_bytes(int64_t B, int64_t n_kv_heads, int64_t budget) {
-  if (B <= 0 || n_kv_heads <= 0 || budget <= 0) return 0;
+  constexpr int64_t kMost = 1ll << 31;
+  if (B <= 0 || n_kv_heads <= 0 || budget <= 0 || B >= kMost || n_kv_heads >= kMost || B * n_kv_heads >= (1ll << 16) || budget >= kMost) return 0;
   return ((size_t)B * n_kv_heads * (budget + 1) * 4 + 255) / 256 * 256;
 }
 

@@ -550,6 +550,11 @@ struct PagedPlan {
   size_t total() const { return o_bytes + ml_bytes + score_bytes + lse_bytes; }
 };
 
+static bool paged_batch(int64_t B, int64_t H) {
+  constexpr int64_t kMost = 1ll << 20;
+  return B > 0 && H > 0 && B < kMost && H < kMost && B * H < kMost;
+}
+
 static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
 
 static bool paged_in_tiles(const Paged& c, int es) {
@@ -625,7 +630,7 @@ extern "C" {
 size_t lh_hip_paged_attention_workspace_bytes(const lh_paged_cache* cache, int64_t B, int64_t H, int32_t with_weights) {
   Paged c;
   if (paged_cache(cache, "lh_hip_paged_attention_workspace_bytes", &c) != LH_OK) return 0;
-  if (B <= 0 || H <= 0 || H % c.heads != 0) return 0;
+  if (!paged_batch(B, H) || H % c.heads != 0) return 0;
   return paged_plan(c, cache->dtype, B, H, with_weights != 0).total();
 }
 
@@ -638,7 +643,7 @@ int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q
   if (B == 0) return LH_OK;
   LH_REQUIRE(out && q && lengths, "lh_hip_paged_attention: null pointer");
   LH_REQUIRE(B >= 0 && H > 0 && H % a.c.heads == 0, "lh_hip_paged_attention: %lld heads are no multiple of %d key / value heads", (long long)H, a.c.heads);
-  LH_REQUIRE(B * H < (1ll << 20), "lh_hip_paged_attention: bad batch (fewer than 2^20 heads of sequences)");
+  LH_REQUIRE(paged_batch(B, H), "lh_hip_paged_attention: bad batch (fewer than 2^20 heads of sequences)");
   LH_REQUIRE(dtype == cache->dtype || (cache->dtype == LH_F8E4M3 && (dtype == LH_BF16 || dtype == LH_F16)),
              "lh_hip_paged_attention: queries must have the cache's dtype (bf16 or f16 for a cache of e4m3)");
   LH_REQUIRE(weights == nullptr || ((a.c.heads == 1 || weights_stride_h >= a.c.capacity()) && (B <= 1 || weights_stride_b >= a.c.capacity())),

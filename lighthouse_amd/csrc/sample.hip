@@ -1108,7 +1108,7 @@ static int launch_sample(const SampleArgs& a, int64_t B, hipStream_t s) {
 extern "C" {
 
 size_t lh_hip_sample_workspace_bytes(int64_t B, int64_t V) {
-  return B <= 0 || V <= 0 ? 0 : ((size_t)B * sample_chunks(V) * sizeof(SampleChunk) + 255) / 256 * 256;
+  return B <= 0 || B >= (1ll << 18) || V <= 0 ? 0 : ((size_t)B * sample_chunks(V) * sizeof(SampleChunk) + 255) / 256 * 256;
 }
 
 int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int64_t B, int64_t V, int64_t ld, int32_t dtype,

@@ -182,6 +182,24 @@ def test_the_c_entry_points_refuse_without_a_gpu():
         assert b"workspace" in lib.lh_hip_last_error()
 
 
+def test_sizes_beyond_every_limit_need_no_workspace_and_are_refused():
+    """Products of sizes that pass 64 bits do not come out as something small."""
+    lib = _lib.load()
+    st = _lib.Strides3(64, 32, 8)
+    c = ctypes.byref(_lib.PagedCache(4096, 8192, 12288, 2, st, st, 6, 2, 4, 2, 8, _lib.BF16, 1.0, 1.0))
+    opts = _lib.SampleOpts(temperature_all=1.0, top_p_all=1.0)
+    for B, H in ((2**62, 4), (2**40, 2**26), (2**32, 2**32), (2**20, 2), (-3, 4), (3, -4)):
+        assert lib.lh_hip_paged_attention_workspace_bytes(c, B, H, 1) == 0
+        assert lib.lh_hip_paged_attention(c, 4096, 4096, 32, 8, 32, 8, 4096, None, 0, 0, B, H, 1.0, _lib.BF16, None, 0, None) == _lib.LH_ERR_INVALID
+    for B, heads, budget in ((2**62, 4, 4), (2**33, 2**31, 8), (2, 2**62, 2), (2, 2, 2**62), (2**16, 1, 4)):
+        assert lib.lh_hip_kv_evict_workspace_bytes(B, heads, budget) == 0
+    for B in (2**62, 2**33, 2**18):
+        assert lib.lh_hip_kv_evict(c, 4096, 16, 8, 4096, 4096, B, 4, 0, 4096, 1 << 40, None) == _lib.LH_ERR_INVALID
+        assert lib.lh_hip_kv_append(c, 4096, 4096, 64, 32, 8, 64, 32, 8, 4096, None, B, 2**31, _lib.BF16, None) == _lib.LH_ERR_INVALID
+        assert lib.lh_hip_sample_workspace_bytes(B, 20000) == 0
+        assert lib.lh_hip_sample(4096, 4096, 4096, B, 20000, 20000, _lib.F32, ctypes.byref(opts), 4096, 1 << 40, None) == _lib.LH_ERR_INVALID
+
+
 def test_packed_structs_are_laid_out_like_the_c_ones():
     import struct
 
