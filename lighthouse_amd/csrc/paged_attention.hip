@@ -564,15 +564,17 @@ static bool paged_in_tiles(const Paged& c, int es) {
 }
 
 // How many positions a workgroup takes of a sequence; `items` (sequence, head, group of queries), `per_cu` workgroups that a CU
-// holds at once, `row_bytes` of a position's key and value.  There are to be two workgroups per CU (one, if no more fit): with few items the
-// shares are short.  (One sequence of 1000, 12 heads of 64: 7.9 us with 128 positions a share, 9.8 in one; one of 32768, 8 heads of 128: 35 with
-// 512, 57 with 4096, 362 in one; heads of 256, 16 sequences of 1024 to 4096: 73 with 2048, 94 with 512.)  With items enough for that, up to 8 per CU
+// holds at once, `row_bytes` of a position's key and value.  There are to be two workgroups per CU (one, if no more fit; one also where the
+// shares would be shorter than 1024 positions, of which their start and end take too much).  (One sequence of 1000, 12 heads of 64: 7.9 us with 128
+// positions a share, 9.8 in one; one of 32768, 8 heads of 128: 31.8 with 1024, 33.5 with 512, 362 in one; 4 of 1024 to 4096, 8 heads of 128 with 4 queries: 14.8 with
+// 512, 15.8 with 256; heads of 256, 16 sequences of 1024 to 4096: 73 with 2048, 94 with 512.)  With items enough for that, up to 8 per CU
 // even out sequences of unlike length, while a share has 512 KB of keys and values, which the join's launch costs nothing against.  (16
 // sequences of 8192 to 32768, 8 heads of 128: 255 with 2048, 263 with 512, 384 in one; 64 of 256 to 1024, 12 heads of 64, 30 in one, 33 with 512.)
 static int paged_share(int64_t items, int capacity, int per_cu, int64_t row_bytes) {
   const int64_t cus = num_cus();
   int64_t splits = ((per_cu < 2 ? 1 : 2) * cus + items - 1) / items;
   if (per_cu >= 3) {
+    if (capacity < 1024 * splits) splits = (cus + items - 1) / items;
     const int64_t level = (8 * cus + items - 1) / items, most = capacity * row_bytes >> 19;
     splits = splits > level ? splits : level < most ? level : splits > most ? splits : most;
   }
