@@ -67,9 +67,10 @@ __device__ __forceinline__ uint32_t paged_e4m3(uint32_t w) {
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
 }
 
-// BYTES from p, of which `left` lie inside the row (elements of ES bytes at their own alignment); the others are 0.
+// BYTES from p, of which `left` lie inside the row (elements of ES bytes at their own alignment); the others are 0.  `width`: bytes of a row
+// (the same for the wave, which jumps over the loads by element where no piece needs them).
 template <int BYTES, int ES>
-__device__ __forceinline__ void load_row_piece(uint32_t* out, const uint8_t* p, int left) {
+__device__ __forceinline__ void load_row_piece(uint32_t* out, const uint8_t* p, int left, int width) {
   if (left >= BYTES) {
     if constexpr (BYTES >= 16) {
 #pragma unroll
@@ -84,6 +85,9 @@ __device__ __forceinline__ void load_row_piece(uint32_t* out, const uint8_t* p, 
     }
     return;
   }
+#pragma unroll
+  for (int i = 0; i < BYTES / 4; ++i) out[i] = 0;
+  if (width % BYTES == 0) return;
 #pragma unroll
   for (int i = 0; i < BYTES / 4; ++i) {
     uint32_t w = 0;
@@ -174,7 +178,7 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
 #pragma unroll
       for (int i = 0; i < QP; ++i) {
         const int d0 = s * (4 * KE) + g4 * KE + i * (16 / QES);
-        load_row_piece<16, QES>(qf[s * QP + i], q + d0 * QES, q_live ? (a.c.d - d0) * QES : 0);
+        load_row_piece<16, QES>(qf[s * QP + i], q + d0 * QES, q_live ? (a.c.d - d0) * QES : 0, a.c.d * QES);
       }
   }
 
@@ -238,7 +242,7 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           const int d0 = s * (4 * KE) + g4 * KE;
-          load_row_piece<KB, ES>(kr[t][s], row + d0 * ES, page < 0 ? 0 : (a.c.d - d0) * ES);
+          load_row_piece<KB, ES>(kr[t][s], row + d0 * ES, page < 0 ? 0 : (a.c.d - d0) * ES, row_bytes);
         }
       }
     }
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
           const int key = k0 + step * KEYS + 16 * t + 4 * g4 + r, page = __shfl(pages[t], 4 * g4 + r);
           const int slot = key - (int)a.c.by_size.div((uint32_t)key) * a.c.size;
           const uint8_t* row = vb + (max(page, 0) * a.c.sv.z + hk * a.c.sv.h + slot * a.c.sv.t) * ES;
-          load_row_piece<VB, ES>(vr[t * 4 + r], row + l16 * VB, page < 0 ? 0 : row_bytes - l16 * VB);
+          load_row_piece<VB, ES>(vr[t * 4 + r], row + l16 * VB, page < 0 ? 0 : row_bytes - l16 * VB, row_bytes);
           live |= (page >= 0 ? 1u : 0u) << (t * 4 + r);
         }
       }
