@@ -522,7 +522,14 @@ __global__ void __launch_bounds__(256) paged_attention_finish(PagedAttnArgs a, i
   if (t0 >= n) return;
   const int parts = (n + a.share - 1) / a.share;
   const int64_t first = (int64_t)b * a.H + hk * a.G;
-  float sum = 0.0f;
+  // (What does not wait for the sums is requested before them: the scores of the first heads and the weight that grows.)
+  constexpr int EARLY = 8;
+  float early[EARLY], sum = 0.0f, old = 0.0f;
+  float* const to = weights + b * sw_b + hk * sw_h + t;
+  const float* const scores = a.scores + first * a.cap_pad + t;
+#pragma unroll
+  for (int g = 0; g < EARLY; ++g) early[g] = t < n && g < a.G ? scores[(int64_t)g * a.cap_pad] : -INFINITY;
+  if (t < n) old = *to;
   for (int g0 = 0; g0 < a.G; g0 += 256) {  // (up to 256 heads of a group at a time)
     const int many = min(256, a.G - g0);
     if (g0 > 0) __syncthreads();
@@ -536,13 +543,17 @@ __global__ void __launch_bounds__(256) paged_attention_finish(PagedAttnArgs a, i
       }
     }
     __syncthreads();
+    auto add = [&](float x, int g) { sum += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - lse[g]); };
+    if (g0 == 0) {
+#pragma unroll
+      for (int g = 0; g < EARLY; ++g)
+        if (g < many) add(early[g], g);
+    }
     if (t < n)
-      for (int g = 0; g < many; ++g) {
-        const float x = a.scores[(first + g0 + g) * a.cap_pad + t];
-        sum += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - lse[g]);
-      }
+#pragma unroll 4
+      for (int g = g0 == 0 ? EARLY : 0; g < many; ++g) add(scores[(int64_t)(g0 + g) * a.cap_pad], g);
   }
-  if (t < n) weights[b * sw_b + hk * sw_h + t] += sum;
+  if (t < n) *to = old + sum;
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
