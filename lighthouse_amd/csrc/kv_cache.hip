@@ -362,11 +362,18 @@ __global__ void __launch_bounds__(THREADS) kv_evict_select(EvictArgs a) {
 
 // Rows move up, row kept[j] to row j: kept[j] >= j, so what a block of rows j .. j + R - 1 overwrites no later block reads,
 // and within the block every row is in registers before any is written.  A workgroup takes a column slice of 128 bytes
-// of the keys or the values of a head, or its weights: slices know nothing of each other.  512 of 1024 positions of 192 heads of 64 in bf16:
-// 50 MB in 10.7 us; 4096 of 4096 to 16384 of 32 heads of 128: 17.4 us.
+// of the keys or the values of a head, or its weights: slices know nothing of each other.  What bounds it is that there are only so many slices,
+// each a CU's chain of blocks.  Where there are fewer than one for every four CUs they are 64 bytes wide: half a line of memory, but twice
+// the CUs.  (Both launches of an eviction, us, slices of 128 and of 64 bytes: 4096 of 16384 positions of 8 heads of 128 in bf16 36.9 and 29.3, of 16 heads 39.4 and
+// 37.6, of 32 heads of ragged lengths 48.4 and 50.5, 2048 of 4096 of 64 heads 46.0 and 51.6.)
 constexpr int kMoveThreads = 1024;
-constexpr int kMoveRows = 4;  // of a thread, in flight at once
+constexpr int kMoveRows = 2;  // of a thread, in flight at once
 
+// PIECES of 16 bytes: a slice.  WHOLE: rows are whole pieces, and the blocks go through a pipeline: while one is written, the rows of the next, the
+// table's entries of the one after it and what `kept` says of the third are on their way.  (Rows of the next block are not among those
+// that this one overwrites.  One block after the other, of twice the size, 4096 of 16384 positions of 32 heads took 81 us instead of 48, 512 of 1024 of 192 heads
+// of 64 24 instead of 18.)  Lanes that have nothing to move load the first row of all: nothing but the stores branches.
+template <int PIECES, bool WHOLE>
 __global__ void __launch_bounds__(kMoveThreads) kv_evict_move(EvictArgs a) {
   const int per_head = 1 + 2 * a.slices;
   const int bh = blockIdx.x / per_head, what = blockIdx.x % per_head;
@@ -395,9 +402,73 @@ __global__ void __launch_bounds__(kMoveThreads) kv_evict_move(EvictArgs a) {
   const int es = a.elem_bytes, row_bytes = a.c.d * es;
   uint8_t* base = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + h * cs.h * es;
   typedef typename Chunk<1>::type any16;
-  const int col = slice * 128 + (tid & 7) * 16;  // 8 threads a row
+  const int col = (slice * PIECES + tid % PIECES) * 16;  // a thread each
   const int bytes = min(16, row_bytes - col);    // (none, or less than a chunk, where the row ends)
-  constexpr int kRows = kMoveThreads / 8;
+  constexpr int kRows = kMoveThreads / PIECES;
+  if constexpr (WHOLE) {
+    struct Block {
+      int j[kMoveRows], from[kMoveRows], entry_from[kMoveRows], entry_to[kMoveRows];
+    };
+    const int64_t table_row = b * a.c.table_stride;
+    uint8_t* const cache = base + min(col, row_bytes - 16);
+    const bool live = bytes > 0;
+    auto look_up = [&](int j0, Block& k) {
+#pragma unroll
+      for (int r = 0; r < kMoveRows; ++r) k.j[r] = j0 + r * kRows + tid / PIECES, k.from[r] = kept[min(k.j[r], a.budget - 1)];
+    };
+    auto find_pages = [&](Block& k) {
+#pragma unroll
+      for (int r = 0; r < kMoveRows; ++r) {
+        k.entry_from[r] = a.c.entry(table_row + a.c.by_size.div((uint32_t)k.from[r]));
+        k.entry_to[r] = a.c.entry(table_row + a.c.by_size.div((uint32_t)min(k.j[r], a.budget - 1)));
+      }
+    };
+    auto place = [&](int entry, int t) -> uint8_t* {
+      const int slot = t - (int)a.c.by_size.div((uint32_t)t) * a.c.size;
+      return cache + (entry * cs.z + slot * cs.t) * es;
+    };
+    auto request = [&](const Block& k, any16* x, uint8_t** to) {
+#pragma unroll
+      for (int r = 0; r < kMoveRows; ++r) {
+        const bool moves = live && k.j[r] < a.budget && k.from[r] != k.j[r] && (uint32_t)k.entry_from[r] < (uint32_t)a.c.pages && (uint32_t)k.entry_to[r] < (uint32_t)a.c.pages;
+        x[r] = *reinterpret_cast<const any16*>(moves ? place(k.entry_from[r], k.from[r]) : cache);
+        to[r] = moves ? place(k.entry_to[r], k.j[r]) : nullptr;
+      }
+    };
+    constexpr int ROWS = kRows * kMoveRows;
+    any16 x[2][kMoveRows];
+    uint8_t* to[2][kMoveRows];
+    Block k[3];  // of this block, of the next, of the one after it, in turn
+    look_up(0, k[0]);
+    look_up(ROWS, k[1]);
+    find_pages(k[0]);
+    find_pages(k[1]);
+    look_up(2 * ROWS, k[2]);
+    request(k[0], x[0], to[0]);
+    // Block at j0: its rows are in x[now], `next` knows the pages of the one behind it, `after` the positions of the one behind that.
+    auto step = [&](int j0, int now, Block& own, Block& next, Block& after) {
+      find_pages(after);
+      look_up(j0 + 3 * ROWS, own);
+      request(next, x[now ^ 1], to[now ^ 1]);
+#pragma unroll
+      for (int r = 0; r < kMoveRows; ++r)
+        asm volatile("" : "+v"(x[now][r][0]), "+v"(x[now][r][1]), "+v"(x[now][r][2]), "+v"(x[now][r][3]));
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < kMoveRows; ++r)
+        if (to[now][r] != nullptr) *reinterpret_cast<any16*>(to[now][r]) = x[now][r];
+    };
+#pragma unroll 1
+    for (int j0 = 0; j0 < a.budget; j0 += 6 * ROWS) {
+      step(j0, 0, k[0], k[1], k[2]);
+      if (j0 + ROWS < a.budget) step(j0 + ROWS, 1, k[1], k[2], k[0]);
+      if (j0 + 2 * ROWS < a.budget) step(j0 + 2 * ROWS, 0, k[2], k[0], k[1]);
+      if (j0 + 3 * ROWS < a.budget) step(j0 + 3 * ROWS, 1, k[0], k[1], k[2]);
+      if (j0 + 4 * ROWS < a.budget) step(j0 + 4 * ROWS, 0, k[1], k[2], k[0]);
+      if (j0 + 5 * ROWS < a.budget) step(j0 + 5 * ROWS, 1, k[2], k[0], k[1]);
+    }
+    return;
+  }
   auto row = [&](int t) -> uint8_t* {
     int slot;
     const int page = a.c.page_of(b, t, &slot);
@@ -408,7 +479,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_evict_move(EvictArgs a) {
     uint8_t* to[kMoveRows];
 #pragma unroll
     for (int r = 0; r < kMoveRows; ++r) {
-      const int j = j0 + r * kRows + (tid >> 3);
+      const int j = j0 + r * kRows + tid / PIECES;
       to[r] = nullptr;
       x[r] = any16{0u, 0u, 0u, 0u};
       if (j >= a.budget || bytes <= 0) continue;
@@ -522,13 +593,18 @@ int lh_hip_kv_evict(const lh_paged_cache* cache, float* weights, int64_t weights
   a.held = a.kept + B * a.c.heads * budget;
   a.B = (int32_t)B, a.budget = (int32_t)budget, a.recent = (int32_t)recent;
   a.elem_bytes = (int32_t)dtype_size(cache->dtype);
-  a.slices = (a.c.d * a.elem_bytes + 127) / 128;
+  const int row_bytes = a.c.d * a.elem_bytes;
+  const bool narrow = row_bytes % 16 == 0 && B * a.c.heads * 2 * ((row_bytes + 127) / 128) <= num_cus() / 4;
+  a.slices = narrow ? (row_bytes + 63) / 64 : (row_bytes + 127) / 128;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 heads((unsigned)(B * a.c.heads));
   if (a.c.capacity() <= 256 * kEvictKeys) LH_LAUNCH(kv_evict_select<256>, heads, dim3(256), 0, s, a);
   else LH_LAUNCH(kv_evict_select<1024>, heads, dim3(1024), 0, s, a);
   if (const int rc = check_launch("kv_evict_select")) return rc;
-  LH_LAUNCH(kv_evict_move, dim3((unsigned)(B * a.c.heads * (1 + 2 * a.slices))), dim3(kMoveThreads), 0, s, a);
+  const dim3 moves((unsigned)(B * a.c.heads * (1 + 2 * a.slices)));
+  if (row_bytes % 16 != 0) LH_LAUNCH((kv_evict_move<8, false>), moves, dim3(kMoveThreads), 0, s, a);
+  else if (narrow) LH_LAUNCH((kv_evict_move<4, true>), moves, dim3(kMoveThreads), 0, s, a);
+  else LH_LAUNCH((kv_evict_move<8, true>), moves, dim3(kMoveThreads), 0, s, a);
   return check_launch("kv_evict_move");
 }
 

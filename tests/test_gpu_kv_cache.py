@@ -164,3 +164,39 @@ def test_evict_with_a_strided_weight_tensor_and_a_workspace():
     assert (full[:, 2] == 5).all() and (full[:, :, c.capacity:] == 5).all()
     with pytest.raises(ValueError, match="workspace"):
         ops.kv_evict(c.k_cache, c.v_cache, weights, c.table, c.device_lengths, 64, workspace=torch.empty(need - 1, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_evict_of_many_heads(d):
+    """Workgroups enough for slices of whole lines, several blocks of rows each, the last of them cut anywhere."""
+    c = ref.Cache([1500, 701, 2000, 5, 1024, 769], 8, 16, d, f16, seed=6)
+    check_evict(c, weights_like(c, 6), 700, 30)
+    c = ref.Cache([1500, 770, 2000, 5, 1024, 769], 8, 16, d, f16, seed=7)
+    check_evict(c, weights_like(c, 7, "ties"), 769, 0)
+
+
+@pytest.mark.parametrize("d", [64, 7])
+@pytest.mark.parametrize("heads", [2, 40])
+def test_rows_on_pages_that_hold_nothing_do_not_move(heads, d):
+    """A row stays where it is if its page, or the one it would go to, is none; all others and the weights move."""
+    c = ref.Cache([600, 333], heads, 16, d, bf16, seed=8)
+    table = c.table_cpu.clone()
+    table[0, 3], table[0, 30], table[1, 0], table[1, 20] = -1, c.pages, 2**31 - 1, -(2**31)
+    weights = weights_like(c, 8)
+    caches = [ref.as_bits(x).cpu().clone() for x in (c.k_cache, c.v_cache)]
+    w = weights.cpu().clone()
+    for b, n in enumerate(c.lengths):
+        for h in range(heads):
+            kept = ref.evict(w[b, h], n, 300, 40)
+            for bits in caches:
+                before = bits[:, h].clone()
+                for j, t in enumerate(kept):
+                    source, target = int(table[b, t // 16]), int(table[b, j // 16])
+                    if 0 <= source < c.pages and 0 <= target < c.pages:
+                        bits[target, h, j % 16] = before[source, t % 16]
+            w[b, h, :300] = w[b, h][kept].clone()
+            w[b, h, 300:n] = 0
+    assert ops.kv_evict(c.k_cache, c.v_cache, weights, table.cuda(), c.device_lengths, 300, recent=40).tolist() == [300, 300]
+    for cache, bits in zip((c.k_cache, c.v_cache), caches):
+        assert torch.equal(ref.as_bits(cache).cpu(), bits)
+    assert torch.equal(ref.as_bits(weights).cpu(), ref.as_bits(w))
