@@ -48,6 +48,7 @@ struct PagedAttnArgs {
 };
 
 constexpr int kPagedWaves = 4;
+typedef float any_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kPagedShare = 32 * kPagedWaves;  // positions a share is a multiple of
 
 __device__ __forceinline__ int paged_length(const PagedAttnArgs& a, int b) { return min(max(a.lengths[b], 0), a.c.capacity()); }
@@ -68,8 +69,8 @@ __device__ __forceinline__ uint32_t paged_e4m3(uint32_t w) {
 }
 
 // BYTES from p, of which `left` lie inside the row (elements of ES bytes at their own alignment); the others are 0.  `width`: bytes of a row
-// (the same for the wave, which jumps over the loads by element where no piece needs them).
-template <int BYTES, int ES>
+// (the same for the wave, which jumps over the loads by element where no piece needs them).  WHOLE: none does.
+template <int BYTES, int ES, bool WHOLE>
 __device__ __forceinline__ void load_row_piece(uint32_t* out, const uint8_t* p, int left, int width) {
   if (left >= BYTES) {
     if constexpr (BYTES >= 16) {
@@ -87,7 +88,7 @@ __device__ __forceinline__ void load_row_piece(uint32_t* out, const uint8_t* p, 
   }
 #pragma unroll
   for (int i = 0; i < BYTES / 4; ++i) out[i] = 0;
-  if (width % BYTES == 0) return;
+  if (WHOLE || width % BYTES == 0) return;
 #pragma unroll
   for (int i = 0; i < BYTES / 4; ++i) {
     uint32_t w = 0;
@@ -99,6 +100,18 @@ __device__ __forceinline__ void load_row_piece(uint32_t* out, const uint8_t* p, 
         else w = reinterpret_cast<const uint32_t*>(p)[i];
       }
     out[i] = w;
+  }
+}
+
+// The first `skip` elements of a piece become 0.
+template <int BYTES, int ES>
+__device__ __forceinline__ void clear_first(uint32_t* w, int skip) {
+#pragma unroll
+  for (int i = 0; i < BYTES / 4; ++i) {
+    uint32_t keep = 0;
+#pragma unroll
+    for (int e = 0; e < 4 / ES; ++e) keep |= i * (4 / ES) + e >= skip ? (ES == 4 ? ~0u : ((1u << (8 * ES % 32)) - 1) << (8 * ES * e)) : 0u;
+    w[i] &= keep;
   }
 }
 
@@ -117,16 +130,17 @@ __device__ __forceinline__ void load_buffer(uint32_t* out, __amdgpu_buffer_rsrc_
 }
 
 // CDT: the cache's type, QDT: the queries' (the cache's, or a 16-bit type with e4m3).  DP: width that d is padded to.
-// TILES: the pages are multiples of 16 positions and rows 16-byte aligned, so that a tile of 16 keys has one base and its rows
+// kTiles: the pages are multiples of 16 positions and rows 16-byte aligned, so that a tile of 16 keys has one base and its rows
 // are loaded through a buffer resource whose size is that of the rows that exist: what lies behind comes back as 0 without a
-// test.  Otherwise every lane finds the page of every row it loads.
+// test.  Otherwise every lane finds the page of every row it loads; kWholeRows: rows that are whole pieces, however aligned.
+enum PagedMode { kTiles, kWholeRows, kOddRows };
 // Waves of a SIMD that the registers have to suffice for: as many as they do without scratch memory.
-constexpr int paged_occupancy(int cdt, int dp, bool tiles) {
-  return dp == 64 ? 4 : dp == 256 ? 1 : tiles && cdt != LH_F32 ? 3 : 2;
+constexpr int paged_occupancy(int cdt, int dp, int mode) {
+  return dp == 64 ? (mode == kOddRows ? 3 : 4) : dp == 256 ? 1 : mode == kTiles && cdt != LH_F32 ? 3 : 2;
 }
-template <int CDT, int QDT, int DP, int NW, bool TILES>
-__global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) paged_attention_kernel(PagedAttnArgs a) {
-  constexpr bool F32 = CDT == LH_F32;
+template <int CDT, int QDT, int DP, int NW, int MODE>
+__global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE)) paged_attention_kernel(PagedAttnArgs a) {
+  constexpr bool F32 = CDT == LH_F32, TILES = MODE == kTiles;
   constexpr int ES = CDT == LH_F8E4M3 ? 1 : F32 ? 4 : 2;
   constexpr int KT = F32 ? 1 : 2;            // 16-key tiles a step
   constexpr int KEYS = 16 * KT;
@@ -138,6 +152,10 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
   constexpr int VP = VB > 16 ? VB / 16 : 1;    // loads for them
   constexpr int VPB = VB / VP;
   constexpr int kOutside = 0x40000000;         // an offset behind every buffer
+  // Rows that are no whole pieces (and longer than one): the last piece moves back to end with the row.  Of a key and a query it gives only the
+  // columns that the piece before has not; columns of a value may come from two lanes, which are of one mind.  (By element, 16 sequences of
+  // 1024 to 4096, 8 heads of 136 with 4 queries, e4m3: 211 us instead of 73; 32 of 40 to 161, 7 heads of 181 with 16 queries, bf16: 41 instead of 34.)
+  const bool k_back = MODE == kOddRows && a.c.d % KE != 0 && a.c.d > KE, v_back = MODE == kOddRows && a.c.d % CE != 0 && a.c.d > CE;
   __shared__ __attribute__((aligned(16))) f32x4 sums[NW / 2][CE][64];
   __shared__ float2 stats[NW][16];
 
@@ -177,8 +195,10 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int i = 0; i < QP; ++i) {
-        const int d0 = s * (4 * KE) + g4 * KE + i * (16 / QES);
-        load_row_piece<16, QES>(qf[s * QP + i], q + d0 * QES, q_live ? (a.c.d - d0) * QES : 0, a.c.d * QES);
+        const int k_d0 = s * (4 * KE) + g4 * KE, back = k_back ? max(k_d0 - (a.c.d - KE), 0) : 0, d0 = k_d0 + i * (16 / QES);
+        const int left = !q_live ? 0 : !k_back ? (a.c.d - d0) * QES : k_d0 < a.c.d ? 16 : 0;
+        load_row_piece<16, QES, MODE != kOddRows>(qf[s * QP + i], q + (d0 - back) * QES, left, k_back ? 16 : a.c.d * QES);
+        if (k_back) clear_first<16, QES>(qf[s * QP + i], back - i * (16 / QES));
       }
   }
 
@@ -194,7 +214,7 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
   const int row_bytes = a.c.d * ES;
   uint32_t kr[KT][KS][KB / 4], vr[KT * 4][VB / 4];
   int pages[KT];       // of the step that is requested next: of its tiles, or of the key 16 t + l16 that is the lane's
-  int held[KT];        // TILES: how many rows of its tiles exist
+  int held[KT];        // kTiles: how many rows of its tiles exist
   uint32_t live = 0;   // otherwise: which of the lane's KT * 4 keys do
 
   int koff[KS], voff[4][VP];
@@ -212,7 +232,7 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
         voff[r][p] = col < row_bytes ? (g4 * 4 + r) * (int)a.c.sv.t * ES + col : kOutside;
       }
   }
-  // TILES: where the rows of a tile of the next step begin (keys and values are laid out alike), and how many bytes there are.
+  // kTiles: where the rows of a tile of the next step begin (keys and values are laid out alike), and how many bytes there are.
   int64_t tile_at[KT];
   int tile_bytes[KT];
   auto next_pages = [&](int step, const int* found) {
@@ -242,7 +262,13 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           const int d0 = s * (4 * KE) + g4 * KE;
-          load_row_piece<KB, ES>(kr[t][s], row + d0 * ES, page < 0 ? 0 : (a.c.d - d0) * ES, row_bytes);
+          if (!k_back) {
+            load_row_piece<KB, ES, MODE != kOddRows>(kr[t][s], row + d0 * ES, page < 0 ? 0 : (a.c.d - d0) * ES, row_bytes);
+          } else {
+            const int back = max(d0 - (a.c.d - KE), 0);
+            load_row_piece<KB, ES, MODE != kOddRows>(kr[t][s], row + (d0 - back) * ES, page >= 0 && d0 < a.c.d ? KB : 0, KB);
+            if ((s + 1) * (4 * KE) > a.c.d) clear_first<KB, ES>(kr[t][s], back);
+          }
         }
       }
     }
@@ -265,7 +291,8 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
           const int key = k0 + step * KEYS + 16 * t + 4 * g4 + r, page = __shfl(pages[t], 4 * g4 + r);
           const int slot = key - (int)a.c.by_size.div((uint32_t)key) * a.c.size;
           const uint8_t* row = vb + (max(page, 0) * a.c.sv.z + hk * a.c.sv.h + slot * a.c.sv.t) * ES;
-          load_row_piece<VB, ES>(vr[t * 4 + r], row + l16 * VB, page < 0 ? 0 : row_bytes - l16 * VB, row_bytes);
+          const int col = v_back ? min(l16 * CE, a.c.d - CE) : l16 * CE, left = !v_back ? row_bytes - l16 * VB : l16 * CE < a.c.d ? VB : 0;
+          load_row_piece<VB, ES, MODE != kOddRows>(vr[t * 4 + r], row + col * ES, page < 0 ? 0 : left, v_back ? VB : row_bytes);
           live |= (page >= 0 ? 1u : 0u) << (t * 4 + r);
         }
       }
@@ -407,7 +434,8 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
     if (next < steps) request_values(next);
   }
 
-  // acc[i][r] = sum p v of query l16, column (4 g4 + r) CE + i, over this wave's positions and relative to its maximum.
+  // acc[i][r] = sum p v of query l16, column first_col(r) + i, over this wave's positions and relative to its maximum.
+  auto first_col = [&](int r) { return v_back ? min((4 * g4 + r) * CE, a.c.d - CE) : (4 * g4 + r) * CE; };
   l_run += __shfl_xor(l_run, 16);
   l_run += __shfl_xor(l_run, 32);
   if (g4 == 0) stats[wave][l16] = make_float2(m_run, l_run);
@@ -440,7 +468,8 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int i = 0; i < CE; i += 4)
-        *reinterpret_cast<f32x4*>(a.part_o + part * DP + (4 * g4 + r) * CE + i) = f32x4{acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+        if ((4 * g4 + r) * CE < a.c.d)
+          *reinterpret_cast<any_f32x4*>(a.part_o + part * DP + first_col(r) + i) = any_f32x4{acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
     return;
   }
   if (a.lse != nullptr && g4 == 0) a.lse[(int64_t)b * a.H + head] = m_all + __builtin_amdgcn_logf(l_all);
@@ -449,8 +478,8 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, TILES)) page
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int i = 0; i < CE; ++i) {
-      const int col = (4 * g4 + r) * CE + i;
-      if (col < a.c.d) store_from_f32<QDT>(a.out, b * a.so_z + head * a.so_h + col, acc[i][r] * inv);
+      const int col = first_col(r) + i;
+      if ((4 * g4 + r) * CE < a.c.d && col < a.c.d) store_from_f32<QDT>(a.out, b * a.so_z + head * a.so_h + col, acc[i][r] * inv);
     }
 }
 
@@ -560,7 +589,7 @@ __global__ void __launch_bounds__(256) paged_attention_finish(PagedAttnArgs a, i
 
 struct PagedPlan {
   int rows, groups, share, splits, dp, cap_pad;
-  bool tiles;
+  int mode;
   size_t o_bytes, ml_bytes, score_bytes, lse_bytes;
   size_t total() const { return o_bytes + ml_bytes + score_bytes + lse_bytes; }
 };
@@ -602,9 +631,10 @@ static PagedPlan paged_plan(const Paged& c, int cache_dtype, int64_t B, int64_t 
   const int G = (int)(H / c.heads);
   p.rows = G < 16 ? G : 16, p.groups = (G + 15) / 16;
   p.dp = c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
-  p.tiles = paged_in_tiles(c, (int)dtype_size(cache_dtype));
+  const int es = (int)dtype_size(cache_dtype);
+  p.mode = paged_in_tiles(c, es) ? kTiles : c.d * es % 16 == 0 && c.d % (p.dp / 16) == 0 ? kWholeRows : kOddRows;
   const int64_t items = B * c.heads * p.groups;
-  p.share = paged_share(items, c.capacity(), paged_occupancy(cache_dtype, p.dp, p.tiles), 2 * (int64_t)c.d * (int64_t)dtype_size(cache_dtype));
+  p.share = paged_share(items, c.capacity(), paged_occupancy(cache_dtype, p.dp, p.mode), 2 * (int64_t)c.d * es);
   p.splits = (c.capacity() + p.share - 1) / p.share;
   if (p.splits > 1) {
     p.o_bytes = granules((size_t)items * p.splits * p.rows * p.dp * 4);
@@ -619,10 +649,11 @@ static PagedPlan paged_plan(const Paged& c, int cache_dtype, int64_t B, int64_t 
 }
 
 template <int CDT, int QDT, int DP>
-static int launch_paged(const PagedAttnArgs& a, bool tiles, float* weights, int64_t sw_b, int64_t sw_h, hipStream_t s) {
+static int launch_paged(const PagedAttnArgs& a, int mode, float* weights, int64_t sw_b, int64_t sw_h, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.B * a.c.heads * a.groups * a.splits)), block(kPagedWaves * 64);
-  if (tiles) LH_LAUNCH((paged_attention_kernel<CDT, QDT, DP, kPagedWaves, true>), grid, block, 0, s, a);
-  else LH_LAUNCH((paged_attention_kernel<CDT, QDT, DP, kPagedWaves, false>), grid, block, 0, s, a);
+  if (mode == kTiles) LH_LAUNCH((paged_attention_kernel<CDT, QDT, DP, kPagedWaves, kTiles>), grid, block, 0, s, a);
+  else if (mode == kWholeRows) LH_LAUNCH((paged_attention_kernel<CDT, QDT, DP, kPagedWaves, kWholeRows>), grid, block, 0, s, a);
+  else LH_LAUNCH((paged_attention_kernel<CDT, QDT, DP, kPagedWaves, kOddRows>), grid, block, 0, s, a);
   if (const int rc = check_launch("paged_attention")) return rc;
   const int joins = a.splits > 1 ? a.B * a.H : 0;
   const unsigned blocks = joins + (weights ? (unsigned)((a.c.capacity() + 255) / 256 * (int64_t)a.B * a.c.heads) : 0u);
@@ -632,10 +663,10 @@ static int launch_paged(const PagedAttnArgs& a, bool tiles, float* weights, int6
 }
 
 template <int CDT, int QDT>
-static int launch_paged_dp(const PagedAttnArgs& a, int dp, bool tiles, float* w, int64_t sw_b, int64_t sw_h, hipStream_t s) {
-  if (dp == 64) return launch_paged<CDT, QDT, 64>(a, tiles, w, sw_b, sw_h, s);
-  if (dp == 128) return launch_paged<CDT, QDT, 128>(a, tiles, w, sw_b, sw_h, s);
-  return launch_paged<CDT, QDT, 256>(a, tiles, w, sw_b, sw_h, s);
+static int launch_paged_dp(const PagedAttnArgs& a, int dp, int mode, float* w, int64_t sw_b, int64_t sw_h, hipStream_t s) {
+  if (dp == 64) return launch_paged<CDT, QDT, 64>(a, mode, w, sw_b, sw_h, s);
+  if (dp == 128) return launch_paged<CDT, QDT, 128>(a, mode, w, sw_b, sw_h, s);
+  return launch_paged<CDT, QDT, 256>(a, mode, w, sw_b, sw_h, s);
 }
 
 }  // namespace lh
@@ -677,14 +708,13 @@ int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q
   if (p.splits > 1) a.part_o = reinterpret_cast<float*>(ws), a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
   if (weights) a.scores = reinterpret_cast<float*>(ws + p.o_bytes + p.ml_bytes), a.lse = reinterpret_cast<float*>(ws + p.o_bytes + p.ml_bytes + p.score_bytes);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const bool tiles = p.tiles;
   const int64_t sb = weights_stride_b, sh = weights_stride_h;
   if (cache->dtype == LH_F8E4M3)
-    return dtype == LH_BF16 ? launch_paged_dp<LH_F8E4M3, LH_BF16>(a, p.dp, tiles, weights, sb, sh, s)
-                            : launch_paged_dp<LH_F8E4M3, LH_F16>(a, p.dp, tiles, weights, sb, sh, s);
-  if (dtype == LH_BF16) return launch_paged_dp<LH_BF16, LH_BF16>(a, p.dp, tiles, weights, sb, sh, s);
-  if (dtype == LH_F16) return launch_paged_dp<LH_F16, LH_F16>(a, p.dp, tiles, weights, sb, sh, s);
-  return launch_paged_dp<LH_F32, LH_F32>(a, p.dp, tiles, weights, sb, sh, s);
+    return dtype == LH_BF16 ? launch_paged_dp<LH_F8E4M3, LH_BF16>(a, p.dp, p.mode, weights, sb, sh, s)
+                            : launch_paged_dp<LH_F8E4M3, LH_F16>(a, p.dp, p.mode, weights, sb, sh, s);
+  if (dtype == LH_BF16) return launch_paged_dp<LH_BF16, LH_BF16>(a, p.dp, p.mode, weights, sb, sh, s);
+  if (dtype == LH_F16) return launch_paged_dp<LH_F16, LH_F16>(a, p.dp, p.mode, weights, sb, sh, s);
+  return launch_paged_dp<LH_F32, LH_F32>(a, p.dp, p.mode, weights, sb, sh, s);
 }
 
 }  // extern "C"

@@ -63,6 +63,16 @@ def test_odd_head_dimensions_and_row_strides(dtype, d, pad):
     check(q, c, ops.paged_attention(q, c.k_cache, c.v_cache, c.table, c.device_lengths, k_scale=c.k_scale, v_scale=c.v_scale))
 
 
+@pytest.mark.parametrize("dtype,d,pad", [(bf16, 33, 0), (f16, 181, 2), (f32, 101, 0), (e4m3, 136, 0), (e4m3, 250, 1), (bf16, 9, 0), (f32, 5, 3), (e4m3, 17, 0)])
+def test_odd_rows_of_long_caches(dtype, d, pad):
+    """Rows that are no whole pieces, in several shares, with weights."""
+    c = ref.Cache([3100, 17, 0, 1025], 2, 16, d, dtype, seed=d, pad=pad)
+    q = torch.randn(4, 6, d, generator=torch.Generator().manual_seed(4)).to(bf16 if dtype == e4m3 else dtype).cuda()
+    weights = torch.rand(4, 2, c.capacity, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4))
+    before = weights.clone()
+    check(q, c, ops.paged_attention(q, c.k_cache, c.v_cache, c.table, c.device_lengths, weights=weights), weights=weights, before=before)
+
+
 @pytest.mark.parametrize("q_dtype", [bf16, f16])
 @pytest.mark.parametrize("d", [32, 64, 96, 128, 256])
 def test_cache_of_8_bits(q_dtype, d):
