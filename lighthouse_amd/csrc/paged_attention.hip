@@ -17,10 +17,10 @@
 //    each leaving (maximum, sum, sum of p v), which a second launch joins.
 //  * The table is read two steps ahead by the scalar unit, so that no step waits for a lookup or drains the loads on the way.
 //
-// Measured, keys and values out of memory: 16 sequences of 8192 to 32768 in bf16, 8 heads of 128 with 4 queries each, 255 us (5.2 TB/s) and 5 for
-// the join; 64 sequences of 256 to 1024, 12 heads of 64, 29 us (4.3 TB/s); 32 sequences of 2048 to 8192 in e4m3, 4 heads of 128 with 8 queries
-// each, 38 us (4.4 TB/s) and 5.  Out of the caches the same take 131, 20 and 31: the longer ones are bound by memory, and by what one CU draws of it
-// (31 B/ns) where the sequences' lengths do not fill all CUs to the end.  One sequence of 1000, 12 heads of 64: 5.3 us and 3.2, the chain of table, keys, values
+// Measured, keys and values out of memory: 16 sequences of 8192 to 32768 in bf16, 8 heads of 128 with 4 queries each, 254 us (5.2 TB/s) and 5 for
+// the join; 64 sequences of 256 to 1024, 12 heads of 64, 28 us (4.4 TB/s); 32 sequences of 2048 to 8192 in e4m3, 4 heads of 128 with 8 queries
+// each, 37 us (4.5 TB/s) and 5.  Out of the caches the same take 131, 20 and 31: the longer ones are bound by memory, and by what one CU draws of it
+// (31 B/ns) where the sequences' lengths do not fill all CUs to the end.  One sequence of 1000, 12 heads of 64: 5.1 us and 3.3, the chain of table, keys, values
 // and join.
 //
 // 16-bit types: P is split into a value of the type and the value of the type nearest to what that leaves, two matrix
@@ -609,7 +609,7 @@ static bool paged_in_tiles(const Paged& c, int es) {
 
 // How many positions a workgroup takes of a sequence; `items` (sequence, head, group of queries), `per_cu` workgroups that a CU
 // holds at once, `row_bytes` of a position's key and value.  There are to be two workgroups per CU (one, if no more fit; one also where the
-// shares would be shorter than 1024 positions, of which their start and end take too much).  (One sequence of 1000, 12 heads of 64: 7.9 us with 128
+// shares would be shorter than 1024 positions, of which their start and end take too much).  (One sequence of 1000, 12 heads of 64: 7.6 us with 128
 // positions a share, 9.8 in one; one of 32768, 8 heads of 128: 31.8 with 1024, 33.5 with 512, 362 in one; 4 of 1024 to 4096, 8 heads of 128 with 4 queries: 14.8 with
 // 512, 15.8 with 256; heads of 256, 16 sequences of 1024 to 4096: 73 with 2048, 94 with 512.)  With items enough for that, up to 8 per CU
 // even out sequences of unlike length, while a share has 512 KB of keys and values, which the join's launch costs nothing against.  (16
