@@ -415,7 +415,7 @@ int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, 
  * stride along d), H a multiple of n_kv_heads, head h reads key / value head h / (H / n_kv_heads):
  *   out[b, h] = sum_t p_t v_t,  p = softmax over t < lengths[b] of scale q . k_t  (an infinite v_t may give a NaN),
  * positions on pages that hold nothing left out; 0 where nothing is left.  `lengths` counts the new token if it has been
- * appended and is clamped to 0 .. max_pages * page_size.  Scores, softmax and sums are f32.  dtype (of q and out) is the
+ * appended and is clamped to 0 .. max_pages * page_size.  Scores, softmax and sums are f32 (with queries of f16, p_t in front of v_t has 22 places).  dtype (of q and out) is the
  * cache's, or BF16 or F16 for a cache of e4m3.  With `weights` ([B, n_kv_heads, >= max_pages * page_size] f32, element strides
  * weights_stride_b, weights_stride_h), weights[b, g, t] grows by the sum of p_t over the H / n_kv_heads heads of group g.
  * B H < 2^20, and with weights B n_kv_heads ceil(max_pages * page_size / 256) < 2^23.

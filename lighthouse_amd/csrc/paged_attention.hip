@@ -23,10 +23,11 @@
 // (31 B/ns) where the sequences' lengths do not fill all CUs to the end.  One sequence of 1000, 12 heads of 64: 5.1 us and 3.3, the chain of table, keys, values
 // and join.
 //
-// 16-bit types: P is split into a value of the type and the value of the type nearest to what that leaves, two matrix
-// instructions instead of one (they cost nothing here): P alone rounded once to bf16 would add an error as large as the
-// rounding of the result.  f32 runs on v_mfma_f32_16x16x4_f32 with one 16-key tile a step.  e4m3 codes are converted to the queries' type, in
-// which every code has an exact value.
+// 16-bit types: P is split into values of the type, each nearest to what the ones before leave: three of bf16 have all 24 places of an f32, two of
+// f16 have 22, and there is a matrix instruction for each.  (Where values cancel, what P has lost shows in the result: with two of bf16,
+// 2^-18 of the largest values.  The third costs long caches less than 1 %, 8 sequences of 256 to 1024, 16 heads of 64, 12.0 us instead of 11.7.)
+// f32 runs on v_mfma_f32_16x16x4_f32 with one 16-key tile a step.  e4m3 codes are converted to the queries' type, in which every code has
+// an exact value.
 #include "paged.h"
 
 namespace lh {
@@ -151,6 +152,7 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE)) paged
   constexpr int VB = CE * ES;
   constexpr int VP = VB > 16 ? VB / 16 : 1;    // loads for them
   constexpr int VPB = VB / VP;
+  constexpr int PARTS = QDT == LH_BF16 ? 3 : 2;  // 16-bit values that a probability is the sum of
   constexpr int kOutside = 0x40000000;         // an offset behind every buffer
   // Rows that are no whole pieces (and longer than one): the last piece moves back to end with the row.  Of a key and a query it gives only the
   // columns that the piece before has not; columns of a value may come from two lanes, which are of one mind.  (By element, 16 sequences of
@@ -403,11 +405,15 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE)) paged
         for (int i = 0; i < CE; ++i)
           acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[j][i]), p[j], acc[i], 0, 0, 0);
     } else {
-      u32x4 hi, lo;
+      u32x4 part[PARTS];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        hi[e] = pack2<QDT>(p[2 * e], p[2 * e + 1]);
-        lo[e] = pack2<QDT>(p[2 * e] - unpack_lo<QDT>(hi[e]), p[2 * e + 1] - unpack_hi<QDT>(hi[e]));
+        float p0 = p[2 * e], p1 = p[2 * e + 1];
+#pragma unroll
+        for (int n = 0; n < PARTS; ++n) {
+          part[n][e] = pack2<QDT>(p0, p1);
+          p0 -= unpack_lo<QDT>(part[n][e]), p1 -= unpack_hi<QDT>(part[n][e]);
+        }
       }
       uint32_t vw[8][CE / 2];  // [key][pair of columns]
 #pragma unroll
@@ -425,10 +431,11 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE)) paged
           even[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e], vw[2 * j][e], 0x05040100u);
           odd[j] = __builtin_amdgcn_perm(vw[2 * j + 1][e], vw[2 * j][e], 0x07060302u);
         }
-        acc[2 * e] = paged_mma<QDT>(even, hi, acc[2 * e]);
-        acc[2 * e + 1] = paged_mma<QDT>(odd, hi, acc[2 * e + 1]);
-        acc[2 * e] = paged_mma<QDT>(even, lo, acc[2 * e]);
-        acc[2 * e + 1] = paged_mma<QDT>(odd, lo, acc[2 * e + 1]);
+#pragma unroll
+        for (int n = 0; n < PARTS; ++n) {
+          acc[2 * e] = paged_mma<QDT>(even, part[n], acc[2 * e]);
+          acc[2 * e + 1] = paged_mma<QDT>(odd, part[n], acc[2 * e + 1]);
+        }
       }
     }
     if (next < steps) request_values(next);

@@ -219,3 +219,29 @@ def test_the_same_call_gives_the_same_bits_with_any_workspace():
     with pytest.raises(ValueError, match="workspace"):
         ops.paged_attention(q, c.k_cache, c.v_cache, c.table, c.device_lengths, weights=weights,
                             workspace=torch.empty(need + 256, dtype=torch.uint8, device="cuda")[16:])
+
+
+@pytest.mark.parametrize("dtype", [bf16, f16, e4m3])
+def test_probabilities_keep_the_places_of_f32(dtype):
+    """Two values of +-256 whose probabilities differ by 2^-12 of themselves: what is left of their difference shows every place that a
+    probability has lost on its way into the second product."""
+    d, B, G = 64, 32, 16
+    q_dtype = bf16 if dtype == e4m3 else dtype
+    a = (1.0 + torch.arange(B * G) / 512.0).to(q_dtype).view(B, G)  # scores of -a and -a - 2^-12 beside one of 0
+    q = torch.zeros(B, G, d, dtype=q_dtype)
+    q[:, :, 0], q[:, :, 1] = a, 2.0**-12
+    k, v = torch.zeros(1, 1, 16, d), torch.zeros(1, 1, 16, d)
+    k[0, 0, 1:3, 0], k[0, 0, 2, 1] = -1.0, -1.0
+    v[0, 0, 1], v[0, 0, 2] = 256.0, -256.0
+    table = torch.zeros(B, 1, dtype=torch.int32).cuda()
+    out = ops.paged_attention(q.cuda(), k.to(dtype).cuda(), v.to(dtype).cuda(), table, torch.full((B,), 3, dtype=torch.int32).cuda(), scale=1.0)
+    s = a.double()
+    p = torch.exp(-s)
+    want = 256.0 * p * -math.expm1(-(2.0**-12)) / (1.0 + p + p * math.exp(-(2.0**-12)))
+    # Scores are exact.  Times log2(e) in f32: 2^-25 of the factor and half a step of the product, both times ln 2 |x| <= 2: 2^-24 + 2^-24;
+    # exp2 and the sum a step of 2^-23 each: 6 steps of 2^-24 for each probability.  The second product: six terms of at most 256 p
+    # added in f32, 6 more; the quotient 2, relative to what is small.
+    share = 256.0 * p / (1.0 + 2.0 * p)
+    half = torch.finfo(q_dtype).eps / 2
+    off = (out.cpu().double() - want[:, :, None]).abs()
+    assert (off <= (half * want + share * (2 * 6 + 6) * 2.0**-24)[:, :, None]).all(), float(off.max())
