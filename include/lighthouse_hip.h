@@ -444,7 +444,8 @@ int lh_hip_kv_evict(const lh_paged_cache* cache, float* weights, int64_t weights
 
 /*
  * The next token of every row of logits [B, V] (dtype F32, BF16 or F16, row stride ld): with w_i = exp((x_i - max x) / T)
- * in 64 bits and the words in falling order of x (equal ones: lowest index first), the first top_k words stay; of those the shortest
+ * in 64 bits (to 6e-12; sums of them to 2^-33 of the whole, V 2^-59 in rows of more than 2^26 words) and the words in falling order of x
+ * (equal ones: lowest index first), the first top_k words stay; of those the shortest
  * beginning that holds top_p of their mass (a word stays while the mass before it is below); of those the ones with
  * w_i >= min_p.  The first always stays.  tokens[b] is the lowest index whose running sum of w over the words that
  * stayed, in the order of the indices, exceeds u = uniform[b] times their sum (u below 0 counts as 0, u at or above 1, or NaN,

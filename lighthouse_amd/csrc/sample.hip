@@ -4,15 +4,19 @@
 // that order: the first k; the words before which less than top_p of the mass lies; the words with w >= min_p.  So what stays
 // is described by its last word, and no row is ever sorted.  The draw is a search in the running sum over the indices.
 //
-// Masses are whole numbers, w in units of 2^-bits with w from a 64-bit exponential: sums of them are exact in any order, so
-// neither atomics nor the split over lanes and waves can change a token, and a sum over 131072 words is off by about 1e-12
-// of the whole: as good as a sum in 64-bit floating point.  (In 32 bits a row of 5000 likely words would get another token about
-// once in 10^4 rows.)
+// Masses are whole numbers, w in units of 2^-bits with w from a 64-bit exponential (to 6e-12 of itself): sums of them are exact in any
+// order, so neither atomics nor the split over lanes and waves can change a token.  (In 32 bits a row of 5000 likely words would get another
+// token about once in 10^4 rows.)  What a word has beside whole units is lost, and a row may hold one likely word and unlikely ones
+// without end, so the units follow from the sums: 2^-49 of the largest weight for up to 8192 words, which lose half a unit each, 2^-36 of the
+// whole at most; the same for each chunk of a longer row, and for the row that its chunks make up, units by their sum.  Where one
+// workgroup takes a row of several chunks they are 2^-51, or what the sum leaves room for, and V words lose V 2^-52; in rows without
+// chunks down to 2^-60, cut off instead of rounded, and V words lose V 2^-59.  (With units by V alone, such that V likely words fit,
+// 131072 unlikely ones lost 2^-28, 2^24 of them 2^-15.)
 //
 // A row of more than 8192 words is digested first, 8192 words a workgroup: for top-k (up to 512) a chunk lists its own largest words, otherwise
 // it adds up its masses, in units of a power of two near its largest word's, and, where a filter will ask for it, by sixteenths of an octave
-// of w below it.  Whole powers and a grid that starts at them let another workgroup put the chunks of a row together
-// exactly.  That one then has the candidates of top-k to sort, or finds in the sums the bin that the last word lies in, collects the words
+// of w below it.  Whole powers and a grid that starts at them let another workgroup put the chunks of a row together,
+// what falls below its units aside.  That one then has the candidates of top-k to sort, or finds in the sums the bin that the last word lies in, collects the words
 // of that bin from the chunks that have any, and evaluates one chunk, the one that the draw falls into.
 //
 // Rows of one chunk, and what a digest does not settle (top-k above 512, thousands of words in the bin of the cut, infinite logits), take
@@ -31,16 +35,16 @@ namespace lh {
 
 constexpr int kChunkWords = 8192, kChunkBins = 512, kChunkList = 1024, kChunks = 64;  // words of a chunk, ..., most chunks of a row
 constexpr int kDigestThreads = 512;
+constexpr int kChunkBits = 49;  // of a mass behind the point: a chunk's words of weight 1 add up to 2^62
 
 enum SampleMode {  // what a chunk holds: the same for all of a row
-  kDigestNone = 0,    // nothing
   kDigestTop = 1,     // its largest word
   kDigestList = 2,    // its largest words, top_k of them or more, or all
-  kDigestTotal = 3,   // its mass
+  kDigestTotal = 3,   // its mass (all that is known of a row with a larger top_k)
   kDigestBins = 4     // and by bins
 };
 struct SampleChunk {
-  double power;               // masses are in units of 2^(power - bits); bins count sixteenths of an octave down from 2^power
+  double power;               // masses are in units of 2^(power - kChunkBits); bins count sixteenths of an octave down from 2^power
   unsigned long long total;
   float top;                  // -inf: no words
   int32_t top_i;
@@ -58,7 +62,6 @@ struct SampleArgs {
   const float* uniform;
   int64_t ld;
   int32_t V;
-  int32_t bits;  // of a mass behind the point: V words of weight 1 stay below 2^62
   lh_sample_opts o;
   SampleChunk* chunks;  // [B][n_chunks], or null
   int32_t n_chunks;
@@ -152,14 +155,14 @@ __device__ __forceinline__ uint64_t part_of(uint64_t all, float f, bool up) {
   return whole + (up && rest != 0);
 }
 
-// w of a word of a chunk, in the units that the chunk counts in: sixteenths of an octave above 2^(power - bits), t = 16 (x c - power + bits).
+// w of a word of a chunk, in the units that the chunk counts in: sixteenths of an octave above 2^(power - bits), t = 16 (x c - power + bits), bits = kChunkBits.
 // With n the nearest whole number and f the rest, 2^(t / 16) = 2^(n / 16) 2^(f / 16): a table of sixteenths, and 1 + f p(f) with p of degree 3
 // through the values at the Chebyshev nodes (relative error 5.1e-12).  x c - power is rounded once, so words of all chunks keep
 // their ratios; what is no word (-inf) comes out as 0 and in the last bin.
 struct ChunkScale {
   double c16, offset;
-  int top;  // n of the power itself
-  __device__ __forceinline__ ChunkScale(double c, double power, int bits) : c16(16.0 * c), offset(16.0 * ((double)bits - power)), top(16 * bits) {}
+  static constexpr int top = 16 * kChunkBits;  // n of the power itself
+  __device__ __forceinline__ ChunkScale(double c, double power) : c16(16.0 * c), offset(16.0 * ((double)kChunkBits - power)) {}
   __device__ __forceinline__ double split(float x, int* n) const {
     const double t = fmax(__builtin_fma((double)x, c16, offset), -32768.0), whole = __builtin_rint(t);
     *n = (int)whole;
@@ -210,28 +213,29 @@ struct SampleShared {
   int32_t cut_i;
   unsigned long long above;
   double chunk_power[kChunks], sixteenths[16];
-  int32_t chunk_shift[kChunks];
+  int32_t chunk_down[kChunks];
   unsigned long long chunk_kept[kChunks];
   uint32_t wave_chunk[kChunks];
 };
 
-template <int DT>
+enum RowKind { kRowOfOne, kRowOfChunks, kRowLong };  // one chunk or less: fixed units; up to kChunks of them; without a digest
+template <int DT, RowKind KIND>
 struct Sampler {
-  static constexpr int E = SampleRow<DT>::E;
+  static constexpr int E = SampleRow<DT>::E, kMostBits = KIND == kRowLong ? 60 : 51;
   SampleShared& s;
   SampleRow<DT> row;
   int tid, lane, wave;
   float top;       // the largest logit
   double c;        // log2(e) / T
   double inv_t;
-  int bits;
+  int row_bits;    // of a mass behind the point, unless kRowOfOne
   float cut_x;     // words below (cut_x, cut_i) have been dropped
   int32_t cut_i;
 
-  // 2^(t + shift): n + f = t with |f| <= 1/2, 2^f = 1 + f p(f) with p of degree 7 through the values at the
+  // 2^t = 2^n 2^f: n + f = t with |f| <= 1/2, 2^f = 1 + f p(f) with p of degree 7 through the values at the
   // Chebyshev nodes of the interval (relative error 2.2e-12, at top exactly 1).
-  __device__ __forceinline__ static double power(double t, int shift) {
-    const double n = __builtin_rint(t), f = t - n;
+  __device__ __forceinline__ static double fraction(double t, int* n) {
+    const double whole = __builtin_rint(t), f = t - whole;
     double p = 1.325080551750225e-06;
     p = __builtin_fma(p, f, 1.5303700711365693e-05);
     p = __builtin_fma(p, f, 0.00015403475186530786);
@@ -241,14 +245,54 @@ struct Sampler {
     p = __builtin_fma(p, f, 0.24022650695888503);
     p = __builtin_fma(p, f, 0.6931471805568324);
     p = __builtin_fma(p, f, 1.0);
-    return __builtin_ldexp(p, (int)fmax(n, -2000.0) + shift);
+    *n = (int)fmax(whole, -2000.0);
+    return p;
   }
-  __device__ __forceinline__ double weight(float x) const { return x == top ? 1.0 : power(((double)x - (double)top) * c, 0); }
+  __device__ __forceinline__ double weight(float x) const {
+    int n;
+    const double p = fraction(((double)x - (double)top) * c, &n);
+    return x == top ? 1.0 : __builtin_ldexp(p, n);
+  }
   __device__ __forceinline__ uint64_t mass(float x) const {
-    const uint64_t m = ChunkScale::whole_of(power(((double)x - (double)top) * c, bits));
+    int n;
+    const double p = fraction(((double)x - (double)top) * c, &n);
+    // (Of what is no word, or stands beside infinite ones, t may be -inf or a NaN: it has no mass whatever comes out.)
+    uint64_t m;
+    const int bits = KIND == kRowOfOne ? kChunkBits : row_bits;
+    if constexpr (KIND == kRowLong) m = ChunkScale::whole_of(p * 0x1p51) << 9 >> min(60 - n - bits, 63);  // (up to 2^60, rounded down)
+    else m = ChunkScale::whole_of(__builtin_ldexp(p, n + bits));
     return x == top ? 1ull << bits : x > -INFINITY ? m : 0;
   }
-  __device__ __forceinline__ static uint64_t whole(double w) { return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & ((1ull << 52) - 1); }
+  // So many bits that the masses of all words add up to at most 2^61: up to 60, or 51 where a mass comes out of the lower bits of a
+  // double (with 64-bit shifts 128 rows of 131072 words, top-k 3000, took 243 us instead of 216).  The sum of all w, in the same order in
+  // every run, decides it, in 32 bits: an eighth is added for what 2^20 additions in a lane lose (2^20 steps of 2^-24) and for the exponentials.
+  __device__ __forceinline__ int bits_of_row() {
+    float sum = 0.0f;
+    row.each([&](const float* x, int) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += x[e] == top ? 1.0f : x[e] > -INFINITY ? __builtin_amdgcn_exp2f((float)(((double)x[e] - (double)top) * c)) : 0.0f;
+    });
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    __syncthreads();
+    if (lane == 0) s.wave_hi[wave] = sum;
+    __syncthreads();
+    sum = 0.0f;
+    for (int w = 0; w < kSampleWaves; ++w) sum += s.wave_hi[w];
+    __syncthreads();
+    return min(61 - __builtin_amdgcn_frexp_expf(1.125f * sum), kMostBits);
+  }
+  // The same from the chunks' masses, if they all have one; otherwise 0.  (Relative to the whole octave below the largest word: up to
+  // twice the sum.)
+  __device__ __forceinline__ int bits_of_chunks(const SampleChunk* chunks, int n_chunks, int mode) const {
+    const SampleChunk& mine = chunks[min(lane, n_chunks - 1)];
+    const bool own = lane < n_chunks;
+    if (mode == kDigestList || __any(own && mine.listed < 0)) return 0;
+    double sum = own && mine.total != 0 ? __builtin_ldexp((double)mine.total, (int)fmax(mine.power - floor((double)top * c), -2000.0) - kChunkBits) : 0.0;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    return min(61 - __builtin_amdgcn_frexp_exp(sum), kMostBits);
+  }
   __device__ __forceinline__ bool stays(float x, int i) const { return x > cut_x || (x == cut_x && i <= cut_i); }
   __device__ __forceinline__ static unsigned long long entry(float x, int i) { return (unsigned long long)order_of(x) << 32 | (uint32_t)~i; }
   __device__ __forceinline__ static float entry_x(unsigned long long e) { return of_order((uint32_t)(e >> 32)); }
@@ -474,19 +518,25 @@ struct Sampler {
       return on_list(n, (int)top_k >= n, top_k, top_p, least, u, 0, token);
     }
 
-    // Every wave has the chunks in its lanes: the row's unit is that of the largest power.
+    // Every wave has the chunks in its lanes.  The row counts octaves from the largest power down, and masses in units in which all
+    // of it comes to between 2^60 and 2^61, by `units` octaves above those of the chunk with the largest power.
     const bool words = lane < n_chunks && mine.total != 0;
     const double own_power = words ? mine.power : -INFINITY;
     double power_of_row = own_power;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) power_of_row = fmax(power_of_row, __shfl_xor(power_of_row, o));
     fill_sixteenths(s.sixteenths);
-    const int shift = words ? (int)fmin(power_of_row - own_power, 63.0) : 63;
+    const int down = words ? (int)fmin(power_of_row - own_power, 80.0) : 80;  // (of what lies 80 octaves below, nothing is left)
     const uint64_t total = words ? mine.total : 0;
-    if (wave == 0) s.chunk_power[lane] = mine.power, s.chunk_shift[lane] = shift, s.chunk_kept[lane] = total;
+    double sum_of_row = __builtin_ldexp((double)total, -down);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum_of_row += __shfl_xor(sum_of_row, o);
+    const int units = __builtin_amdgcn_frexp_exp(sum_of_row) - 61;  // -12 to 8
+    auto to_row = [&](uint64_t m, int down) { return down + units >= 0 ? m >> min(down + units, 63) : m << -(down + units); };
+    if (wave == 0) s.chunk_power[lane] = mine.power, s.chunk_down[lane] = down, s.chunk_kept[lane] = total;
     int last = kChunkBins;                   // words of bins before it stay, and those of it down to the cut
     if (mode == kDigestBins) {
-      const uint64_t all = wave_total(total >> shift);
+      const uint64_t all = wave_total(to_row(total, down));
       const uint64_t goal = top_p < 1.0f ? top_goal(top_p, all) : ~0ull;
       // The row's bins: a wave adds those of a chunk.
       if (tid < kChunkBins) s.mass[tid] = 0;
@@ -497,13 +547,13 @@ struct Sampler {
         for (int i = 0; i < kChunkBins / 64; ++i) early[i] = chunks[k].bins[64 * i + lane];
       };
       for (int k = wave; k < n_chunks; k += kSampleWaves) {
-        const int down = s.chunk_shift[k];
+        const int octaves = s.chunk_down[k];
         if (s.chunk_kept[k] == 0) continue;
         if (k != wave) fetch(k);  // (those are there already)
 #pragma unroll
         for (int i = 0; i < kChunkBins / 64; ++i) {
           const int at = 64 * i + lane;  // (the last one is not in use)
-          if (at < kChunkBins - 1 && at + 16 * down < kChunkBins - 1) atomicAdd(&s.mass[at + 16 * down], early[i] >> down);
+          if (at < kChunkBins - 1 && at + 16 * octaves < kChunkBins - 1) atomicAdd(&s.mass[at + 16 * octaves], (unsigned long long)to_row(early[i], octaves));
         }
       }
       __syncthreads();
@@ -516,13 +566,13 @@ struct Sampler {
       if (least > 0.0) {  // the bin of the least weight, but none before the largest word's, which stays (least may be above 1)
         const double t = power_of_row - ((double)top * c + log2(least));
         const int of_least = t <= 0.0 ? 0 : (int)fmin(__builtin_rint(16.0 * t), (double)(kChunkBins - 1));
-        last = min(last, max(of_least, ChunkScale(c, power_of_row, bits).bin(top)));
+        last = min(last, max(of_least, ChunkScale(c, power_of_row).bin(top)));
       }
       if (last == kChunkBins - 1) return false;
       if (tid == last) s.above = before;
       // What a chunk has in the bins before it, and which chunks have words of it.
       for (int k = wave; k < n_chunks; k += kSampleWaves) {
-        const int bins = s.chunk_kept[k] == 0 ? 0 : last - 16 * s.chunk_shift[k];
+        const int bins = s.chunk_kept[k] == 0 ? 0 : last - 16 * s.chunk_down[k];
         uint64_t m = 0;
         if (n_chunks > kSampleWaves) fetch(k);
 #pragma unroll
@@ -587,7 +637,7 @@ struct Sampler {
         if (tid + i * kSampleThreads < range) {
           const unsigned long long e = s.list[tid + i * kSampleThreads];
           const int k = entry_i(e) / kChunkWords;
-          if (ChunkScale(c, s.chunk_power[k], bits).bin(entry_x(e)) + 16 * s.chunk_shift[k] == last) member[i] = e;
+          if (ChunkScale(c, s.chunk_power[k]).bin(entry_x(e)) + 16 * s.chunk_down[k] == last) member[i] = e;
         }
       __syncthreads();
       if (tid == 0) s.listed = 0;
@@ -604,9 +654,9 @@ struct Sampler {
       const unsigned long long e0 = j0 < n ? s.list[j0] : 0, e1 = j1 < n ? s.list[j1] : 0;
       const int k0 = j0 < n ? entry_i(e0) / kChunkWords : 0, k1 = j1 < n ? entry_i(e1) / kChunkWords : 0;
       int bin;
-      const uint64_t m0 = j0 < n ? ChunkScale(c, s.chunk_power[k0], bits).mass(entry_x(e0), s.sixteenths, &bin) : 0;
-      const uint64_t m1 = j1 < n ? ChunkScale(c, s.chunk_power[k1], bits).mass(entry_x(e1), s.sixteenths, &bin) : 0;
-      const uint64_t r0 = m0 >> s.chunk_shift[k0], r1 = m1 >> s.chunk_shift[k1];
+      const uint64_t m0 = j0 < n ? ChunkScale(c, s.chunk_power[k0]).mass(entry_x(e0), s.sixteenths, &bin) : 0;
+      const uint64_t m1 = j1 < n ? ChunkScale(c, s.chunk_power[k1]).mass(entry_x(e1), s.sixteenths, &bin) : 0;
+      const uint64_t r0 = to_row(m0, s.chunk_down[k0]), r1 = to_row(m1, s.chunk_down[k1]);
       uint64_t of_list, kept;
       const uint64_t front = above + block_before(r0 + r1, &of_list);
       block_before((uint64_t)(j0 < n && front < goal && (weight(entry_x(e0)) >= least || entry_i(e0) == top_i)) +
@@ -618,22 +668,24 @@ struct Sampler {
     }
     __syncthreads();
     // The chunk that the draw falls into.
-    const uint64_t kept = lane < n_chunks ? s.chunk_kept[lane] : 0, units = kept >> shift;
-    const uint64_t run = wave_scan(units), all = wave_last(run);
+    const uint64_t kept = lane < n_chunks ? s.chunk_kept[lane] : 0, own_units = to_row(kept, down);
+    const uint64_t run = wave_scan(own_units), all = wave_last(run);
     if (all == 0) return false;  // (the largest word stays: this does not happen, and without it there would be no chunk to find)
     int k;
     uint64_t goal;
     if (u < 1.0f) {
       const uint64_t of_row = goal_of(u, all);
       k = __ffsll((unsigned long long)__ballot(of_row < run)) - 1;
-      goal = (of_row - __shfl((unsigned long long)(run - units), k)) << s.chunk_shift[k];
+      goal = of_row - __shfl((unsigned long long)(run - own_units), k);
+      const int by = s.chunk_down[k] + units;  // (below 62: the chunk has a unit of the row's)
+      goal = by >= 0 ? goal << by : goal >> -by;
     } else {
       k = 63 - __clzll((unsigned long long)__ballot(kept != 0));
       goal = s.chunk_kept[k] - 1;
     }
     k = __builtin_amdgcn_readfirstlane(k);
-    const ChunkScale scale(c, s.chunk_power[k], bits);
-    const int bin_shift = 16 * s.chunk_shift[k];
+    const ChunkScale scale(c, s.chunk_power[k]);
+    const int bin_shift = 16 * s.chunk_down[k];
     cut_x = s.cut_x, cut_i = s.cut_i;
     constexpr int EACH = kChunkWords / kSampleThreads;  // neighbouring words of a thread
     const int i0 = k * kChunkWords + tid * EACH;
@@ -821,7 +873,7 @@ struct Sampler {
 // A chunk's words in registers, and what the row's settings will ask of it.
 template <int DT>
 __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
-  typedef Sampler<DT> S;
+  typedef Sampler<DT, kRowOfChunks> S;
   constexpr int E = SampleRow<DT>::E, ES = DT == LH_F32 ? 4 : 2, PIECES = kChunkWords / (kDigestThreads * E), WAVES = kDigestThreads / 64;
   __shared__ unsigned long long bins[kChunkBins];
   __shared__ unsigned long long wave_mass[WAVES];
@@ -864,7 +916,7 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
   for (int w = 0; w < WAVES; ++w) top = fmaxf(top, wave_top[w]);
   int mode = kDigestTotal;
   if (!(temperature > 0.0f) || top_k == 1) mode = kDigestTop;
-  else if (top_k > 0 && top_k < a.V) mode = top_k <= kSampleTopK ? kDigestList : kDigestNone;
+  else if (top_k > 0 && top_k < a.V) mode = top_k <= kSampleTopK ? kDigestList : kDigestTotal;
   else if (top_p < 1.0f || min_p > 0.0f) mode = kDigestBins;
   int top_i = 0x7fffffff;
   if (mode == kDigestTop || min_p > 1.0f) {  // (otherwise nobody asks which it is)
@@ -880,7 +932,7 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
   const double c = 1.0 / (double)temperature * 1.4426950408889634, exponent = (double)top * c;
   const bool some = top > -INFINITY, words = some && fabs(exponent) <= 0x1p40;
   const double power = words ? ceil(exponent) : 0.0;
-  const ChunkScale scale(c, power, a.bits);
+  const ChunkScale scale(c, power);
   unsigned long long total = 0;
   int in_list = 0;
   if (words && mode == kDigestTotal) {
@@ -944,7 +996,7 @@ __global__ void __launch_bounds__(kDigestThreads) sample_digest(SampleArgs a) {
   }
 }
 
-template <int DT>
+template <int DT, RowKind KIND>
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   __shared__ SampleShared s;
   constexpr int E = SampleRow<DT>::E, ES = DT == LH_F32 ? 4 : 2;
@@ -962,7 +1014,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
 
   const double inv_t = 1.0 / (double)temperature;
   const double least = min_p > 0.0f ? (double)min_p : 0.0;
-  if (a.chunks != nullptr) {
+  int bits = 0;
+  if constexpr (KIND == kRowOfChunks) {
     const SampleChunk* chunks = a.chunks + (int64_t)b * a.n_chunks;
     const SampleChunk& mine = chunks[min(lane, a.n_chunks - 1)];
     unsigned long long early[kChunkBins / 64];  // (on the way before anything is known)
@@ -982,8 +1035,9 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
       if (tid == 0) a.tokens[b] = top == -INFINITY ? -1 : top_i;
       return;
     }
-    Sampler<DT> f = {s, row, tid, lane, wave, top, inv_t * 1.4426950408889634, inv_t, a.bits, -INFINITY, -1};
-    if (mode != kDigestNone && top < INFINITY && f.by_chunks(chunks, a.n_chunks, early, mode, top_i, (uint32_t)top_k, top_p, least, u, a.tokens + b)) return;
+    Sampler<DT, KIND> f = {s, row, tid, lane, wave, top, inv_t * 1.4426950408889634, inv_t, kChunkBits, -INFINITY, -1};
+    if ((top_k <= kSampleTopK || top_k >= a.V) && top < INFINITY && f.by_chunks(chunks, a.n_chunks, early, mode, top_i, (uint32_t)top_k, top_p, least, u, a.tokens + b)) return;
+    if (top < INFINITY) bits = f.bits_of_chunks(chunks, a.n_chunks, mode);
     __syncthreads();
   }
 
@@ -1022,7 +1076,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
     return;
   }
 
-  Sampler<DT> f = {s, row, tid, lane, wave, top, inv_t * 1.4426950408889634, inv_t, a.bits, -INFINITY, -1};
+  Sampler<DT, KIND> f = {s, row, tid, lane, wave, top, inv_t * 1.4426950408889634, inv_t, kChunkBits, -INFINITY, -1};
+  if (KIND != kRowOfOne) f.row_bits = bits > 0 ? bits : f.bits_of_row();
   const bool few = top_k > 0 && (uint32_t)top_k < words;
   if (top < INFINITY && (few ? top_k <= kSampleTopK : top_p < 1.0f || least > 0.0))
     if (f.by_list(mine, words, few ? top_k : 0, top_p, least, u, a.tokens + b)) return;
@@ -1101,7 +1156,9 @@ static int launch_sample(const SampleArgs& a, int64_t B, hipStream_t s) {
     LH_LAUNCH(sample_digest<DT>, dim3((unsigned)(B * a.n_chunks)), dim3(kDigestThreads), 0, s, a);
     if (const int rc = check_launch("sample_digest")) return rc;
   }
-  LH_LAUNCH(sample_kernel<DT>, dim3((unsigned)B), dim3(kSampleThreads), 0, s, a);
+  if (a.chunks) LH_LAUNCH((sample_kernel<DT, kRowOfChunks>), dim3((unsigned)B), dim3(kSampleThreads), 0, s, a);
+  else if (a.V <= kChunkWords) LH_LAUNCH((sample_kernel<DT, kRowOfOne>), dim3((unsigned)B), dim3(kSampleThreads), 0, s, a);
+  else LH_LAUNCH((sample_kernel<DT, kRowLong>), dim3((unsigned)B), dim3(kSampleThreads), 0, s, a);
   return check_launch("sample");
 }
 
@@ -1122,8 +1179,7 @@ int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int
   const size_t need = lh_hip_sample_workspace_bytes(B, V);
   LH_REQUIRE(need == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= need),
              "lh_hip_sample: workspace too small or not 256-byte aligned: %zu of %zu bytes", workspace_bytes, need);
-  SampleArgs a = {tokens, logits, uniform, ld, (int32_t)V, 50, *opts, need ? static_cast<SampleChunk*>(workspace) : nullptr, sample_chunks(V), 0};
-  while ((V >> (62 - a.bits)) != 0) --a.bits;
+  SampleArgs a = {tokens, logits, uniform, ld, (int32_t)V, *opts, need ? static_cast<SampleChunk*>(workspace) : nullptr, sample_chunks(V), 0};
   a.may_bin = (opts->top_k || opts->top_k_all <= 0 || opts->top_k_all >= V) && (opts->top_p || opts->min_p || opts->top_p_all < 1.0f || opts->min_p_all > 0.0f);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == LH_F32) return launch_sample<LH_F32>(a, B, s);

@@ -742,8 +742,8 @@ def kv_evict_workspace_bytes(k_cache, block_table, budget) -> int:
 def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, workspace=None):
     """The next token of every row of logits [B, V] (float32, bfloat16 or float16, rows of any stride): int64 [B].
 
-    With w = exp((x - max) / temperature) in 64 bits and the words in falling order of x (equal ones: lowest index first): the first
-    top_k words stay, of those the shortest beginning with at least top_p of their mass, of those the ones with w >= min_p;
+    With w = exp((x - max) / temperature) in 64 bits (to 6e-12; sums of them to 2^-33 of the whole) and the words in falling order of x
+    (equal ones: lowest index first): the first top_k words stay, of those the shortest beginning with at least top_p of their mass, of those the ones with w >= min_p;
     the first always does.  The token is the lowest index whose running sum of w over what stayed, by index, exceeds uniform[b] (float32
     [B], in [0, 1)) times their sum.  temperature <= 0: the largest logit.  top_k <= 0, top_p >= 1 and min_p <= 0 keep everything.
     NaN and -inf are no words, a +inf leaves only those, a row without words gives -1.

@@ -182,3 +182,39 @@ def test_workspace_of_the_caller():
     assert torch.equal(ops.sample(x, u, top_p=0.9, workspace=ws), ops.sample(x, u, top_p=0.9))
     with pytest.raises(ValueError, match="workspace"):
         ops.sample(x, u, workspace=ws[: need - 256])
+
+
+@pytest.mark.parametrize("V", [8192, 20011, 131072, 524288, 2**20, 2**24])
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_a_likely_word_and_a_long_tail_of_unlikely_ones(V, dtype):
+    """One word of weight 1 at the end, all others 2^-40 to 2^-52 of it: their sum is small, but not lost, and a draw below it falls on
+    the one that it says, to what the units lose."""
+    # Units of 2^-49 of a chunk's largest weight, half of one lost for each of 8192 words, the largest at least half of 2^power: 2^-36.  Where
+    # one workgroup takes a row of several chunks, 2^-51, half of one for each: V 2^-52.  Without chunks and with a sum of 1, 2^-60, all of one.
+    allowed = max(2.0**-36, V * (2.0**-52 if V <= 524288 else 2.0**-60))
+    for octaves in (40.0, 42.9, 43.1, 44.9, 45.1, 47.0, 49.9, 50.1, 52.0):
+        tail = torch.tensor(-octaves * math.log(2.0)).to(dtype)
+        x = torch.full((1, V), tail.item()).to(dtype)
+        x[0, -1] = 0.0
+        w = math.exp(tail.double().item())
+        for options, words in (({}, V - 1), ({"min_p": 1e-30}, V - 1), ({"top_k": 3000}, 2999), ({"top_k": 300}, 299)):
+            u = torch.tensor([words * w * f for f in (0.0, 0.1, 0.5, 0.9)] + [0.5], dtype=f32)
+            got = ops.sample(x.cuda().repeat(len(u), 1), u.cuda(), **options).tolist()
+            whole = 1.0 + words * w
+            for token, part in zip(got, u.double().tolist()):
+                before = (words if token == V - 1 else token) * w
+                assert token == V - 1 or 0 <= token < words
+                assert before <= (part + allowed) * whole, (octaves, options, part, token)
+                assert before + (1.0 if token == V - 1 else w) >= (part - allowed) * whole, (octaves, options, part, token)
+
+
+def test_sums_of_chunks_far_apart():
+    """A chunk holds one likely word, the others only unlikely ones of many sizes: top-p cuts where the sums in 64 bits do."""
+    V = 131072
+    g = torch.Generator().manual_seed(9)
+    x = -25.0 - 15.0 * torch.rand(4, V, generator=g)
+    x[0, 70000] = x[1, 0] = x[2, V - 1] = x[3, 8192] = 0.0
+    x[:, 8192 * 4:8192 * 8] += torch.linspace(0.0, 20.0, 8192 * 4)
+    check(x, [0.1, 0.9, 0.5, 0.999])
+    check(x, [0.1, 0.9, 0.5, 0.999], top_p=0.9)
+    check(x, [1e-4, 0.9, 0.5, 0.999], top_p=0.999)
