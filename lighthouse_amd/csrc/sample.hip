@@ -518,6 +518,7 @@ struct Sampler {
       return on_list(n, (int)top_k >= n, top_k, top_p, least, u, 0, token);
     }
 
+    if (!(u < 1.0f)) return false;  // (which word is the last with any weight, masses do not tell)
     // Every wave has the chunks in its lanes.  The row counts octaves from the largest power down, and masses in units in which all
     // of it comes to between 2^60 and 2^61, by `units` octaves above those of the chunk with the largest power.
     const bool words = lane < n_chunks && mine.total != 0;
@@ -671,18 +672,11 @@ struct Sampler {
     const uint64_t kept = lane < n_chunks ? s.chunk_kept[lane] : 0, own_units = to_row(kept, down);
     const uint64_t run = wave_scan(own_units), all = wave_last(run);
     if (all == 0) return false;  // (the largest word stays: this does not happen, and without it there would be no chunk to find)
-    int k;
-    uint64_t goal;
-    if (u < 1.0f) {
-      const uint64_t of_row = goal_of(u, all);
-      k = __ffsll((unsigned long long)__ballot(of_row < run)) - 1;
-      goal = of_row - __shfl((unsigned long long)(run - own_units), k);
-      const int by = s.chunk_down[k] + units;  // (below 62: the chunk has a unit of the row's)
-      goal = by >= 0 ? goal << by : goal >> -by;
-    } else {
-      k = 63 - __clzll((unsigned long long)__ballot(kept != 0));
-      goal = s.chunk_kept[k] - 1;
-    }
+    const uint64_t of_row = goal_of(u, all);
+    int k = __ffsll((unsigned long long)__ballot(of_row < run)) - 1;
+    uint64_t goal = of_row - __shfl((unsigned long long)(run - own_units), k);
+    const int by = s.chunk_down[k] + units;  // (below 62: the chunk has a unit of the row's)
+    goal = by >= 0 ? goal << by : goal >> -by;
     k = __builtin_amdgcn_readfirstlane(k);
     const ChunkScale scale(c, s.chunk_power[k]);
     const int bin_shift = 16 * s.chunk_down[k];
@@ -746,9 +740,17 @@ struct Sampler {
     return s.cut_i;
   }
 
-  // u * all as the whole number that the running sum has to exceed.
-  __device__ __forceinline__ static uint64_t goal_of(float u, uint64_t all) {
-    return u < 1.0f ? u > 0.0f ? part_of(all, u, false) : 0 : all - 1;
+  // u * all as the whole number that the running sum has to exceed, for u below 1.
+  __device__ __forceinline__ static uint64_t goal_of(float u, uint64_t all) { return u > 0.0f ? part_of(all, u, false) : 0; }
+  // For another u: the last word with any weight, of the workgroup, given that of each thread (or -1).
+  __device__ __forceinline__ void take_last(int own, int64_t* token) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) own = max(own, __shfl_xor(own, o));
+    __syncthreads();
+    if (lane == 0) s.wave_i[wave] = own;
+    __syncthreads();
+    for (int w = 0; w < kSampleWaves; ++w) own = max(own, s.wave_i[w]);
+    if (tid == 0) *token = own;
   }
   __device__ __forceinline__ static uint64_t top_goal(float top_p, uint64_t all) {
     const uint64_t goal = top_p > 0.0f ? part_of(all, top_p, true) : 1;
@@ -828,6 +830,13 @@ struct Sampler {
     const uint64_t m = first ? mass(entry_x(e)) : 0, run = wave_scan(m), of_list = wave_last(run);
     const uint64_t goal = top_p < 1.0f ? top_goal(top_p, of_list) : ~0ull;
     const int kept = __popcll(__ballot(lane == 0 || (first && run - m < goal && weight(entry_x(e)) >= least)));
+    if (!(u < 1.0f)) {
+      int last = lane < kept && weight(entry_x(e)) > 0.0 ? entry_i(e) : -1;
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) last = max(last, __shfl_xor(last, o));
+      if (lane == 0) *token = last;
+      return;
+    }
     const uint64_t own = lane < kept ? m : 0, aim = goal_of(u, wave_total(own));
     const unsigned long long by_index = wave_sort(lane < kept ? (unsigned long long)(uint32_t)~entry_i(e) << 32 | (uint32_t)lane : 0);
     const uint64_t here = lane < kept ? __shfl((unsigned long long)own, (int)(by_index & 63)) : 0, end = wave_scan(here);
@@ -852,6 +861,10 @@ struct Sampler {
     const bool in0 = j0 < (int)kept, in1 = j1 < (int)kept;
     // All of the list stays, and words that are not on it might: it was too short.
     if (kept == (uint64_t)n && !complete && !(top_k > 0 && (int)top_k <= n) && of_list < goal) return false;
+    if (!(u < 1.0f)) {
+      take_last(max(in0 && weight(entry_x(e0)) > 0.0 ? entry_i(e0) : -1, in1 && weight(entry_x(e1)) > 0.0 ? entry_i(e1) : -1), token);
+      return true;
+    }
     uint64_t all;
     block_before((in0 ? m0 : 0) + (in1 ? m1 : 0), &all);
     const uint64_t aim_mass = goal_of(u, all);
@@ -1090,11 +1103,22 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   }
   __syncthreads();
 
+  auto keeps = [&](float x, int i) { return x > -INFINITY && f.stays(x, i) && (least == 0.0 || f.weight(x) >= least || i == top_i); };
+  if (!(u < 1.0f)) {
+    int last = -1;
+    row.each([&](const float* x, int i0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (keeps(x[e], i0 + e) && f.weight(x[e]) > 0.0) last = i0 + e;
+    });
+    f.take_last(last, a.tokens + b);
+    return;
+  }
+
   // What stays: its mass by waves, and within a wave by up to 64 groups of pieces, lane g has group g's.
   auto left = [&](float x, int i) -> uint64_t {
     const uint64_t m = f.mass(x);
-    if (!(x > -INFINITY) || !f.stays(x, i)) return 0;
-    return least == 0.0 || f.weight(x) >= least || i == top_i ? m : 0;
+    return keeps(x, i) ? m : 0;
   };
   const int group = ((share / (64 * E) + 63) / 64) * 64 * E;  // words
   uint64_t of_group = 0, total = 0;
