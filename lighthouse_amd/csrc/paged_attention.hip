@@ -53,6 +53,8 @@ typedef float any_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kPagedShare = 32 * kPagedWaves;  // positions a share is a multiple of
 
 __device__ __forceinline__ int paged_length(const PagedAttnArgs& a, int b) { return min(max(a.lengths[b], 0), a.c.capacity()); }
+// Shares that n positions take.
+__device__ __forceinline__ int paged_parts(const PagedAttnArgs& a, int n) { return (int)(((uint32_t)n + (uint32_t)a.share - 1u) / (uint32_t)a.share); }
 
 template <int DT>
 __device__ __forceinline__ f32x4 paged_mma(u32x4 a, u32x4 b, f32x4 c) {
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE)) paged
   const int item = (int)((blockIdx.x - (unsigned)split * items + split) % (unsigned)items);
   const int group = item % a.groups, rest = item / a.groups;
   const int hk = rest % a.c.heads, b = rest / a.c.heads;
-  const int k0 = split * a.share, table_end = min(a.c.capacity(), k0 + a.share);
+  const int k0 = split * a.share, table_end = k0 + min(a.c.capacity() - k0, a.share);  // (k0 + share may pass 2^31)
   const int64_t table_row = b * a.c.table_stride;
   int ahead[KT];       // what the table says for a later step
   auto find_pages = [&](int step, int* found) {
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE)) paged
   float m_run = -INFINITY, l_run = 0.0f;
 
   if (k0 >= n && split > 0) return;
-  const int k1 = min(n, k0 + a.share);
+  const int k1 = k0 + min(n - k0, a.share);
   const uint8_t* kb = static_cast<const uint8_t*>(a.c.k);
   const uint8_t* vb = static_cast<const uint8_t*>(a.c.v);
   const int row_bytes = a.c.d * ES;
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(256) paged_attention_finish(PagedAttnArgs a, i
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if ((int)blockIdx.x < joins) {
     const int bh = blockIdx.x, b = bh / a.H, head = bh % a.H;
-    const int n = paged_length(a, b), parts = (n + a.share - 1) / a.share;
+    const int n = paged_length(a, b), parts = paged_parts(a, n);
     if (parts <= 1) return;  // (written at once)
     const int hk = head / a.G, q_row = head % a.G, col = tid % DP, first = tid / DP;
     const int64_t at = ((int64_t)(b * a.c.heads + hk) * a.groups + q_row / 16) * a.splits * a.rows + q_row % 16;
@@ -556,7 +558,7 @@ __global__ void __launch_bounds__(256) paged_attention_finish(PagedAttnArgs a, i
   const int t0 = (blockIdx.x - joins - bh * per_head) * 256, t = t0 + tid;
   const int n = paged_length(a, b);
   if (t0 >= n) return;
-  const int parts = (n + a.share - 1) / a.share;
+  const int parts = paged_parts(a, n);
   const int64_t first = (int64_t)b * a.H + hk * a.G;
   // (What does not wait for the sums is requested before them: the scores of the first heads and the weight that grows.)
   constexpr int EARLY = 8;
@@ -642,7 +644,7 @@ static PagedPlan paged_plan(const Paged& c, int cache_dtype, int64_t B, int64_t 
   p.mode = paged_in_tiles(c, es) ? kTiles : c.d * es % 16 == 0 && c.d % (p.dp / 16) == 0 ? kWholeRows : kOddRows;
   const int64_t items = B * c.heads * p.groups;
   p.share = paged_share(items, c.capacity(), paged_occupancy(cache_dtype, p.dp, p.mode), 2 * (int64_t)c.d * es);
-  p.splits = (c.capacity() + p.share - 1) / p.share;
+  p.splits = (int)(((int64_t)c.capacity() + p.share - 1) / p.share);
   if (p.splits > 1) {
     p.o_bytes = granules((size_t)items * p.splits * p.rows * p.dp * 4);
     p.ml_bytes = granules((size_t)items * p.splits * p.rows * 8);

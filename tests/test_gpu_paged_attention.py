@@ -245,3 +245,31 @@ def test_probabilities_keep_the_places_of_f32(dtype):
     half = torch.finfo(q_dtype).eps / 2
     off = (out.cpu().double() - want[:, :, None]).abs()
     assert (off <= (half * want + share * (2 * 6 + 6) * 2.0**-24)[:, :, None]).all(), float(off.max())
+
+
+def test_the_widest_table():
+    """A table of nearly 2^31 positions, all on three pages; those of the last have nearly all the weight, and lie in the last share."""
+    size, pages, d = 65536, 32766, 16
+    k = torch.zeros(3, 1, size, d)
+    k[2, :, :, 0] = 24.0
+    v = (0.5 + torch.rand(3, 1, size, d, generator=torch.Generator().manual_seed(16))).to(e4m3)
+    table = (torch.arange(pages, dtype=torch.int32) % 2).view(1, pages)
+    table[0, -1] = 2
+    q = torch.zeros(1, 1, d, dtype=bf16)
+    q[0, 0, 0] = 1.0
+    out = ops.paged_attention(q.cuda(), k.to(e4m3).cuda(), v.cuda(), table.cuda(), torch.full((1,), 2**31 - 1, dtype=torch.int32).cuda(), scale=1.0)
+    mean = v.double().mean(2)[:, 0]
+    rest = (pages - 1) // 2 * math.exp(-24.0)
+    want = (mean[2] + rest * mean[0] + (rest + math.exp(-24.0)) * mean[1]) / (1.0 + 2 * rest + math.exp(-24.0))
+    # Up to 2^18 positions of a lane and 2^16 steps of a wave are added one after the other in f32, and the result rounded to 2^-9.
+    assert ((out[0, 0].cpu().double() - want).abs() <= want * (2.0**-6 + 2.0**-8 + 2.0**-9)).all()
+    # Heads for every CU: a share is the whole table.
+    B, heads = 129, 16
+    k, v = (torch.randn(3, heads, size, d, generator=torch.Generator().manual_seed(17)).to(bf16) for _ in range(2))
+    q = torch.randn(B, heads, d, generator=torch.Generator().manual_seed(18)).to(bf16)
+    wide = torch.full((B, pages), -1, dtype=torch.int32)
+    wide[:, 0] = torch.arange(B) % 3
+    out = ops.paged_attention(q.cuda(), k.cuda(), v.cuda(), wide.cuda(), torch.arange(B, dtype=torch.int32).cuda())
+    for b in range(B):
+        want, _, allowed, _ = ref.attention(q[b], k[b % 3, :, :b], v[b % 3, :, :b], 0.25)
+        assert ((out[b].cpu().double() - want).abs() <= allowed).all(), b

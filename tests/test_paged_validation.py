@@ -229,3 +229,16 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
     refused("current device", ops._on_current_device, On(1), None, On(1))
     refused(ON_GPU, ops._on_current_device, On(-1), On(-1))
     refused(ON_GPU, ops._on_current_device, On(0), On(-1))
+
+
+def test_shares_of_the_widest_tables():
+    """Positions of the table and of a share add up to more than 2^31: there are as many shares all the same."""
+    lib = _lib.load()
+    size, pages = 65536, 32766
+    st = _lib.Strides3(size * 64, size * 64, 64)
+    c = _lib.PagedCache(4096, 8192, 12288, pages, st, st, 2, pages, size, 1, 64, _lib.BF16, 1.0, 1.0)
+    per_share = 64 * 4 + 8  # sums of a head, maximum and sum
+    need = lib.lh_hip_paged_attention_workspace_bytes(ctypes.byref(c), 1, 1, 0)
+    assert need >= 1024 * per_share and need <= 4096 * per_share
+    # With heads for every CU a share is the table, and nothing is joined.
+    assert lib.lh_hip_paged_attention_workspace_bytes(ctypes.byref(c), 2**14, 1, 0) == 0
