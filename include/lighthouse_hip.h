@@ -420,7 +420,7 @@ int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, 
  * weights_stride_b, weights_stride_h), weights[b, g, t] grows by the sum of p_t over the H / n_kv_heads heads of group g.
  * B H < 2^20, and with weights B n_kv_heads ceil(max_pages * page_size / 256) < 2^23.
  * `workspace`, 256-byte aligned, of lh_hip_paged_attention_workspace_bytes(...): the call allocates nothing, and two calls
- * that overlap in time need a workspace each.  It needs no clearing.
+ * that overlap in time need a workspace each.  It needs no clearing.  Its size goes by sizes, strides and types, not by where the cache begins.
  */
 size_t lh_hip_paged_attention_workspace_bytes(const lh_paged_cache* cache, int64_t B, int64_t H, int32_t with_weights);
 int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q, int64_t out_stride_b, int64_t out_stride_h,

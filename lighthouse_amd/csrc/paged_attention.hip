@@ -610,10 +610,11 @@ static bool paged_batch(int64_t B, int64_t H) {
 
 static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
 
-static bool paged_in_tiles(const Paged& c, int es) {
+// `aligned`: keys and values begin at multiples of 16 bytes.
+static bool paged_in_tiles(const Paged& c, int es, bool aligned) {
   const lh_strides3& s = c.sk;
-  return c.size % 16 == 0 && c.d * es % 16 == 0 && s.z == c.sv.z && s.h == c.sv.h && s.t == c.sv.t && s.z * es % 16 == 0 && s.h * es % 16 == 0 &&
-         s.t * es % 16 == 0 && 16 * s.t * es < 0x40000000 && s.t >= c.d && aligned16(c.k) && aligned16(c.v);
+  return aligned && c.size % 16 == 0 && c.d * es % 16 == 0 && s.z == c.sv.z && s.h == c.sv.h && s.t == c.sv.t && s.z * es % 16 == 0 && s.h * es % 16 == 0 &&
+         s.t * es % 16 == 0 && 16 * s.t * es < 0x40000000 && s.t >= c.d;
 }
 
 // How many positions a workgroup takes of a sequence; `items` (sequence, head, group of queries), `per_cu` workgroups that a CU
@@ -635,13 +636,13 @@ static int paged_share(int64_t items, int capacity, int per_cu, int64_t row_byte
   return (int)((share + kPagedShare - 1) / kPagedShare * kPagedShare);
 }
 
-static PagedPlan paged_plan(const Paged& c, int cache_dtype, int64_t B, int64_t H, bool with_weights) {
+static PagedPlan paged_plan(const Paged& c, int cache_dtype, int64_t B, int64_t H, bool with_weights, bool aligned) {
   PagedPlan p = {};
   const int G = (int)(H / c.heads);
   p.rows = G < 16 ? G : 16, p.groups = (G + 15) / 16;
   p.dp = c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
   const int es = (int)dtype_size(cache_dtype);
-  p.mode = paged_in_tiles(c, es) ? kTiles : c.d * es % 16 == 0 && c.d % (p.dp / 16) == 0 ? kWholeRows : kOddRows;
+  p.mode = paged_in_tiles(c, es, aligned) ? kTiles : c.d * es % 16 == 0 && c.d % (p.dp / 16) == 0 ? kWholeRows : kOddRows;
   const int64_t items = B * c.heads * p.groups;
   p.share = paged_share(items, c.capacity(), paged_occupancy(cache_dtype, p.dp, p.mode), 2 * (int64_t)c.d * es);
   p.splits = (int)(((int64_t)c.capacity() + p.share - 1) / p.share);
@@ -688,7 +689,9 @@ size_t lh_hip_paged_attention_workspace_bytes(const lh_paged_cache* cache, int64
   Paged c;
   if (paged_cache(cache, "lh_hip_paged_attention_workspace_bytes", &c) != LH_OK) return 0;
   if (!paged_batch(B, H) || H % c.heads != 0) return 0;
-  return paged_plan(c, cache->dtype, B, H, with_weights != 0).total();
+  // (Room for either alignment: a caller may size it with one cache and pass a view of another.)
+  const size_t one = paged_plan(c, cache->dtype, B, H, with_weights != 0, true).total(), other = paged_plan(c, cache->dtype, B, H, with_weights != 0, false).total();
+  return one > other ? one : other;
 }
 
 int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q, int64_t out_stride_b, int64_t out_stride_h,
@@ -706,7 +709,7 @@ int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q
   LH_REQUIRE(weights == nullptr || ((a.c.heads == 1 || weights_stride_h >= a.c.capacity()) && (B <= 1 || weights_stride_b >= a.c.capacity())),
              "lh_hip_paged_attention: rows of the weights overlap");
   LH_REQUIRE(weights == nullptr || (a.c.capacity() + 255) / 256 * B * a.c.heads < (1ll << 23), "lh_hip_paged_attention: too many weights (fewer than 2^31)");
-  const PagedPlan p = paged_plan(a.c, cache->dtype, B, H, weights != nullptr);
+  const PagedPlan p = paged_plan(a.c, cache->dtype, B, H, weights != nullptr, aligned16(a.c.k) && aligned16(a.c.v));
   LH_REQUIRE(p.total() == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= p.total()),
              "lh_hip_paged_attention: workspace too small or not 256-byte aligned: %zu of %zu bytes", workspace_bytes, p.total());
   a.out = out, a.q = q, a.so_z = out_stride_b, a.so_h = out_stride_h, a.sq_z = q_stride_b, a.sq_h = q_stride_h, a.lengths = lengths;

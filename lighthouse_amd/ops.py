@@ -700,7 +700,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, *, scale=None, ou
 
 
 def paged_attention_workspace_bytes(q, k_cache, v_cache, block_table, *, weights=False) -> int:
-    """Bytes of temporary memory that paged_attention takes for these tensors (only their shapes and strides matter);
+    """Bytes of temporary memory that paged_attention takes for these tensors (only their shapes, strides and types matter);
     `weights`: whether the call passes any."""
     cache = _paged_cache(k_cache, v_cache, block_table, q.shape[0], 1.0, 1.0)[0]
     return int(_lib.load().lh_hip_paged_attention_workspace_bytes(cache, q.shape[0], q.shape[1], 1 if weights else 0))

@@ -273,3 +273,18 @@ def test_the_widest_table():
     for b in range(B):
         want, _, allowed, _ = ref.attention(q[b], k[b % 3, :, :b], v[b % 3, :, :b], 0.25)
         assert ((out[b].cpu().double() - want).abs() <= allowed).all(), b
+
+
+def test_a_workspace_sized_for_an_aligned_cache_serves_a_view():
+    c = ref.Cache([4000, 17, 2100, 1], 8, 16, 128, f16, seed=19)
+    q = torch.randn(4, 16, 128, generator=torch.Generator().manual_seed(19)).to(f16).cuda()
+    need = ops.paged_attention_workspace_bytes(q, c.k_cache, c.v_cache, c.table)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    check(q, c, ops.paged_attention(q, c.k_cache, c.v_cache, c.table, c.device_lengths, workspace=ws))
+    store = torch.empty(2, c.k_cache.numel() + 4, dtype=f16, device="cuda")
+    views = []
+    for row, cache in zip(store, (c.k_cache, c.v_cache)):
+        view = row[4:].view(cache.shape)  # 8 bytes further
+        ref.as_bits(view).copy_(ref.as_bits(cache))
+        views.append(view)
+    check(q, c, ops.paged_attention(q, *views, c.table, c.device_lengths, workspace=ws))

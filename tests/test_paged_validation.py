@@ -242,3 +242,15 @@ def test_shares_of_the_widest_tables():
     assert need >= 1024 * per_share and need <= 4096 * per_share
     # With heads for every CU a share is the table, and nothing is joined.
     assert lib.lh_hip_paged_attention_workspace_bytes(ctypes.byref(c), 2**14, 1, 0) == 0
+
+
+@pytest.mark.parametrize("B,heads,d,size,pages,dtype", [(4, 8, 128, 16, 256, _lib.F16), (32, 1, 128, 16, 256, _lib.BF16), (1, 12, 64, 16, 63, _lib.BF16),
+                                                        (2, 2, 256, 64, 100, _lib.F32), (3, 4, 128, 32, 700, _lib.F8E4M3)])
+@pytest.mark.parametrize("weights", [0, 1])
+def test_a_workspace_serves_a_cache_of_any_alignment(B, heads, d, size, pages, dtype, weights):
+    """Sized with keys and values at multiples of 16 bytes, it holds a call with a view that begins elsewhere, and the other way round."""
+    lib = _lib.load()
+    st = _lib.Strides3(heads * size * d, size * d, d)
+    need = [lib.lh_hip_paged_attention_workspace_bytes(ctypes.byref(_lib.PagedCache(4096 + k, 8192 + v, 12288, pages, st, st, 9, pages, size, heads, d, dtype, 1.0, 1.0)),
+                                                       B, 4 * heads, weights) for k, v in ((0, 0), (8, 0), (0, 8), (8, 8))]
+    assert len(set(need)) == 1 and need[0] % 256 == 0
