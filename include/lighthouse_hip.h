@@ -435,7 +435,7 @@ int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q
  * 0 .. budget - 1; weights behind them up to the old length become 0; rows behind them stay as they were.
  * new_lengths[b] = min(lengths[b], budget); it may be `lengths`.  Every position below the length must
  * lie on a page of its own that holds something (rows on others do not move).  1 <= budget, 0 <= recent <= budget,
- * B n_kv_heads < 2^16.
+ * B n_kv_heads < 2^16.  `workspace` as for lh_hip_paged_attention, of lh_hip_kv_evict_workspace_bytes(...).
  */
 size_t lh_hip_kv_evict_workspace_bytes(int64_t B, int64_t n_kv_heads, int64_t budget);
 int lh_hip_kv_evict(const lh_paged_cache* cache, float* weights, int64_t weights_stride_b, int64_t weights_stride_h,

@@ -587,7 +587,8 @@ int lh_hip_kv_evict(const lh_paged_cache* cache, float* weights, int64_t weights
   if (budget > a.c.capacity()) budget = a.c.capacity();  // nothing is longer: nothing goes
   if (recent > budget) recent = budget;
   const size_t need = lh_hip_kv_evict_workspace_bytes(B, a.c.heads, budget);
-  LH_REQUIRE(workspace != nullptr && workspace_bytes >= need, "lh_hip_kv_evict: workspace too small: %zu of %zu bytes", workspace_bytes, need);
+  LH_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= need,
+             "lh_hip_kv_evict: workspace too small or not 256-byte aligned: %zu of %zu bytes", workspace_bytes, need);
   a.weights = weights, a.sw_b = weights_stride_b, a.sw_h = weights_stride_h;
   a.lengths = lengths, a.new_lengths = new_lengths, a.kept = static_cast<int32_t*>(workspace);
   a.held = a.kept + B * a.c.heads * budget;

@@ -254,3 +254,13 @@ def test_a_workspace_serves_a_cache_of_any_alignment(B, heads, d, size, pages, d
     need = [lib.lh_hip_paged_attention_workspace_bytes(ctypes.byref(_lib.PagedCache(4096 + k, 8192 + v, 12288, pages, st, st, 9, pages, size, heads, d, dtype, 1.0, 1.0)),
                                                        B, 4 * heads, weights) for k, v in ((0, 0), (8, 0), (0, 8), (8, 8))]
     assert len(set(need)) == 1 and need[0] % 256 == 0
+
+
+def test_kv_evict_refuses_a_workspace_that_is_not_aligned():
+    lib = _lib.load()
+    st = _lib.Strides3(64, 32, 8)
+    c = ctypes.byref(_lib.PagedCache(4096, 8192, 12288, 2, st, st, 6, 2, 4, 2, 8, _lib.BF16, 1.0, 1.0))
+    need = lib.lh_hip_kv_evict_workspace_bytes(3, 2, 4)
+    for ws in (4096 + 1, 4096 + 4, 4096 + 128):
+        assert lib.lh_hip_kv_evict(c, 4096, 16, 8, 4096, 4096, 3, 4, 0, ws, need, None) == _lib.LH_ERR_INVALID
+        assert b"aligned" in lib.lh_hip_last_error()
