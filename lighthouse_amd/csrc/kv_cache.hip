@@ -171,7 +171,7 @@ struct EvictArgs {
   int32_t* new_lengths;
   int32_t* kept;  // [B * heads][budget]
   int32_t* held;  // [B * heads]: the length before
-  int32_t B, budget, recent;
+  int32_t budget, recent;
   int32_t elem_bytes;
   int32_t slices;  // column slices of a row of keys (and of values)
 };
@@ -592,7 +592,7 @@ int lh_hip_kv_evict(const lh_paged_cache* cache, float* weights, int64_t weights
   a.weights = weights, a.sw_b = weights_stride_b, a.sw_h = weights_stride_h;
   a.lengths = lengths, a.new_lengths = new_lengths, a.kept = static_cast<int32_t*>(workspace);
   a.held = a.kept + B * a.c.heads * budget;
-  a.B = (int32_t)B, a.budget = (int32_t)budget, a.recent = (int32_t)recent;
+  a.budget = (int32_t)budget, a.recent = (int32_t)recent;
   a.elem_bytes = (int32_t)dtype_size(cache->dtype);
   const int row_bytes = a.c.d * a.elem_bytes;
   const bool narrow = row_bytes % 16 == 0 && B * a.c.heads * 2 * ((row_bytes + 127) / 128) <= num_cus() / 4;
