@@ -200,3 +200,41 @@ def test_rows_on_pages_that_hold_nothing_do_not_move(heads, d):
     for cache, bits in zip((c.k_cache, c.v_cache), caches):
         assert torch.equal(ref.as_bits(cache).cpu(), bits)
     assert torch.equal(ref.as_bits(weights).cpu(), ref.as_bits(w))
+
+
+@pytest.mark.parametrize("dtype,cache_dtype", [(bf16, bf16), (f32, f32), (bf16, e4m3), (f32, e4m3)])
+@pytest.mark.parametrize("B,T,heads,d", [(2, 2101, 2, 64), (3, 5001, 1, 7), (5, 903, 16, 128), (1, 36003, 1, 16), (4, 4500, 3, 20)])
+def test_append_of_prompts_whose_workgroups_take_several_tokens(dtype, cache_dtype, B, T, heads, d):
+    """2 to 16 tokens a workgroup; counts that end anywhere in its share, positions that leave the table, a page that is none."""
+    c = ref.Cache([0] * B, heads, 16, d, cache_dtype, room=T + 40, seed=T)
+    g = torch.Generator().manual_seed(T)
+    k, v = ((100 * torch.randn(B, T, heads, d, generator=g)).to(dtype).cuda().transpose(1, 2) for _ in range(2))
+    positions = [0, 39, 45, -6, 3][:B]
+    counts = [T - 1, T - 18, T + 5, 1, T // 2][:B]
+    c.table[0, 7] = -1
+    table = c.table.cpu()
+    scales = (0.37, 1.7) if cache_dtype == e4m3 else (1.0, 1.0)
+    device = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for many in (counts, None):
+        want = [written(cache, table, x, positions, many, s) for cache, x, s in ((c.k_cache, k, scales[0]), (c.v_cache, v, scales[1]))]
+        ops.kv_append(k, v, c.k_cache, c.v_cache, c.table, device(positions), counts=None if many is None else device(many), k_scale=scales[0], v_scale=scales[1])
+        for cache, bits in zip((c.k_cache, c.v_cache), want):
+            assert torch.equal(ref.as_bits(cache).cpu(), bits)
+
+
+def written(cache, table, x, positions, counts, scale):
+    """`appended` for many tokens: a sequence at a time."""
+    bits = ref.as_bits(cache).cpu().clone()
+    B, _, T, _ = x.shape
+    size = cache.shape[2]
+    for b in range(B):
+        t = torch.arange(T if counts is None else min(T, counts[b]))
+        at = positions[b] + t
+        t, at = (y[(at >= 0) & (at < table.shape[1] * size)] for y in (t, at))
+        page = table[b].long()[at // size]
+        there = (page >= 0) & (page < cache.shape[0])
+        rows = x[b].cpu()[:, t[there]].transpose(0, 1)
+        if cache.dtype == e4m3:
+            rows = torch.clamp(rows.float() / scale, -448.0, 448.0)
+        bits[page[there], :, (at % size)[there]] = ref.as_bits(rows.to(cache.dtype).contiguous())
+    return bits

@@ -288,3 +288,22 @@ def test_a_workspace_sized_for_an_aligned_cache_serves_a_view():
         ref.as_bits(view).copy_(ref.as_bits(cache))
         views.append(view)
     check(q, c, ops.paged_attention(q, *views, c.table, c.device_lengths, workspace=ws))
+
+
+@pytest.mark.parametrize("q_dtype", [bf16, f16])
+@pytest.mark.parametrize("d,size,layout,pad", [(64, 24, "heads", 0), (128, 7, "slots", 0), (192, 24, "heads", 0), (256, 10, "slots", 16), (160, 8, "heads", 3), (32, 8, "heads", 0)])
+def test_cache_of_8_bits_on_any_pages(q_dtype, d, size, layout, pad):
+    c = ref.Cache([0, 1, size, 3 * size + 1, 1300], 2, size, d, e4m3, seed=d + size, layout=layout, pad=pad, scales=(0.75, 1.5))
+    q = torch.randn(5, 8, d, generator=torch.Generator().manual_seed(20)).to(q_dtype).cuda()
+    weights = torch.zeros(5, 2, c.capacity, device="cuda")
+    before = weights.clone()
+    check(q, c, ops.paged_attention(q, c.k_cache, c.v_cache, c.table, c.device_lengths, weights=weights, k_scale=0.75, v_scale=1.5), weights=weights, before=before)
+
+
+@pytest.mark.parametrize("d,size", [(64, 8), (128, 24), (256, 8), (32, 24), (24, 40)])
+@pytest.mark.parametrize("dtype", [bf16, f32])
+def test_pages_that_end_inside_a_tile(dtype, d, size):
+    """Several shares of positions on pages that are a multiple of 8 but not of 16, tables with unused entries."""
+    c = ref.Cache([2500, 8, 0, 777], 3, size, d, dtype, seed=d, room=3)
+    q = torch.randn(4, 6, d, generator=torch.Generator().manual_seed(21)).to(dtype).cuda()
+    check(q, c, ops.paged_attention(q, c.k_cache, c.v_cache, c.table, c.device_lengths))
