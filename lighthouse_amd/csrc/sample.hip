@@ -518,7 +518,7 @@ struct Sampler {
       return on_list(n, (int)top_k >= n, top_k, top_p, least, u, 0, token);
     }
 
-    if (!(u < 1.0f)) return false;  // (which word is the last with any weight, masses do not tell)
+    if (at_end(u)) return false;  // (which word is the first or last with any weight, masses do not tell)
     // Every wave has the chunks in its lanes.  The row counts octaves from the largest power down, and masses in units in which all
     // of it comes to between 2^60 and 2^61, by `units` octaves above those of the chunk with the largest power.
     const bool words = lane < n_chunks && mine.total != 0;
@@ -740,17 +740,24 @@ struct Sampler {
     return s.cut_i;
   }
 
-  // u * all as the whole number that the running sum has to exceed, for u below 1.
-  __device__ __forceinline__ static uint64_t goal_of(float u, uint64_t all) { return u > 0.0f ? part_of(all, u, false) : 0; }
-  // For another u: the last word with any weight, of the workgroup, given that of each thread (or -1).
-  __device__ __forceinline__ void take_last(int own, int64_t* token) {
+  // u * all as the whole number that the running sum has to exceed, for u between 0 and 1.
+  __device__ __forceinline__ static uint64_t goal_of(float u, uint64_t all) { return part_of(all, u, false); }
+  // Another u takes the first word with any weight, or the last one (1 and more, NaN): the largest `rank` among the candidates, 0 or more.
+  __device__ __forceinline__ static bool at_end(float u) { return !(u > 0.0f && u < 1.0f); }
+  __device__ __forceinline__ static int rank(float u, int i) { return u < 1.0f ? 0x7fffffff - i : i; }
+  __device__ __forceinline__ int rank_of(float u, unsigned long long e) const { return weight(entry_x(e)) > 0.0 ? rank(u, entry_i(e)) : -1; }
+  __device__ __forceinline__ static int wave_best(int own) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) own = max(own, __shfl_xor(own, o));
+    return own;
+  }
+  __device__ __forceinline__ void take_end(float u, int own, int64_t* token) {
+    own = wave_best(own);
     __syncthreads();
     if (lane == 0) s.wave_i[wave] = own;
     __syncthreads();
     for (int w = 0; w < kSampleWaves; ++w) own = max(own, s.wave_i[w]);
-    if (tid == 0) *token = own;
+    if (tid == 0) *token = rank(u, own);  // (its own inverse)
   }
   __device__ __forceinline__ static uint64_t top_goal(float top_p, uint64_t all) {
     const uint64_t goal = top_p > 0.0f ? part_of(all, top_p, true) : 1;
@@ -830,11 +837,9 @@ struct Sampler {
     const uint64_t m = first ? mass(entry_x(e)) : 0, run = wave_scan(m), of_list = wave_last(run);
     const uint64_t goal = top_p < 1.0f ? top_goal(top_p, of_list) : ~0ull;
     const int kept = __popcll(__ballot(lane == 0 || (first && run - m < goal && weight(entry_x(e)) >= least)));
-    if (!(u < 1.0f)) {
-      int last = lane < kept && weight(entry_x(e)) > 0.0 ? entry_i(e) : -1;
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) last = max(last, __shfl_xor(last, o));
-      if (lane == 0) *token = last;
+    if (at_end(u)) {
+      const int best = wave_best(lane < kept ? rank_of(u, e) : -1);
+      if (lane == 0) *token = rank(u, best);
       return;
     }
     const uint64_t own = lane < kept ? m : 0, aim = goal_of(u, wave_total(own));
@@ -861,8 +866,8 @@ struct Sampler {
     const bool in0 = j0 < (int)kept, in1 = j1 < (int)kept;
     // All of the list stays, and words that are not on it might: it was too short.
     if (kept == (uint64_t)n && !complete && !(top_k > 0 && (int)top_k <= n) && of_list < goal) return false;
-    if (!(u < 1.0f)) {
-      take_last(max(in0 && weight(entry_x(e0)) > 0.0 ? entry_i(e0) : -1, in1 && weight(entry_x(e1)) > 0.0 ? entry_i(e1) : -1), token);
+    if (at_end(u)) {
+      take_end(u, max(in0 ? rank_of(u, e0) : -1, in1 ? rank_of(u, e1) : -1), token);
       return true;
     }
     uint64_t all;
@@ -1104,14 +1109,14 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
   __syncthreads();
 
   auto keeps = [&](float x, int i) { return x > -INFINITY && f.stays(x, i) && (least == 0.0 || f.weight(x) >= least || i == top_i); };
-  if (!(u < 1.0f)) {
-    int last = -1;
+  if (f.at_end(u)) {
+    int best = -1;
     row.each([&](const float* x, int i0) {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (keeps(x[e], i0 + e) && f.weight(x[e]) > 0.0) last = i0 + e;
+        if (keeps(x[e], i0 + e) && f.weight(x[e]) > 0.0) best = max(best, f.rank(u, i0 + e));
     });
-    f.take_last(last, a.tokens + b);
+    f.take_end(u, best, a.tokens + b);
     return;
   }
 

@@ -230,3 +230,14 @@ def test_a_number_of_one_or_none_takes_the_last_word_with_any_weight(u, V):
         x[b, 0], x[b, V - 1] = 0.0, least
     for options in ({}, {"top_k": 2}, {"top_k": 600}, {"top_p": 0.9}, {"min_p": 1e-20}, {"temperature": 2.0}, {"temperature": 0.5, "top_k": 700}, {"top_k": 1}):
         check(x, [u] * 7, **options)
+
+
+@pytest.mark.parametrize("u", [0.0, -0.0, -1.0, -math.inf])
+@pytest.mark.parametrize("V", [2, 900, 8192, 20000, 600000])
+def test_a_number_of_zero_or_less_takes_the_first_word_with_any_weight(u, V):
+    x = torch.full((7, V), -math.inf)
+    for b, least in enumerate((-20.0, -40.0, -300.0, -700.0, -744.0, -746.0, -1e30)):
+        x[b, 1:] = -800.0
+        x[b, 0], x[b, V - 1] = least, 0.0
+    for options in ({}, {"top_k": 2}, {"top_k": 600}, {"top_p": 0.9}, {"min_p": 1e-20}, {"temperature": 2.0}, {"temperature": 0.5, "top_k": 700}, {"top_k": 1}):
+        check(x, [u] * 7, **options)
