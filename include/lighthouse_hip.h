@@ -433,7 +433,7 @@ int lh_hip_paged_attention(const lh_paged_cache* cache, void* out, const void* q
  * the last `recent` positions stay, and of the others the budget - recent with the largest weight (equal weights: the
  * lowest positions; a NaN is below every number).  Rows of keys, values and weights that stay move up, in order, to the positions
  * 0 .. budget - 1; weights behind them up to the old length become 0; rows behind them stay as they were.
- * new_lengths[b] = min(lengths[b], budget); it may be `lengths`.  Every position below the length must
+ * new_lengths[b] = min(lengths[b], budget), lengths[b] clamped to 0 .. max_pages * page_size; it may be `lengths`.  Every position below the length must
  * lie on a page of its own that holds something (rows on others do not move).  1 <= budget, 0 <= recent <= budget,
  * B n_kv_heads < 2^16.  `workspace` as for lh_hip_paged_attention, of lh_hip_kv_evict_workspace_bytes(...).
  */

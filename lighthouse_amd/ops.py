@@ -710,7 +710,8 @@ def kv_evict(k_cache, v_cache, weights, block_table, lengths, budget, *, recent=
     """Shrinks every sequence longer than `budget` to it and returns the new lengths (int32 [B]; written to `out` if given, which may be
     `lengths`).  Of each kv head the last `recent` positions stay, and of the others the budget - recent with the largest weight
     (ties: the lowest positions; NaN is below every number).  Keys, values and weights of what stays move up, in order; weights behind
-    them up to the old length become 0.  Every position below the length must lie on a page of its own.
+    them up to the old length become 0.  Every position below the length must lie on a page of its own; lengths are clamped to 0 and the
+    positions of the block table.
     Cache, block table and weights are those of kv_append and paged_attention; `workspace` as there (kv_evict_workspace_bytes)."""
     B = lengths.shape[0] if lengths.dim() == 1 else -1
     _is_index(lengths, B, "lengths")

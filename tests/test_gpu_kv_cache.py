@@ -238,3 +238,16 @@ def written(cache, table, x, positions, counts, scale):
             rows = torch.clamp(rows.float() / scale, -448.0, 448.0)
         bits[page[there], :, (at % size)[there]] = ref.as_bits(rows.to(cache.dtype).contiguous())
     return bits
+
+
+def test_evict_clamps_the_lengths_to_the_table():
+    c = ref.Cache([48, 48, 48, 48], 2, 16, 64, bf16, seed=10)
+    weights = weights_like(c, 10)
+    given = torch.tensor([-5, 2**31 - 1, 49, 20], dtype=torch.int32, device="cuda")
+    c.lengths = [0, 48, 48, 20]
+    new, caches, w = evicted(c, weights, 30, 4)
+    assert ops.kv_evict(c.k_cache, c.v_cache, weights, c.table, given, 30, recent=4).tolist() == new == [0, 30, 30, 20]
+    for cache, bits in zip((c.k_cache, c.v_cache), caches):
+        assert torch.equal(ref.as_bits(cache).cpu(), bits)
+    assert torch.equal(weights.cpu(), w)
+    assert ops.kv_evict(c.k_cache, c.v_cache, weights, c.table, given, 60).tolist() == [0, 48, 48, 20]
