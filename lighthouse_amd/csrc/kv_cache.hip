@@ -83,9 +83,9 @@ __device__ __forceinline__ void e4m3_divide(float* x, float scale, float inv) {
 // A thread takes one chunk (16 bytes of the source; 8 elements for a cache of 8 bits) of one head's key or value, of several
 // tokens of a sequence one after the other, four at a time; a token's chunks are neighbours, so that both sides are read and
 // written in whole lines whatever the layout of heads and tokens.  The slot of a token is the same for the workgroup: the scalar
-// unit finds it.  Eight prompts of up to 1024 tokens, 12 heads of 64, bf16 into a cache of 8 bits: 9 us (with a token per workgroup and the slot found
-// by every thread 13.4); one token for each of 64 sequences: 3 us, a launch.  Any strides and alignment: gfx9 global memory takes 16 bytes at element alignment, the end of a row that
-// is no whole chunk goes element by element.
+// unit finds it.  Eight prompts of up to 1024 tokens, 12 heads of 64, bf16 into a cache of 8 bits: 12 us from memory, 9 from
+// the caches (with a token per workgroup and the slot found by every thread 13.4); one token for each of 64 sequences: 4 us, a launch.  Any
+// strides and alignment: gfx9 global memory takes 16 bytes at element alignment, the end of a row that is no whole chunk goes element by element.
 template <int SDT, int CDT>
 __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
   constexpr int E = SDT == LH_F32 && CDT == LH_F32 ? 4 : 8;
@@ -193,7 +193,7 @@ constexpr int kEvictBins = 2048;  // 11 bits of the key a pass
 // they are ranked against each other; of the positions that share it the lowest stay.  A thread has up to 16 neighbouring
 // positions, whose place among those that stay comes from one running sum over the workgroup.  4 waves for tables of up to 4096
 // positions, 16 for longer ones; up to 16384 positions the keys stay in registers, a longer sequence reads its weights (which the L2 holds) in
-// every pass, 16384 at a time.  What bounds it is the chain of passes: 16384 positions of 32 heads 14 us, 1024 of 192 heads 6.4.
+// every pass, 16384 at a time.  What bounds it is the chain of passes: 16384 positions of 32 heads 16 us, 1024 of 192 heads 7.
 constexpr int kEvictKeys = 16;   // of a thread
 constexpr int kEvictRank = 128;  // keys that are ranked
 template <int THREADS>

@@ -17,11 +17,11 @@
 //    each leaving (maximum, sum, sum of p v), which a second launch joins.
 //  * The table is read two steps ahead by the scalar unit, so that no step waits for a lookup or drains the loads on the way.
 //
-// Measured, keys and values out of memory: 16 sequences of 8192 to 32768 in bf16, 8 heads of 128 with 4 queries each, 254 us (5.2 TB/s) and 5 for
-// the join; 64 sequences of 256 to 1024, 12 heads of 64, 28 us (4.4 TB/s); 32 sequences of 2048 to 8192 in e4m3, 4 heads of 128 with 8 queries
-// each, 37 us (4.5 TB/s) and 5.  Out of the caches the same take 131, 20 and 31: the longer ones are bound by memory, and by what one CU draws of it
-// (31 B/ns) where the sequences' lengths do not fill all CUs to the end.  One sequence of 1000, 12 heads of 64: 5.1 us and 3.3, the chain of table, keys, values
-// and join.
+// Measured, keys and values out of memory: 16 sequences of 8192 to 32768 in bf16, 8 heads of 128 with 4 queries each, 256 us (5.2 TB/s) and 5 for
+// the join; 64 sequences of 256 to 1024, 12 heads of 64, 31 us (4.1 TB/s); 32 sequences of 2048 to 8192 in e4m3, 4 heads of 128 with 8 queries
+// each, 38 us (4.4 TB/s) and 5.  Out of the caches all of it takes 136, 19 and 34: the longer ones are bound by memory, and by what one CU draws of
+// it (31 B/ns) where the sequences' lengths do not fill all CUs to the end.  One sequence of 1000, 12 heads of 64: 6.1 us and 3.6, the chain of
+// table, keys, values and join.
 //
 // 16-bit types: P is split into values of the type, each nearest to what the ones before leave: three of bf16 have all 24 places of an f32, two of
 // f16 have 22, and there is a matrix instruction for each.  (Where values cancel, what P has lost shows in the result: with two of bf16,

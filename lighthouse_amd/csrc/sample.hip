@@ -25,8 +25,8 @@
 // word is found in a histogram of the distance max - x, by counts (top-k) or masses (top-p), and then among the words of the bin it
 // lies in.
 //
-// Measured: one row of 50257 f32 with top-k 50 and top-p 6 us for the digest and 9 for the rest, both a chain of a dozen dependent steps (in one
-// workgroup 24); 128 rows of 131072 bf16 with top-p and min-p 20.6 and 24.4 (without a digest 260).  Of that digest about 10 us are the loads and the largest
+// Measured: one row of 50257 f32 with top-k 50 and top-p 6.4 us for the digest and 9.5 for the rest, both a chain of a dozen dependent steps (in one
+// workgroup 24); 128 rows of 131072 bf16 with top-p and min-p 21.7 and 25.0 (without a digest 260).  Of that digest about 10 us are the loads and the largest
 // word, 4 the masses and 6 their addition to bins in LDS; loading the next chunk during that (103 registers instead of 64, half the waves) took 3 us longer.
 #include "common.h"
 #include "wave_scan.h"
