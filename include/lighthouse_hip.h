@@ -470,6 +470,85 @@ size_t lh_hip_sample_workspace_bytes(int64_t B, int64_t V);
 int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int64_t B, int64_t V, int64_t ld, int32_t dtype,
                   const lh_sample_opts* opts, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------- packed tokens of many sequences over a paged cache ---- */
+
+/*
+ * A step of a server packs the new tokens of B sequences into N rows: sequence b has the rows starts[b] .. starts[b + 1] - 1 (starts
+ * [B + 1], ascending from 0), rows from starts[B] on belong to none.  The cache is lh_paged_cache's.
+ */
+
+/*
+ * The pages of a step.  The first entries of a row of the table are the sequence's pages, the ones behind them are negative; free_pages
+ * [n_pages] begins with the *n_free pages that no sequence has, the last of them taken first.  With size = page_size, of sequence b:
+ *   counts[b] >= 0: it gets counts[b] tokens, behind its first lengths[b] (clamped to 0 .. max_pages * size) positions;
+ *   counts[b] < 0: it has ended, its length becomes 0.
+ * A sequence is refused if the new length passes max_pages * size or its tokens pass N.  Of the others the pages behind
+ * ceil(new length / size) go back to the end of free_pages, in the order of sequences and positions, their entries become -1.  Then,
+ * sequence after sequence, missing pages are taken from the end of the list; a sequence that misses more than there are, with
+ * all that the ones before it missed, is refused, too.  A refused one keeps its pages and length, and its tokens have no place.
+ * new_lengths[b] (may be `lengths`): the length.  starts[b]: running sum of the counts (a negative one is 0), at most N.  Of row i of
+ * sequence b: positions[i] = lengths[b] + i - starts[b] and slots[i] = page * size + position % size; -1 both where it has no place.
+ * Everything is on the device.  B < 2^20, N < 2^30, max_pages * page_size < 2^31 - 65536.
+ */
+int lh_hip_kv_pages(int32_t* block_table, int64_t table_stride, const int32_t* lengths, const int32_t* counts, int32_t* new_lengths,
+                    int32_t* free_pages, int32_t* n_free, int32_t* starts, int32_t* positions, int64_t* slots, int64_t B,
+                    int64_t max_pages, int64_t n_pages, int64_t page_size, int64_t N, void* stream);
+
+/*
+ * Rotary positions: of the first `turned` (even) of a head's d columns the pairs (i, i + turned / 2), or (2 i, 2 i + 1) if interleaved, turn
+ * by positions[n] * freqs[i] (radians, in 64 bits), times `amplitude`:
+ *   a' = amplitude (a cos - b sin),  b' = amplitude (b cos + a sin);  the other columns stay.
+ * Sines, cosines and sums are f32.  x, out [N, H, d] in F32, BF16 or F16 (element strides of token and head, unit stride along d); out
+ * may be x, but not another view of its memory.  Negated freqs turn back (and take the gradient back, at amplitude 1).  N H (d + 30) < 2^34.
+ */
+typedef struct lh_rotary {
+  const int32_t* positions; /* [N] */
+  const double* freqs;      /* [turned / 2] */
+  int32_t turned;
+  int32_t interleaved;
+  float amplitude;
+} lh_rotary;
+int lh_hip_rotary(void* out, const void* x, int64_t out_stride_n, int64_t out_stride_h, int64_t x_stride_n, int64_t x_stride_h,
+                  const lh_rotary* turn, int64_t N, int64_t H, int64_t d, int32_t dtype, void* stream);
+
+/*
+ * Keys and values of packed tokens into their slots: k, v [N, n_kv_heads, d] (element strides of token and head) in the cache's dtype,
+ * or F32, BF16 or F16 for a cache of e4m3, which holds e4m3(clamp(x / scale, +-448)), rounded to nearest even.  slots[n] = page * page_size + slot;
+ * a token with a slot outside 0 .. n_pages * page_size - 1 is dropped; two for one slot leave either.  The cache's table is not read.
+ * With `turn` the keys turn on their way (one rounding), and so do q [N, H, d] to q_out (which may be q), in the dtype of k, of every row, where H > 0.
+ */
+int lh_hip_kv_store(const lh_paged_cache* cache, const void* k, const void* v, int64_t k_stride_n, int64_t k_stride_h, int64_t v_stride_n,
+                    int64_t v_stride_h, const int64_t* slots, void* q_out, const void* q, int64_t out_stride_n, int64_t out_stride_h,
+                    int64_t q_stride_n, int64_t q_stride_h, const lh_rotary* turn, int64_t N, int64_t H, int32_t dtype, void* stream);
+
+/*
+ * Attention of packed new tokens over their sequences' caches: q, out [N, H, d] (element strides of token and head, unit stride along d), H a
+ * multiple of n_kv_heads, head h reads key / value head h / (H / n_kv_heads).  Row i of sequence b is its token at position
+ *   p = lengths[b] - (starts[b + 1] - starts[b]) + i - starts[b],   lengths clamped to 0 .. max_pages * page_size,
+ * and out[i, h] = sum_t w_t v_t, w = softmax over t <= p of scale q . k_t: `lengths` counts the new tokens, which have been stored.
+ * Positions on pages that hold nothing are left out; 0 where nothing is left; what lies at positions that a row does not see does not matter to it.
+ * Rows from starts[B] on stay as they were.  starts are taken as clamped to 0 .. N, a sequence whose end is not behind its beginning has no rows.
+ * Scores, softmax and sums are f32 (with 16-bit queries w_t in front of v_t is the sum of two values of their type, 16 places in bf16 and 22 in
+ * f16).  dtype (of q and out) is the cache's, or BF16 or F16 for a cache of e4m3.  B < 2^20, N < 2^30, N H < 2^31 - 256,
+ * (N H / n_kv_heads / 32 + B) n_kv_heads < 2^30.
+ * `workspace` as for lh_hip_paged_attention, of lh_hip_paged_attention_chunk_workspace_bytes(...), which goes by sizes and types.
+ */
+size_t lh_hip_paged_attention_chunk_workspace_bytes(const lh_paged_cache* cache, int64_t N, int64_t B, int64_t H);
+int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const void* q, int64_t out_stride_n, int64_t out_stride_h,
+                                 int64_t q_stride_n, int64_t q_stride_h, const int32_t* lengths, const int32_t* starts, int64_t N,
+                                 int64_t B, int64_t H, float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/*
+ * Root-mean-square norm of rows: s = x + residual (f32; without residual: x), out = s / sqrt(mean(s^2) + eps) * gamma, and
+ * residual_out = s, rounded to residual_dtype (residual_out may be residual).  x, out, residual [M, C] with row strides, gamma [C] f32.
+ * x_dtype F32, BF16 or F16, residual_dtype F32 or x_dtype; out_dtype F32, BF16, F16 or F8E4M3.  A result of e4m3 is e4m3(clamp(y / scale,
+ * +-448)), with `scale`, or, where row_scales is not NULL, row_scales[m] = max |y| / 448 of its row (1 for a row of zeros).
+ */
+int lh_hip_rms_norm(void* out, const void* x, const float* gamma, const void* residual, void* residual_out, float* row_scales,
+                    float scale, int64_t M, int64_t C, int64_t ld_out, int64_t ld_x, int64_t ld_residual, int64_t ld_residual_out,
+                    float eps, int32_t x_dtype, int32_t residual_dtype, int32_t out_dtype, void* stream);
+
 /* ------------------------------------------------- packed-argument payloads ---- */
 
 /*

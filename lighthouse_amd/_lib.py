@@ -122,15 +122,21 @@ class PagedCache(ctypes.Structure):
                 ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
 
 
-# These two for struct.pack, a fifth of the time: the entry points take their bytes.
+# These for struct.pack, a fifth of the time: the entry points take their bytes.
 PAGED_CACHE_FORMAT = "@PPPq3q3q5qi2f4x"
 SAMPLE_OPTS_FORMAT = "@4Pfi2f"
+ROTARY_FORMAT = "@2P2if4x"
 
 
 class SampleOpts(ctypes.Structure):
     _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p),
                 ("temperature_all", ctypes.c_float), ("top_k_all", ctypes.c_int32), ("top_p_all", ctypes.c_float),
                 ("min_p_all", ctypes.c_float)]
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [("positions", ctypes.c_void_p), ("freqs", ctypes.c_void_p), ("turned", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("amplitude", ctypes.c_float)]
 
 
 _vp, _i64, _i32, _u32, _f32, _sz = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32,
@@ -182,6 +188,12 @@ PROTOTYPES = {
     "lh_hip_kv_evict": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
     "lh_hip_sample_workspace_bytes": (_sz, [_i64, _i64]),
     "lh_hip_sample": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _sz, _vp]),
+    "lh_hip_kv_pages": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "lh_hip_rotary": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "lh_hip_kv_store": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i32, _vp]),
+    "lh_hip_rms_norm": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _f32, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _i32, _vp]),
+    "lh_hip_paged_attention_chunk_workspace_bytes": (_sz, [_vp, _i64, _i64, _i64]),
+    "lh_hip_paged_attention_chunk": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _f32, _i32, _vp, _sz, _vp]),
     "lh_hip_payload_matmul": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MatmulAttrs)]),
     "lh_hip_payload_matmul_fp8": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MatmulFp8Attrs)]),
     "lh_hip_payload_mlp": (_i32, [ctypes.POINTER(_vp), _i32, ctypes.POINTER(MlpAttrs)]),

@@ -1,0 +1,131 @@
+// Attention of packed chunks of new tokens over a paged cache: how a call is cut into workgroups, the join of shares of positions, the
+// entry points.  The kernel is in chunk_attention_kernel.hip.
+#include "chunk_attention.h"
+
+namespace lh {
+
+// One wave per row of the result whose positions were cut into shares: brings them to the common maximum and adds them in order.
+template <int QDT>
+__global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row_all = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int n = (int)(row_all / a.H), head = (int)(row_all - (int64_t)n * a.H);
+  if (n >= chunk_start(a, a.B)) return;
+  const int b = chunk_last(a, n, [&](int i) { return chunk_start(a, i); });
+  const int start = chunk_start(a, b), count = max(chunk_start(a, b + 1) - start, 0), token = n - start;
+  if (token < 0 || token >= count) return;
+  const int hk = head / a.G, row = token * a.G + head % a.G, tile = row >> a.tile_shift;
+  const int base = min(max(a.lengths[b], 0), a.c.capacity()) - count;
+  const int sees = base + (min(count * a.G, (tile + 1) << a.tile_shift) - 1) / a.G + 1;
+  if (sees <= a.share) return;  // (written at once)
+  const int parts = (sees + a.share - 1) / a.share;
+  const int64_t place = (int64_t)((uint32_t)(start * a.G) >> a.tile_shift) + b + tile;
+  const int64_t at = (place * a.c.heads + hk) * a.splits * a.tile_rows + (row - tile * a.tile_rows);
+  float m = -INFINITY;
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[at + (int64_t)p * a.tile_rows].x);
+  const float safe = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const int64_t part = at + (int64_t)p * a.tile_rows;
+    const float2 ml = a.part_ml[part];
+    const float w = __builtin_amdgcn_exp2f(ml.x - safe);
+    l = __builtin_fmaf(ml.y, w, l);
+    if (4 * lane < a.c.d) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + part * a.width + 4 * lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], w, o[e]);
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : a.c.v_scale / l;
+  const int64_t to = n * a.so_n + head * a.so_h + 4 * lane;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (4 * lane + e < a.c.d) store_from_f32<QDT>(a.out, to + e, o[e] * inv);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+
+static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
+
+static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H) {
+  ChunkPlan p = {};
+  const int64_t G = H / c.heads;
+  const int piece = cache_dtype == LH_F32 ? 4 : 8;
+  p.odd = c.d % piece != 0;
+  const int blocks = (c.d + 31) / 32;
+  p.blocks = p.odd ? (blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8) : blocks <= 2 ? 2 : blocks <= 4 ? blocks : blocks <= 6 ? 6 : 8;
+  // Tiles of 32 rows where the sequences have no more on average.
+  p.few = cache_dtype != LH_F32 && N * G <= 32 * B;
+  p.tile_rows = p.few ? 32 : 128;
+  const int64_t slots = N * G / p.tile_rows + B;
+  p.slots = (int)slots;
+  const int64_t items = slots * c.heads, cus = num_cus();
+  int64_t splits = (2 * cus + items - 1) / items;
+  const int64_t most = (c.capacity() + 255) / 256;
+  splits = splits > most ? most : splits;
+  const int64_t share = (c.capacity() + splits - 1) / splits;
+  p.share = (int)((share + 127) / 128 * 128);
+  p.splits = (int)(((int64_t)c.capacity() + p.share - 1) / p.share);
+  if (p.splits > 1) {
+    p.o_bytes = granules((size_t)items * p.splits * p.tile_rows * p.blocks * 32 * 4);
+    p.ml_bytes = granules((size_t)items * p.splits * p.tile_rows * 8);
+  }
+  return p;
+}
+
+static bool chunk_sizes(const Paged& c, int64_t N, int64_t B, int64_t H) {
+  return N > 0 && B > 0 && H > 0 && B < (1ll << 20) && N < (1ll << 30) && H < (1ll << 20) && H % c.heads == 0 && N * (H / c.heads) < (1ll << 31) - 256 &&
+         N * H < (1ll << 32) && (N * (H / c.heads) / 32 + B) * c.heads < (1ll << 30);
+}
+
+}  // namespace lh
+
+using namespace lh;
+
+extern "C" {
+
+size_t lh_hip_paged_attention_chunk_workspace_bytes(const lh_paged_cache* cache, int64_t N, int64_t B, int64_t H) {
+  Paged c;
+  if (paged_cache(cache, "lh_hip_paged_attention_chunk_workspace_bytes", &c) != LH_OK || !chunk_sizes(c, N, B, H)) return 0;
+  return chunk_plan(c, cache->dtype, N, B, H).total();
+}
+
+int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const void* q, int64_t out_stride_n, int64_t out_stride_h, int64_t q_stride_n,
+                                 int64_t q_stride_h, const int32_t* lengths, const int32_t* starts, int64_t N, int64_t B, int64_t H, float scale,
+                                 int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "lh_hip_paged_attention_chunk";
+  ChunkArgs a = {};
+  if (const int rc = paged_cache(cache, what, &a.c)) return rc;
+  if (N == 0 || B == 0) return LH_OK;
+  LH_REQUIRE(H > 0 && H % a.c.heads == 0, "%s: %lld heads are no multiple of %d key / value heads", what, (long long)H, a.c.heads);
+  LH_REQUIRE(chunk_sizes(a.c, N, B, H), "%s: bad sizes (fewer than 2^20 sequences, 2^30 rows, 2^32 rows of heads)", what);
+  LH_REQUIRE(out && q && lengths && starts, "%s: null pointer", what);
+  LH_REQUIRE(dtype == cache->dtype || (cache->dtype == LH_F8E4M3 && (dtype == LH_BF16 || dtype == LH_F16)),
+             "%s: queries must have the cache's dtype (bf16 or f16 for a cache of e4m3)", what);
+  const ChunkPlan p = chunk_plan(a.c, cache->dtype, N, B, H);
+  LH_REQUIRE(p.total() == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= p.total()),
+             "%s: workspace too small or not 256-byte aligned: %zu of %zu bytes", what, workspace_bytes, p.total());
+  a.out = out, a.q = q, a.so_n = out_stride_n, a.so_h = out_stride_h, a.sq_n = q_stride_n, a.sq_h = q_stride_h, a.lengths = lengths, a.starts = starts;
+  a.N = (int32_t)N, a.B = (int32_t)B, a.H = (int32_t)H, a.G = (int32_t)(H / a.c.heads), a.by_group = FastDiv((uint32_t)a.G);
+  a.tile_rows = p.tile_rows, a.tile_shift = p.few ? 5 : 7, a.slots = p.slots, a.share = p.share, a.splits = p.splits, a.width = 32 * p.blocks;
+  const double factor = (double)scale * a.c.k_scale * 1.4426950408889634;
+  a.scale_log2e = scale == 0.0f ? 1.0f : (float)(factor < 0.0 ? -factor : factor);
+  a.q_and = scale == 0.0f ? 0u : ~0u, a.q_xor = scale < 0.0f ? (dtype == LH_F32 ? 0x80000000u : 0x80008000u) : 0u;
+  LH_REQUIRE(a.scale_log2e > 0.0f && a.scale_log2e < INFINITY, "%s: scale times the keys' scale must be finite", what);
+  if (p.splits > 1) a.part_o = static_cast<float*>(workspace), a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.o_bytes);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int rc = cache->dtype == LH_F32    ? chunk_launch_f32(a, p, s)
+                 : cache->dtype == LH_BF16 ? chunk_launch_bf16(a, p, s)
+                 : cache->dtype == LH_F16  ? chunk_launch_f16(a, p, s)
+                 : dtype == LH_BF16        ? chunk_launch_e4m3_bf16(a, p, s)
+                                           : chunk_launch_e4m3_f16(a, p, s);
+  if (rc != LH_OK || p.splits == 1) return rc;
+  const dim3 grid((unsigned)((N * H + 3) / 4)), block(256);
+  if (dtype == LH_BF16) LH_LAUNCH((chunk_join_kernel<LH_BF16>), grid, block, 0, s, a);
+  else if (dtype == LH_F16) LH_LAUNCH((chunk_join_kernel<LH_F16>), grid, block, 0, s, a);
+  else LH_LAUNCH((chunk_join_kernel<LH_F32>), grid, block, 0, s, a);
+  return check_launch("chunk_join");
+}
+
+}  // extern "C"

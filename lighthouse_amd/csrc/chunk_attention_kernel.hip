@@ -1,0 +1,522 @@
+// Attention of packed chunks of new tokens over a paged cache, for one pair of types (the cache's LH_CHUNK_CDT, the queries' LH_CHUNK_QDT).
+//
+// The rows of a sequence and key / value head are its tokens' queries of the G heads that share it, token by token: row r is token r / G.  A
+// workgroup takes a tile of them and walks over the positions up to the last one that any of them sees:
+//
+//  * Both products are transposed, S^T = K Q^T and O^T = V^T P^T on 32-wide matrix instructions: a lane has one row, its softmax state
+//    is a scalar per lane, and the accumulators of S^T are, rounded, the second operand of O^T.
+//  * Keys and values of a step go through registers into LDS, requested while the step before is computed; where each position's
+//    row lies is looked up two steps ahead, one position a thread, so that any page size and any strides cost the same.
+//  * Many rows: 128 a workgroup, 32 for each of four waves, 64 positions a step, which all waves read.  Few rows: 32, and a step's 128
+//    positions are shared out between the waves, whose results are brought together at the end.
+//  * Long caches of few tiles are cut into shares of positions; a second launch joins them.
+//
+// P in 16 bits is split into two values of the type, the second what the first has lost: with one alone the result's error against 64 bits is
+// 1.4 times that of its own rounding.
+#include "chunk_attention.h"
+
+#ifndef LH_CHUNK_CDT
+#error "compiled with -DLH_CHUNK_CDT=... -DLH_CHUNK_QDT=... -DLH_CHUNK_NAME=..."
+#endif
+
+namespace lh {
+namespace {
+
+constexpr int CDT = LH_CHUNK_CDT, QDT = LH_CHUNK_QDT;
+constexpr bool F32 = CDT == LH_F32;
+constexpr int CES = CDT == LH_F8E4M3 ? 1 : F32 ? 4 : 2;  // bytes of an element in the cache
+constexpr int QES = F32 ? 4 : 2;                         // of a query's, and in LDS
+constexpr int PE = F32 ? 4 : 8;                          // elements of a piece: 16 bytes in LDS
+constexpr int PW = PE * CES / 4;                         // its words in the cache
+constexpr int PARTS = F32 ? 1 : 2;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x16 mma(u32x4 x, u32x4 y, f32x16 c) {
+  if constexpr (QDT == LH_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+}
+
+// (By value: a bit cast of a vector's element itself reads its first one.)
+__device__ __forceinline__ float f32_of(uint32_t u) { return __builtin_bit_cast(float, u); }
+
+// Waits for this wave's LDS accesses and for the workgroup, but for no load on its way to registers.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A piece of W words whose elements are of ES bytes, moved down by `skip` elements (those behind them become 0).
+template <int W, int ES>
+__device__ __forceinline__ void move_down(uint32_t* w, int skip) {
+  const int bits = skip * ES * 8;
+#pragma unroll
+  for (int step = 2; step >= 1; step /= 2)
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const uint32_t from = i + step < W ? w[i + step] : 0u;
+      w[i] = bits / 32 & step ? from : w[i];
+    }
+  if constexpr (ES < 4) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = (uint32_t)(((uint64_t)(i + 1 < W ? w[i + 1] : 0u) << 32 | w[i]) >> (bits & 31));
+  }
+}
+
+// Columns col .. col + PE - 1 of a row of d elements of ES bytes; those behind its end are 0.  The row is there in any case.  ODD: d is no multiple
+// of a piece; the last piece is loaded so that it ends with the row and moved down.
+template <int ES, bool ODD>
+__device__ __forceinline__ void load_columns(uint32_t* w, const uint8_t* row, int col, int d) {
+  constexpr int W = PE * ES / 4;
+  if (ODD && d < PE) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = 0;
+#pragma unroll
+    for (int e = 0; e < PE; ++e)
+      if (col + e < d) {
+        if constexpr (ES == 4) w[e] = reinterpret_cast<const uint32_t*>(row)[col + e];
+        else if constexpr (ES == 2) w[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[col + e] << (16 * (e % 2));
+        else w[e / 4] |= (uint32_t)row[col + e] << (8 * (e % 4));
+      }
+    return;
+  }
+  const int from = ODD ? min(col, d - PE) : col < d ? col : 0;
+  if constexpr (W == 4) {
+    const typename Chunk<ES>::type v = *reinterpret_cast<const typename Chunk<ES>::type*>(row + from * ES);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = v[i];
+  } else {
+    typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+    const u32x2_any v = *reinterpret_cast<const u32x2_any*>(row + from * ES);
+    w[0] = v[0], w[1] = v[1];
+  }
+}
+// What of it is not in the row becomes 0 (apart from the load, so that nothing waits for that).
+template <int ES, bool ODD>
+__device__ __forceinline__ void settle_columns(uint32_t* w, int col, int d, bool there) {
+  constexpr int W = PE * ES / 4;
+  if (ODD && d >= PE) {
+    const int skip = max(col - (d - PE), 0);
+    if (skip > 0) move_down<W, ES>(w, min(skip, PE - 1));
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i) w[i] = there && col < d ? w[i] : 0u;
+}
+
+// Two e4m3 codes (the lower or upper two of a word) as two values of the queries' type: exact.
+template <bool HI>
+__device__ __forceinline__ uint32_t of_e4m3(uint32_t w) {
+  if constexpr (QDT == LH_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+}
+__device__ __forceinline__ u32x4 in_lds(const uint32_t* w) {
+  if constexpr (CDT == LH_F8E4M3) return u32x4{of_e4m3<false>(w[0]), of_e4m3<true>(w[0]), of_e4m3<false>(w[1]), of_e4m3<true>(w[1])};
+  else return u32x4{w[0], w[1], w[2], w[3]};
+}
+// Whether a piece in LDS holds an infinity or a NaN.
+__device__ __forceinline__ bool any_wild(u32x4 w) {
+  bool wild = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (F32) {
+      wild |= (w[i] & 0x7f800000u) == 0x7f800000u;
+    } else {
+      constexpr uint32_t top = QDT == LH_BF16 ? 0x7f80u : 0x7c00u;
+      wild |= (w[i] & top) == top || (w[i] >> 16 & top) == top;
+    }
+  }
+  return wild;
+}
+
+// Widths that leave a CU two workgroups (registers).
+constexpr int occupancy(int blocks, bool few) { return blocks <= (few ? 3 : 4) ? 2 : 1; }
+
+constexpr int keys_of(bool few) { return few && !F32 ? 128 : 64; }
+constexpr size_t row_elems(int blocks) { return 32 * blocks + 8; }  // (16 or 32 bytes apart: the banks of neighbouring rows differ)
+constexpr size_t lds_bytes(int blocks, bool few) { return 2 * keys_of(few) * row_elems(blocks) * QES; }
+
+// DB: width in 32 columns.  FEW: 32 rows, positions shared out between the waves; otherwise 128 rows.
+template <int CACHE, int QUERY, int DB, bool ODD, bool FEW>  // (the types: for the name)
+__global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kernel(ChunkArgs a) {
+  constexpr int D = 32 * DB, KROW = row_elems(DB), KEYS = keys_of(FEW);
+  constexpr int WK = FEW ? 4 : 1;                 // waves that share out a step's positions
+  constexpr int NI = KEYS / 32 / WK;              // 32-position tiles of a wave
+  constexpr int CPR = D / PE;                     // pieces of a row
+  constexpr int NP = KEYS * CPR / 256;            // pieces a thread brings, of keys and of values
+  constexpr int SD = F32 ? D / 8 : D / 16;
+  constexpr bool AHEAD = !F32 && DB <= (FEW ? 4 : 6);                    // a step's keys and values are requested a step ahead
+  static_assert(NI >= 1 && NP * 256 == KEYS * CPR, "");
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  typedef typename std::conditional<F32, float, uint16_t>::type elem;
+  elem* const Ks = reinterpret_cast<elem*>(smem);
+  elem* const Vs = Ks + KEYS * KROW;
+  __shared__ int64_t k_at[2][KEYS], v_at[2][KEYS];  // where the rows of a step lie, in elements; below 0: nowhere
+  __shared__ uint64_t held[3][KEYS / 64];           // which positions of a step there are (read while a wave ahead notes those of two steps later)
+  __shared__ int32_t wild[4], first_wild[D];
+  __shared__ float2 stats[4][32];
+
+  const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int items = a.slots * a.c.heads, split = blockIdx.x / items, item = blockIdx.x - split * items;
+  // Later tiles of a sequence see more positions: they begin first.
+  const int place = a.slots - 1 - item / a.c.heads, hk = item % a.c.heads;
+
+  // The sequence whose places hold this one: the last that begins at or before it.
+  const int b = chunk_last(a, place, [&](int i) { return chunk_place(a, i); });
+  const int start = __builtin_amdgcn_readfirstlane(chunk_start(a, b));
+  const int count = max(__builtin_amdgcn_readfirstlane(chunk_start(a, b + 1)) - start, 0);
+  const int tile = place - (int)((uint32_t)(start * a.G) >> a.tile_shift) - b;
+  if (tile < 0 || tile > (count * a.G - 1) >> a.tile_shift) return;
+  const int first = tile << a.tile_shift, rows = min(a.tile_rows, count * a.G - first);
+  const int length = __builtin_amdgcn_readfirstlane(min(max(a.lengths[b], 0), a.c.capacity()));
+  const int base = length - count;  // position of the sequence's first new token
+  const int sees = base + (int)a.by_group.div((uint32_t)(first + rows - 1)) + 1;  // positions that the last row sees
+  const int k0 = split * a.share;
+  if (k0 >= sees && split > 0) return;
+  const int k1 = k0 + max(min(sees - k0, a.share), 0);
+  const bool cut = sees > a.share;
+
+  const int row0 = FEW ? 0 : 32 * wave;  // of the wave, in the tile
+  const int row = first + row0 + r32;
+  const bool row_live = row0 + r32 < rows;
+  const int token = (int)a.by_group.div((uint32_t)row), head = hk * a.G + (row - token * a.G);
+  const int last_seen = row_live ? min(base + token, k1 - 1) : -1;
+  const bool wave_live = row0 < rows;
+  const int wave_first = base + (int)a.by_group.div((uint32_t)(first + min(row0, rows - 1)));                  // what its first row sees
+  const int wave_last = min(base + (int)a.by_group.div((uint32_t)(first + min(row0 + 31, rows - 1))), k1 - 1);  // and its last one
+
+  // Queries: lane (r32, h) has columns 16 s + 8 h .. + 7 of its row (f32: 8 s + 4 h .. + 3); where the registers do not suffice for them, they are
+  // read again in every step.
+  constexpr bool Q_HELD = F32 ? DB <= 3 || DB == 6 : !(DB == 8 && ODD && FEW);
+  const uint8_t* const q = static_cast<const uint8_t*>(a.q) + ((start + (row_live ? token : 0)) * a.sq_n + (row_live ? head : hk * a.G) * a.sq_h) * QES;
+  auto query = [&](const uint8_t* from, int s, int d) {
+    const int col = (2 * s + h) * PE;
+    uint32_t w[4];
+    load_columns<QES, ODD>(w, from, col, d);
+    settle_columns<QES, ODD>(w, col, d, row_live);
+    // (A scale below 0 is that of the queries, so that -inf is the score of what a row does not see; with one of 0 they are 0.)
+    return (u32x4{w[0], w[1], w[2], w[3]} & a.q_and) ^ a.q_xor;
+  };
+  u32x4 qf[Q_HELD ? SD : 1];
+  if constexpr (Q_HELD)
+#pragma unroll
+    for (int s = 0; s < SD; ++s) qf[s] = query(q, s, a.c.d);
+
+  f32x16 acc[DB];
+#pragma unroll
+  for (int j = 0; j < DB; ++j)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[j][v] = 0.0f;
+  // What p is relative to: the maximum, or, in f16, 2^12 below it, so that small probabilities keep their part in a long row (the
+  // smallest number of f16 is 2^-24).  It moves only when a p would pass 2^slack.
+  constexpr float below = QDT == LH_F16 ? 12.0f : 0.0f, slack = QDT == LH_F16 ? 14.0f : 10.0f;
+  float m_run = row_live ? -INFINITY : 0.0f, l_run = 0.0f;  // (a row that is none waits for no maximum)
+
+  const int steps = (k1 - k0 + KEYS - 1) / KEYS;
+  const int64_t table_row = b * a.c.table_stride;
+  const uint8_t* const kb = static_cast<const uint8_t*>(a.c.k) + hk * a.c.sk.h * CES;
+  const uint8_t* const vb = static_cast<const uint8_t*>(a.c.v) + hk * a.c.sv.h * CES;
+  // Position k0 + step KEYS + tid, for tid < KEYS: its page, or -1; then where it lies.
+  auto look_up = [&](int step) {
+    const int key = k0 + step * KEYS + tid;
+    return tid < KEYS && key < k1 ? a.c.table[table_row + a.c.by_size.div((uint32_t)key)] : -1;
+  };
+  auto note = [&](int step, int page) {
+    if (tid >= KEYS) return;
+    const int key = k0 + step * KEYS + tid;
+    const bool there = key < k1 && (uint32_t)page < (uint32_t)a.c.pages;
+    const int slot = there ? key - (int)a.c.by_size.div((uint32_t)key) * a.c.size : 0;
+    k_at[step & 1][tid] = there ? page * a.c.sk.z + slot * a.c.sk.t : -1;
+    v_at[step & 1][tid] = there ? page * a.c.sv.z + slot * a.c.sv.t : -1;
+    const uint64_t some = __builtin_amdgcn_ballot_w64(there);
+    if (lane == 0) held[step % 3][wave] = some;
+  };
+  uint32_t kr[AHEAD ? NP : 1][PW], vr[AHEAD ? NP : 1][PW];
+  uint32_t there = 0;  // which of the thread's rows there are
+  auto request = [&](int step, int i, uint32_t* k, uint32_t* v) {
+    const int piece = tid + 256 * i, key = piece / CPR, col = (piece - key * CPR) * PE;
+    const int64_t k_row = k_at[step & 1][key], v_row = v_at[step & 1][key];
+    there = (there & ~(1u << i)) | (uint32_t)(k_row >= 0) << i;
+    load_columns<CES, ODD>(k, kb + max(k_row, (int64_t)0) * CES, col, a.c.d);
+    load_columns<CES, ODD>(v, vb + max(v_row, (int64_t)0) * CES, col, a.c.d);
+  };
+  auto put = [&](int i, uint32_t* k, uint32_t* v, bool look) {  // into LDS; whether a value is an infinity or a NaN, if asked for
+    const int piece = tid + 256 * i, key = piece / CPR, col = (piece - key * CPR) * PE;
+    settle_columns<CES, ODD>(k, col, a.c.d, there >> i & 1);
+    settle_columns<CES, ODD>(v, col, a.c.d, there >> i & 1);
+    const u32x4 kw = in_lds(k), vw = in_lds(v);
+    *reinterpret_cast<u32x4*>(Ks + key * KROW + col) = kw;
+    *reinterpret_cast<u32x4*>(Vs + key * KROW + col) = vw;
+    return look && any_wild(vw);
+  };
+
+  if (steps > 0) {
+    const int p0 = look_up(0), p1 = look_up(1);
+    note(0, p0);
+    note(1, p1);
+    lds_barrier();
+    if constexpr (AHEAD)
+#pragma unroll
+      for (int i = 0; i < NP; ++i) request(0, i, kr[i], vr[i]);
+  }
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    const int j0 = k0 + step * KEYS;
+    // Some row does not see all of this step's positions: those it does not see must not reach it by a 0 times an infinity.
+    const bool partial = j0 + KEYS > base + (int)a.by_group.div((uint32_t)first) + 1;
+    if (step > 0) lds_barrier();  // the step before has been read
+    bool odd_one = false;
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) odd_one |= put(i, kr[i], vr[i], partial);
+      if (step + 1 < steps)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) request(step + 1, i, kr[i], vr[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        uint32_t k[PW], v[PW];
+        request(step, i, k, v);
+        odd_one |= put(i, k, v, partial);
+        if (i % (ODD ? 2 : 4) == 1) asm volatile("" ::: "memory");  // (a few of each on their way at once)
+      }
+    }
+    const int page = look_up(step + 2);
+    if (partial) {
+      const bool some = __any(odd_one);
+      if (lane == 0) wild[wave] = some;
+    }
+    lds_barrier();
+    bool some_wild = false;
+    if (partial) some_wild = wild[0] | wild[1] | wild[2] | wild[3];
+    if (__builtin_expect(some_wild, 0)) {
+      // Such values become 0; a column's first one makes a NaN of the rows that see it (below).
+      for (int c = tid; c < D; c += 256) first_wild[c] = 0x7fffffff;
+      lds_barrier();
+#pragma unroll 1
+      for (int c = tid; c < KEYS * D; c += 256) {
+        elem* const x = Vs + c / D * KROW + c % D;
+        const uint32_t bits = F32 ? __builtin_bit_cast(uint32_t, (float)*x) : (uint32_t)*x, top = F32 ? 0x7f800000u : QDT == LH_BF16 ? 0x7f80u : 0x7c00u;
+        if ((bits & top) == top) {
+          *x = 0;
+          atomicMin(&first_wild[c % D], c / D);
+        }
+      }
+      lds_barrier();
+    }
+    const uint64_t all_held = KEYS == 64 ? held[step % 3][0] : held[step % 3][wave / 2] >> (32 * (wave & 1)) | 0xffffffff00000000ull;
+    const int kw0 = FEW && WK > 1 ? 32 * NI * wave : 0;  // the wave's first position of the step
+    const int j0w = j0 + kw0;
+    if (wave_live && wave_last >= j0w) {
+      f32x16 s[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[i][v] = 0.0f;
+      const uint8_t* q_now = q;
+      int d_now = a.c.d;
+      if constexpr (!Q_HELD) asm volatile("" : "+v"(q_now), "+s"(d_now));  // (read here, not held over the steps)
+#pragma unroll
+      for (int e = 0; e < SD; ++e) {
+        u32x4 qe;
+        if constexpr (Q_HELD) qe = qf[e];
+        else qe = query(q_now, e, d_now);
+        if (!Q_HELD && (F32 || e % 2 == 1)) asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(Ks + (kw0 + 32 * i + r32) * KROW + (2 * e + h) * PE);
+          if constexpr (F32) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              s[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(f32_of(kf[t]), f32_of(qe[t]), s[i], 0, 0, 0);
+          } else {
+            s[i] = mma(kf, qe, s[i]);
+          }
+        }
+      }
+      // s[i][v] = q . k of row r32 and position j0w + 32 i + 8 (v / 4) + 4 h + v % 4
+      const bool whole = j0w + 32 * NI - 1 <= min(wave_first, k1 - 1) && row0 + 31 < rows && all_held == ~0ull;
+      if (!whole) {
+        // Bit p of `seen`: whether the row sees position j0w + p.
+        uint64_t seen = last_seen < j0w ? 0ull : last_seen - j0w >= 63 ? ~0ull : (2ull << (last_seen - j0w)) - 1;
+        seen = (seen & all_held) >> (4 * h);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (!(seen >> (32 * i + 8 * (v >> 2) + (v & 3)) & 1)) s[i][v] = -INFINITY;
+      }
+      // The maximum is followed with a delay: nothing moves until a p would pass 2^10, which is as accurate as one of 1, and then for all lanes.
+      float mx = s[0][0];
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[i][v]);
+      mx *= a.scale_log2e;
+      if (__any(mx > m_run + slack)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float m_new = fmaxf(m_run, mx - below);
+        const float safe = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_run - safe);
+        l_run *= alpha;
+#pragma unroll
+        for (int j = 0; j < DB; ++j) acc[j] *= alpha;
+        m_run = m_new;
+      }
+      const float off = m_run == -INFINITY ? 0.0f : m_run;  // (nothing seen yet: every p is exp2(-inf))
+      // p takes the place of s: one rounding of s scale - maximum.
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          s[i][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][v], a.scale_log2e, -off));
+          l_run += s[i][v];
+        }
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const float* vrow = reinterpret_cast<const float*>(Vs) + (kw0 + 32 * i + 8 * (v >> 2) + 4 * h + (v & 3)) * KROW + r32;
+#pragma unroll
+            for (int j = 0; j < DB; ++j) acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[32 * j], s[i][v], acc[j], 0, 0, 0);
+            if (v % (DB > 6 ? 2 : 4) == (DB > 6 ? 1 : 3)) asm volatile("" ::: "memory");  // (values of a few positions fetched ahead)
+          }
+      } else {
+        // Values through the transposing read: lane (g4 = lane / 16, j16 = lane % 16) addresses position 4 h + j16 / 4 of 16 (+ 8 for the second
+        // read), columns 32 j + 16 (g4 % 2) + 4 (j16 % 4) .. + 3, and receives 8 positions of one column in the order of p's registers.
+        const int tr_row = 4 * h + ((lane & 15) >> 2), tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            u32x4 pf[PARTS];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float p0 = s[i][8 * u + 2 * e], p1 = s[i][8 * u + 2 * e + 1];
+              pf[0][e] = pack2<QDT>(p0, p1);
+              if constexpr (PARTS == 2) pf[PARTS - 1][e] = pack2<QDT>(p0 - unpack_lo<QDT>(pf[0][e]), p1 - unpack_hi<QDT>(pf[0][e]));
+            }
+#pragma unroll
+            for (int j = 0; j < DB; ++j) {
+              const elem* p0 = Vs + (kw0 + 32 * i + 16 * u + tr_row) * KROW + 32 * j + tr_col;
+              const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p0);
+              const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p0 + 8 * KROW));
+              const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+              const u32x4 vf = {l2[0], l2[1], h2[0], h2[1]};
+#pragma unroll
+              for (int n = 0; n < PARTS; ++n) acc[j] = mma(vf, pf[n], acc[j]);
+            }
+          }
+      }
+      if (__builtin_expect(some_wild, 0)) {
+#pragma unroll
+        for (int j = 0; j < DB; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (first_wild[32 * j + 8 * (v >> 2) + 4 * h + (v & 3)] <= last_seen - j0) acc[j][v] = NAN;
+      }
+    }
+    note(step + 2, page);
+  }
+
+  // acc[j][v] = sum of p v of row r32, column 32 j + 8 (v / 4) + 4 h + v % 4, relative to m_run
+  l_run += __shfl_xor(l_run, 32);
+  if constexpr (WK > 1) {
+    __syncthreads();  // (the last step has been read: its place is taken)
+    if (h == 0) stats[wave][r32] = make_float2(m_run, l_run);
+    __syncthreads();
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, stats[w][r32].x);
+    const float safe = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) l += stats[w][r32].y * __builtin_amdgcn_exp2f(stats[w][r32].x - safe);
+    const float own = __builtin_amdgcn_exp2f(m_run - safe);
+#pragma unroll
+    for (int j = 0; j < DB; ++j) acc[j] *= own;
+    f32x16* const sums = reinterpret_cast<f32x16*>(smem);  // [2][DB][64]
+#pragma unroll
+    for (int half = 2; half >= 1; half /= 2) {
+      if (wave >= half && wave < 2 * half)
+#pragma unroll
+        for (int j = 0; j < DB; ++j) sums[((wave - half) * DB + j) * 64 + lane] = acc[j];
+      __syncthreads();
+      if (wave < half)
+#pragma unroll
+        for (int j = 0; j < DB; ++j) acc[j] += sums[(wave * DB + j) * 64 + lane];
+      if (half > 1) __syncthreads();
+    }
+    if (wave != 0) return;
+    m_run = m, l_run = l;
+  }
+  if (!row_live) return;
+  if (cut) {
+    const int64_t part = (((int64_t)place * a.c.heads + hk) * a.splits + split) * a.tile_rows + row0 + r32;
+    if (h == 0) a.part_ml[part] = make_float2(m_run, l_run);
+    float* to = a.part_o + part * a.width;
+#pragma unroll
+    for (int j = 0; j < DB; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(to + 32 * j + 8 * g + 4 * h) = f32x4{acc[j][4 * g], acc[j][4 * g + 1], acc[j][4 * g + 2], acc[j][4 * g + 3]};
+    return;
+  }
+  const float inv = l_run == 0.0f ? 0.0f : a.c.v_scale / l_run;  // (no position seen: 0)
+  uint8_t* out = static_cast<uint8_t*>(a.out) + ((start + token) * a.so_n + head * a.so_h) * QES;
+#pragma unroll
+  for (int j = 0; j < DB; ++j)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * j + 8 * g + 4 * h;
+      const float x0 = acc[j][4 * g] * inv, x1 = acc[j][4 * g + 1] * inv, x2 = acc[j][4 * g + 2] * inv, x3 = acc[j][4 * g + 3] * inv;
+      if (col + 3 < a.c.d) {
+        if constexpr (F32) {
+          typedef float any_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+          *reinterpret_cast<any_f32x4*>(out + col * 4) = any_f32x4{x0, x1, x2, x3};
+        } else {
+          typedef uint32_t any_u32x2 __attribute__((ext_vector_type(2), aligned(2)));
+          *reinterpret_cast<any_u32x2*>(out + col * 2) = any_u32x2{pack2<QDT>(x0, x1), pack2<QDT>(x2, x3)};
+        }
+      } else {
+        if (col < a.c.d) store_from_f32<QDT>(out, col, x0);
+        if (col + 1 < a.c.d) store_from_f32<QDT>(out, col + 1, x1);
+        if (col + 2 < a.c.d) store_from_f32<QDT>(out, col + 2, x2);
+      }
+    }
+}
+
+template <int DB, bool ODD, bool FEW>
+int launch(const ChunkArgs& a, hipStream_t s) {
+  auto kernel = chunk_attention_kernel<CDT, QDT, DB, ODD, FEW>;
+  constexpr size_t sums = FEW ? (size_t)2 * DB * 64 * 64 : 0, lds = sums > lds_bytes(DB, FEW) ? sums : lds_bytes(DB, FEW);
+  if (lds > 65536 && !planning())
+    LH_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  LH_LAUNCH(kernel, dim3((unsigned)((int64_t)a.slots * a.c.heads * a.splits)), dim3(256), lds, s, a);
+  return check_launch("chunk_attention");
+}
+
+template <int DB, bool ODD>
+int launch_rows(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s) {
+  if constexpr (!F32)
+    if (p.few) return launch<DB, ODD, true>(a, s);
+  return launch<DB, ODD, false>(a, s);
+}
+
+}  // namespace
+
+int LH_CHUNK_NAME(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s) {
+  if (p.odd) {
+    if (p.blocks <= 2) return launch_rows<2, true>(a, p, s);
+    if (p.blocks <= 4) return launch_rows<4, true>(a, p, s);
+    return launch_rows<8, true>(a, p, s);
+  }
+  switch (p.blocks) {
+    case 2: return launch_rows<2, false>(a, p, s);
+    case 3: return launch_rows<3, false>(a, p, s);
+    case 4: return launch_rows<4, false>(a, p, s);
+    case 6: return launch_rows<6, false>(a, p, s);
+    default: return launch_rows<8, false>(a, p, s);
+  }
+}
+
+}  // namespace lh

@@ -535,6 +535,7 @@ _CACHE_DTYPES = (torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3
 _SAMPLE_OPTIONS = ("temperature", "top_k", "top_p", "min_p")
 _PACK_SAMPLE = struct.Struct(_lib.SAMPLE_OPTS_FORMAT).pack
 _PACK_CACHE = struct.Struct(_lib.PAGED_CACHE_FORMAT).pack
+_PACK_ROTARY = struct.Struct(_lib.ROTARY_FORMAT).pack
 _F32_MAX = torch.finfo(torch.float32).max
 
 
@@ -573,16 +574,20 @@ def _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale):
             raise ValueError("k_cache and v_cache: innermost stride must be 1")
         if (st[0] < d and pages > 1) or (st[1] < d and heads > 1) or (st[2] < d and size > 1):
             raise ValueError("k_cache and v_cache: rows overlap")
-    rows = block_table.shape
-    if len(rows) != 2 or rows[0] != B or rows[1] < 1 or block_table.dtype != torch.int32:
-        raise ValueError(f"block_table must be an int32 tensor of shape [{B}, pages of a sequence], got {tuple(rows)} {block_table.dtype}")
-    step, inner = block_table.stride()
-    if inner != 1 and rows[1] > 1:
-        raise ValueError("block_table: innermost stride must be 1")
-    if step < rows[1]:
-        if B > 1:
-            raise ValueError("rows of block_table overlap")
-        step = rows[1]
+    if block_table is None:  # (for calls that name slots, which read none)
+        rows, step, table = (B, 1), 1, k_cache.data_ptr()
+    else:
+        table = block_table.data_ptr()
+        rows = block_table.shape
+        if len(rows) != 2 or rows[0] != B or rows[1] < 1 or block_table.dtype != torch.int32:
+            raise ValueError(f"block_table must be an int32 tensor of shape [{B}, pages of a sequence], got {tuple(rows)} {block_table.dtype}")
+        step, inner = block_table.stride()
+        if inner != 1 and rows[1] > 1:
+            raise ValueError("block_table: innermost stride must be 1")
+        if step < rows[1]:
+            if B > 1:
+                raise ValueError("rows of block_table overlap")
+            step = rows[1]
     if rows[1] * size >= 2**31 - 65536:
         raise ValueError("the block table must hold fewer than 2^31 - 65536 positions")
     if not (k_scale == 1.0 and v_scale == 1.0):
@@ -590,7 +595,7 @@ def _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale):
             raise ValueError("k_scale and v_scale belong to a cache of float8_e4m3fn")
         if not (0.0 < k_scale <= _F32_MAX and 0.0 < v_scale <= _F32_MAX):
             raise ValueError("k_scale and v_scale must be positive numbers")
-    return (_PACK_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), step, *sk[:3], *sv[:3], pages, rows[1], size,
+    return (_PACK_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), table, step, *sk[:3], *sv[:3], pages, rows[1], size,
                         heads, d, lh_dtype(dtype), k_scale, v_scale), heads, d, rows[1] * size)
 
 
@@ -789,6 +794,257 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, o
 def sample_workspace_bytes(B, V) -> int:
     """Bytes of temporary memory that sample takes for B rows of V words."""
     return int(_lib.load().lh_hip_sample_workspace_bytes(B, V))
+
+
+# ---- packed tokens of many sequences over a paged cache ------------------------------------------------------------------------
+def kv_pages(block_table, lengths, counts, free_pages, n_free, page_size, tokens, *, out=None):
+    """The pages of a step, and where its packed tokens lie: (lengths int32 [B], starts int32 [B + 1], positions int32 [tokens], slots int64 [tokens]).
+
+    Sequence b has `lengths[b]` positions (int32 [B]) and gets `counts[b]` tokens (int32 [B]), or has ended, where that is negative: its
+    length becomes 0.  block_table (int32 [B, P]) is updated: its first entries are the pages that the new length needs, those behind
+    them -1, as at the beginning.  free_pages (int32, one entry for every page of the cache) begins with the n_free (int32 [1]) pages that no sequence
+    has; both are updated.  Pages that are needed no longer go back first, in the order of sequences and positions; then missing ones are taken from
+    the list's end.  A sequence whose pages, with those that the ones before it miss, are more than there are, whose length would
+    pass the table or whose rows pass `tokens`, is refused: pages and length stay, its rows have no place.
+    Row i of the `tokens` packed ones belongs to the sequence with starts[b] <= i < starts[b + 1]; its position is positions[i], its slot (page *
+    page_size + slot of the page) slots[i], -1 both where it has no place.  `out` receives the lengths (may be `lengths`)."""
+    rows = block_table.shape
+    if len(rows) != 2 or rows[1] < 1 or block_table.dtype != torch.int32:
+        raise ValueError(f"block_table must be an int32 tensor of shape [sequences, pages of a sequence], got {tuple(rows)} {block_table.dtype}")
+    B, P = rows
+    step, inner = block_table.stride()
+    if inner != 1 and P > 1:
+        raise ValueError("block_table: innermost stride must be 1")
+    if step < P and B > 1:
+        raise ValueError("rows of block_table overlap")
+    _is_index(lengths, B, "lengths")
+    _is_index(counts, B, "counts")
+    if free_pages.dim() != 1 or free_pages.shape[0] < 1:
+        raise ValueError("free_pages must be an int32 vector with an entry for every page of the cache")
+    _is_index(free_pages, free_pages.shape[0], "free_pages")
+    _is_index(n_free, 1, "n_free")
+    size, tokens = int(page_size), int(tokens)
+    if size < 1 or P * size >= 2**31 - 65536:
+        raise ValueError("the block table must hold fewer than 2^31 - 65536 positions, with at least one on a page")
+    if not 0 <= tokens < 2**30:
+        raise ValueError(f"tokens must be between 0 and 2^30, got {tokens}")
+    if out is None:
+        out = lengths.new_empty(B)
+    _is_index(out, B, "out")
+    _on_current_device(block_table, lengths, counts, free_pages, n_free, out)
+    starts, positions = lengths.new_empty(B + 1), lengths.new_empty(tokens)
+    slots = lengths.new_empty(tokens, dtype=torch.int64)
+    _lib.check(_lib.load().lh_hip_kv_pages(
+        block_table.data_ptr(), step, lengths.data_ptr(), counts.data_ptr(), out.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(),
+        starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), B, P, free_pages.shape[0], size, tokens, _stream()), "kv_pages")
+    return out, starts, positions, slots
+
+
+def rotary_frequencies(turned, *, base=10000.0, factor=1.0, context=None, low=1.0, high=32.0, device="cuda"):
+    """Radians a position for the pairs of columns of `rotary`: float64 [turned / 2], base^(-2 i / turned).
+
+    For contexts `factor` times as long as those a model has seen: without `context` every frequency is divided by the factor.  With it (the
+    length that was seen) those that turn at most `low` times over it are divided, those that turn at least `high` times stay, between
+    them the two are mixed in proportion."""
+    turned = int(turned)
+    if turned < 2 or turned % 2:
+        raise ValueError(f"an even number of columns turns, got {turned}")
+    if not (base > 0 and factor > 0 and (context is None or (context > 0 and low < high))):
+        raise ValueError("base, factor and context must be positive, low below high")
+    f = base ** (-torch.arange(0, turned, 2, dtype=torch.float64) / turned)
+    if context is None:
+        f = f / factor
+    else:
+        stays = ((f * context / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        f = stays * f + (1.0 - stays) * f / factor
+    return f.to(device)
+
+
+def _packed_rows(t, what: str):
+    """(shape, strides of token and head) of a [N, heads, d] tensor."""
+    if t.dim() != 3 or t.dtype not in _FLOATS:
+        raise ValueError(f"{what} must be a float32, bfloat16 or float16 tensor of shape [tokens, heads, d], got {tuple(t.shape)} {t.dtype}")
+    st = t.stride()
+    if t.shape[2] != 1 and st[2] != 1:
+        raise ValueError("innermost stride must be 1")
+    return t.shape, st
+
+
+def _packed_out(out, x, what: str):
+    """The result of a call on x [N, heads, d], with rows of its own."""
+    if out is None:
+        return x.new_empty(x.shape)
+    if out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError(f"{what} must have the shape and dtype of its input")
+    (n, heads, d), st = out.shape, out.stride()
+    if d != 1 and st[2] != 1:
+        raise ValueError("innermost stride must be 1")
+    if n and heads and ((heads > 1 and st[1] < d) or (n > 1 and st[0] < d) or (n > 1 and heads > 1 and st[0] < (heads - 1) * st[1] + d and st[1] < (n - 1) * st[0] + d)):
+        raise ValueError(f"rows of {what} overlap")
+    return out
+
+
+def _turn(positions, freqs, N, d, interleaved, amplitude):
+    _is_index(positions, N, "positions")
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not 1 <= freqs.shape[0] <= d // 2 or (freqs.shape[0] > 1 and freqs.stride(0) != 1):
+        raise ValueError(f"freqs must be a contiguous float64 vector of 1 to {d // 2}, got {tuple(freqs.shape)} {freqs.dtype}")
+    return _PACK_ROTARY(positions.data_ptr(), freqs.data_ptr(), 2 * freqs.shape[0], 1 if interleaved else 0, amplitude)
+
+
+def rotary(x, positions, freqs, *, interleaved=False, amplitude=1.0, out=None):
+    """Rotary positions: of every head of x [N, heads, d] (any strides with unit stride along d) the column pairs (i, i + R / 2), or (2 i, 2 i + 1)
+    if `interleaved`, turn by positions[n] * freqs[i]: (a cos - b sin, b cos + a sin), times `amplitude`.  freqs: float64 [R / 2] (see
+    rotary_frequencies), radians a position; columns from R on stay.  positions: int32 [N].  `out` may be x.
+    Turning by -freqs takes it back, and takes a gradient from the result to x."""
+    (N, heads, d), sx = _packed_rows(x, "x")
+    turn = _turn(positions, freqs, N, d, interleaved, amplitude)
+    out = _packed_out(out, x, "out")
+    _on_current_device(x, positions, freqs, out)
+    if N and heads:
+        so = out.stride()
+        _lib.check(_lib.load().lh_hip_rotary(out.data_ptr(), x.data_ptr(), so[0], so[1], sx[0], sx[1], turn, N, heads, d, lh_dtype(x.dtype),
+                                             _stream()), "rotary")
+    return out
+
+
+def kv_store(k, v, k_cache, v_cache, slots, *, q=None, q_out=None, positions=None, freqs=None, interleaved=False, amplitude=1.0, k_scale=1.0,
+             v_scale=1.0):
+    """Keys and values of packed tokens into their slots of a paged cache (see kv_pages): returns (k_cache, v_cache).
+
+    k, v: [N, kv heads, d] (any strides with unit stride along d, so a projection's output can be passed as views) in the cache's dtype, or in
+    float32, bfloat16 or float16 for a cache of float8_e4m3fn, which holds e4m3(x / scale), clamped to +-448.  k_cache, v_cache:
+    [pages, kv heads, page size, d] as for kv_append.  slots int64 [N]: page * page size + slot; a token whose slot lies outside the cache (-1)
+    is left out, two tokens must not share one.  With `positions` and `freqs` the keys turn on their way (see rotary).  `q` [N, H, d] turns
+    with them, all rows of it, into `q_out` (which may be q; otherwise made here): then the result is (q_out, k_cache, v_cache)."""
+    (N, heads, d), sk = _packed_rows(k, "k")
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("k and v must have the same shape [tokens, kv heads, d] and dtype")
+    sv = v.stride()
+    if d != 1 and sv[2] != 1:
+        raise ValueError("innermost stride must be 1")
+    cache, cache_heads, cache_d = _paged_cache(k_cache, v_cache, None, 1, k_scale, v_scale)[:3]
+    if heads != cache_heads or d != cache_d:
+        raise ValueError(f"k and v have {heads} heads of {d}, the cache {cache_heads} of {cache_d}")
+    dtype = k.dtype
+    if dtype != k_cache.dtype and k_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError("k and v must have the cache's dtype (float32, bfloat16 or float16 for a cache of float8_e4m3fn)")
+    if slots.dtype != torch.int64:
+        raise ValueError(f"slots must be int64, got {slots.dtype}")
+    _is_vector(slots, N, torch.int64, "slots")
+    if (positions is None) != (freqs is None):
+        raise ValueError("positions and freqs go together")
+    turn = None if freqs is None else _turn(positions, freqs, N, d, interleaved, amplitude)
+    H, sq, so = 0, (0, 0), (0, 0)
+    if q is not None:
+        if turn is None:
+            raise ValueError("q is passed to be turned: positions and freqs are missing")
+        (rows, H, q_d), sq = _packed_rows(q, "q")
+        if rows != N or q_d != d or q.dtype != dtype:
+            raise ValueError(f"q must have shape [{N}, heads, {d}] and the dtype of k, got {tuple(q.shape)} {q.dtype}")
+        q_out = _packed_out(q_out, q, "q_out")
+        so = q_out.stride()
+    elif q_out is not None:
+        raise ValueError("q_out needs q")
+    _on_current_device(k, v, k_cache, v_cache, slots, q, q_out, positions, freqs)
+    if N:
+        _lib.check(_lib.load().lh_hip_kv_store(
+            cache, k.data_ptr(), v.data_ptr(), sk[0], sk[1], sv[0], sv[1], slots.data_ptr(), q_out.data_ptr() if H else None,
+            q.data_ptr() if H else None, so[0], so[1], sq[0], sq[1], turn, N, H, lh_dtype(dtype), _stream()), "kv_store")
+    return (k_cache, v_cache) if q is None else (q_out, k_cache, v_cache)
+
+
+def paged_attention_chunk(q, k_cache, v_cache, block_table, lengths, starts, *, scale=None, out=None, k_scale=1.0, v_scale=1.0, workspace=None):
+    """Causal attention of packed chunks of new tokens over their sequences' paged caches (laid out as for kv_append).
+
+    q, out: [N, H, d] (unit stride along d) in the cache's dtype, or bfloat16 / float16 for a cache of float8_e4m3fn, whose codes stand for
+    code * k_scale and code * v_scale.  H is a multiple of the cache's heads; head h reads head h // (H // kv heads).  Sequence b has the rows
+    starts[b] .. starts[b + 1] - 1 (int32 [B + 1], from 0 up); the last one is at position lengths[b] - 1 (int32 [B]: the new tokens count, and
+    have been stored), the others right before it, and each sees the positions up to its own: softmax(scale q . k_t) v_t, 0 where it sees none.
+    What lies at positions that a row does not see does not matter to it.  Rows from starts[B] on stay as they were.  scale: 1 / sqrt(d) if None.
+    `workspace` (uint8, see paged_attention_chunk_workspace_bytes): temporary memory, otherwise torch's allocator is asked; two
+    calls that overlap in time need one each."""
+    (N, H, d), sq = _packed_rows(q, "q")
+    dtype = q.dtype
+    B = block_table.shape[0]
+    cache, heads, cache_d, _ = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
+    if d != cache_d:
+        raise ValueError(f"q has a head dimension of {d}, the cache of {cache_d}")
+    if H == 0 or H % heads:
+        raise ValueError(f"{H} heads are no multiple of the cache's {heads}")
+    if dtype != k_cache.dtype and (k_cache.dtype != torch.float8_e4m3fn or dtype == torch.float32):
+        raise ValueError("q must have the cache's dtype (bfloat16 or float16 for a cache of float8_e4m3fn)")
+    _is_index(lengths, B, "lengths")
+    _is_index(starts, B + 1, "starts")
+    out = _packed_out(out, q, "out")
+    _on_current_device(q, k_cache, v_cache, block_table, lengths, starts, out)
+    if N == 0 or B == 0:
+        return out
+    lib = _lib.load()
+    need = lib.lh_hip_paged_attention_chunk_workspace_bytes(cache, N, B, H)
+    if need:
+        workspace = _vector_workspace(workspace, need, q)
+    so = out.stride()
+    _lib.check(lib.lh_hip_paged_attention_chunk(
+        cache, out.data_ptr(), q.data_ptr(), so[0], so[1], sq[0], sq[1], lengths.data_ptr(), starts.data_ptr(), N, B, H,
+        1.0 / math.sqrt(d) if scale is None else scale, lh_dtype(dtype), workspace.data_ptr() if need else None, need, _stream()),
+        "paged_attention_chunk")
+    return out
+
+
+def paged_attention_chunk_workspace_bytes(q, k_cache, v_cache, block_table) -> int:
+    """Bytes of temporary memory that paged_attention_chunk takes for these tensors (only their shapes and types matter)."""
+    cache = _paged_cache(k_cache, v_cache, block_table, block_table.shape[0], 1.0, 1.0)[0]
+    return int(_lib.load().lh_hip_paged_attention_chunk_workspace_bytes(cache, q.shape[0], block_table.shape[0], q.shape[1]))
+
+
+def rms_norm(x, gamma, eps=1e-5, *, residual=None, residual_out=None, out=None, out_dtype=None, scale=None, row_scales=None):
+    """Root-mean-square norm of the rows of x [M, C]: s / sqrt(mean(s^2) + eps) * gamma with s = x + residual (x where there is none), in f32.
+
+    x: float32, bfloat16 or float16, rows of any stride; gamma: float32 [C].  `residual` [M, C], float32 or of the dtype of x, becomes s, or
+    stays where `residual_out` (of its dtype) receives it.  out_dtype (default: that of x): float32, bfloat16, float16 or float8_e4m3fn; that one holds
+    e4m3(y / scale), clamped to +-448: with `scale` given (a number: what gemm_fp8 takes as scale_a) the result is `out`; without, every row has
+    the scale max |y| / 448 of its own (1 for a row of zeros) and the result is (out, row_scales), float32 [M]."""
+    if x.dim() != 2 or x.dtype not in _FLOATS or x.shape[1] < 1:
+        raise ValueError("rms_norm expects x of shape [M, C] in float32, bfloat16 or float16")
+    M, C = x.shape
+    _is_vector(gamma, C, torch.float32, "gamma")
+    if out is None:
+        out = x.new_empty((M, C), dtype=out_dtype or x.dtype)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError(f"out must be {out_dtype}, got {out.dtype}")
+    if out.dtype not in _CACHE_DTYPES:
+        raise ValueError("out must be float32, bfloat16, float16 or float8_e4m3fn")
+    _is_matrix(out, M, C, "out")
+    _is_matrix(x, M, C, "x")
+    if residual is not None:
+        _is_matrix(residual, M, C, "residual")
+        if residual.dtype != x.dtype and residual.dtype != torch.float32:
+            raise ValueError("residual must be float32 or have the dtype of x")
+        if residual_out is None:
+            residual_out = residual
+        elif residual_out.dtype != residual.dtype:
+            raise ValueError("residual_out must have the dtype of residual")
+        _is_matrix(residual_out, M, C, "residual_out")
+    elif residual_out is not None:
+        raise ValueError("residual_out needs residual")
+    coded = out.dtype == torch.float8_e4m3fn
+    if scale is not None and not (coded and 0.0 < scale <= _F32_MAX):
+        raise ValueError("scale belongs to a result of float8_e4m3fn, and must be a positive number")
+    if coded and scale is None:
+        if row_scales is None:
+            row_scales = gamma.new_empty(M)
+        _is_vector(row_scales, M, torch.float32, "row_scales")
+    elif row_scales is not None:
+        raise ValueError("row_scales belong to a result of float8_e4m3fn without a scale")
+    _on_current_device(x, gamma, residual, residual_out, out, row_scales)
+    if M:
+        _lib.check(_lib.load().lh_hip_rms_norm(
+            out.data_ptr(), x.data_ptr(), gamma.data_ptr(), residual.data_ptr() if residual is not None else None,
+            residual_out.data_ptr() if residual is not None else None, row_scales.data_ptr() if row_scales is not None else None,
+            scale or 1.0, M, C, out.stride(0), x.stride(0), residual.stride(0) if residual is not None else 0,
+            residual_out.stride(0) if residual is not None else 0, eps, lh_dtype(x.dtype),
+            lh_dtype(residual.dtype) if residual is not None else 0, lh_dtype(out.dtype), _stream()), "rms_norm")
+    return out if row_scales is None else (out, row_scales)
 
 
 def release_scratch() -> None:
