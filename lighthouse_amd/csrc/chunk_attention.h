@@ -18,6 +18,7 @@ struct ChunkArgs {
   FastDiv by_group;        // rows of a sequence and key / value head: G of a token
   int32_t tile_rows, tile_shift;  // rows a workgroup takes, a power of 2
   int32_t slots;           // workgroups' places for tiles
+  int32_t ranked;          // tiles by weight, or by place
   int32_t share, splits;   // positions a workgroup takes, workgroups for the positions of the table
   float scale_log2e;       // above 0
   uint32_t q_and, q_xor;   // on the queries' words: their signs change, or they become 0
@@ -52,6 +53,41 @@ __device__ __forceinline__ int chunk_last(const ChunkArgs& a, int at, F begins) 
     span = min(step, span - last * step);
   }
   return __builtin_amdgcn_readfirstlane(b);
+}
+
+// The tile that workgroup `rank` of a head takes, heaviest first: for up to 32 sequences (`ranked`) first each one's last tile, then each one's last
+// but one, and so on, since a later tile sees more positions; otherwise the places in falling order.
+__device__ __forceinline__ bool chunk_tile(const ChunkArgs& a, int rank, int* seq, int* tile) {
+  if (a.ranked) {
+    const int lane = threadIdx.x & 63, i = min(lane, a.B - 1);
+    const int rows = max(chunk_start(a, i + 1) - chunk_start(a, i), 0) * a.G;
+    const int tiles = lane < a.B ? (int)((uint32_t)(rows + a.tile_rows - 1) >> a.tile_shift) : 0;
+    for (int level = 0;;) {  // (of each sequence, counted from its last tile)
+      const uint64_t live = __builtin_amdgcn_ballot_w64(tiles > level);
+      const int n = (int)__popcll(live);
+      if (n == 0) return false;
+      int same = tiles > level ? tiles : 0x7fffffff;  // up to here as many sequences have a tile
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) same = min(same, __shfl_xor(same, o));
+      same = __builtin_amdgcn_readfirstlane(same);
+      const int64_t there = (int64_t)n * (same - level);
+      if (rank < there) {
+        level += rank / n;
+        uint64_t left = live;
+        for (int k = rank % n; k > 0; --k) left &= left - 1;
+        *seq = (int)__builtin_ctzll(left);
+        *tile = __builtin_amdgcn_readlane(tiles, *seq) - 1 - level;
+        return true;
+      }
+      rank -= (int)there;
+      level = same;
+    }
+  }
+  const int place = a.slots - 1 - rank;
+  *seq = chunk_last(a, place, [&](int i) { return chunk_place(a, i); });
+  const int start = __builtin_amdgcn_readfirstlane(chunk_start(a, *seq)), count = __builtin_amdgcn_readfirstlane(chunk_start(a, *seq + 1)) - start;
+  *tile = place - __builtin_amdgcn_readfirstlane(chunk_place(a, *seq));
+  return *tile >= 0 && count > 0 && *tile <= (count * a.G - 1) >> a.tile_shift;
 }
 
 // Launches the kernel of a pair of types (in chunk_attention.hip, compiled once for each).

@@ -55,13 +55,16 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
   p.odd = c.d % piece != 0;
   const int blocks = (c.d + 31) / 32;
   p.blocks = p.odd ? (blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8) : blocks <= 2 ? 2 : blocks <= 4 ? blocks : blocks <= 6 ? 6 : 8;
-  // Tiles of 32 rows where the sequences have no more on average.
-  p.few = cache_dtype != LH_F32 && N * G <= 32 * B;
+  // Tiles of 32 rows where the sequences have no more on average (and the registers suffice for two waves' worth of positions).
+  p.few = cache_dtype != LH_F32 && p.blocks <= 6 && N * G <= 32 * B;
   p.tile_rows = p.few ? 32 : 128;
   const int64_t slots = N * G / p.tile_rows + B;
   p.slots = (int)slots;
-  const int64_t items = slots * c.heads, cus = num_cus();
-  int64_t splits = (2 * cus + items - 1) / items;
+  // As many shares of positions as the workgroups that run at once allow for, of tiles that there probably are (a place more per sequence may
+  // be empty).  One more would be a second round of workgroups for a few.
+  const int64_t items = slots * c.heads, tiles = N * G / p.tile_rows > B ? N * G / p.tile_rows : B < N ? B : N;
+  int64_t splits = (p.few && p.blocks > 2 ? 1 : 2) * num_cus() / (tiles * c.heads);
+  splits = splits < 1 ? 1 : splits;
   const int64_t most = (c.capacity() + 255) / 256;
   splits = splits > most ? most : splits;
   const int64_t share = (c.capacity() + splits - 1) / splits;
@@ -108,7 +111,7 @@ int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const v
              "%s: workspace too small or not 256-byte aligned: %zu of %zu bytes", what, workspace_bytes, p.total());
   a.out = out, a.q = q, a.so_n = out_stride_n, a.so_h = out_stride_h, a.sq_n = q_stride_n, a.sq_h = q_stride_h, a.lengths = lengths, a.starts = starts;
   a.N = (int32_t)N, a.B = (int32_t)B, a.H = (int32_t)H, a.G = (int32_t)(H / a.c.heads), a.by_group = FastDiv((uint32_t)a.G);
-  a.tile_rows = p.tile_rows, a.tile_shift = p.few ? 5 : 7, a.slots = p.slots, a.share = p.share, a.splits = p.splits, a.width = 32 * p.blocks;
+  a.tile_rows = p.tile_rows, a.tile_shift = p.few ? 5 : 7, a.slots = p.slots, a.ranked = B > 1 && B <= 32, a.share = p.share, a.splits = p.splits, a.width = 32 * p.blocks;
   const double factor = (double)scale * a.c.k_scale * 1.4426950408889634;
   a.scale_log2e = scale == 0.0f ? 1.0f : (float)(factor < 0.0 ? -factor : factor);
   a.q_and = scale == 0.0f ? 0u : ~0u, a.q_xor = scale < 0.0f ? (dtype == LH_F32 ? 0x80000000u : 0x80008000u) : 0u;

@@ -11,8 +11,9 @@
 //    positions are shared out between the waves, whose results are brought together at the end.
 //  * Long caches of few tiles are cut into shares of positions; a second launch joins them.
 //
-// P in 16 bits is split into two values of the type, the second what the first has lost: with one alone the result's error against 64 bits is
-// 1.4 times that of its own rounding.
+// Many rows are bound by the arithmetic: P is rounded to 16 bits once, as in attention over tensors, and the sum is that of the rounded values,
+// so that the weights add up to 1; the result's error against 64 bits is up to 1.4 times that of its own rounding.  Few rows are bound by
+// memory: there P is the sum of two values of the type, the second what the first has lost.
 #include "chunk_attention.h"
 
 #ifndef LH_CHUNK_CDT
@@ -28,7 +29,6 @@ constexpr int CES = CDT == LH_F8E4M3 ? 1 : F32 ? 4 : 2;  // bytes of an element 
 constexpr int QES = F32 ? 4 : 2;                         // of a query's, and in LDS
 constexpr int PE = F32 ? 4 : 8;                          // elements of a piece: 16 bytes in LDS
 constexpr int PW = PE * CES / 4;                         // its words in the cache
-constexpr int PARTS = F32 ? 1 : 2;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -41,6 +41,15 @@ __device__ __forceinline__ f32x16 mma(u32x4 x, u32x4 y, f32x16 c) {
 
 // (By value: a bit cast of a vector's element itself reads its first one.)
 __device__ __forceinline__ float f32_of(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
+
+// The same number, which the compiler takes for another: comparisons with it are made where they are used and not held over the loop (a
+// pair of scalar registers each; where those did not suffice, hipcc of ROCm 7.2 put copies of vector registers at the wrong side of the
+// lanes' return from a branch).
+__device__ __forceinline__ int hide(int x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
 
 // Waits for this wave's LDS accesses and for the workgroup, but for no load on its way to registers.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -63,11 +72,11 @@ __device__ __forceinline__ void move_down(uint32_t* w, int skip) {
 }
 
 // Columns col .. col + PE - 1 of a row of d elements of ES bytes; those behind its end are 0.  The row is there in any case.  ODD: d is no multiple
-// of a piece; the last piece is loaded so that it ends with the row and moved down.
-template <int ES, bool ODD>
+// of a piece; the last piece is loaded so that it ends with the row and moved down.  SHORT: a row may be shorter than a piece.
+template <int ES, bool ODD, bool SHORT>
 __device__ __forceinline__ void load_columns(uint32_t* w, const uint8_t* row, int col, int d) {
   constexpr int W = PE * ES / 4;
-  if (ODD && d < PE) {
+  if (SHORT && d < PE) {
 #pragma unroll
     for (int i = 0; i < W; ++i) w[i] = 0;
 #pragma unroll
@@ -90,16 +99,24 @@ __device__ __forceinline__ void load_columns(uint32_t* w, const uint8_t* row, in
     w[0] = v[0], w[1] = v[1];
   }
 }
-// What of it is not in the row becomes 0 (apart from the load, so that nothing waits for that).
-template <int ES, bool ODD>
-__device__ __forceinline__ void settle_columns(uint32_t* w, int col, int d, bool there) {
+// What of it is not in the row becomes 0, all of it if `there` is (otherwise ones), apart from the load, so that nothing waits for that.  (Masks in
+// vector registers: as conditions they would take a pair of scalar ones each.)
+template <int ES, bool ODD, bool SHORT>
+__device__ __forceinline__ void settle_columns(uint32_t* w, int col, int d, uint32_t there) {
   constexpr int W = PE * ES / 4;
-  if (ODD && d >= PE) {
+  if (ODD && (!SHORT || d >= PE)) {
     const int skip = max(col - (d - PE), 0);
     if (skip > 0) move_down<W, ES>(w, min(skip, PE - 1));
   }
+  const uint32_t keep = there & (uint32_t)((col - d) >> 31);
 #pragma unroll
-  for (int i = 0; i < W; ++i) w[i] = there && col < d ? w[i] : 0u;
+  for (int i = 0; i < W; ++i) w[i] &= keep;
+}
+
+// The sum of two values of the queries' type and of x.
+__device__ __forceinline__ float add_pair(uint32_t w, float x) {
+  if constexpr (QDT == LH_BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), bf16x2_t{(__bf16)1.0f, (__bf16)1.0f}, x, false);
+  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), f16x2_t{(_Float16)1.0f, (_Float16)1.0f}, x, false);
 }
 
 // Two e4m3 codes (the lower or upper two of a word) as two values of the queries' type: exact.
@@ -112,60 +129,59 @@ __device__ __forceinline__ u32x4 in_lds(const uint32_t* w) {
   if constexpr (CDT == LH_F8E4M3) return u32x4{of_e4m3<false>(w[0]), of_e4m3<true>(w[0]), of_e4m3<false>(w[1]), of_e4m3<true>(w[1])};
   else return u32x4{w[0], w[1], w[2], w[3]};
 }
-// Whether a piece in LDS holds an infinity or a NaN.
-__device__ __forceinline__ bool any_wild(u32x4 w) {
-  bool wild = false;
+// Not 0 where a piece in LDS holds an infinity or a NaN: an exponent of ones carries into the sign's place.
+__device__ __forceinline__ uint32_t wild_bits(u32x4 w) {
+  constexpr uint32_t top = F32 ? 0x7f800000u : QDT == LH_BF16 ? 0x7f807f80u : 0x7c007c00u, one = F32 ? 0x00800000u : QDT == LH_BF16 ? 0x00800080u : 0x04000400u;
+  uint32_t bits = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (F32) {
-      wild |= (w[i] & 0x7f800000u) == 0x7f800000u;
-    } else {
-      constexpr uint32_t top = QDT == LH_BF16 ? 0x7f80u : 0x7c00u;
-      wild |= (w[i] & top) == top || (w[i] >> 16 & top) == top;
-    }
-  }
-  return wild;
+  for (int i = 0; i < 4; ++i) bits |= (w[i] & top) + one;
+  return bits & (F32 ? 0x80000000u : 0x80008000u);
 }
 
-// Widths that leave a CU two workgroups (registers).
-constexpr int occupancy(int blocks, bool few) { return blocks <= (few ? 3 : 4) ? 2 : 1; }
+// Workgroups that a CU holds, by their registers.
+constexpr int occupancy(int blocks, bool few) { return blocks <= (few ? 2 : 4) ? 2 : 1; }
+// Steps ahead whose keys and values are on their way to registers: as many as these suffice for.  0: they are asked for when their place is free.
+constexpr int ahead(int blocks, bool odd, bool few) { return F32 || (CES == 1 && odd && !few && blocks == 4) ? 0 : few ? (blocks <= 4 ? 2 : 1) : blocks <= 3 ? 2 : blocks <= 6 ? 1 : 0; }
 
 constexpr int keys_of(bool few) { return few && !F32 ? 128 : 64; }
-constexpr size_t row_elems(int blocks) { return 32 * blocks + 8; }  // (16 or 32 bytes apart: the banks of neighbouring rows differ)
-constexpr size_t lds_bytes(int blocks, bool few) { return 2 * keys_of(few) * row_elems(blocks) * QES; }
+// Elements from one row to the next: of keys, whose rows are read 16 bytes a lane, so that neighbours lie 4 (f32: 8) banks apart; of values, of
+// which 16-bit ones are read four rows at a time, 64 bytes of each: 16 or 48 banks apart.
+constexpr int k_row_elems(int blocks) { return 32 * blocks + 8; }
+constexpr int v_row_elems(int blocks) { return F32 ? 32 * blocks + 8 : blocks == 3 ? 96 : 32 * blocks + 32; }
+constexpr size_t stage_bytes(int blocks, bool few) { return (size_t)keys_of(few) * (k_row_elems(blocks) + v_row_elems(blocks)) * QES; }
+// Steps that are in LDS: the next one beside the one that is read, where two do not cost a CU a workgroup.
+constexpr int stages(int blocks, bool few) { return 2 * stage_bytes(blocks, few) <= (occupancy(blocks, few) == 2 ? 77000 : 153000) ? 2 : 1; }
+constexpr size_t lds_bytes(int blocks, bool few) { return stages(blocks, few) * stage_bytes(blocks, few); }
 
 // DB: width in 32 columns.  FEW: 32 rows, positions shared out between the waves; otherwise 128 rows.
 template <int CACHE, int QUERY, int DB, bool ODD, bool FEW>  // (the types: for the name)
 __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kernel(ChunkArgs a) {
-  constexpr int D = 32 * DB, KROW = row_elems(DB), KEYS = keys_of(FEW);
+  constexpr int D = 32 * DB, KROW = k_row_elems(DB), VROW = v_row_elems(DB), KEYS = keys_of(FEW);
+  constexpr int PARTS = FEW ? 2 : 1;              // 16-bit values that a probability is the sum of
   constexpr int WK = FEW ? 4 : 1;                 // waves that share out a step's positions
   constexpr int NI = KEYS / 32 / WK;              // 32-position tiles of a wave
   constexpr int CPR = D / PE;                     // pieces of a row
   constexpr int NP = KEYS * CPR / 256;            // pieces a thread brings, of keys and of values
   constexpr int SD = F32 ? D / 8 : D / 16;
-  constexpr bool AHEAD = !F32 && DB <= (FEW ? 4 : 6);                    // a step's keys and values are requested a step ahead
+  constexpr int RS = ahead(DB, ODD, FEW), STAGES = stages(DB, FEW);
+  constexpr bool SHORT = ODD && DB == 2;
+  constexpr bool TWO = STAGES == 2 || RS == 2;    // steps go by in pairs
   static_assert(NI >= 1 && NP * 256 == KEYS * CPR, "");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   typedef typename std::conditional<F32, float, uint16_t>::type elem;
-  elem* const Ks = reinterpret_cast<elem*>(smem);
-  elem* const Vs = Ks + KEYS * KROW;
   __shared__ int64_t k_at[2][KEYS], v_at[2][KEYS];  // where the rows of a step lie, in elements; below 0: nowhere
-  __shared__ uint64_t held[3][KEYS / 64];           // which positions of a step there are (read while a wave ahead notes those of two steps later)
-  __shared__ int32_t wild[4], first_wild[D];
+  __shared__ uint64_t held[8][KEYS / 64];           // which positions of a step there are (noted up to four steps before they are read)
+  __shared__ int32_t wild[2][4], first_wild[D];
   __shared__ float2 stats[4][32];
 
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int items = a.slots * a.c.heads, split = blockIdx.x / items, item = blockIdx.x - split * items;
-  // Later tiles of a sequence see more positions: they begin first.
-  const int place = a.slots - 1 - item / a.c.heads, hk = item % a.c.heads;
-
-  // The sequence whose places hold this one: the last that begins at or before it.
-  const int b = chunk_last(a, place, [&](int i) { return chunk_place(a, i); });
+  const int hk = item % a.c.heads;
+  int b, tile;
+  if (!chunk_tile(a, item / a.c.heads, &b, &tile)) return;
   const int start = __builtin_amdgcn_readfirstlane(chunk_start(a, b));
   const int count = max(__builtin_amdgcn_readfirstlane(chunk_start(a, b + 1)) - start, 0);
-  const int tile = place - (int)((uint32_t)(start * a.G) >> a.tile_shift) - b;
-  if (tile < 0 || tile > (count * a.G - 1) >> a.tile_shift) return;
   const int first = tile << a.tile_shift, rows = min(a.tile_rows, count * a.G - first);
   const int length = __builtin_amdgcn_readfirstlane(min(max(a.lengths[b], 0), a.c.capacity()));
   const int base = length - count;  // position of the sequence's first new token
@@ -186,13 +202,13 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
 
   // Queries: lane (r32, h) has columns 16 s + 8 h .. + 7 of its row (f32: 8 s + 4 h .. + 3); where the registers do not suffice for them, they are
   // read again in every step.
-  constexpr bool Q_HELD = F32 ? DB <= 3 || DB == 6 : !(DB == 8 && ODD && FEW);
+  constexpr bool Q_HELD = F32 ? DB <= 3 || DB == 6 : !(DB == 8 && ODD);
   const uint8_t* const q = static_cast<const uint8_t*>(a.q) + ((start + (row_live ? token : 0)) * a.sq_n + (row_live ? head : hk * a.G) * a.sq_h) * QES;
   auto query = [&](const uint8_t* from, int s, int d) {
     const int col = (2 * s + h) * PE;
     uint32_t w[4];
-    load_columns<QES, ODD>(w, from, col, d);
-    settle_columns<QES, ODD>(w, col, d, row_live);
+    load_columns<QES, ODD, SHORT>(w, from, col, d);
+    settle_columns<QES, ODD, SHORT>(w, col, d, row_live ? ~0u : 0u);
     // (A scale below 0 is that of the queries, so that -inf is the score of what a row does not see; with one of 0 they are 0.)
     return (u32x4{w[0], w[1], w[2], w[3]} & a.q_and) ^ a.q_xor;
   };
@@ -228,73 +244,108 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
     k_at[step & 1][tid] = there ? page * a.c.sk.z + slot * a.c.sk.t : -1;
     v_at[step & 1][tid] = there ? page * a.c.sv.z + slot * a.c.sv.t : -1;
     const uint64_t some = __builtin_amdgcn_ballot_w64(there);
-    if (lane == 0) held[step % 3][wave] = some;
+    if (lane == 0) held[step & 7][wave] = some;
   };
-  uint32_t kr[AHEAD ? NP : 1][PW], vr[AHEAD ? NP : 1][PW];
-  uint32_t there = 0;  // which of the thread's rows there are
-  auto request = [&](int step, int i, uint32_t* k, uint32_t* v) {
+  uint32_t kr[RS > 0 ? RS : 1][RS > 0 ? NP : 1][PW], vr[RS > 0 ? RS : 1][RS > 0 ? NP : 1][PW];
+  uint32_t there[RS > 0 ? RS : 1] = {};  // which of the thread's rows there are
+  auto request = [&](int step, int i, uint32_t* k, uint32_t* v, uint32_t& some) {
     const int piece = tid + 256 * i, key = piece / CPR, col = (piece - key * CPR) * PE;
     const int64_t k_row = k_at[step & 1][key], v_row = v_at[step & 1][key];
-    there = (there & ~(1u << i)) | (uint32_t)(k_row >= 0) << i;
-    load_columns<CES, ODD>(k, kb + max(k_row, (int64_t)0) * CES, col, a.c.d);
-    load_columns<CES, ODD>(v, vb + max(v_row, (int64_t)0) * CES, col, a.c.d);
+    some = (some & ~(1u << i)) | (uint32_t)(k_row >= 0) << i;
+    const int d = hide(a.c.d);
+    load_columns<CES, ODD, SHORT>(k, kb + max(k_row, (int64_t)0) * CES, col, d);
+    load_columns<CES, ODD, SHORT>(v, vb + max(v_row, (int64_t)0) * CES, col, d);
   };
-  auto put = [&](int i, uint32_t* k, uint32_t* v, bool look) {  // into LDS; whether a value is an infinity or a NaN, if asked for
+  auto put = [&](elem* Ks, int i, uint32_t* k, uint32_t* v, uint32_t some, bool full, bool look) {  // into LDS; not 0 where a value is an infinity or a NaN, if asked for
     const int piece = tid + 256 * i, key = piece / CPR, col = (piece - key * CPR) * PE;
-    settle_columns<CES, ODD>(k, col, a.c.d, there >> i & 1);
-    settle_columns<CES, ODD>(v, col, a.c.d, there >> i & 1);
+    if (!full) {
+      const int d = hide(a.c.d);
+      const uint32_t there = (uint32_t)((int32_t)(some << (31 - i)) >> 31);
+      settle_columns<CES, ODD, SHORT>(k, col, d, there);
+      settle_columns<CES, ODD, SHORT>(v, col, d, there);
+    }
     const u32x4 kw = in_lds(k), vw = in_lds(v);
     *reinterpret_cast<u32x4*>(Ks + key * KROW + col) = kw;
-    *reinterpret_cast<u32x4*>(Vs + key * KROW + col) = vw;
-    return look && any_wild(vw);
+    *reinterpret_cast<u32x4*>(Ks + KEYS * KROW + key * VROW + col) = vw;
+    return look ? wild_bits(vw) : 0u;
   };
-
-  if (steps > 0) {
-    const int p0 = look_up(0), p1 = look_up(1);
-    note(0, p0);
-    note(1, p1);
-    lds_barrier();
-    if constexpr (AHEAD)
+  // Some row does not see all of a step's positions: those it does not see must not reach it by a 0 times an infinity.
+  auto partial = [&](int step) { return k0 + (step + 1) * KEYS > base + (int)a.by_group.div((uint32_t)first) + 1; };
+  elem* const stage0 = reinterpret_cast<elem*>(smem);
+  constexpr int kStage = STAGES == 2 ? KEYS * (KROW + VROW) : 0;  // elements from one stage to the other
+  // A step's keys and values into its stage, those RS steps later on their way.
+  auto bring = [&](int step, auto set) {
+    constexpr int S = decltype(set)::value;
+    elem* const Ks = stage0 + (step & 1) * kStage;
+    const bool look = partial(step);
+    bool full = a.c.d == D;  // nothing of the step has to become 0
 #pragma unroll
-      for (int i = 0; i < NP; ++i) request(0, i, kr[i], vr[i]);
-  }
-#pragma unroll 1
-  for (int step = 0; step < steps; ++step) {
-    const int j0 = k0 + step * KEYS;
-    // Some row does not see all of this step's positions: those it does not see must not reach it by a 0 times an infinity.
-    const bool partial = j0 + KEYS > base + (int)a.by_group.div((uint32_t)first) + 1;
-    if (step > 0) lds_barrier();  // the step before has been read
-    bool odd_one = false;
-    if constexpr (AHEAD) {
+    for (int w = 0; w < KEYS / 64; ++w) full = full && held[step & 7][w] == ~0ull;
+    full = __builtin_amdgcn_readfirstlane(full);
+    uint32_t odd_one = 0;
+    if constexpr (RS > 0) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) odd_one |= put(i, kr[i], vr[i], partial);
-      if (step + 1 < steps)
+      for (int i = 0; i < NP; ++i) odd_one |= put(Ks, i, kr[S % RS][i], vr[S % RS][i], there[S % RS], full, look);
+      if (step + RS < steps)
 #pragma unroll
-        for (int i = 0; i < NP; ++i) request(step + 1, i, kr[i], vr[i]);
+        for (int i = 0; i < NP; ++i) request(step + RS, i, kr[S % RS][i], vr[S % RS][i], there[S % RS]);
     } else {
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        uint32_t k[PW], v[PW];
-        request(step, i, k, v);
-        odd_one |= put(i, k, v, partial);
+        uint32_t k[PW], v[PW], some = 0;
+        request(step, i, k, v, some);
+        odd_one |= put(Ks, i, k, v, some, full, look);
         if (i % (ODD ? 2 : 4) == 1) asm volatile("" ::: "memory");  // (a few of each on their way at once)
       }
     }
-    const int page = look_up(step + 2);
-    if (partial) {
-      const bool some = __any(odd_one);
-      if (lane == 0) wild[wave] = some;
+    if (look) {
+      const bool some = __any(odd_one != 0);
+      if (lane == 0) wild[TWO ? step & 1 : 0][wave] = some;
     }
+  };
+  typedef std::integral_constant<int, 0> even_t;
+
+  // What the table says for later steps: asked for as long ahead as keys and values are, since what is asked for later comes later.
+  constexpr int QUEUE = RS > 0 ? RS : 1;
+  int queue[QUEUE];
+  if (steps > 0) {
+    int pages[RS + 2];
+#pragma unroll
+    for (int i = 0; i < RS + 2; ++i) pages[i] = look_up(i);
+#pragma unroll
+    for (int i = 0; i < QUEUE; ++i) queue[i] = look_up(RS + 2 + i);
+    note(0, pages[0]);
+    note(1, pages[1]);
     lds_barrier();
+    if constexpr (RS > 0) {
+#pragma unroll
+      for (int r = 0; r < RS; ++r)
+        if (r < steps)
+#pragma unroll
+          for (int i = 0; i < NP; ++i) request(r, i, kr[r][i], vr[r][i], there[r]);
+      lds_barrier();  // (where the first ones lie has been read)
+#pragma unroll
+      for (int i = 2; i < RS + 2; ++i) note(i, pages[i]);
+      lds_barrier();
+    }
+    bring(0, even_t());
+  }
+  // Step `step`, whose parity is known to the compiler.
+  auto take = [&](int step, auto parity) {
+    constexpr int P = decltype(parity)::value;
+    elem* const Ks = stage0 + P * kStage;
+    elem* const Vs = Ks + KEYS * KROW;
+    const int j0 = k0 + step * KEYS;
+    lds_barrier();  // this step is in its place; the one before has been read
     bool some_wild = false;
-    if (partial) some_wild = wild[0] | wild[1] | wild[2] | wild[3];
+    if (partial(step)) some_wild = wild[P][0] | wild[P][1] | wild[P][2] | wild[P][3];
     if (__builtin_expect(some_wild, 0)) {
       // Such values become 0; a column's first one makes a NaN of the rows that see it (below).
       for (int c = tid; c < D; c += 256) first_wild[c] = 0x7fffffff;
       lds_barrier();
 #pragma unroll 1
       for (int c = tid; c < KEYS * D; c += 256) {
-        elem* const x = Vs + c / D * KROW + c % D;
+        elem* const x = Vs + c / D * VROW + c % D;
         const uint32_t bits = F32 ? __builtin_bit_cast(uint32_t, (float)*x) : (uint32_t)*x, top = F32 ? 0x7f800000u : QDT == LH_BF16 ? 0x7f80u : 0x7c00u;
         if ((bits & top) == top) {
           *x = 0;
@@ -303,7 +354,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
       }
       lds_barrier();
     }
-    const uint64_t all_held = KEYS == 64 ? held[step % 3][0] : held[step % 3][wave / 2] >> (32 * (wave & 1)) | 0xffffffff00000000ull;
+    const uint64_t all_held = KEYS == 64 ? held[step & 7][0] : held[step & 7][wave / 2] >> (32 * (wave & 1)) | 0xffffffff00000000ull;
     const int kw0 = FEW && WK > 1 ? 32 * NI * wave : 0;  // the wave's first position of the step
     const int j0w = j0 + kw0;
     if (wave_live && wave_last >= j0w) {
@@ -339,11 +390,15 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
         // Bit p of `seen`: whether the row sees position j0w + p.
         uint64_t seen = last_seen < j0w ? 0ull : last_seen - j0w >= 63 ? ~0ull : (2ull << (last_seen - j0w)) - 1;
         seen = (seen & all_held) >> (4 * h);
+        const uint32_t half[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-          for (int v = 0; v < 16; ++v)
-            if (!(seen >> (32 * i + 8 * (v >> 2) + (v & 3)) & 1)) s[i][v] = -INFINITY;
+          for (int v = 0; v < 16; ++v) {
+            const int bit = 8 * (v >> 2) + (v & 3);
+            const uint32_t keep = (uint32_t)((int32_t)(half[i] << (31 - bit)) >> 31);  // (bit by bit, no condition)
+            s[i][v] = f32_of((bits_of(s[i][v]) & keep) | (0xff800000u & ~keep));
+          }
       }
       // The maximum is followed with a delay: nothing moves until a p would pass 2^10, which is as accurate as one of 1, and then for all lanes.
       float mx = s[0][0];
@@ -369,14 +424,14 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           s[i][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][v], a.scale_log2e, -off));
-          l_run += s[i][v];
+          if constexpr (F32 || PARTS == 2) l_run += s[i][v];
         }
       if constexpr (F32) {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const float* vrow = reinterpret_cast<const float*>(Vs) + (kw0 + 32 * i + 8 * (v >> 2) + 4 * h + (v & 3)) * KROW + r32;
+            const float* vrow = reinterpret_cast<const float*>(Vs) + (kw0 + 32 * i + 8 * (v >> 2) + 4 * h + (v & 3)) * VROW + r32;
 #pragma unroll
             for (int j = 0; j < DB; ++j) acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[32 * j], s[i][v], acc[j], 0, 0, 0);
             if (v % (DB > 6 ? 2 : 4) == (DB > 6 ? 1 : 3)) asm volatile("" ::: "memory");  // (values of a few positions fetched ahead)
@@ -394,13 +449,14 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
             for (int e = 0; e < 4; ++e) {
               const float p0 = s[i][8 * u + 2 * e], p1 = s[i][8 * u + 2 * e + 1];
               pf[0][e] = pack2<QDT>(p0, p1);
+              if constexpr (PARTS == 1) l_run = add_pair(pf[0][e], l_run);  // (what the values are weighted with)
               if constexpr (PARTS == 2) pf[PARTS - 1][e] = pack2<QDT>(p0 - unpack_lo<QDT>(pf[0][e]), p1 - unpack_hi<QDT>(pf[0][e]));
             }
 #pragma unroll
             for (int j = 0; j < DB; ++j) {
-              const elem* p0 = Vs + (kw0 + 32 * i + 16 * u + tr_row) * KROW + 32 * j + tr_col;
+              const elem* p0 = Vs + (kw0 + 32 * i + 16 * u + tr_row) * VROW + 32 * j + tr_col;
               const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p0);
-              const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p0 + 8 * KROW));
+              const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p0 + 8 * VROW));
               const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
               const u32x4 vf = {l2[0], l2[1], h2[0], h2[1]};
 #pragma unroll
@@ -409,14 +465,28 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
           }
       }
       if (__builtin_expect(some_wild, 0)) {
+        const int sees_up_to = min(max(last_seen - j0, -1), KEYS);
 #pragma unroll
         for (int j = 0; j < DB; ++j)
 #pragma unroll
-          for (int v = 0; v < 16; ++v)
-            if (first_wild[32 * j + 8 * (v >> 2) + 4 * h + (v & 3)] <= last_seen - j0) acc[j][v] = NAN;
+          for (int v = 0; v < 16; ++v) {
+            const uint32_t reached = (uint32_t)((first_wild[32 * j + 8 * (v >> 2) + 4 * h + (v & 3)] - 1 - sees_up_to) >> 31);
+            acc[j][v] = f32_of(bits_of(acc[j][v]) | reached);  // (all ones: a NaN)
+          }
       }
     }
-    note(step + 2, page);
+    __builtin_amdgcn_sched_barrier(0);  // (what waits for memory comes behind the arithmetic)
+    if (step + 1 < steps) {
+      if constexpr (STAGES == 1) lds_barrier();
+      bring(step + 1, std::integral_constant<int, TWO ? 1 - P : 0>());
+    }
+    note(step + RS + 2, queue[P % QUEUE]);
+    queue[P % QUEUE] = look_up(step + RS + 2 + QUEUE);
+  };
+#pragma unroll 1
+  for (int step = 0; step < steps; step += TWO ? 2 : 1) {
+    take(step, even_t());
+    if (TWO && step + 1 < steps) take(step + 1, std::integral_constant<int, TWO ? 1 : 0>());
   }
 
   // acc[j][v] = sum of p v of row r32, column 32 j + 8 (v / 4) + 4 h + v % 4, relative to m_run
@@ -451,7 +521,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
   }
   if (!row_live) return;
   if (cut) {
-    const int64_t part = (((int64_t)place * a.c.heads + hk) * a.splits + split) * a.tile_rows + row0 + r32;
+    const int64_t part = ((((int64_t)chunk_place(a, b) + tile) * a.c.heads + hk) * a.splits + split) * a.tile_rows + row0 + r32;
     if (h == 0) a.part_ml[part] = make_float2(m_run, l_run);
     float* to = a.part_o + part * a.width;
 #pragma unroll
@@ -467,9 +537,9 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
   for (int j = 0; j < DB; ++j)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int col = 32 * j + 8 * g + 4 * h;
+      const int col = 32 * j + 8 * g + 4 * h, d = hide(a.c.d);
       const float x0 = acc[j][4 * g] * inv, x1 = acc[j][4 * g + 1] * inv, x2 = acc[j][4 * g + 2] * inv, x3 = acc[j][4 * g + 3] * inv;
-      if (col + 3 < a.c.d) {
+      if (col + 3 < d) {
         if constexpr (F32) {
           typedef float any_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
           *reinterpret_cast<any_f32x4*>(out + col * 4) = any_f32x4{x0, x1, x2, x3};
@@ -477,10 +547,10 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
           typedef uint32_t any_u32x2 __attribute__((ext_vector_type(2), aligned(2)));
           *reinterpret_cast<any_u32x2*>(out + col * 2) = any_u32x2{pack2<QDT>(x0, x1), pack2<QDT>(x2, x3)};
         }
-      } else {
-        if (col < a.c.d) store_from_f32<QDT>(out, col, x0);
-        if (col + 1 < a.c.d) store_from_f32<QDT>(out, col + 1, x1);
-        if (col + 2 < a.c.d) store_from_f32<QDT>(out, col + 2, x2);
+      } else if (ODD) {
+        if (col < d) store_from_f32<QDT>(out, col, x0);
+        if (col + 1 < d) store_from_f32<QDT>(out, col + 1, x1);
+        if (col + 2 < d) store_from_f32<QDT>(out, col + 2, x2);
       }
     }
 }
@@ -497,7 +567,7 @@ int launch(const ChunkArgs& a, hipStream_t s) {
 
 template <int DB, bool ODD>
 int launch_rows(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s) {
-  if constexpr (!F32)
+  if constexpr (!F32 && DB <= 6)
     if (p.few) return launch<DB, ODD, true>(a, s);
   return launch<DB, ODD, false>(a, s);
 }
