@@ -20,7 +20,7 @@ LIB_PATH = LIB_DIR / "liblighthouse_hip.so"
 PROBE_LIB = LIB_DIR / "liblighthouse_probe.so"  # bench.py's MFMA-rate probe, not part of the product library
 
 HIP_SOURCES = ["runtime.hip", "gemm16.hip", "gemm16_direct.hip", "gemm32.hip", "gemm8.hip", "gemm_small.hip", "gemm_small_norm.hip", "attention.hip", "attention_small.hip", "rowwise.hip", "kv_cache.hip", "paged_attention.hip", "sample.hip",
-               "kv_pages.hip", "rotary.hip", "rms_norm.hip", "chunk_attention.hip", "chunk_attention_kernel.hip",
+               "kv_pages.hip", "rotary.hip", "rms_norm.hip", "chunk_attention.hip", "chunk_attention_kernel.hip", "chunk_attention_few.hip",
                "api.hip"]
 
 # A lone workgroup's main loop fetches a line more of instructions a turn where it starts at the end of one: the same loop 4 bytes
@@ -38,12 +38,13 @@ INSTANCES = {
                                    f"-DLH_GEMM16_{kind.upper()}=1"] + ALIGNED_LOOPS * (kind == "deep")
         for kind, tm, tn in (("odd", 2, 1), ("deep", 2, 1), ("deep", 2, 3), ("deep", 2, 2), ("deep", 4, 1)) for dt in ("bf16", "f16")
     },
-    # the types of a cache and of queries
-    "chunk_attention_kernel.hip": {
-        f"_{name}": [f"-DLH_CHUNK_CDT=LH_{cache}", f"-DLH_CHUNK_QDT=LH_{q}", f"-DLH_CHUNK_NAME=chunk_launch_{name}"]
+} | {
+    source: {
+        f"_{name}": [f"-DLH_CHUNK_CDT=LH_{cache}", f"-DLH_CHUNK_QDT=LH_{q}", f"-DLH_CHUNK_NAME={launch}_{name}"]
         for name, cache, q in (("f32", "F32", "F32"), ("bf16", "BF16", "BF16"), ("f16", "F16", "F16"), ("e4m3_bf16", "F8E4M3", "BF16"),
-                               ("e4m3_f16", "F8E4M3", "F16"))
-    },
+                               ("e4m3_f16", "F8E4M3", "F16"))  # the types of a cache and of queries
+    }
+    for source, launch in (("chunk_attention_kernel.hip", "chunk_many"), ("chunk_attention_few.hip", "chunk_few"))
 }
 
 HIPCC_FLAGS = [

@@ -28,10 +28,11 @@ struct ChunkArgs {
 };
 
 struct ChunkPlan {
-  int blocks;              // width of the kernel's rows, in 32 columns
-  bool odd;                // rows that are no whole pieces
-  bool few;                // 32 rows a workgroup, whose waves share the positions out; otherwise 128, 32 a wave
-  int tile_rows, slots, share, splits;
+  bool few;                // 16 rows a workgroup, otherwise 128
+  int blocks;              // of the many: width of the kernel's rows, in 32 columns
+  bool odd;                //   rows that are no whole pieces
+  int mode;                // of the few: PagedMode
+  int tile_rows, slots, share, splits, width;
   size_t o_bytes, ml_bytes;
   size_t total() const { return o_bytes + ml_bytes; }
 };
@@ -90,11 +91,16 @@ __device__ __forceinline__ bool chunk_tile(const ChunkArgs& a, int rank, int* se
   return *tile >= 0 && count > 0 && *tile <= (count * a.G - 1) >> a.tile_shift;
 }
 
-// Launches the kernel of a pair of types (in chunk_attention.hip, compiled once for each).
-int chunk_launch_f32(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
-int chunk_launch_bf16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
-int chunk_launch_f16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
-int chunk_launch_e4m3_bf16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
-int chunk_launch_e4m3_f16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+// Launch the kernel of a pair of types (chunk_attention_kernel.hip and chunk_attention_few.hip, compiled once for each).
+int chunk_many_f32(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+int chunk_many_bf16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+int chunk_many_f16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+int chunk_many_e4m3_bf16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+int chunk_many_e4m3_f16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+int chunk_few_f32(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+int chunk_few_bf16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+int chunk_few_f16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+int chunk_few_e4m3_bf16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
+int chunk_few_e4m3_f16(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s);
 
 }  // namespace lh

@@ -1,6 +1,6 @@
 // Attention of packed chunks of new tokens over a paged cache: how a call is cut into workgroups, the join of shares of positions, the
 // entry points.  The kernel is in chunk_attention_kernel.hip.
-#include "chunk_attention.h"
+#include "paged_rows.h"
 
 namespace lh {
 
@@ -48,30 +48,37 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a) {
 
 static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
 
-static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H) {
+// `aligned`: keys and values begin at multiples of 16 bytes.
+static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H, bool aligned) {
   ChunkPlan p = {};
   const int64_t G = H / c.heads;
-  const int piece = cache_dtype == LH_F32 ? 4 : 8;
-  p.odd = c.d % piece != 0;
-  const int blocks = (c.d + 31) / 32;
-  p.blocks = p.odd ? (blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8) : blocks <= 2 ? 2 : blocks <= 4 ? blocks : blocks <= 6 ? 6 : 8;
-  // Tiles of 32 rows where the sequences have no more on average (and the registers suffice for two waves' worth of positions).
-  p.few = cache_dtype != LH_F32 && p.blocks <= 6 && N * G <= 32 * B;
-  p.tile_rows = p.few ? 32 : 128;
+  const int es = (int)dtype_size(cache_dtype);
+  // Tiles of 16 rows where the sequences have no more than two of them on average.
+  p.few = N * G <= 32 * B;
+  p.tile_rows = p.few ? 16 : 128;
   const int64_t slots = N * G / p.tile_rows + B;
   p.slots = (int)slots;
-  // As many shares of positions as the workgroups that run at once allow for, of tiles that there probably are (a place more per sequence may
-  // be empty).  One more would be a second round of workgroups for a few.
+  // (A place more per sequence may be empty: the tiles that there probably are.)
   const int64_t items = slots * c.heads, tiles = N * G / p.tile_rows > B ? N * G / p.tile_rows : B < N ? B : N;
-  int64_t splits = (p.few && p.blocks > 2 ? 1 : 2) * num_cus() / (tiles * c.heads);
-  splits = splits < 1 ? 1 : splits;
-  const int64_t most = (c.capacity() + 255) / 256;
-  splits = splits > most ? most : splits;
-  const int64_t share = (c.capacity() + splits - 1) / splits;
-  p.share = (int)((share + 127) / 128 * 128);
+  if (p.few) {
+    p.mode = paged_mode(c, es, aligned);
+    p.width = paged_width(c.d);
+    p.share = paged_share(tiles * c.heads, c.capacity(), paged_occupancy(cache_dtype, p.width, p.mode, true), 2 * (int64_t)c.d * es);
+  } else {
+    p.odd = c.d % (cache_dtype == LH_F32 ? 4 : 8) != 0;
+    const int blocks = (c.d + 31) / 32;
+    p.blocks = p.odd ? (blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8) : blocks <= 2 ? 2 : blocks <= 4 ? blocks : blocks <= 6 ? 6 : 8;
+    p.width = 32 * p.blocks;
+    // As many shares of positions as the workgroups that run at once allow for.  One more would be a second round of workgroups for a few.
+    int64_t splits = 2 * num_cus() / (tiles * c.heads);
+    const int64_t most = (c.capacity() + 255) / 256;
+    splits = splits < 1 ? 1 : splits > most ? most : splits;
+    const int64_t share = (c.capacity() + splits - 1) / splits;
+    p.share = (int)((share + 127) / 128 * 128);
+  }
   p.splits = (int)(((int64_t)c.capacity() + p.share - 1) / p.share);
   if (p.splits > 1) {
-    p.o_bytes = granules((size_t)items * p.splits * p.tile_rows * p.blocks * 32 * 4);
+    p.o_bytes = granules((size_t)items * p.splits * p.tile_rows * p.width * 4);
     p.ml_bytes = granules((size_t)items * p.splits * p.tile_rows * 8);
   }
   return p;
@@ -79,7 +86,7 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
 
 static bool chunk_sizes(const Paged& c, int64_t N, int64_t B, int64_t H) {
   return N > 0 && B > 0 && H > 0 && B < (1ll << 20) && N < (1ll << 30) && H < (1ll << 20) && H % c.heads == 0 && N * (H / c.heads) < (1ll << 31) - 256 &&
-         N * H < (1ll << 32) && (N * (H / c.heads) / 32 + B) * c.heads < (1ll << 30);
+         N * H < (1ll << 32) && (N * (H / c.heads) / 16 + B) * c.heads < (1ll << 30);
 }
 
 }  // namespace lh
@@ -91,7 +98,9 @@ extern "C" {
 size_t lh_hip_paged_attention_chunk_workspace_bytes(const lh_paged_cache* cache, int64_t N, int64_t B, int64_t H) {
   Paged c;
   if (paged_cache(cache, "lh_hip_paged_attention_chunk_workspace_bytes", &c) != LH_OK || !chunk_sizes(c, N, B, H)) return 0;
-  return chunk_plan(c, cache->dtype, N, B, H).total();
+  // (Room for either alignment: a caller may size it with one cache and pass a view of another.)
+  const size_t one = chunk_plan(c, cache->dtype, N, B, H, true).total(), other = chunk_plan(c, cache->dtype, N, B, H, false).total();
+  return one > other ? one : other;
 }
 
 int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const void* q, int64_t out_stride_n, int64_t out_stride_h, int64_t q_stride_n,
@@ -106,23 +115,24 @@ int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const v
   LH_REQUIRE(out && q && lengths && starts, "%s: null pointer", what);
   LH_REQUIRE(dtype == cache->dtype || (cache->dtype == LH_F8E4M3 && (dtype == LH_BF16 || dtype == LH_F16)),
              "%s: queries must have the cache's dtype (bf16 or f16 for a cache of e4m3)", what);
-  const ChunkPlan p = chunk_plan(a.c, cache->dtype, N, B, H);
+  const ChunkPlan p = chunk_plan(a.c, cache->dtype, N, B, H, aligned16(a.c.k) && aligned16(a.c.v));
   LH_REQUIRE(p.total() == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= p.total()),
              "%s: workspace too small or not 256-byte aligned: %zu of %zu bytes", what, workspace_bytes, p.total());
   a.out = out, a.q = q, a.so_n = out_stride_n, a.so_h = out_stride_h, a.sq_n = q_stride_n, a.sq_h = q_stride_h, a.lengths = lengths, a.starts = starts;
   a.N = (int32_t)N, a.B = (int32_t)B, a.H = (int32_t)H, a.G = (int32_t)(H / a.c.heads), a.by_group = FastDiv((uint32_t)a.G);
-  a.tile_rows = p.tile_rows, a.tile_shift = p.few ? 5 : 7, a.slots = p.slots, a.ranked = B > 1 && B <= 32, a.share = p.share, a.splits = p.splits, a.width = 32 * p.blocks;
+  a.tile_rows = p.tile_rows, a.tile_shift = p.few ? 4 : 7, a.slots = p.slots, a.ranked = B > 1 && B <= 32, a.share = p.share, a.splits = p.splits, a.width = p.width;
   const double factor = (double)scale * a.c.k_scale * 1.4426950408889634;
   a.scale_log2e = scale == 0.0f ? 1.0f : (float)(factor < 0.0 ? -factor : factor);
   a.q_and = scale == 0.0f ? 0u : ~0u, a.q_xor = scale < 0.0f ? (dtype == LH_F32 ? 0x80000000u : 0x80008000u) : 0u;
   LH_REQUIRE(a.scale_log2e > 0.0f && a.scale_log2e < INFINITY, "%s: scale times the keys' scale must be finite", what);
   if (p.splits > 1) a.part_o = static_cast<float*>(workspace), a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.o_bytes);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int rc = cache->dtype == LH_F32    ? chunk_launch_f32(a, p, s)
-                 : cache->dtype == LH_BF16 ? chunk_launch_bf16(a, p, s)
-                 : cache->dtype == LH_F16  ? chunk_launch_f16(a, p, s)
-                 : dtype == LH_BF16        ? chunk_launch_e4m3_bf16(a, p, s)
-                                           : chunk_launch_e4m3_f16(a, p, s);
+  const auto launch = cache->dtype == LH_F32    ? (p.few ? chunk_few_f32 : chunk_many_f32)
+                      : cache->dtype == LH_BF16 ? (p.few ? chunk_few_bf16 : chunk_many_bf16)
+                      : cache->dtype == LH_F16  ? (p.few ? chunk_few_f16 : chunk_many_f16)
+                      : dtype == LH_BF16        ? (p.few ? chunk_few_e4m3_bf16 : chunk_many_e4m3_bf16)
+                                                : (p.few ? chunk_few_e4m3_f16 : chunk_many_e4m3_f16);
+  const int rc = launch(a, p, s);
   if (rc != LH_OK || p.splits == 1) return rc;
   const dim3 grid((unsigned)((N * H + 3) / 4)), block(256);
   if (dtype == LH_BF16) LH_LAUNCH((chunk_join_kernel<LH_BF16>), grid, block, 0, s, a);

@@ -7,13 +7,12 @@
 //    is a scalar per lane, and the accumulators of S^T are, rounded, the second operand of O^T.
 //  * Keys and values of a step go through registers into LDS, requested while the step before is computed; where each position's
 //    row lies is looked up two steps ahead, one position a thread, so that any page size and any strides cost the same.
-//  * Many rows: 128 a workgroup, 32 for each of four waves, 64 positions a step, which all waves read.  Few rows: 32, and a step's 128
-//    positions are shared out between the waves, whose results are brought together at the end.
+//  * 128 rows a workgroup, 32 for each of four waves, 64 positions a step, which all waves read.  (Sequences with few rows have a kernel
+//    without LDS, in chunk_attention_few.hip.)
 //  * Long caches of few tiles are cut into shares of positions; a second launch joins them.
 //
-// Many rows are bound by the arithmetic: P is rounded to 16 bits once, as in attention over tensors, and the sum is that of the rounded values,
-// so that the weights add up to 1; the result's error against 64 bits is up to 1.4 times that of its own rounding.  Few rows are bound by
-// memory: there P is the sum of two values of the type, the second what the first has lost.
+// The arithmetic bounds it: P is rounded to 16 bits once, as in attention over tensors, and the sum is that of the rounded values, so that the
+// weights add up to 1; the result's error against 64 bits is up to 1.4 times that of its own rounding.
 #include "chunk_attention.h"
 
 #ifndef LH_CHUNK_CDT
@@ -139,40 +138,37 @@ __device__ __forceinline__ uint32_t wild_bits(u32x4 w) {
 }
 
 // Workgroups that a CU holds, by their registers.
-constexpr int occupancy(int blocks, bool few) { return blocks <= (few ? 2 : 4) ? 2 : 1; }
+constexpr int occupancy(int blocks) { return blocks <= 4 ? 2 : 1; }
 // Steps ahead whose keys and values are on their way to registers: as many as these suffice for.  0: they are asked for when their place is free.
-constexpr int ahead(int blocks, bool odd, bool few) { return F32 || (CES == 1 && odd && !few && blocks == 4) ? 0 : few ? (blocks <= 4 ? 2 : 1) : blocks <= 3 ? 2 : blocks <= 6 ? 1 : 0; }
+constexpr int ahead(int blocks, bool odd) { return F32 || (CES == 1 && odd && blocks == 4) ? 0 : blocks <= 3 ? 2 : blocks <= 6 ? 1 : 0; }
 
-constexpr int keys_of(bool few) { return few && !F32 ? 128 : 64; }
+constexpr int KEYS = 64;  // positions of a step
 // Elements from one row to the next: of keys, whose rows are read 16 bytes a lane, so that neighbours lie 4 (f32: 8) banks apart; of values, of
 // which 16-bit ones are read four rows at a time, 64 bytes of each: 16 or 48 banks apart.
 constexpr int k_row_elems(int blocks) { return 32 * blocks + 8; }
 constexpr int v_row_elems(int blocks) { return F32 ? 32 * blocks + 8 : blocks == 3 ? 96 : 32 * blocks + 32; }
-constexpr size_t stage_bytes(int blocks, bool few) { return (size_t)keys_of(few) * (k_row_elems(blocks) + v_row_elems(blocks)) * QES; }
+constexpr size_t stage_bytes(int blocks) { return (size_t)KEYS * (k_row_elems(blocks) + v_row_elems(blocks)) * QES; }
 // Steps that are in LDS: the next one beside the one that is read, where two do not cost a CU a workgroup.
-constexpr int stages(int blocks, bool few) { return 2 * stage_bytes(blocks, few) <= (occupancy(blocks, few) == 2 ? 77000 : 153000) ? 2 : 1; }
-constexpr size_t lds_bytes(int blocks, bool few) { return stages(blocks, few) * stage_bytes(blocks, few); }
+constexpr int stages(int blocks) { return 2 * stage_bytes(blocks) <= (occupancy(blocks) == 2 ? 77000 : 153000) ? 2 : 1; }
+constexpr size_t lds_bytes(int blocks) { return stages(blocks) * stage_bytes(blocks); }
 
-// DB: width in 32 columns.  FEW: 32 rows, positions shared out between the waves; otherwise 128 rows.
-template <int CACHE, int QUERY, int DB, bool ODD, bool FEW>  // (the types: for the name)
-__global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kernel(ChunkArgs a) {
-  constexpr int D = 32 * DB, KROW = k_row_elems(DB), VROW = v_row_elems(DB), KEYS = keys_of(FEW);
-  constexpr int PARTS = FEW ? 2 : 1;              // 16-bit values that a probability is the sum of
-  constexpr int WK = FEW ? 4 : 1;                 // waves that share out a step's positions
-  constexpr int NI = KEYS / 32 / WK;              // 32-position tiles of a wave
+// DB: width in 32 columns.
+template <int CACHE, int QUERY, int DB, bool ODD>  // (the types: for the name)
+__global__ void __launch_bounds__(256, occupancy(DB)) chunk_attention_kernel(ChunkArgs a) {
+  constexpr int D = 32 * DB, KROW = k_row_elems(DB), VROW = v_row_elems(DB);
+  constexpr int NI = KEYS / 32;                   // 32-position tiles
   constexpr int CPR = D / PE;                     // pieces of a row
   constexpr int NP = KEYS * CPR / 256;            // pieces a thread brings, of keys and of values
   constexpr int SD = F32 ? D / 8 : D / 16;
-  constexpr int RS = ahead(DB, ODD, FEW), STAGES = stages(DB, FEW);
+  constexpr int RS = ahead(DB, ODD), STAGES = stages(DB);
   constexpr bool SHORT = ODD && DB == 2;
   constexpr bool TWO = STAGES == 2 || RS == 2;    // steps go by in pairs
   static_assert(NI >= 1 && NP * 256 == KEYS * CPR, "");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   typedef typename std::conditional<F32, float, uint16_t>::type elem;
   __shared__ int64_t k_at[2][KEYS], v_at[2][KEYS];  // where the rows of a step lie, in elements; below 0: nowhere
-  __shared__ uint64_t held[8][KEYS / 64];           // which positions of a step there are (noted up to four steps before they are read)
+  __shared__ uint64_t held[8];           // which positions of a step there are (noted up to four steps before they are read)
   __shared__ int32_t wild[2][4], first_wild[D];
-  __shared__ float2 stats[4][32];
 
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -191,7 +187,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
   const int k1 = k0 + max(min(sees - k0, a.share), 0);
   const bool cut = sees > a.share;
 
-  const int row0 = FEW ? 0 : 32 * wave;  // of the wave, in the tile
+  const int row0 = 32 * wave;  // of the wave, in the tile
   const int row = first + row0 + r32;
   const bool row_live = row0 + r32 < rows;
   const int token = (int)a.by_group.div((uint32_t)row), head = hk * a.G + (row - token * a.G);
@@ -244,7 +240,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
     k_at[step & 1][tid] = there ? page * a.c.sk.z + slot * a.c.sk.t : -1;
     v_at[step & 1][tid] = there ? page * a.c.sv.z + slot * a.c.sv.t : -1;
     const uint64_t some = __builtin_amdgcn_ballot_w64(there);
-    if (lane == 0) held[step & 7][wave] = some;
+    if (lane == 0) held[step & 7] = some;
   };
   uint32_t kr[RS > 0 ? RS : 1][RS > 0 ? NP : 1][PW], vr[RS > 0 ? RS : 1][RS > 0 ? NP : 1][PW];
   uint32_t there[RS > 0 ? RS : 1] = {};  // which of the thread's rows there are
@@ -278,10 +274,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
     constexpr int S = decltype(set)::value;
     elem* const Ks = stage0 + (step & 1) * kStage;
     const bool look = partial(step);
-    bool full = a.c.d == D;  // nothing of the step has to become 0
-#pragma unroll
-    for (int w = 0; w < KEYS / 64; ++w) full = full && held[step & 7][w] == ~0ull;
-    full = __builtin_amdgcn_readfirstlane(full);
+    const bool full = __builtin_amdgcn_readfirstlane(a.c.d == D && held[step & 7] == ~0ull);  // nothing of the step has to become 0
     uint32_t odd_one = 0;
     if constexpr (RS > 0) {
 #pragma unroll
@@ -354,10 +347,8 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
       }
       lds_barrier();
     }
-    const uint64_t all_held = KEYS == 64 ? held[step & 7][0] : held[step & 7][wave / 2] >> (32 * (wave & 1)) | 0xffffffff00000000ull;
-    const int kw0 = FEW && WK > 1 ? 32 * NI * wave : 0;  // the wave's first position of the step
-    const int j0w = j0 + kw0;
-    if (wave_live && wave_last >= j0w) {
+    const uint64_t all_held = held[step & 7];
+    if (wave_live && wave_last >= j0) {
       f32x16 s[NI];
 #pragma unroll
       for (int i = 0; i < NI; ++i)
@@ -374,7 +365,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
         if (!Q_HELD && (F32 || e % 2 == 1)) asm volatile("" ::: "memory");
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(Ks + (kw0 + 32 * i + r32) * KROW + (2 * e + h) * PE);
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(Ks + (32 * i + r32) * KROW + (2 * e + h) * PE);
           if constexpr (F32) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
@@ -384,11 +375,11 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
           }
         }
       }
-      // s[i][v] = q . k of row r32 and position j0w + 32 i + 8 (v / 4) + 4 h + v % 4
-      const bool whole = j0w + 32 * NI - 1 <= min(wave_first, k1 - 1) && row0 + 31 < rows && all_held == ~0ull;
+      // s[i][v] = q . k of row r32 and position j0 + 32 i + 8 (v / 4) + 4 h + v % 4
+      const bool whole = j0 + 32 * NI - 1 <= min(wave_first, k1 - 1) && row0 + 31 < rows && all_held == ~0ull;
       if (!whole) {
-        // Bit p of `seen`: whether the row sees position j0w + p.
-        uint64_t seen = last_seen < j0w ? 0ull : last_seen - j0w >= 63 ? ~0ull : (2ull << (last_seen - j0w)) - 1;
+        // Bit p of `seen`: whether the row sees position j0 + p.
+        uint64_t seen = last_seen < j0 ? 0ull : last_seen - j0 >= 63 ? ~0ull : (2ull << (last_seen - j0)) - 1;
         seen = (seen & all_held) >> (4 * h);
         const uint32_t half[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
 #pragma unroll
@@ -424,14 +415,14 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           s[i][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][v], a.scale_log2e, -off));
-          if constexpr (F32 || PARTS == 2) l_run += s[i][v];
+          if constexpr (F32) l_run += s[i][v];
         }
       if constexpr (F32) {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const float* vrow = reinterpret_cast<const float*>(Vs) + (kw0 + 32 * i + 8 * (v >> 2) + 4 * h + (v & 3)) * VROW + r32;
+            const float* vrow = reinterpret_cast<const float*>(Vs) + (32 * i + 8 * (v >> 2) + 4 * h + (v & 3)) * VROW + r32;
 #pragma unroll
             for (int j = 0; j < DB; ++j) acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[32 * j], s[i][v], acc[j], 0, 0, 0);
             if (v % (DB > 6 ? 2 : 4) == (DB > 6 ? 1 : 3)) asm volatile("" ::: "memory");  // (values of a few positions fetched ahead)
@@ -444,23 +435,19 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
         for (int i = 0; i < NI; ++i)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            u32x4 pf[PARTS];
+            u32x4 pf;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float p0 = s[i][8 * u + 2 * e], p1 = s[i][8 * u + 2 * e + 1];
-              pf[0][e] = pack2<QDT>(p0, p1);
-              if constexpr (PARTS == 1) l_run = add_pair(pf[0][e], l_run);  // (what the values are weighted with)
-              if constexpr (PARTS == 2) pf[PARTS - 1][e] = pack2<QDT>(p0 - unpack_lo<QDT>(pf[0][e]), p1 - unpack_hi<QDT>(pf[0][e]));
+              pf[e] = pack2<QDT>(s[i][8 * u + 2 * e], s[i][8 * u + 2 * e + 1]);
+              l_run = add_pair(pf[e], l_run);  // (what the values are weighted with)
             }
 #pragma unroll
             for (int j = 0; j < DB; ++j) {
-              const elem* p0 = Vs + (kw0 + 32 * i + 16 * u + tr_row) * VROW + 32 * j + tr_col;
+              const elem* p0 = Vs + (32 * i + 16 * u + tr_row) * VROW + 32 * j + tr_col;
               const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p0);
               const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p0 + 8 * VROW));
               const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
-              const u32x4 vf = {l2[0], l2[1], h2[0], h2[1]};
-#pragma unroll
-              for (int n = 0; n < PARTS; ++n) acc[j] = mma(vf, pf[n], acc[j]);
+              acc[j] = mma(u32x4{l2[0], l2[1], h2[0], h2[1]}, pf, acc[j]);
             }
           }
       }
@@ -491,34 +478,6 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
 
   // acc[j][v] = sum of p v of row r32, column 32 j + 8 (v / 4) + 4 h + v % 4, relative to m_run
   l_run += __shfl_xor(l_run, 32);
-  if constexpr (WK > 1) {
-    __syncthreads();  // (the last step has been read: its place is taken)
-    if (h == 0) stats[wave][r32] = make_float2(m_run, l_run);
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, stats[w][r32].x);
-    const float safe = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) l += stats[w][r32].y * __builtin_amdgcn_exp2f(stats[w][r32].x - safe);
-    const float own = __builtin_amdgcn_exp2f(m_run - safe);
-#pragma unroll
-    for (int j = 0; j < DB; ++j) acc[j] *= own;
-    f32x16* const sums = reinterpret_cast<f32x16*>(smem);  // [2][DB][64]
-#pragma unroll
-    for (int half = 2; half >= 1; half /= 2) {
-      if (wave >= half && wave < 2 * half)
-#pragma unroll
-        for (int j = 0; j < DB; ++j) sums[((wave - half) * DB + j) * 64 + lane] = acc[j];
-      __syncthreads();
-      if (wave < half)
-#pragma unroll
-        for (int j = 0; j < DB; ++j) acc[j] += sums[(wave * DB + j) * 64 + lane];
-      if (half > 1) __syncthreads();
-    }
-    if (wave != 0) return;
-    m_run = m, l_run = l;
-  }
   if (!row_live) return;
   if (cut) {
     const int64_t part = ((((int64_t)chunk_place(a, b) + tile) * a.c.heads + hk) * a.splits + split) * a.tile_rows + row0 + r32;
@@ -555,37 +514,30 @@ __global__ void __launch_bounds__(256, occupancy(DB, FEW)) chunk_attention_kerne
     }
 }
 
-template <int DB, bool ODD, bool FEW>
+template <int DB, bool ODD>
 int launch(const ChunkArgs& a, hipStream_t s) {
-  auto kernel = chunk_attention_kernel<CDT, QDT, DB, ODD, FEW>;
-  constexpr size_t sums = FEW ? (size_t)2 * DB * 64 * 64 : 0, lds = sums > lds_bytes(DB, FEW) ? sums : lds_bytes(DB, FEW);
+  auto kernel = chunk_attention_kernel<CDT, QDT, DB, ODD>;
+  constexpr size_t lds = lds_bytes(DB);
   if (lds > 65536 && !planning())
     LH_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   LH_LAUNCH(kernel, dim3((unsigned)((int64_t)a.slots * a.c.heads * a.splits)), dim3(256), lds, s, a);
   return check_launch("chunk_attention");
 }
 
-template <int DB, bool ODD>
-int launch_rows(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s) {
-  if constexpr (!F32 && DB <= 6)
-    if (p.few) return launch<DB, ODD, true>(a, s);
-  return launch<DB, ODD, false>(a, s);
-}
-
 }  // namespace
 
 int LH_CHUNK_NAME(const ChunkArgs& a, const ChunkPlan& p, hipStream_t s) {
   if (p.odd) {
-    if (p.blocks <= 2) return launch_rows<2, true>(a, p, s);
-    if (p.blocks <= 4) return launch_rows<4, true>(a, p, s);
-    return launch_rows<8, true>(a, p, s);
+    if (p.blocks <= 2) return launch<2, true>(a, s);
+    if (p.blocks <= 4) return launch<4, true>(a, s);
+    return launch<8, true>(a, s);
   }
   switch (p.blocks) {
-    case 2: return launch_rows<2, false>(a, p, s);
-    case 3: return launch_rows<3, false>(a, p, s);
-    case 4: return launch_rows<4, false>(a, p, s);
-    case 6: return launch_rows<6, false>(a, p, s);
-    default: return launch_rows<8, false>(a, p, s);
+    case 2: return launch<2, false>(a, s);
+    case 3: return launch<3, false>(a, s);
+    case 4: return launch<4, false>(a, s);
+    case 6: return launch<6, false>(a, s);
+    default: return launch<8, false>(a, s);
   }
 }
 
