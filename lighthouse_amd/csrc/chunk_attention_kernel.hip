@@ -138,9 +138,9 @@ __device__ __forceinline__ uint32_t wild_bits(u32x4 w) {
 }
 
 // Workgroups that a CU holds, by their registers.
-constexpr int occupancy(int blocks) { return blocks <= 4 ? 2 : 1; }
+constexpr int occupancy(int blocks, bool odd) { return blocks <= 2 && !F32 && !odd ? 3 : blocks <= 4 ? 2 : 1; }
 // Steps ahead whose keys and values are on their way to registers: as many as these suffice for.  0: they are asked for when their place is free.
-constexpr int ahead(int blocks, bool odd) { return F32 || (CES == 1 && odd && blocks == 4) ? 0 : blocks <= 3 ? 2 : blocks <= 6 ? 1 : 0; }
+constexpr int ahead(int blocks, bool odd) { return F32 || (CES == 1 && odd && blocks == 4) ? 0 : blocks == 3 ? 2 : blocks <= 6 ? 1 : 0; }
 
 constexpr int KEYS = 64;  // positions of a step
 // Elements from one row to the next: of keys, whose rows are read 16 bytes a lane, so that neighbours lie 4 (f32: 8) banks apart; of values, of
@@ -149,18 +149,18 @@ constexpr int k_row_elems(int blocks) { return 32 * blocks + 8; }
 constexpr int v_row_elems(int blocks) { return F32 ? 32 * blocks + 8 : blocks == 3 ? 96 : 32 * blocks + 32; }
 constexpr size_t stage_bytes(int blocks) { return (size_t)KEYS * (k_row_elems(blocks) + v_row_elems(blocks)) * QES; }
 // Steps that are in LDS: the next one beside the one that is read, where two do not cost a CU a workgroup.
-constexpr int stages(int blocks) { return 2 * stage_bytes(blocks) <= (occupancy(blocks) == 2 ? 77000 : 153000) ? 2 : 1; }
-constexpr size_t lds_bytes(int blocks) { return stages(blocks) * stage_bytes(blocks); }
+constexpr int stages(int blocks, bool odd) { return 2 * stage_bytes(blocks) <= (occupancy(blocks, odd) == 3 ? 51000 : occupancy(blocks, odd) == 2 ? 77000 : 153000) ? 2 : 1; }
+constexpr size_t lds_bytes(int blocks, bool odd) { return stages(blocks, odd) * stage_bytes(blocks); }
 
 // DB: width in 32 columns.
 template <int CACHE, int QUERY, int DB, bool ODD>  // (the types: for the name)
-__global__ void __launch_bounds__(256, occupancy(DB)) chunk_attention_kernel(ChunkArgs a) {
+__global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kernel(ChunkArgs a) {
   constexpr int D = 32 * DB, KROW = k_row_elems(DB), VROW = v_row_elems(DB);
   constexpr int NI = KEYS / 32;                   // 32-position tiles
   constexpr int CPR = D / PE;                     // pieces of a row
   constexpr int NP = KEYS * CPR / 256;            // pieces a thread brings, of keys and of values
   constexpr int SD = F32 ? D / 8 : D / 16;
-  constexpr int RS = ahead(DB, ODD), STAGES = stages(DB);
+  constexpr int RS = ahead(DB, ODD), STAGES = stages(DB, ODD);
   constexpr bool SHORT = ODD && DB == 2;
   constexpr bool TWO = STAGES == 2 || RS == 2;    // steps go by in pairs
   static_assert(NI >= 1 && NP * 256 == KEYS * CPR, "");
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(256, occupancy(DB)) chunk_attention_kernel(Chu
 template <int DB, bool ODD>
 int launch(const ChunkArgs& a, hipStream_t s) {
   auto kernel = chunk_attention_kernel<CDT, QDT, DB, ODD>;
-  constexpr size_t lds = lds_bytes(DB);
+  constexpr size_t lds = lds_bytes(DB, ODD);
   if (lds > 65536 && !planning())
     LH_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   LH_LAUNCH(kernel, dim3((unsigned)((int64_t)a.slots * a.c.heads * a.splits)), dim3(256), lds, s, a);
