@@ -17,6 +17,7 @@ struct ChunkArgs {
   int32_t N, B, H, G;
   FastDiv by_group;        // rows of a sequence and key / value head: G of a token
   int32_t tile_rows, tile_shift;  // rows a workgroup takes, a power of 2
+  int32_t least, most;     // rows of the sequences that the launch is for
   int32_t slots;           // workgroups' places for tiles
   int32_t ranked;          // tiles by weight, or by place
   int32_t share, splits;   // positions a workgroup takes, workgroups for the positions of the table
@@ -32,14 +33,19 @@ struct ChunkPlan {
   int blocks;              // of the many: width of the kernel's rows, in 32 columns
   bool odd;                //   rows that are no whole pieces
   int mode;                // of the few: PagedMode
-  int tile_rows, slots, share, splits, width;
+  int least, most, tile_rows, slots, share, splits, width;
   size_t o_bytes, ml_bytes;
   size_t total() const { return o_bytes + ml_bytes; }
 };
 
-// Places for the tiles of sequence b begin at rows / tile_rows (of the rows before it) + b: at least as many as its rows need.
+constexpr int kChunkFew = 32;  // rows of a sequence: two tiles of the few
+
+// Places for the tiles of sequence b begin at rows / tile_rows (of the rows before it) + b: at least as many as its rows need.  Where a launch is
+// for sequences with few rows only, each has two.
 __device__ __forceinline__ int chunk_start(const ChunkArgs& a, int b) { return min(max(a.starts[b], 0), a.N); }
-__device__ __forceinline__ int chunk_place(const ChunkArgs& a, int b) { return (int)((uint32_t)(chunk_start(a, b) * a.G) >> a.tile_shift) + b; }
+__device__ __forceinline__ int chunk_place(const ChunkArgs& a, int b) {
+  return a.most == kChunkFew ? 2 * b : (int)((uint32_t)(chunk_start(a, b) * a.G) >> a.tile_shift) + b;
+}
 
 // The last of the B sequences for which `begins(b) <= at` (ascending), 0 if there is none, by all lanes of a wave: 64 a round.
 template <typename F>
@@ -62,7 +68,7 @@ __device__ __forceinline__ bool chunk_tile(const ChunkArgs& a, int rank, int* se
   if (a.ranked) {
     const int lane = threadIdx.x & 63, i = min(lane, a.B - 1);
     const int rows = max(chunk_start(a, i + 1) - chunk_start(a, i), 0) * a.G;
-    const int tiles = lane < a.B ? (int)((uint32_t)(rows + a.tile_rows - 1) >> a.tile_shift) : 0;
+    const int tiles = lane < a.B && rows >= a.least && rows <= a.most ? (int)((uint32_t)(rows + a.tile_rows - 1) >> a.tile_shift) : 0;
     for (int level = 0;;) {  // (of each sequence, counted from its last tile)
       const uint64_t live = __builtin_amdgcn_ballot_w64(tiles > level);
       const int n = (int)__popcll(live);
@@ -88,7 +94,7 @@ __device__ __forceinline__ bool chunk_tile(const ChunkArgs& a, int rank, int* se
   *seq = chunk_last(a, place, [&](int i) { return chunk_place(a, i); });
   const int start = __builtin_amdgcn_readfirstlane(chunk_start(a, *seq)), count = __builtin_amdgcn_readfirstlane(chunk_start(a, *seq + 1)) - start;
   *tile = place - __builtin_amdgcn_readfirstlane(chunk_place(a, *seq));
-  return *tile >= 0 && count > 0 && *tile <= (count * a.G - 1) >> a.tile_shift;
+  return *tile >= 0 && count > 0 && count * a.G >= a.least && count * a.G <= a.most && *tile <= (count * a.G - 1) >> a.tile_shift;
 }
 
 // Launch the kernel of a pair of types (chunk_attention_kernel.hip and chunk_attention_few.hip, compiled once for each).

@@ -6,20 +6,14 @@ namespace lh {
 
 // One wave per row of the result whose positions were cut into shares: brings them to the common maximum and adds them in order.
 template <int QDT>
-__global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row_all = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int n = (int)(row_all / a.H), head = (int)(row_all - (int64_t)n * a.H);
-  if (n >= chunk_start(a, a.B)) return;
-  const int b = chunk_last(a, n, [&](int i) { return chunk_start(a, i); });
-  const int start = chunk_start(a, b), count = max(chunk_start(a, b + 1) - start, 0), token = n - start;
-  if (token < 0 || token >= count) return;
+__device__ __forceinline__ void chunk_join(const ChunkArgs& a, int n, int head, int b, int start, int count) {
+  const int lane = threadIdx.x & 63, token = n - start;
   const int hk = head / a.G, row = token * a.G + head % a.G, tile = row >> a.tile_shift;
   const int base = min(max(a.lengths[b], 0), a.c.capacity()) - count;
   const int sees = base + (min(count * a.G, (tile + 1) << a.tile_shift) - 1) / a.G + 1;
   if (sees <= a.share) return;  // (written at once)
   const int parts = (sees + a.share - 1) / a.share;
-  const int64_t place = (int64_t)((uint32_t)(start * a.G) >> a.tile_shift) + b + tile;
+  const int64_t place = chunk_place(a, b) + tile;
   const int64_t at = (place * a.c.heads + hk) * a.splits * a.tile_rows + (row - tile * a.tile_rows);
   float m = -INFINITY;
   for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[at + (int64_t)p * a.tile_rows].x);
@@ -44,22 +38,44 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a) {
     if (4 * lane + e < a.c.d) store_from_f32<QDT>(a.out, to + e, o[e] * inv);
 }
 
+// few: of the sequences with up to few.most rows.
+template <int QDT>
+__global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a, ChunkArgs few) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int n = (int)(row / a.H), head = (int)(row - (int64_t)n * a.H);
+  if (n >= chunk_start(a, a.B)) return;
+  const int b = chunk_last(a, n, [&](int i) { return chunk_start(a, i); });
+  const int start = chunk_start(a, b), count = max(chunk_start(a, b + 1) - start, 0);
+  if (n < start || n - start >= count) return;
+  if (count * a.G > few.most) chunk_join<QDT>(a, n, head, b, start, count);
+  else chunk_join<QDT>(few, n, head, b, start, count);
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------------
 
 static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
 
+// Sequences with up to 32 rows are for the kernel of the few, those with more for that of the many; but where they have no more than 32 on
+// average, all are for the first, and where a tile of 128 for each would add less than a quarter to the rows that there are, all for the second.
+enum ChunkPart { kAllFew, kAllMany, kTheFew, kTheMany };
+static ChunkPart chunk_part(const Paged& c, int64_t N, int64_t B, int64_t H) {
+  const int64_t rows = N * (H / c.heads);
+  return rows <= kChunkFew * B ? kAllFew : B == 1 || rows >= 4 * 128 * B ? kAllMany : kTheMany;
+}
+
 // `aligned`: keys and values begin at multiples of 16 bytes.
-static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H, bool aligned) {
+static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H, bool aligned, ChunkPart part) {
   ChunkPlan p = {};
   const int64_t G = H / c.heads;
   const int es = (int)dtype_size(cache_dtype);
-  // Tiles of 16 rows where the sequences have no more than two of them on average.
-  p.few = N * G <= 32 * B;
+  p.few = part == kAllFew || part == kTheFew;
+  p.least = part == kTheMany ? kChunkFew + 1 : 0, p.most = part == kTheFew ? kChunkFew : 0x7fffffff;
   p.tile_rows = p.few ? 16 : 128;
-  const int64_t slots = N * G / p.tile_rows + B;
+  const int64_t slots = part == kTheFew ? 2 * B : N * G / p.tile_rows + B;
   p.slots = (int)slots;
   // (A place more per sequence may be empty: the tiles that there probably are.)
-  const int64_t items = slots * c.heads, tiles = N * G / p.tile_rows > B ? N * G / p.tile_rows : B < N ? B : N;
+  const int64_t full = N * G / p.tile_rows, some = part == kTheMany ? 1 : B < N ? B : N;
+  const int64_t items = slots * c.heads, tiles = part == kTheFew || full < some ? some : full;
   if (p.few) {
     p.mode = paged_mode(c, es, aligned);
     p.width = paged_width(c.d);
@@ -99,8 +115,14 @@ size_t lh_hip_paged_attention_chunk_workspace_bytes(const lh_paged_cache* cache,
   Paged c;
   if (paged_cache(cache, "lh_hip_paged_attention_chunk_workspace_bytes", &c) != LH_OK || !chunk_sizes(c, N, B, H)) return 0;
   // (Room for either alignment: a caller may size it with one cache and pass a view of another.)
-  const size_t one = chunk_plan(c, cache->dtype, N, B, H, true).total(), other = chunk_plan(c, cache->dtype, N, B, H, false).total();
-  return one > other ? one : other;
+  const ChunkPart part = chunk_part(c, N, B, H);
+  size_t bytes = 0;
+  for (int aligned = 0; aligned < 2; ++aligned) {
+    size_t sum = chunk_plan(c, cache->dtype, N, B, H, aligned, part).total();
+    if (part == kTheMany) sum += chunk_plan(c, cache->dtype, N, B, H, aligned, kTheFew).total();
+    bytes = sum > bytes ? sum : bytes;
+  }
+  return bytes;
 }
 
 int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const void* q, int64_t out_stride_n, int64_t out_stride_h, int64_t q_stride_n,
@@ -115,29 +137,45 @@ int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const v
   LH_REQUIRE(out && q && lengths && starts, "%s: null pointer", what);
   LH_REQUIRE(dtype == cache->dtype || (cache->dtype == LH_F8E4M3 && (dtype == LH_BF16 || dtype == LH_F16)),
              "%s: queries must have the cache's dtype (bf16 or f16 for a cache of e4m3)", what);
-  const ChunkPlan p = chunk_plan(a.c, cache->dtype, N, B, H, aligned16(a.c.k) && aligned16(a.c.v));
-  LH_REQUIRE(p.total() == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= p.total()),
-             "%s: workspace too small or not 256-byte aligned: %zu of %zu bytes", what, workspace_bytes, p.total());
+  const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
+  const ChunkPart part = chunk_part(a.c, N, B, H);
+  const ChunkPlan p = chunk_plan(a.c, cache->dtype, N, B, H, aligned, part);
+  ChunkPlan f = {};
+  if (part == kTheMany) f = chunk_plan(a.c, cache->dtype, N, B, H, aligned, kTheFew);
+  const size_t need = p.total() + f.total();
+  LH_REQUIRE(need == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= need),
+             "%s: workspace too small or not 256-byte aligned: %zu of %zu bytes", what, workspace_bytes, need);
   a.out = out, a.q = q, a.so_n = out_stride_n, a.so_h = out_stride_h, a.sq_n = q_stride_n, a.sq_h = q_stride_h, a.lengths = lengths, a.starts = starts;
-  a.N = (int32_t)N, a.B = (int32_t)B, a.H = (int32_t)H, a.G = (int32_t)(H / a.c.heads), a.by_group = FastDiv((uint32_t)a.G);
-  a.tile_rows = p.tile_rows, a.tile_shift = p.few ? 4 : 7, a.slots = p.slots, a.ranked = B > 1 && B <= 32, a.share = p.share, a.splits = p.splits, a.width = p.width;
+  a.N = (int32_t)N, a.B = (int32_t)B, a.H = (int32_t)H, a.G = (int32_t)(H / a.c.heads), a.by_group = FastDiv((uint32_t)a.G), a.ranked = B > 1 && B <= 32;
   const double factor = (double)scale * a.c.k_scale * 1.4426950408889634;
   a.scale_log2e = scale == 0.0f ? 1.0f : (float)(factor < 0.0 ? -factor : factor);
   a.q_and = scale == 0.0f ? 0u : ~0u, a.q_xor = scale < 0.0f ? (dtype == LH_F32 ? 0x80000000u : 0x80008000u) : 0u;
   LH_REQUIRE(a.scale_log2e > 0.0f && a.scale_log2e < INFINITY, "%s: scale times the keys' scale must be finite", what);
-  if (p.splits > 1) a.part_o = static_cast<float*>(workspace), a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.o_bytes);
+  auto planned = [&](const ChunkPlan& plan, char* space) {
+    ChunkArgs x = a;
+    x.least = plan.least, x.most = plan.most, x.tile_rows = plan.tile_rows, x.tile_shift = plan.few ? 4 : 7, x.slots = plan.slots;
+    x.share = plan.share, x.splits = plan.splits, x.width = plan.width;
+    if (plan.splits > 1) x.part_o = reinterpret_cast<float*>(space), x.part_ml = reinterpret_cast<float2*>(space + plan.o_bytes);
+    return x;
+  };
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const auto launch = cache->dtype == LH_F32    ? (p.few ? chunk_few_f32 : chunk_many_f32)
-                      : cache->dtype == LH_BF16 ? (p.few ? chunk_few_bf16 : chunk_many_bf16)
-                      : cache->dtype == LH_F16  ? (p.few ? chunk_few_f16 : chunk_many_f16)
-                      : dtype == LH_BF16        ? (p.few ? chunk_few_e4m3_bf16 : chunk_many_e4m3_bf16)
-                                                : (p.few ? chunk_few_e4m3_f16 : chunk_many_e4m3_f16);
-  const int rc = launch(a, p, s);
-  if (rc != LH_OK || p.splits == 1) return rc;
+  auto launch = [&](const ChunkArgs& x, const ChunkPlan& plan) {
+    const auto kernel = cache->dtype == LH_F32    ? (plan.few ? chunk_few_f32 : chunk_many_f32)
+                        : cache->dtype == LH_BF16 ? (plan.few ? chunk_few_bf16 : chunk_many_bf16)
+                        : cache->dtype == LH_F16  ? (plan.few ? chunk_few_f16 : chunk_many_f16)
+                        : dtype == LH_BF16        ? (plan.few ? chunk_few_e4m3_bf16 : chunk_many_e4m3_bf16)
+                                                  : (plan.few ? chunk_few_e4m3_f16 : chunk_many_e4m3_f16);
+    return kernel(x, plan, s);
+  };
+  const ChunkArgs main = planned(p, static_cast<char*>(workspace)), few = part == kTheMany ? planned(f, static_cast<char*>(workspace) + p.total()) : main;
+  if (const int rc = launch(main, p)) return rc;
+  if (part == kTheMany)
+    if (const int rc = launch(few, f)) return rc;
+  if (need == 0) return LH_OK;
   const dim3 grid((unsigned)((N * H + 3) / 4)), block(256);
-  if (dtype == LH_BF16) LH_LAUNCH((chunk_join_kernel<LH_BF16>), grid, block, 0, s, a);
-  else if (dtype == LH_F16) LH_LAUNCH((chunk_join_kernel<LH_F16>), grid, block, 0, s, a);
-  else LH_LAUNCH((chunk_join_kernel<LH_F32>), grid, block, 0, s, a);
+  if (dtype == LH_BF16) LH_LAUNCH((chunk_join_kernel<LH_BF16>), grid, block, 0, s, main, few);
+  else if (dtype == LH_F16) LH_LAUNCH((chunk_join_kernel<LH_F16>), grid, block, 0, s, main, few);
+  else LH_LAUNCH((chunk_join_kernel<LH_F32>), grid, block, 0, s, main, few);
   return check_launch("chunk_join");
 }
 
