@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
   static_assert(NI >= 1 && NP * 256 == KEYS * CPR, "");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   typedef typename std::conditional<F32, float, uint16_t>::type elem;
-  __shared__ int64_t k_at[2][KEYS], v_at[2][KEYS];  // where the rows of a step lie, in elements; below 0: nowhere
+  __shared__ int64_t k_at[2][KEYS], v_at[2][KEYS];  // where the rows of a step lie, in elements; 0 where there is none
   __shared__ uint64_t held[8];           // which positions of a step there are (noted up to four steps before they are read)
   __shared__ int32_t wild[2][4], first_wild[D];
 
@@ -237,26 +237,24 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
     const int key = k0 + step * KEYS + tid;
     const bool there = key < k1 && (uint32_t)page < (uint32_t)a.c.pages;
     const int slot = there ? key - (int)a.c.by_size.div((uint32_t)key) * a.c.size : 0;
-    k_at[step & 1][tid] = there ? page * a.c.sk.z + slot * a.c.sk.t : -1;
-    v_at[step & 1][tid] = there ? page * a.c.sv.z + slot * a.c.sv.t : -1;
+    k_at[step & 1][tid] = there ? page * a.c.sk.z + slot * a.c.sk.t : 0;
+    v_at[step & 1][tid] = there ? page * a.c.sv.z + slot * a.c.sv.t : 0;
     const uint64_t some = __builtin_amdgcn_ballot_w64(there);
     if (lane == 0) held[step & 7] = some;
   };
   uint32_t kr[RS > 0 ? RS : 1][RS > 0 ? NP : 1][PW], vr[RS > 0 ? RS : 1][RS > 0 ? NP : 1][PW];
-  uint32_t there[RS > 0 ? RS : 1] = {};  // which of the thread's rows there are
-  auto request = [&](int step, int i, uint32_t* k, uint32_t* v, uint32_t& some) {
+  auto request = [&](int step, int i, uint32_t* k, uint32_t* v) {
     const int piece = tid + 256 * i, key = piece / CPR, col = (piece - key * CPR) * PE;
     const int64_t k_row = k_at[step & 1][key], v_row = v_at[step & 1][key];
-    some = (some & ~(1u << i)) | (uint32_t)(k_row >= 0) << i;
     const int d = hide(a.c.d);
-    load_columns<CES, ODD, SHORT>(k, kb + max(k_row, (int64_t)0) * CES, col, d);
-    load_columns<CES, ODD, SHORT>(v, vb + max(v_row, (int64_t)0) * CES, col, d);
+    load_columns<CES, ODD, SHORT>(k, kb + k_row * CES, col, d);
+    load_columns<CES, ODD, SHORT>(v, vb + v_row * CES, col, d);
   };
-  auto put = [&](elem* Ks, int i, uint32_t* k, uint32_t* v, uint32_t some, bool full, bool look) {  // into LDS; not 0 where a value is an infinity or a NaN, if asked for
+  auto put = [&](elem* Ks, int i, uint32_t* k, uint32_t* v, uint64_t some, bool full, bool look) {  // into LDS; not 0 where a value is an infinity or a NaN, if asked for
     const int piece = tid + 256 * i, key = piece / CPR, col = (piece - key * CPR) * PE;
     if (!full) {
       const int d = hide(a.c.d);
-      const uint32_t there = (uint32_t)((int32_t)(some << (31 - i)) >> 31);
+      const uint32_t there = 0u - ((uint32_t)(some >> key) & 1u);
       settle_columns<CES, ODD, SHORT>(k, col, d, there);
       settle_columns<CES, ODD, SHORT>(v, col, d, there);
     }
@@ -274,26 +272,27 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
     constexpr int S = decltype(set)::value;
     elem* const Ks = stage0 + (step & 1) * kStage;
     const bool look = partial(step);
-    const bool full = __builtin_amdgcn_readfirstlane(a.c.d == D && held[step & 7] == ~0ull);  // nothing of the step has to become 0
+    const uint64_t some = held[step & 7];
+    const bool full = __builtin_amdgcn_readfirstlane(a.c.d == D && some == ~0ull);  // nothing of the step has to become 0
     uint32_t odd_one = 0;
     if constexpr (RS > 0) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) odd_one |= put(Ks, i, kr[S % RS][i], vr[S % RS][i], there[S % RS], full, look);
+      for (int i = 0; i < NP; ++i) odd_one |= put(Ks, i, kr[S % RS][i], vr[S % RS][i], some, full, look);
       if (step + RS < steps)
 #pragma unroll
-        for (int i = 0; i < NP; ++i) request(step + RS, i, kr[S % RS][i], vr[S % RS][i], there[S % RS]);
+        for (int i = 0; i < NP; ++i) request(step + RS, i, kr[S % RS][i], vr[S % RS][i]);
     } else {
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        uint32_t k[PW], v[PW], some = 0;
-        request(step, i, k, v, some);
+        uint32_t k[PW], v[PW];
+        request(step, i, k, v);
         odd_one |= put(Ks, i, k, v, some, full, look);
         if (i % (ODD ? 2 : 4) == 1) asm volatile("" ::: "memory");  // (a few of each on their way at once)
       }
     }
     if (look) {
-      const bool some = __any(odd_one != 0);
-      if (lane == 0) wild[TWO ? step & 1 : 0][wave] = some;
+      const bool found = __any(odd_one != 0);
+      if (lane == 0) wild[TWO ? step & 1 : 0][wave] = found;
     }
   };
   typedef std::integral_constant<int, 0> even_t;
@@ -315,7 +314,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
       for (int r = 0; r < RS; ++r)
         if (r < steps)
 #pragma unroll
-          for (int i = 0; i < NP; ++i) request(r, i, kr[r][i], vr[r][i], there[r]);
+          for (int i = 0; i < NP; ++i) request(r, i, kr[r][i], vr[r][i]);
       lds_barrier();  // (where the first ones lie has been read)
 #pragma unroll
       for (int i = 2; i < RS + 2; ++i) note(i, pages[i]);
@@ -374,6 +373,15 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
             s[i] = mma(kf, qe, s[i]);
           }
         }
+      }
+      if constexpr (!F32 && Q_HELD) {  // (keys are read from LDS four matrix instructions ahead)
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int e = 0; e < NI * SD - 4; ++e) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
       }
       // s[i][v] = q . k of row r32 and position j0 + 32 i + 8 (v / 4) + 4 h + v % 4
       const bool whole = j0 + 32 * NI - 1 <= min(wave_first, k1 - 1) && row0 + 31 < rows && all_held == ~0ull;
