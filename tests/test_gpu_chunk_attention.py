@@ -112,6 +112,18 @@ def test_long_caches_are_split_and_joined(dtype, d, counts):
     check(q, c, counts, out, rows=(0, 1, 63, 64, 65, 1000, -1))
 
 
+@pytest.mark.parametrize("dtype,d", [(bf16, 128), (f32, 64), (e4m3, 128), (f16, 96)])
+@pytest.mark.parametrize("B", [2, 20, 33, 70])
+def test_pieces_among_single_tokens(dtype, d, B):
+    """Sequences with few rows beside ones with many, around the number of rows (32: 8 tokens here) that parts them, up to 12 shares of positions."""
+    counts = [(1, 8, 9, 0, 300, 2, 33)[b % 7] if b < 14 else b % 2 for b in range(B)]
+    counts[-1] = 140
+    lengths = [n + (0, 1, 64, 250, 2700, 500)[b % 6] if b < 14 else n + b for b, n in enumerate(counts)]
+    c = ref.Cache(lengths, 2, 16, d, dtype, seed=B, scales=(0.75, 1.5) if dtype == e4m3 else (1.0, 1.0))
+    q, out = run(c, counts, 8, seed=B)
+    check(q, c, counts, out, rows=(0, 31, 32, -1))
+
+
 def test_a_whole_prompt_is_what_attention_gives():
     c = ref.Cache([700, 300], 4, 16, 64, f32, seed=3)
     counts = [700, 300]
