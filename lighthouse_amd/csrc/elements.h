@@ -69,7 +69,8 @@ __device__ __forceinline__ Piece<DT> piece_of_f32(const float* x) {
 }
 
 // The first n (1 to 8) elements to p.
-template <int DT>
+// STREAM: whole pieces are not kept in the caches.
+template <int DT, bool STREAM = false>
 __device__ __forceinline__ void store_piece(void* p, const Piece<DT>& v, int n) {
   constexpr int ES = elem_bytes<DT>();
   typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
@@ -78,8 +79,11 @@ __device__ __forceinline__ void store_piece(void* p, const Piece<DT>& v, int n) 
       *reinterpret_cast<u32x2_any*>(p) = u32x2_any{v.w[0], v.w[1]};
     } else {
 #pragma unroll
-      for (int l = 0; l < kPiece * ES / 16; ++l)
-        reinterpret_cast<typename Chunk<ES>::type*>(p)[l] = typename Chunk<ES>::type{v.w[4 * l], v.w[4 * l + 1], v.w[4 * l + 2], v.w[4 * l + 3]};
+      for (int l = 0; l < kPiece * ES / 16; ++l) {
+        const typename Chunk<ES>::type w = {v.w[4 * l], v.w[4 * l + 1], v.w[4 * l + 2], v.w[4 * l + 3]};
+        if constexpr (STREAM) __builtin_nontemporal_store(w, reinterpret_cast<typename Chunk<ES>::type*>(p) + l);
+        else reinterpret_cast<typename Chunk<ES>::type*>(p)[l] = w;
+      }
     }
   } else {
 #pragma unroll

@@ -3,7 +3,7 @@
 // Column pairs (a, b) of a head, (i, i + R / 2) or (2 i, 2 i + 1) for i < R / 2, turn by the angle position * freqs[i]:
 //   a' = a cos - b sin,  b' = b cos + a sin,
 // the other columns stay.  A token's angles are the same for all of its heads: a thread makes the eight it needs and uses them for up to
-// four heads, whose loads are on their way meanwhile.  The angle is reduced in 64 bits (a position of 10^6 times a frequency of 1 leaves an
+// two heads, whose loads are on their way meanwhile.  The angle is reduced in 64 bits (a position of 10^6 times a frequency of 1 leaves an
 // f32 4 places after the point), the reduced one has a sine and cosine by their Taylor series, in f32.
 //
 // Both operators read and write every value once and are bound by memory, or by the launch for a step of one token a sequence.
@@ -30,7 +30,7 @@ struct RotaryArgs {
   int32_t H, heads, d, half;  // heads of q (0: none), of the cache (0: nothing is stored), columns, pairs that turn (0: none)
   int64_t all_slots;
   FastDiv by_size, by_chunks, by_groups;
-  int32_t turning;        // chunks of a head that turn: 8 pairs each; the others hold 16 columns
+  int32_t turning;        // chunks of a head that turn: 8 pairs each
   int32_t threads;
 };
 
@@ -60,8 +60,9 @@ __device__ __forceinline__ void cos_sin(int position, double freq, float* c, flo
   *s = n >= 2 ? -sq : sq;
 }
 
-// A thread takes one chunk of PER heads of a token (of q, keys and values counted through): chunk c < turning has the pairs 8 c .. 8 c + 7, the
-// others 16 columns behind those that turn.  Values, and keys that do not turn, are chunks of 16 columns from 0 on.
+// A thread takes one chunk, two pieces of 8 columns, of PER heads of a token (of q, keys and values counted through).  The pieces of what turns, of
+// what is behind it, and of a value, each are cut in two halves, and a chunk has one of either, so that neighbours read and write neighbouring
+// pieces (16 neighbouring columns a chunk: 41.5 us, so 38.1, 8192 tokens of 40 heads of 128, 96 of which turn in neighbouring pairs, f16).
 template <int SDT, int CDT, bool INTERLEAVED, int PER>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
   constexpr int SES = elem_bytes<SDT>(), CES = elem_bytes<CDT>();
@@ -91,12 +92,12 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
     n0[i] = n1[i] = 0, c0[i] = c1[i] = 0;
     if (head < heads_all && (!stored || page >= 0)) {
       if (value || chunk >= a.turning) {
-        const int first = value ? 16 * chunk : 2 * a.half + 16 * (chunk - a.turning);
-        c0[i] = first, c1[i] = first + 8;
-        n0[i] = min(max(a.d - first, 0), 8), n1[i] = min(max(a.d - first - 8, 0), 8);
+        const int from = value ? 0 : 2 * a.half, at = value ? chunk : chunk - a.turning, chunks_here = (a.d - from + 15) >> 4;
+        c0[i] = from + 8 * at, c1[i] = c0[i] + 8 * chunks_here;
+        n0[i] = at < chunks_here ? min(a.d - c0[i], 8) : 0, n1[i] = at < chunks_here ? min(max(a.d - c1[i], 0), 8) : 0;
       } else if (INTERLEAVED) {
-        c0[i] = 16 * chunk, c1[i] = 16 * chunk + 8;
-        n0[i] = min(2 * a.half - 16 * chunk, 8), n1[i] = min(max(2 * a.half - 16 * chunk - 8, 0), 8);
+        c0[i] = 8 * chunk, c1[i] = 8 * (chunk + a.turning);
+        n0[i] = min(2 * a.half - c0[i], 8), n1[i] = min(max(2 * a.half - c1[i], 0), 8);
       } else {
         c0[i] = 8 * chunk, c1[i] = a.half + 8 * chunk;
         n0[i] = n1[i] = min(a.half - 8 * chunk, 8);
@@ -112,7 +113,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
   if (chunk < a.turning) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      cos_sin(position, a.freqs[min(8 * chunk + e, a.half - 1)], &c[e], &s[e]);
+      const int pair = INTERLEAVED ? 4 * (e < 4 ? chunk : chunk + a.turning) + e % 4 : 8 * chunk + e;
+      cos_sin(position, a.freqs[min(pair, a.half - 1)], &c[e], &s[e]);
       c[e] *= a.amplitude, s[e] *= a.amplitude;
     }
   }
@@ -148,8 +150,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
     if (!stored) {
       uint8_t* to = static_cast<uint8_t*>(a.out) + (n * a.so_n + head * a.so_h) * SES;
       const Piece<SDT> first = turns ? piece_of_f32<SDT>(x) : lo[i], second = turns ? piece_of_f32<SDT>(y) : hi[i];
-      store_piece<SDT>(to + (int64_t)c0[i] * SES, first, n0[i]);
-      if (n1[i] > 0) store_piece<SDT>(to + (int64_t)c1[i] * SES, second, n1[i]);
+      store_piece<SDT, (PER > 1)>(to + (int64_t)c0[i] * SES, first, n0[i]);
+      if (n1[i] > 0) store_piece<SDT, (PER > 1)>(to + (int64_t)c1[i] * SES, second, n1[i]);
     } else {
       const lh_strides3 cs = value ? a.cv : a.ck;
       uint8_t* to = static_cast<uint8_t*>(value ? a.v_cache : a.k_cache) + (page * cs.z + (head - a.H - (value ? a.heads : 0)) * cs.h + slot * cs.t) * CES;
@@ -163,22 +165,23 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
         first = turns ? piece_of_f32<CDT>(x) : __builtin_bit_cast(Piece<CDT>, lo[i]);
         second = turns ? piece_of_f32<CDT>(y) : __builtin_bit_cast(Piece<CDT>, hi[i]);
       }
-      store_piece<CDT>(to + (int64_t)c0[i] * CES, first, n0[i]);
-      if (n1[i] > 0) store_piece<CDT>(to + (int64_t)c1[i] * CES, second, n1[i]);
+      store_piece<CDT, (PER > 1)>(to + (int64_t)c0[i] * CES, first, n0[i]);
+      if (n1[i] > 0) store_piece<CDT, (PER > 1)>(to + (int64_t)c1[i] * CES, second, n1[i]);
     }
   }
 }
 
 template <int SDT, int CDT, bool INTERLEAVED>
 static int launch_rotary(RotaryArgs& a, int64_t N, int heads_all, int chunks, hipStream_t s) {
-  // Four heads a thread where that leaves more threads than the chip holds at once.
+  // Two heads a thread where that leaves more threads than the chip holds at once, and results that no cache would hold for the next reader
+  // (8192 tokens of 40 heads of 128, f16: one head 41.6 us, two 38.7, two and streaming stores 35.2, four 41.2, eight 43.4).
   const bool many = N * heads_all * chunks >= 4ll * num_cus() * 2048;
-  const int groups = many ? (heads_all + 3) / 4 : heads_all;
+  const int groups = many ? (heads_all + 1) / 2 : heads_all;
   const int64_t threads = N * groups * chunks;
   LH_REQUIRE(threads < (1ll << 31) - 256, "rotary positions: too many values");
   a.by_groups = FastDiv((uint32_t)groups), a.threads = (int32_t)threads;
   const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
-  if (many) LH_LAUNCH((rotary_kernel<SDT, CDT, INTERLEAVED, 4>), grid, block, 0, s, a);
+  if (many) LH_LAUNCH((rotary_kernel<SDT, CDT, INTERLEAVED, 2>), grid, block, 0, s, a);
   else LH_LAUNCH((rotary_kernel<SDT, CDT, INTERLEAVED, 1>), grid, block, 0, s, a);
   return check_launch("rotary");
 }
