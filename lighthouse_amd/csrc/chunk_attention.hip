@@ -74,38 +74,55 @@ __device__ __forceinline__ void chunk_join(const ChunkArgs& a, int n, int head, 
     if (4 * lane + e < a.c.d) store_from_f32<QDT>(a.out, to + e, o[e] * inv);
 }
 
-// few: of the sequences with up to few.most rows.  WAVES: a row's, 1 or all 4 of the workgroup.
-template <int QDT, int WAVES>
+// few: of the sequences with up to few.most rows.  WAVES: a row's, 1 or all 4 of the workgroup.  ALL: rows of the result one after the other;
+// otherwise those that a sequence with few rows may have, since no other's positions were cut.
+template <int QDT, int WAVES, bool ALL>
 __global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a, ChunkArgs few) {
   const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
-  const int n = (int)(row / a.H), head = (int)(row - (int64_t)n * a.H);
-  if (n >= chunk_start(a, a.B)) return;
-  const int b = chunk_last(a, n, [&](int i) { return chunk_start(a, i); });
-  const int start = chunk_start(a, b), count = max(chunk_start(a, b + 1) - start, 0);
-  if (n < start || n - start >= count) return;
-  if (count * a.G > few.most) chunk_join<QDT, WAVES>(a, n, head, b, start, count);
+  int n, head, b, start, count;
+  if constexpr (ALL) {
+    n = (int)(row / a.H), head = (int)(row - (int64_t)n * a.H);
+    if (n >= chunk_start(a, a.B)) return;
+    b = chunk_last(a, n, [&](int i) { return chunk_start(a, i); });
+    start = chunk_start(a, b), count = max(chunk_start(a, b + 1) - start, 0);
+    if (n < start || n - start >= count) return;
+  } else {
+    const int item = (int)(row / kChunkFew), at = (int)(row % kChunkFew);
+    b = item / a.c.heads;
+    if (b >= a.B) return;
+    start = chunk_start(a, b), count = max(chunk_start(a, b + 1) - start, 0);
+    if (at >= count * a.G || count * a.G > kChunkFew) return;
+    n = start + at / a.G, head = (item - b * a.c.heads) * a.G + at % a.G;
+  }
+  if (ALL && count * a.G > few.most) chunk_join<QDT, WAVES>(a, n, head, b, start, count);
   else chunk_join<QDT, WAVES>(few, n, head, b, start, count);
 }
 
 template <int QDT>
 static void chunk_join_launch(const ChunkArgs& a, const ChunkArgs& few, hipStream_t s) {
-  const int64_t rows = (int64_t)a.N * a.H;
+  const int64_t rows = (int64_t)a.N * a.H, few_rows = (int64_t)a.B * a.c.heads * kChunkFew;
   // A wave for up to 8 shares, and where the rows are enough to fill the device (4 drafted tokens after 8188 positions, 32 shares: 24.3 us, with
-  // four waves 17.7; 1038 tokens of 16 heads, few of them of 12 shares: 76 us, with four 93).
-  if ((a.splits <= 8 && few.splits <= 8) || rows > 8 * num_cus()) LH_LAUNCH((chunk_join_kernel<QDT, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, few);
-  else LH_LAUNCH((chunk_join_kernel<QDT, 4>), dim3((unsigned)rows), dim3(256), 0, s, a, few);
+  // four waves 17.7; 1038 tokens of 16 heads, few of them of 12 shares: 76 us, with four 93).  (With few rows that are cut, and others that are not,
+  // they are.)
+  if (a.splits == 1) LH_LAUNCH((chunk_join_kernel<QDT, 1, false>), dim3((unsigned)((few_rows + 3) / 4)), dim3(256), 0, s, a, few);
+  else if ((a.splits <= 8 && few.splits <= 8) || rows > 8 * num_cus()) LH_LAUNCH((chunk_join_kernel<QDT, 1, true>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, few);
+  else LH_LAUNCH((chunk_join_kernel<QDT, 4, true>), dim3((unsigned)rows), dim3(256), 0, s, a, few);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 
 static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
 
-// Sequences with up to 32 rows are for the kernel of the few, those with more for that of the many; but where they have no more than 32 on
-// average, all are for the first, and where a tile of 128 for each would add less than a quarter to the rows that there are, all for the second.
+// Sequences with up to 32 rows are for the kernel of the few, those with more for that of the many: two pieces of 512 among 14 tokens of 16 heads
+// take 98 us in the kernel of the many, 82 so; of 32 heads 163 and 146.  But all are for the first where they have no more than 32 rows on average,
+// and all for the second where a tile of 128 for each would add less than a quarter to the rows that there are, or where there are more tiles than
+// workgroups run at once: single tokens, bound by memory, then run beside the others (8 pieces of 512 among 56 tokens of 32 heads: 199 us, 216 in
+// two launches; 32 of 256 among 224: 261, 293).
 enum ChunkPart { kAllFew, kAllMany, kTheFew, kTheMany };
 static ChunkPart chunk_part(const Paged& c, int64_t N, int64_t B, int64_t H) {
   const int64_t rows = N * (H / c.heads);
-  return rows <= kChunkFew * B ? kAllFew : B == 1 || rows >= 4 * 128 * B ? kAllMany : kTheMany;
+  if (rows <= kChunkFew * B) return kAllFew;
+  return B == 1 || rows >= 4 * 128 * B || (rows / 128 + B) * c.heads > 2 * num_cus() ? kAllMany : kTheMany;
 }
 
 // Positions of each of `splits` shares of a sequence's, which have no fewer than 256.

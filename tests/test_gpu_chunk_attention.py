@@ -124,6 +124,14 @@ def test_pieces_among_single_tokens(dtype, d, B):
     check(q, c, counts, out, rows=(0, 31, 32, -1))
 
 
+@pytest.mark.parametrize("dtype", [bf16, f32, e4m3])
+def test_only_sequences_with_few_rows_are_cut(dtype):
+    counts = [300, 2, 8, 10]
+    c = ref.Cache([300, 900, 1500, 700], 32, 16, 64, dtype, seed=18)
+    q, out = run(c, counts, 128)
+    check(q, c, counts, out, rows=(0, 3, 7, 255, -1))
+
+
 def test_a_whole_prompt_is_what_attention_gives():
     c = ref.Cache([700, 300], 4, 16, 64, f32, seed=3)
     counts = [700, 300]
