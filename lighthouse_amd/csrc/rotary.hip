@@ -50,11 +50,11 @@ __device__ __forceinline__ void cos_sin_eighth(float x, float* c, float* s) {
 }
 // Of position * freq radians.
 __device__ __forceinline__ void cos_sin(int position, double freq, float* c, float* s) {
-  const double quarters = (double)position * (freq * 0.63661977236758134308);  // 2 / pi
-  const double whole = __builtin_rint(quarters);
+  const double turns = (double)position * (freq * 0.15915494309189533577);  // 1 / (2 pi)
+  const double quarters = 4.0 * __builtin_amdgcn_fract(turns), whole = __builtin_rint(quarters);
   float c0, s0;
   cos_sin_eighth((float)((quarters - whole) * 0.25), &c0, &s0);
-  const int n = (int)((int64_t)whole & 3);
+  const int n = (int)whole & 3;
   const float cq = n & 1 ? s0 : c0, sq = n & 1 ? c0 : s0;
   *c = n == 1 || n == 2 ? -cq : cq;
   *s = n >= 2 ? -sq : sq;
@@ -150,8 +150,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
     if (!stored) {
       uint8_t* to = static_cast<uint8_t*>(a.out) + (n * a.so_n + head * a.so_h) * SES;
       const Piece<SDT> first = turns ? piece_of_f32<SDT>(x) : lo[i], second = turns ? piece_of_f32<SDT>(y) : hi[i];
-      store_piece<SDT, (PER > 1)>(to + (int64_t)c0[i] * SES, first, n0[i]);
-      if (n1[i] > 0) store_piece<SDT, (PER > 1)>(to + (int64_t)c1[i] * SES, second, n1[i]);
+      store_piece<SDT>(to + (int64_t)c0[i] * SES, first, n0[i]);
+      if (n1[i] > 0) store_piece<SDT>(to + (int64_t)c1[i] * SES, second, n1[i]);
     } else {
       const lh_strides3 cs = value ? a.cv : a.ck;
       uint8_t* to = static_cast<uint8_t*>(value ? a.v_cache : a.k_cache) + (page * cs.z + (head - a.H - (value ? a.heads : 0)) * cs.h + slot * cs.t) * CES;
@@ -165,23 +165,25 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
         first = turns ? piece_of_f32<CDT>(x) : __builtin_bit_cast(Piece<CDT>, lo[i]);
         second = turns ? piece_of_f32<CDT>(y) : __builtin_bit_cast(Piece<CDT>, hi[i]);
       }
-      store_piece<CDT, (PER > 1)>(to + (int64_t)c0[i] * CES, first, n0[i]);
-      if (n1[i] > 0) store_piece<CDT, (PER > 1)>(to + (int64_t)c1[i] * CES, second, n1[i]);
+      store_piece<CDT>(to + (int64_t)c0[i] * CES, first, n0[i]);
+      if (n1[i] > 0) store_piece<CDT>(to + (int64_t)c1[i] * CES, second, n1[i]);
     }
   }
 }
 
 template <int SDT, int CDT, bool INTERLEAVED>
 static int launch_rotary(RotaryArgs& a, int64_t N, int heads_all, int chunks, hipStream_t s) {
-  // Two heads a thread where that leaves more threads than the chip holds at once, and results that no cache would hold for the next reader
-  // (8192 tokens of 40 heads of 128, f16: one head 41.6 us, two 38.7, two and streaming stores 35.2, four 41.2, eight 43.4).
-  const bool many = N * heads_all * chunks >= 4ll * num_cus() * 2048;
-  const int groups = many ? (heads_all + 1) / 2 : heads_all;
+  // Two heads a thread, which share their angles, where half as many threads still fill half of the chip: prompts of 8192 tokens, 24 heads of 64,
+  // into e4m3 13.9 us (one head 16.4, four 13.7); 64 tokens of 24 heads 4.4 us (one head 3.8).  (Stores past the
+  // caches cost their reader more than they save: 8192 tokens of 40 heads of 128, f16, into one buffer that is read after, 92.5 us; 81.1 kept.)
+  const int64_t values = N * heads_all * chunks, at_once = (int64_t)num_cus() * 2048;
+  const int per = 2 * values >= at_once ? 2 : 1;
+  const int groups = (heads_all + per - 1) / per;
   const int64_t threads = N * groups * chunks;
   LH_REQUIRE(threads < (1ll << 31) - 256, "rotary positions: too many values");
   a.by_groups = FastDiv((uint32_t)groups), a.threads = (int32_t)threads;
   const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
-  if (many) LH_LAUNCH((rotary_kernel<SDT, CDT, INTERLEAVED, 2>), grid, block, 0, s, a);
+  if (per == 2) LH_LAUNCH((rotary_kernel<SDT, CDT, INTERLEAVED, 2>), grid, block, 0, s, a);
   else LH_LAUNCH((rotary_kernel<SDT, CDT, INTERLEAVED, 1>), grid, block, 0, s, a);
   return check_launch("rotary");
 }
