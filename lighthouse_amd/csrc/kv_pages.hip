@@ -6,8 +6,10 @@
 // depend on which thread is first.
 //
 // One workgroup does the pages: a step moves few (4096 for 65536 new tokens in pages of 16), and the sums would need the others to wait for
-// each other.  What bounds it is its chain of dependent loads (length, table, list).  The tokens' positions and slots are its work too
-// where they are few; otherwise a second launch finds each token's sequence by bisection of the running sums.
+// each other.  What bounds it is its chain of dependent loads (length, table, list) and barriers: 64 sequences of up to 1024 positions that get a
+// token each take 6.7 us with 256 threads (8.6 with 1024), 1024 sequences that get 66432 tokens 19 us, of which 4 loops over about a thousand
+// pages each, out of memory, are the larger part.  The tokens' positions and slots are its work too where they are few; otherwise a second
+// launch finds each token's sequence by bisection of the running sums (5.2 us for those 66432).
 #include "paged.h"
 #include "wave_scan.h"
 
@@ -28,10 +30,10 @@ struct PagesArgs {
   FastDiv by_size;
 };
 
-constexpr int kPagesThreads = 1024, kPagesWaves = kPagesThreads / 64;
-constexpr int kPagesTokens = 4096;  // tokens that the one workgroup places itself
+constexpr int kPagesThreads = 1024;
 
 // Running sum over the workgroup's threads, up to and with this one; *all: of all of them.  `sums`: one entry per wave, its own.
+template <int WAVES>
 __device__ __forceinline__ uint64_t pages_scan(uint64_t v, uint64_t* sums, uint64_t* all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   v = wave_scan(v);
@@ -40,7 +42,7 @@ __device__ __forceinline__ uint64_t pages_scan(uint64_t v, uint64_t* sums, uint6
   __syncthreads();
   uint64_t before = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < kPagesWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     if (w < wave) before += sums[w];
     total += sums[w];
   }
@@ -98,15 +100,16 @@ __device__ __forceinline__ void pages_place(const PagesArgs& a, int i, int b, in
   a.slots[i] = slot;
 }
 
-__global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(PagesArgs a) {
-  __shared__ uint64_t sums[kPagesThreads];  // running sums of pages, of the sequences of a round
-  __shared__ uint64_t scan[kPagesWaves];
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_pages_kernel(PagesArgs a) {
+  __shared__ uint64_t sums[THREADS];  // running sums of pages, of the sequences of a round
+  __shared__ uint64_t scan[THREADS / 64];
   __shared__ uint64_t most;
-  __shared__ int32_t from[kPagesThreads];   // a table's entry that the pages begin at
-  __shared__ int32_t ends[kPagesThreads];   // running sum of tokens, at most N
-  __shared__ int32_t first_at[kPagesThreads];
+  __shared__ int32_t from[THREADS];   // a table's entry that the pages begin at
+  __shared__ int32_t ends[THREADS];   // running sum of tokens, at most N
+  __shared__ int32_t first_at[THREADS];
   const int tid = threadIdx.x;
-  const int rounds = (a.B + kPagesThreads - 1) / kPagesThreads;
+  const int rounds = (a.B + THREADS - 1) / THREADS;
   const int free_before = min(max(*a.n_free, 0), a.F);
   PagesSequence s = {};
   // Sequence b of this thread; `tokens`: before the round's.
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(PagesArgs a) {
       s.count = a.counts[b];
       s.held = pages_held(a, b, pages_for(a, s.length));
     }
-    const uint64_t end = tokens + pages_scan((uint64_t)max(s.count, (int64_t)0), scan, round_tokens);
+    const uint64_t end = tokens + pages_scan<THREADS / 64>((uint64_t)max(s.count, (int64_t)0), scan, round_tokens);
     const int64_t length = s.count < 0 ? 0 : s.length + s.count;
     s.fits = b < a.B && length <= (int64_t)a.P * a.size && end <= (uint64_t)a.N;
     s.need = s.fits ? pages_for(a, length) : s.held;
@@ -130,16 +133,16 @@ __global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(PagesArgs a) {
   uint64_t tokens = 0, back = 0, round_tokens = 0;
   if (tid == 0) a.starts[0] = 0;
   for (int round = 0; round < rounds; ++round) {
-    const int b = round * kPagesThreads + tid;
+    const int b = round * THREADS + tid;
     look(b, tokens, &round_tokens);
     uint64_t all;
-    const uint64_t up_to = pages_scan((uint64_t)max(s.held - s.need, 0), scan, &all);
+    const uint64_t up_to = pages_scan<THREADS / 64>((uint64_t)max(s.held - s.need, 0), scan, &all);
     sums[tid] = up_to;
     from[tid] = s.need - (int32_t)(up_to - (uint64_t)max(s.held - s.need, 0));  // (modulo 2^32: what is added to it takes it back)
     __syncthreads();
-    for (uint64_t r = tid; r < all; r += kPagesThreads) {
-      const int t = first_above(sums, kPagesThreads, r);
-      int32_t* entry = a.table + (round * kPagesThreads + t) * a.table_stride + (from[t] + (int32_t)r);
+    for (uint64_t r = tid; r < all; r += THREADS) {
+      const int t = first_above(sums, THREADS, r);
+      int32_t* entry = a.table + (round * THREADS + t) * a.table_stride + (from[t] + (int32_t)r);
       const uint64_t to = free_before + back + r;
       if (to < (uint64_t)a.F) a.free_pages[to] = *entry;
       *entry = -1;
@@ -155,7 +158,7 @@ __global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(PagesArgs a) {
   uint64_t wanted = 0, taken = 0;
   tokens = 0;
   for (int round = 0; round < rounds; ++round) {
-    const int b = round * kPagesThreads + tid;
+    const int b = round * THREADS + tid;
     if (rounds > 1) {
       look(b, tokens, &round_tokens);
       tokens += round_tokens;
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(PagesArgs a) {
     }
     const int more = max(s.need - s.held, 0);
     uint64_t all;
-    const uint64_t up_to = pages_scan((uint64_t)more, scan, &all);
+    const uint64_t up_to = pages_scan<THREADS / 64>((uint64_t)more, scan, &all);
     const bool gets = s.fits && (more == 0 || wanted + up_to <= (uint64_t)there);
     if (tid == 0) most = 0;
     sums[tid] = up_to;
@@ -179,19 +182,19 @@ __global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(PagesArgs a) {
     }
     __syncthreads();
     const uint64_t now = most;
-    for (uint64_t r = tid; r < now; r += kPagesThreads) {
-      const int t = first_above(sums, kPagesThreads, r);
-      a.table[(round * kPagesThreads + t) * a.table_stride + (from[t] + (int32_t)r)] = a.free_pages[there - 1 - (int64_t)(wanted + r)];
+    for (uint64_t r = tid; r < now; r += THREADS) {
+      const int t = first_above(sums, THREADS, r);
+      a.table[(round * THREADS + t) * a.table_stride + (from[t] + (int32_t)r)] = a.free_pages[there - 1 - (int64_t)(wanted + r)];
     }
     wanted += all;
     taken += now;
     __syncthreads();
   }
   if (tid == 0) *a.n_free = there - (int)taken;
-  if (rounds > 1 || a.N > kPagesTokens) return;
-  for (int i = tid; i < a.N; i += kPagesThreads) {
-    const int b = first_above(ends, kPagesThreads, i);
-    const bool inside = b < a.B && first_at[min(b, kPagesThreads - 1)] >= 0;
+  if (rounds > 1 || a.N > 4 * THREADS) return;
+  for (int i = tid; i < a.N; i += THREADS) {
+    const int b = first_above(ends, THREADS, i);
+    const bool inside = b < a.B && first_at[min(b, THREADS - 1)] >= 0;
     pages_place(a, i, b, inside ? first_at[b] + i - (b == 0 ? 0 : ends[b - 1]) : -1);
   }
 }
@@ -229,9 +232,11 @@ extern "C" int lh_hip_kv_pages(int32_t* block_table, int64_t table_stride, const
   const PagesArgs a = {block_table, table_stride, lengths, counts, new_lengths, free_pages, n_free, starts, positions, slots,
                        (int32_t)B, (int32_t)max_pages, (int32_t)n_pages, (int32_t)N, (int32_t)page_size, FastDiv((uint32_t)page_size)};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  LH_LAUNCH(kv_pages_kernel, dim3(1), dim3(kPagesThreads), 0, s, a);
+  const bool small = B <= 256 && N <= 1024;  // (fewer waves at a barrier, fewer steps of a bisection)
+  if (small) LH_LAUNCH((kv_pages_kernel<256>), dim3(1), dim3(256), 0, s, a);
+  else LH_LAUNCH((kv_pages_kernel<kPagesThreads>), dim3(1), dim3(kPagesThreads), 0, s, a);
   if (const int rc = check_launch("kv_pages")) return rc;
-  if (N == 0 || (B <= kPagesThreads && N <= kPagesTokens)) return LH_OK;
+  if (N == 0 || (B <= kPagesThreads && N <= 4 * kPagesThreads)) return LH_OK;
   LH_LAUNCH(kv_pages_tokens, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s, a);
   return check_launch("kv_pages_tokens");
 }

@@ -802,7 +802,7 @@ def kv_pages(block_table, lengths, counts, free_pages, n_free, page_size, tokens
 
     Sequence b has `lengths[b]` positions (int32 [B]) and gets `counts[b]` tokens (int32 [B]), or has ended, where that is negative: its
     length becomes 0.  block_table (int32 [B, P]) is updated: its first entries are the pages that the new length needs, those behind
-    them -1, as at the beginning.  free_pages (int32, one entry for every page of the cache) begins with the n_free (int32 [1]) pages that no sequence
+    them -1, as at the beginning; a page is one sequence's.  free_pages (int32, one entry for every page of the cache) begins with the n_free (int32 [1]) pages that no sequence
     has; both are updated.  Pages that are needed no longer go back first, in the order of sequences and positions; then missing ones are taken from
     the list's end.  A sequence whose pages, with those that the ones before it miss, are more than there are, whose length would
     pass the table or whose rows pass `tokens`, is refused: pages and length stay, its rows have no place.
@@ -961,7 +961,7 @@ def paged_attention_chunk(q, k_cache, v_cache, block_table, lengths, starts, *, 
     starts[b] .. starts[b + 1] - 1 (int32 [B + 1], from 0 up); the last one is at position lengths[b] - 1 (int32 [B]: the new tokens count, and
     have been stored), the others right before it, and each sees the positions up to its own: softmax(scale q . k_t) v_t, 0 where it sees none.
     What lies at positions that a row does not see does not matter to it.  Rows from starts[B] on stay as they were.  scale: 1 / sqrt(d) if None.
-    `workspace` (uint8, see paged_attention_chunk_workspace_bytes): temporary memory, otherwise torch's allocator is asked; two
+    `out` may be q.  `workspace` (uint8, see paged_attention_chunk_workspace_bytes): temporary memory, otherwise torch's allocator is asked; two
     calls that overlap in time need one each."""
     (N, H, d), sq = _packed_rows(q, "q")
     dtype = q.dtype

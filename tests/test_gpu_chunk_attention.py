@@ -287,6 +287,14 @@ def test_strided_queries_and_results():
     assert (store == 5).all()
 
 
+@pytest.mark.parametrize("counts", [[2000, 1, 40], [300, 1, 40], [4, 1, 2]])
+def test_the_result_may_take_the_place_of_the_queries(counts):
+    c = ref.Cache([2300, 700, 900], 2, 16, 64, bf16, seed=19)
+    q, want = run(c, counts, 8)
+    got = ops.paged_attention_chunk(q, c.k_cache, c.v_cache, c.table, c.device_lengths, starts_of(counts), out=q)
+    assert got is q and torch.equal(q, want)
+
+
 def test_starts_that_make_no_sense_stay_within_the_rows():
     c = ref.Cache([100, 33, 50], 2, 16, 64, bf16, seed=14)
     q = queries([90], 4, 64, bf16, 14)

@@ -143,6 +143,18 @@ def test_more_tokens_than_one_workgroup_places(B, T):
     p.whole()
 
 
+@pytest.mark.parametrize("B", [255, 256, 257])
+@pytest.mark.parametrize("N", [1023, 1024, 1025])
+def test_around_the_sizes_of_the_smaller_workgroup(B, N):
+    g = torch.Generator().manual_seed(B + N)
+    p = Pool(torch.randint(0, 40, (B,), generator=g).tolist(), 4, 16, 20 * B, seed=B)
+    counts = [(3, 5, -1, 0, 7)[b % 5] for b in range(B)]
+    counts[-1] += N - sum(max(c, 0) for c in counts[:-1]) - max(counts[-1], 0) if N > sum(max(c, 0) for c in counts) else 0
+    p.step(counts, N)
+    p.step([1] * B, N, in_place=False)
+    p.whole()
+
+
 def test_a_captured_step_goes_on_from_replay_to_replay():
     p = Pool([3, 16, 0, 30], 16, 6, 24, seed=3)
     counts, N = dev([1, 1, 1, 1]), 6

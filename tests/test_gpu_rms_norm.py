@@ -70,6 +70,20 @@ def test_8_bits(M, C, dtype, residual, scale):
         check(x, gamma, r, got, after, scale=float(torch.tensor(scale)))
 
 
+@pytest.mark.parametrize("C", [8192, 4099])
+@pytest.mark.parametrize("residual", [bf16, f32])
+def test_large_sums(C, residual):
+    """A sum that no cache holds, and the same rows a few at a time."""
+    M = (36 << 20) // C // (4 if residual == f32 else 2)
+    x, r, gamma = rows(M, C, bf16, 3), rows(M, C, residual, 4), torch.ones(C, device="cuda")
+    after = torch.empty_like(r)
+    out, scales = ops.rms_norm(x, gamma, residual=r, residual_out=after, out_dtype=e4m3)
+    for part in (slice(0, 9), slice(M // 2, M // 2 + 9), slice(M - 9, M)):
+        few = torch.empty_like(r[part])
+        want, each = ops.rms_norm(x[part], gamma, residual=r[part], residual_out=few, out_dtype=e4m3)
+        assert torch.equal(out[part].view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales[part], each) and torch.equal(after[part], few)
+
+
 @pytest.mark.parametrize("C", [30, 768, 3000, 9000, 20000])
 def test_strides(C):
     """Rows further apart than they are long, that begin anywhere; what lies between them stays."""

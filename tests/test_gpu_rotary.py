@@ -54,6 +54,18 @@ def test_few_and_many_tokens(N, heads):
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("heads,d,turned", [(5, 100, 72), (1, 64, 64), (3, 40, 6)])
+def test_many_tokens_are_what_few_are(interleaved, heads, d, turned):
+    """A call with as many values as have two heads a thread, and the same tokens 100 at a time."""
+    x, positions = case(60000 // heads, heads, d, f16, seed=d)
+    freqs = ops.rotary_frequencies(turned)
+    whole = ops.rotary(x, positions, freqs, interleaved=interleaved)
+    for at in range(0, x.shape[0], 1900):
+        part = slice(at, at + 100)
+        assert torch.equal(whole[part], ops.rotary(x[part], positions[part], freqs, interleaved=interleaved))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
 def test_far_positions_and_quarters_of_the_circle(interleaved):
     """Positions up to the largest number and below 0; angles right at, before and behind the borders of the eighths."""
     x = torch.randn(4096, 1, 32, generator=torch.Generator().manual_seed(1)).cuda()
