@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
   constexpr int RS = ahead(DB, ODD), STAGES = stages(DB, ODD);
   constexpr bool SHORT = ODD && DB == 2;
   constexpr bool TWO = STAGES == 2 || RS == 2;    // steps go by in pairs
+  constexpr bool MIDDLE = STAGES == 2 && RS > 0;
   static_assert(NI >= 1 && NP * 256 == KEYS * CPR, "");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   typedef typename std::conditional<F32, float, uint16_t>::type elem;
@@ -355,12 +356,13 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
       lds_barrier();
     }
     const uint64_t all_held = held[step & 7];
-    if (wave_live && wave_last >= j0) {
-      f32x16 s[NI];
+    const bool some_row = wave_live && wave_last >= j0;
+    f32x16 s[NI];
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) s[i][v] = 0.0f;
+      for (int v = 0; v < 16; ++v) s[i][v] = 0.0f;
+    if (some_row) {
       const uint8_t* q_now = q;
       int d_now = a.c.d;
       if constexpr (!Q_HELD) asm volatile("" : "+v"(q_now), "+s"(d_now));  // (read here, not held over the steps)
@@ -391,6 +393,12 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
         }
         __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
       }
+    }
+    // (While the products are made; the other stage has been read.)
+    if constexpr (MIDDLE) {
+      if (step + 1 < steps) bring(step + 1, std::integral_constant<int, TWO ? 1 - P : 0>());
+    }
+    if (some_row) {
       // s[i][v] = q . k of row r32 and position j0 + 32 i + 8 (v / 4) + 4 h + v % 4
       const bool whole = j0 + 32 * NI - 1 <= min(wave_first, k1 - 1) && row0 + 31 < rows && all_held == ~0ull;
       if (!whole) {
@@ -479,9 +487,11 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
       }
     }
     __builtin_amdgcn_sched_barrier(0);  // (what waits for memory comes behind the arithmetic)
-    if (step + 1 < steps) {
-      if constexpr (STAGES == 1) lds_barrier();
-      bring(step + 1, std::integral_constant<int, TWO ? 1 - P : 0>());
+    if constexpr (!MIDDLE) {
+      if (step + 1 < steps) {
+        if constexpr (STAGES == 1) lds_barrier();
+        bring(step + 1, std::integral_constant<int, TWO ? 1 - P : 0>());
+      }
     }
     note(step + RS + 2, queue[P % QUEUE]);
     queue[P % QUEUE] = look_up(step + RS + 2 + QUEUE);
