@@ -5,22 +5,23 @@
 //
 //  * Both products are transposed, S^T = K Q^T and O^T = V^T P^T on 32-wide matrix instructions: a lane has one row, its softmax state
 //    is a scalar per lane, and the accumulators of S^T are, rounded, the second operand of O^T.
-//  * Keys and values of a step go through registers into LDS, two steps of which are there where that costs a CU no workgroup; they are asked for
-//    up to two steps ahead, as far as registers suffice.  Where each position's row lies is looked up before that, one position a thread, so
+//  * Keys and values of a step go through registers into LDS, two steps of which are there where that costs a CU no workgroup (the next one's are
+//    put there between the two products: 2.1 % of a long step's time, 7.5 % of a short one's); they are asked for up to two steps ahead, as far as
+//    registers suffice.  Where each position's row lies is looked up before that, one position a thread, so
 //    that any page size and any strides cost the same.
 //  * 128 rows a workgroup, 32 for each of four waves, 64 positions a step, which all waves read.  (Sequences with few rows have a kernel
 //    without LDS, in chunk_attention_few.hip.)
 //  * Long caches of few tiles are cut into shares of positions; a second launch joins them.
 //
 // The arithmetic bounds it: a step of a wave has 32 matrix instructions of 32 cycles at width 128 beside about 190 vector instructions, 32 of them
-// exponentials, and the two hardly overlap (2048 tokens after 14336, f16, 32 heads of 128: matrix unit 38 % of the cycles, vector unit 37 %).
+// exponentials, and the two hardly overlap (2048 tokens after 14336, f16, 32 heads of 128: matrix unit 38 % of the cycles, vector unit 38 %).
 // So P is rounded to 16 bits once, as in attention over tensors, and the sum is that of the rounded values, so that the weights add up to 1; the
 // result's error against 64 bits is up to 1.4 times that of its own rounding.  Everything that was not needed in a step for which nothing has to be
 // masked is behind a uniform branch.
 //
-// Measured: those 2048 tokens 613 us (840 TFLOP/s of a causal step's products; 1180 is what a large f16 product reaches); 8 prompts of 1024, bf16, 12
-// heads of 64, 30.7 us (420 TFLOP/s: steps of 16 matrix instructions, half of a tile's last two are masked); 512 tokens each of two sequences of 4096
-// and 2560 positions, e4m3, 16 heads of 128, 61 us and 12 for the join.
+// Measured: those 2048 tokens 600 us (859 TFLOP/s of the products that the mask leaves; 1180 is what a large f16 product reaches); 8 prompts of 1024,
+// bf16, 12 heads of 64, 28.4 us (454 TFLOP/s: steps of 16 matrix instructions, half of a tile's last two are masked); 512 tokens each of two sequences
+// of 4096 and 2458 positions, e4m3, 16 heads of 128, 57 us and 13 for the join, which moves 34 MB.
 #include "chunk_attention.h"
 
 #ifndef LH_CHUNK_CDT
