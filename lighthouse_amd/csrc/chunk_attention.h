@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "paged.h"
+#include "wave_scan.h"
 
 namespace lh {
 
@@ -63,7 +64,9 @@ __device__ __forceinline__ int chunk_last(const ChunkArgs& a, int at, F begins) 
 }
 
 // The tile that workgroup `rank` of a head takes, heaviest first: for up to 32 sequences (`ranked`) first each one's last tile, then each one's last
-// but one, and so on, since a later tile sees more positions; otherwise the places in falling order.
+// but one, and so on, since a later tile sees more positions; for up to 4096 the tiles in falling order, found by running sums of the lanes' sequences;
+// otherwise the places in falling order.  (Those have holes, and the device deals workgroups to its CUs in turn, whether they find work or not: with every
+// second place empty half of the CUs did all of it, 64 sequences of 16 rows 105 us instead of 79.)
 __device__ __forceinline__ bool chunk_tile(const ChunkArgs& a, int rank, int* seq, int* tile) {
   if (a.ranked) {
     const int lane = threadIdx.x & 63, i = min(lane, a.B - 1);
@@ -89,6 +92,31 @@ __device__ __forceinline__ bool chunk_tile(const ChunkArgs& a, int rank, int* se
       rank -= (int)there;
       level = same;
     }
+  }
+  if (a.B <= 4096) {
+    const int lane = threadIdx.x & 63, per = (a.B + 63) >> 6;
+    auto tiles_of = [&](int rows) { return rows >= a.least && rows <= a.most ? (int)((uint32_t)(rows + a.tile_rows - 1) >> a.tile_shift) : 0; };
+    uint32_t mine = 0;
+    int from = chunk_start(a, min(lane * per, a.B));
+    for (int i = 0; i < per; ++i) {
+      const int to = chunk_start(a, min(lane * per + i + 1, a.B));
+      mine += (uint32_t)tiles_of(max(to - from, 0) * a.G);
+      from = to;
+    }
+    const uint32_t up_to = wave_scan(mine), all = wave_last(up_to);
+    if ((uint32_t)rank >= all) return false;
+    const uint32_t at = all - 1 - (uint32_t)rank;
+    const int owner = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(up_to > at));  // (the last lane's is)
+    const uint32_t left = at - (uint32_t)__builtin_amdgcn_readlane((int)(up_to - mine), owner);
+    const int b = owner * per + lane;
+    const int tiles = lane < per && b < a.B ? tiles_of(max(chunk_start(a, b + 1) - chunk_start(a, b), 0) * a.G) : 0;
+    const uint32_t up = wave_scan((uint32_t)tiles);
+    const uint64_t above = __builtin_amdgcn_ballot_w64(up > left);
+    if (above == 0) return false;
+    const int which = (int)__builtin_ctzll(above), has = __builtin_amdgcn_readlane(tiles, which);
+    *seq = owner * per + which;
+    *tile = (int)(left - (uint32_t)(__builtin_amdgcn_readlane((int)up, which) - has));
+    return *tile >= 0 && *tile < has;  // (starts that make no sense may have more tiles than an integer holds)
   }
   const int place = a.slots - 1 - rank;
   *seq = chunk_last(a, place, [&](int i) { return chunk_place(a, i); });
