@@ -113,16 +113,21 @@ static void chunk_join_launch(const ChunkArgs& a, const ChunkArgs& few, hipStrea
 
 static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
 
-// Sequences with up to 32 rows are for the kernel of the few, those with more for that of the many: two pieces of 512 among 14 tokens of 16 heads
-// take 98 us in the kernel of the many, 82 so; of 32 heads 163 and 146.  But all are for the first where they have no more than 32 rows on average,
-// and all for the second where a tile of 128 for each would add less than a quarter to the rows that there are, or where there are more tiles than
-// workgroups run at once: single tokens, bound by memory, then run beside the others (8 pieces of 512 among 56 tokens of 32 heads: 199 us, 216 in
-// two launches; 32 of 256 among 224: 261, 293).
+// Which kernel a call is for.  The few read every position once for 16 rows; the many have more to do for a tile of 128, however few rows it has.
+// Rows of a sequence up to which the few are faster, all alike (few against many, us): 16-bit types 16 (64 sequences of up to 1024, 12 heads of 64: 16
+// rows 33.3, 37.3; 17 rows 47.2, 37.4), e4m3 48 (16 of up to 4096, 4 heads of 128: 48 rows 31.7, 34.6; 64 rows 37.3, 35.0), f32 and wide rows 64
+// and more (8 of up to 2048, 4 heads of 128, f32: 34, 91; 32 of them, 4 heads of 256, bf16: 106, 136).
+//
+// Of unlike sequences, those with up to 32 rows are for the few, those with more for the many, in two launches: two pieces of 512 among 14 tokens of 16
+// heads take 98 us in the kernel of the many, 82 so; of 32 heads 163 and 146.  But all are for the many where there are fewer than 128 rows a
+// sequence, so that they may be alike (8 of 20 rows 30.5 us, 38 in two launches), where a tile of 128 for each would add less than a quarter to the
+// rows that there are, and where there are more tiles than workgroups run at once: single tokens, bound by memory, then run beside the others (8
+// pieces of 512 among 56 tokens of 32 heads: 176 us, 188 in two launches; 32 of 256 among 224: 236, 256).
 enum ChunkPart { kAllFew, kAllMany, kTheFew, kTheMany };
-static ChunkPart chunk_part(const Paged& c, int64_t N, int64_t B, int64_t H) {
+static ChunkPart chunk_part(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H) {
   const int64_t rows = N * (H / c.heads);
-  if (rows <= kChunkFew * B) return kAllFew;
-  return B == 1 || rows >= 4 * 128 * B || (rows / 128 + B) * c.heads > 2 * num_cus() ? kAllMany : kTheMany;
+  if (rows <= B * (cache_dtype == LH_F32 || c.d > 192 ? 64 : cache_dtype == LH_F8E4M3 ? 48 : 16)) return kAllFew;
+  return rows < 128 * B || rows >= 4 * 128 * B || (rows / 128 + B) * c.heads > 2 * num_cus() ? kAllMany : kTheMany;
 }
 
 // Positions of each of `splits` shares of a sequence's, which have no fewer than 256.
@@ -184,7 +189,7 @@ size_t lh_hip_paged_attention_chunk_workspace_bytes(const lh_paged_cache* cache,
   Paged c;
   if (paged_cache(cache, "lh_hip_paged_attention_chunk_workspace_bytes", &c) != LH_OK || !chunk_sizes(c, N, B, H)) return 0;
   // (Room for either alignment: a caller may size it with one cache and pass a view of another.)
-  const ChunkPart part = chunk_part(c, N, B, H);
+  const ChunkPart part = chunk_part(c, cache->dtype, N, B, H);
   size_t bytes = 0;
   for (int aligned = 0; aligned < 2; ++aligned) {
     size_t sum = chunk_plan(c, cache->dtype, N, B, H, aligned, part).total();
@@ -207,7 +212,7 @@ int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const v
   LH_REQUIRE(dtype == cache->dtype || (cache->dtype == LH_F8E4M3 && (dtype == LH_BF16 || dtype == LH_F16)),
              "%s: queries must have the cache's dtype (bf16 or f16 for a cache of e4m3)", what);
   const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
-  const ChunkPart part = chunk_part(a.c, N, B, H);
+  const ChunkPart part = chunk_part(a.c, cache->dtype, N, B, H);
   const ChunkPlan p = chunk_plan(a.c, cache->dtype, N, B, H, aligned, part);
   ChunkPlan f = {};
   if (part == kTheMany) f = chunk_plan(a.c, cache->dtype, N, B, H, aligned, kTheFew);
