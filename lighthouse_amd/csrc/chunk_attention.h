@@ -24,8 +24,8 @@ struct ChunkArgs {
   int32_t share, splits;   // positions a workgroup takes, workgroups for the positions of the table
   float scale_log2e;       // above 0
   uint32_t q_and, q_xor;   // on the queries' words: their signs change, or they become 0
-  float* part_o;           // [slots][kv heads][splits][tile_rows][width]
-  float2* part_ml;         // [slots][kv heads][splits][tile_rows]
+  float* part_o;           // [rows of the result, or as chunk_part_row says][splits][width]
+  float2* part_ml;         // [rows][splits]
   int32_t width;           // columns of a row of part_o
 };
 
@@ -41,11 +41,13 @@ struct ChunkPlan {
 
 constexpr int kChunkFew = 32;  // rows of a sequence: two tiles of the few
 
-// Places for the tiles of sequence b begin at rows / tile_rows (of the rows before it) + b: at least as many as its rows need.  Where a launch is
-// for sequences with few rows only, each has two.
+// Places for the tiles of sequence b begin at rows / tile_rows (of the rows before it) + b: at least as many as its rows need.
 __device__ __forceinline__ int chunk_start(const ChunkArgs& a, int b) { return min(max(a.starts[b], 0), a.N); }
-__device__ __forceinline__ int chunk_place(const ChunkArgs& a, int b) {
-  return a.most == kChunkFew ? 2 * b : (int)((uint32_t)(chunk_start(a, b) * a.G) >> a.tile_shift) + b;
+__device__ __forceinline__ int chunk_place(const ChunkArgs& a, int b) { return (int)((uint32_t)(chunk_start(a, b) * a.G) >> a.tile_shift) + b; }
+// Where the shares of a row's result lie: token n of the packed ones and `head`, which are `row` (of the sequence) of key / value head hk of sequence b.  By rows of the
+// result, or, where the launch is for a few of them, by sequence.
+__device__ __forceinline__ int64_t chunk_part_row(const ChunkArgs& a, int b, int hk, int row, int n, int head) {
+  return a.most == kChunkFew ? ((int64_t)b * a.c.heads + hk) * kChunkFew + row : (int64_t)n * a.H + head;
 }
 
 // The last of the B sequences for which `begins(b) <= at` (ascending), 0 if there is none, by all lanes of a wave: 64 a round.

@@ -14,8 +14,7 @@ __device__ __forceinline__ void chunk_join(const ChunkArgs& a, int n, int head, 
   const int sees = base + (min(count * a.G, (tile + 1) << a.tile_shift) - 1) / a.G + 1;
   if (sees <= a.share) return;  // (written at once)
   const int parts = (sees + a.share - 1) / a.share;
-  const int64_t place = chunk_place(a, b) + tile;
-  const int64_t at = (place * a.c.heads + hk) * a.splits * a.tile_rows + (row - tile * a.tile_rows);
+  const int64_t at = chunk_part_row(a, b, hk, row, n, head) * a.splits;
   // Four at a time, asked for together.
   float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   const int col = 4 * lane < a.width ? 4 * lane : 0;
@@ -24,7 +23,7 @@ __device__ __forceinline__ void chunk_join(const ChunkArgs& a, int n, int head, 
     f32x4 x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t part = at + (int64_t)min(p0 + i * WAVES, parts - 1) * a.tile_rows;
+      const int64_t part = at + min(p0 + i * WAVES, parts - 1);
       ml[i] = a.part_ml[part];
       x[i] = *reinterpret_cast<const f32x4*>(a.part_o + part * a.width + col);
     }
@@ -149,7 +148,7 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
   p.slots = (int)slots;
   // (A place more per sequence may be empty: the tiles that there probably are.)
   const int64_t full = N * G / p.tile_rows, some = part == kTheMany ? 1 : B < N ? B : N;
-  const int64_t items = slots * c.heads, tiles = part == kTheFew || full < some ? some : full;
+  const int64_t tiles = part == kTheFew || full < some ? some : full;
   if (p.few) {
     p.mode = paged_mode(c, es, aligned);
     p.width = paged_width(c.d);
@@ -168,8 +167,9 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
   }
   p.splits = (int)(((int64_t)c.capacity() + p.share - 1) / p.share);
   if (p.splits > 1) {
-    p.o_bytes = granules((size_t)items * p.splits * p.tile_rows * p.width * 4);
-    p.ml_bytes = granules((size_t)items * p.splits * p.tile_rows * 8);
+    const size_t rows = (size_t)(part == kTheFew ? B * c.heads * kChunkFew : N * H) * p.splits;
+    p.o_bytes = granules(rows * p.width * 4);
+    p.ml_bytes = granules(rows * 8);
   }
   return p;
 }

@@ -505,9 +505,12 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
 
   // acc[j][v] = sum of p v of row r32, column 32 j + 8 (v / 4) + 4 h + v % 4, relative to m_run
   l_run += __shfl_xor(l_run, 32);
-  if (!row_live) return;
+  int again = r32;
+  asm volatile("" : "+v"(again));  // (where the row belongs: found again and not held over the steps)
+  if (row0 + again >= rows) return;
+  const int to_row = first + row0 + again, to_token = (int)a.by_group.div((uint32_t)to_row), to_head = hk * a.G + (to_row - to_token * a.G);
   if (cut) {
-    const int64_t part = ((((int64_t)chunk_place(a, b) + tile) * a.c.heads + hk) * a.splits + split) * a.tile_rows + row0 + r32;
+    const int64_t part = chunk_part_row(a, b, hk, to_row, start + to_token, to_head) * a.splits + split;
     if (h == 0) a.part_ml[part] = make_float2(m_run, l_run);
     float* to = a.part_o + part * a.width;
 #pragma unroll
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
     return;
   }
   const float inv = l_run == 0.0f ? 0.0f : a.c.v_scale / l_run;  // (no position seen: 0)
-  uint8_t* out = static_cast<uint8_t*>(a.out) + ((start + token) * a.so_n + head * a.so_h) * QES;
+  uint8_t* out = static_cast<uint8_t*>(a.out) + ((start + to_token) * a.so_n + to_head * a.so_h) * QES;
 #pragma unroll
   for (int j = 0; j < DB; ++j)
 #pragma unroll

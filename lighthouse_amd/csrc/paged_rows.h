@@ -179,7 +179,6 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE, std::i
     const int first = tile << a.tile_shift, rows = min(a.tile_rows, count * a.G - first);
     const int base = __builtin_amdgcn_readfirstlane(min(max(a.lengths[b], 0), a.c.capacity())) - count;
     n = max(base + (int)a.by_group.div((uint32_t)(first + rows - 1)) + 1, 0);  // positions that the last row sees
-    item = (chunk_place(a, b) + tile) * a.c.heads + hk;
     q_row = l16, q_live = l16 < rows;
     const int row = first + (q_live ? l16 : 0), of_chunk = (int)a.by_group.div((uint32_t)row);
     token = start + of_chunk, head = hk * a.G + (row - of_chunk * a.G), last_seen = base + of_chunk;
@@ -537,11 +536,17 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE, std::i
     if (half > 1) __syncthreads();
   }
   if (wave != 0 || !q_live) return;
+  if constexpr (CHUNK) {  // (found again and not held over the steps)
+    int of_tile = l16;
+    asm volatile("" : "+v"(of_tile));
+    q_row = first_row + of_tile;
+    const int of_chunk = (int)a.by_group.div((uint32_t)q_row);
+    token = first_token + of_chunk, head = hk * a.G + (q_row - of_chunk * a.G);
+  }
   if (n > a.share) {
-    int of_item;
-    if constexpr (CHUNK) of_item = a.tile_rows;
-    else of_item = a.rows;
-    const int64_t part = ((int64_t)item * a.splits + split) * of_item + l16;
+    int64_t part;
+    if constexpr (CHUNK) part = chunk_part_row(a, b, hk, q_row, token, head) * a.splits + split;
+    else part = ((int64_t)item * a.splits + split) * a.rows + l16;
     if (g4 == 0) a.part_ml[part] = make_float2(m_all, l_all);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -554,12 +559,6 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE, std::i
   if constexpr (!CHUNK)
     if (a.lse != nullptr && g4 == 0) a.lse[(int64_t)b * a.H + head] = m_all + __builtin_amdgcn_logf(l_all);
   const float inv = l_all == 0.0f ? 0.0f : a.c.v_scale / l_all;  // (no position there: 0)
-  if constexpr (CHUNK) {  // (found again and not held over the steps)
-    int of_tile = l16;
-    asm volatile("" : "+v"(of_tile));
-    const int row = first_row + of_tile, of_chunk = (int)a.by_group.div((uint32_t)row);
-    token = first_token + of_chunk, head = hk * a.G + (row - of_chunk * a.G);
-  }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
