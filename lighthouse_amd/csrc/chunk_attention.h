@@ -39,7 +39,8 @@ struct ChunkPlan {
   size_t total() const { return o_bytes + ml_bytes; }
 };
 
-constexpr int kChunkFew = 32;  // rows of a sequence: two tiles of the few
+constexpr int kChunkFew = 32;     // rows of a sequence: two tiles of the few
+constexpr int kChunkSums = 4096;  // sequences whose tiles are found by running sums
 
 // Places for the tiles of sequence b begin at rows / tile_rows (of the rows before it) + b: at least as many as its rows need.
 __device__ __forceinline__ int chunk_start(const ChunkArgs& a, int b) { return min(max(a.starts[b], 0), a.N); }
@@ -95,7 +96,7 @@ __device__ __forceinline__ bool chunk_tile(const ChunkArgs& a, int rank, int* se
       level = same;
     }
   }
-  if (a.B <= 4096) {
+  if (a.B <= kChunkSums) {
     const int lane = threadIdx.x & 63, per = (a.B + 63) >> 6;
     auto tiles_of = [&](int rows) { return rows >= a.least && rows <= a.most ? (int)((uint32_t)(rows + a.tile_rows - 1) >> a.tile_shift) : 0; };
     uint32_t mine = 0;

@@ -144,10 +144,10 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
   p.few = part == kAllFew || part == kTheFew;
   p.least = part == kTheMany ? kChunkFew + 1 : 0, p.most = part == kTheFew ? kChunkFew : 0x7fffffff;
   p.tile_rows = p.few ? 16 : 128;
-  const int64_t slots = part == kTheFew ? 2 * B : N * G / p.tile_rows + B;
-  p.slots = (int)slots;
-  // (A place more per sequence may be empty: the tiles that there probably are.)
-  const int64_t full = N * G / p.tile_rows, some = part == kTheMany ? 1 : B < N ? B : N;
+  // No more sequences than tokens have a tile (but where tiles are found by place, each sequence may have an empty one), and the last tile of each
+  // may not be full: `tiles` is how many there probably are.
+  const int64_t live = B < N ? B : N, full = N * G / p.tile_rows, some = part == kTheMany ? 1 : live;
+  p.slots = (int)(part == kTheFew ? 2 * live : full + (B <= kChunkSums ? live : B));
   const int64_t tiles = part == kTheFew || full < some ? some : full;
   if (p.few) {
     p.mode = paged_mode(c, es, aligned);

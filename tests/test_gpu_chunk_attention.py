@@ -132,6 +132,18 @@ def test_only_sequences_with_few_rows_are_cut(dtype):
     check(q, c, counts, out, rows=(0, 3, 7, 255, -1))
 
 
+@pytest.mark.parametrize("B", [30, 900, 4100])
+@pytest.mark.parametrize("dtype,some", [(bf16, [1, 4, 1, 2]), (f32, [1, 4, 200, 2]), (e4m3, [1, 1, 1, 150])])
+def test_most_sequences_idle(B, dtype, some):
+    counts, lengths = [0] * B, [0] * B
+    for b, n in zip((0, 1, B // 2, B - 1), some):
+        counts[b], lengths[b] = n, n + 1100 + b % 5
+    c = ref.Cache(lengths, 2, 16, 64, dtype, seed=20)
+    q, out = run(c, counts, 8)
+    check(q, c, counts, out, rows=(0, 1, -1))
+    assert ops.paged_attention_chunk_workspace_bytes(q, c.k_cache, c.v_cache, c.table) < 16 << 20  # (256 rows, 8 shares: 1.1 MB)
+
+
 def test_a_whole_prompt_is_what_attention_gives():
     c = ref.Cache([700, 300], 4, 16, 64, f32, seed=3)
     counts = [700, 300]
