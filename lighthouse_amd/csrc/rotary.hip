@@ -53,7 +53,7 @@ __device__ __forceinline__ void cos_sin_eighth(float x, float* c, float* s) {
 // Of position * freq radians.
 __device__ __forceinline__ void cos_sin(int position, double freq, float* c, float* s) {
   const double turns = (double)position * (freq * 0.15915494309189533577);  // 1 / (2 pi)
-  const double quarters = 4.0 * __builtin_amdgcn_fract(turns), whole = __builtin_rint(quarters);
+  const double quarters = 4.0 * (turns - __builtin_rint(turns)), whole = __builtin_rint(quarters);  // -2 .. 2
   float c0, s0;
   cos_sin_eighth((float)((quarters - whole) * 0.25), &c0, &s0);
   const int n = (int)whole & 3;

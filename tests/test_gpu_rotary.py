@@ -80,6 +80,19 @@ def test_far_positions_and_quarters_of_the_circle(interleaved):
     close(ops.rotary(x, at.cuda(), eighths.cuda(), interleaved=interleaved), want, allowed, f32)
 
 
+def test_small_angles_of_either_sign():
+    """Sines of small angles, alone in their columns, are right to the type's last places: a column of 0 beside one of 1."""
+    x = torch.zeros(4, 1, 8, device="cuda")
+    x[..., :4] = 1
+    positions = torch.tensor([1, -1, 3, -70], dtype=torch.int32, device="cuda")
+    freqs = torch.tensor([1e-3, 1e-9, 1e-14, 1e-20], dtype=torch.float64, device="cuda")
+    for turn in (freqs, -freqs):
+        got = ops.rotary(x, positions, turn)[:, 0, 4:].cpu().double()
+        want = torch.sin(positions.cpu().double()[:, None] * turn.cpu())
+        # the reduced angle and its product with 2 pi are rounded, the series' last sum, and the product with the amplitude and 1
+        assert ((got - want).abs() <= 6 * 2.0**-24 * want.abs()).all()
+
+
 def test_turning_back_and_the_gradient():
     x, positions = case(50, 4, 96, f32, seed=5)
     freqs = ops.rotary_frequencies(64)
