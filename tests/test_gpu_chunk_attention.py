@@ -144,6 +144,27 @@ def test_most_sequences_idle(B, dtype, some):
     assert ops.paged_attention_chunk_workspace_bytes(q, c.k_cache, c.v_cache, c.table) < 16 << 20  # (256 rows, 8 shares: 1.1 MB)
 
 
+@pytest.mark.parametrize("d", [128, 125])
+def test_a_cache_behind_2_to_the_31_elements(d):
+    """Stored there and read from there, as few rows and as many."""
+    pages = 2**31 // (16 * 128) + 9
+    k_cache, v_cache = (torch.zeros(pages, 1, 16, 128, dtype=bf16, device="cuda")[..., :d] for _ in range(2))
+    g = torch.Generator().manual_seed(14)
+    k, v = (torch.randn(40, 1, d, generator=g).to(bf16).cuda() for _ in range(2))
+    table = torch.tensor([[pages - 1, 3, pages - 5]], dtype=torch.int32, device="cuda")
+    at = torch.arange(40, device="cuda")
+    ops.kv_store(k, v, k_cache, v_cache, table[0].long()[at // 16] * 16 + at % 16)
+    assert torch.equal(k_cache[pages - 1, 0], k[:16, 0]) and torch.equal(v_cache[pages - 5, 0, :8], v[32:, 0])
+    lengths = torch.tensor([40], dtype=torch.int32, device="cuda")
+    for n in (3, 40):
+        q = queries([n], 2, d, bf16, seed=n)
+        out = ops.paged_attention_chunk(q, k_cache, v_cache, table, lengths, starts_of([n])).cpu().double()
+        for i in range(n):
+            seen = 40 - n + i + 1
+            want, allowed = statement(q[i].cpu(), k[:seen, 0].cpu().double()[None], v[:seen, 0].cpu().double()[None], 1 / math.sqrt(d))
+            assert ((out[i] - want).abs() <= allowed).all()
+
+
 def test_a_whole_prompt_is_what_attention_gives():
     c = ref.Cache([700, 300], 4, 16, 64, f32, seed=3)
     counts = [700, 300]

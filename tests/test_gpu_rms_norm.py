@@ -84,6 +84,15 @@ def test_large_sums(C, residual):
         assert torch.equal(out[part].view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales[part], each) and torch.equal(after[part], few)
 
 
+@pytest.mark.parametrize("C", [1000, 20000])
+def test_more_than_2_to_the_31_values(C):
+    M, gamma = 2**31 // C + 100, torch.ones(C, device="cuda")
+    x = torch.zeros(M, C, dtype=bf16, device="cuda")
+    x[-50:] = rows(50, C, bf16, 5)
+    want = ops.rms_norm(x[-50:], gamma)
+    assert ops.rms_norm(x, gamma, out=x) is x and torch.equal(x[-50:], want) and (x[:-50:997] == 0).all()
+
+
 @pytest.mark.parametrize("C", [30, 768, 3000, 9000, 20000])
 def test_strides(C):
     """Rows further apart than they are long, that begin anywhere; what lies between them stays."""

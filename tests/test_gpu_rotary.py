@@ -80,6 +80,16 @@ def test_far_positions_and_quarters_of_the_circle(interleaved):
     close(ops.rotary(x, at.cuda(), eighths.cuda(), interleaved=interleaved), want, allowed, f32)
 
 
+def test_more_than_2_to_the_31_values():
+    N, heads, d = 2**31 // (128 * 64) + 100, 128, 64
+    x = torch.zeros(N, heads, d, dtype=bf16, device="cuda")
+    x[-50:] = torch.randn(50, heads, d, generator=torch.Generator().manual_seed(1)).to(bf16).cuda()
+    positions = torch.arange(N, dtype=torch.int32, device="cuda")
+    freqs = ops.rotary_frequencies(d)
+    want = ops.rotary(x[-50:], positions[-50:], freqs)
+    assert ops.rotary(x, positions, freqs, out=x) is x and torch.equal(x[-50:], want) and (x[:-50:997] == 0).all()
+
+
 def test_small_angles_of_either_sign():
     """Sines of small angles, alone in their columns, are right to the type's last places: a column of 0 beside one of 1."""
     x = torch.zeros(4, 1, 8, device="cuda")
