@@ -537,6 +537,7 @@ _PACK_SAMPLE = struct.Struct(_lib.SAMPLE_OPTS_FORMAT).pack
 _PACK_CACHE = struct.Struct(_lib.PAGED_CACHE_FORMAT).pack
 _PACK_ROTARY = struct.Struct(_lib.ROTARY_FORMAT).pack
 _F32_MAX = torch.finfo(torch.float32).max
+_LH_DTYPE = {t: lh_dtype(t) for t in (torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn)}  # (in front of launches of a few microseconds)
 
 
 def _on_current_device(*tensors) -> None:
@@ -553,7 +554,7 @@ def _on_current_device(*tensors) -> None:
 
 
 def _is_index(t, n, what: str) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 vector of {n}, got {tuple(t.shape)} {t.dtype}")
 
 
@@ -596,7 +597,7 @@ def _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale):
         if not (0.0 < k_scale <= _F32_MAX and 0.0 < v_scale <= _F32_MAX):
             raise ValueError("k_scale and v_scale must be positive numbers")
     return (_PACK_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), table, step, *sk[:3], *sv[:3], pages, rows[1], size,
-                        heads, d, lh_dtype(dtype), k_scale, v_scale), heads, d, rows[1] * size)
+                        heads, d, _LH_DTYPE[dtype], k_scale, v_scale), heads, d, rows[1] * size)
 
 
 def _cache_weights(weights, B, heads, capacity):
@@ -862,33 +863,46 @@ def rotary_frequencies(turned, *, base=10000.0, factor=1.0, context=None, low=1.
 
 def _packed_rows(t, what: str):
     """(shape, strides of token and head) of a [N, heads, d] tensor."""
-    if t.dim() != 3 or t.dtype not in _FLOATS:
-        raise ValueError(f"{what} must be a float32, bfloat16 or float16 tensor of shape [tokens, heads, d], got {tuple(t.shape)} {t.dtype}")
-    st = t.stride()
-    if t.shape[2] != 1 and st[2] != 1:
+    shape, st = t.shape, t.stride()
+    if len(shape) != 3 or t.dtype not in _FLOATS:
+        raise ValueError(f"{what} must be a float32, bfloat16 or float16 tensor of shape [tokens, heads, d], got {tuple(shape)} {t.dtype}")
+    if st[2] != 1 and shape[2] != 1:
         raise ValueError("innermost stride must be 1")
-    return t.shape, st
+    return shape, st
 
 
-def _packed_out(out, x, what: str):
-    """The result of a call on x [N, heads, d], with rows of its own."""
+def _row_stride(t, rows, cols, what: str) -> int:
+    """Stride of the rows of a [rows, cols] matrix."""
+    shape, st = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != rows or shape[1] != cols:
+        raise ValueError(f"{what} must have shape [{rows}, {cols}], got {tuple(shape)}")
+    if st[1] != 1 and cols != 1:
+        raise ValueError(f"{what}: innermost stride must be 1")
+    if st[0] < cols and rows != 1:
+        raise ValueError(f"{what}: rows overlap (stride {st[0]} < {cols} columns)")
+    return st[0]
+
+
+def _packed_out(out, x, shape, what: str):
+    """(the result of a call on x [N, heads, d], with rows of its own; its strides)."""
     if out is None:
-        return x.new_empty(x.shape)
-    if out.shape != x.shape or out.dtype != x.dtype:
+        return x.new_empty(shape), (shape[1] * shape[2], shape[2])
+    if out.shape != shape or out.dtype != x.dtype:
         raise ValueError(f"{what} must have the shape and dtype of its input")
-    (n, heads, d), st = out.shape, out.stride()
+    (n, heads, d), st = shape, out.stride()
     if d != 1 and st[2] != 1:
         raise ValueError("innermost stride must be 1")
     if n and heads and ((heads > 1 and st[1] < d) or (n > 1 and st[0] < d) or (n > 1 and heads > 1 and st[0] < (heads - 1) * st[1] + d and st[1] < (n - 1) * st[0] + d)):
         raise ValueError(f"rows of {what} overlap")
-    return out
+    return out, st
 
 
 def _turn(positions, freqs, N, d, interleaved, amplitude):
     _is_index(positions, N, "positions")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not 1 <= freqs.shape[0] <= d // 2 or (freqs.shape[0] > 1 and freqs.stride(0) != 1):
+    half = freqs.numel()
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not 1 <= half <= d // 2 or not freqs.is_contiguous():
         raise ValueError(f"freqs must be a contiguous float64 vector of 1 to {d // 2}, got {tuple(freqs.shape)} {freqs.dtype}")
-    return _PACK_ROTARY(positions.data_ptr(), freqs.data_ptr(), 2 * freqs.shape[0], 1 if interleaved else 0, amplitude)
+    return _PACK_ROTARY(positions.data_ptr(), freqs.data_ptr(), 2 * half, 1 if interleaved else 0, amplitude)
 
 
 def rotary(x, positions, freqs, *, interleaved=False, amplitude=1.0, out=None):
@@ -896,13 +910,13 @@ def rotary(x, positions, freqs, *, interleaved=False, amplitude=1.0, out=None):
     if `interleaved`, turn by positions[n] * freqs[i]: (a cos - b sin, b cos + a sin), times `amplitude`.  freqs: float64 [R / 2] (see
     rotary_frequencies), radians a position; columns from R on stay.  positions: int32 [N].  `out` may be x.
     Turning by -freqs takes it back, and takes a gradient from the result to x."""
-    (N, heads, d), sx = _packed_rows(x, "x")
+    shape, sx = _packed_rows(x, "x")
+    N, heads, d = shape
     turn = _turn(positions, freqs, N, d, interleaved, amplitude)
-    out = _packed_out(out, x, "out")
+    out, so = _packed_out(out, x, shape, "out")
     _on_current_device(x, positions, freqs, out)
     if N and heads:
-        so = out.stride()
-        _lib.check(_lib.load().lh_hip_rotary(out.data_ptr(), x.data_ptr(), so[0], so[1], sx[0], sx[1], turn, N, heads, d, lh_dtype(x.dtype),
+        _lib.check(_lib.load().lh_hip_rotary(out.data_ptr(), x.data_ptr(), so[0], so[1], sx[0], sx[1], turn, N, heads, d, _LH_DTYPE[x.dtype],
                                              _stream()), "rotary")
     return out
 
@@ -916,8 +930,10 @@ def kv_store(k, v, k_cache, v_cache, slots, *, q=None, q_out=None, positions=Non
     [pages, kv heads, page size, d] as for kv_append.  slots int64 [N]: page * page size + slot; a token whose slot lies outside the cache (-1)
     is left out, two tokens must not share one.  With `positions` and `freqs` the keys turn on their way (see rotary).  `q` [N, H, d] turns
     with them, all rows of it, into `q_out` (which may be q; otherwise made here): then the result is (q_out, k_cache, v_cache)."""
-    (N, heads, d), sk = _packed_rows(k, "k")
-    if v.shape != k.shape or v.dtype != k.dtype:
+    shape, sk = _packed_rows(k, "k")
+    N, heads, d = shape
+    dtype = k.dtype
+    if v.shape != shape or v.dtype != dtype:
         raise ValueError("k and v must have the same shape [tokens, kv heads, d] and dtype")
     sv = v.stride()
     if d != 1 and sv[2] != 1:
@@ -925,12 +941,10 @@ def kv_store(k, v, k_cache, v_cache, slots, *, q=None, q_out=None, positions=Non
     cache, cache_heads, cache_d = _paged_cache(k_cache, v_cache, None, 1, k_scale, v_scale)[:3]
     if heads != cache_heads or d != cache_d:
         raise ValueError(f"k and v have {heads} heads of {d}, the cache {cache_heads} of {cache_d}")
-    dtype = k.dtype
     if dtype != k_cache.dtype and k_cache.dtype != torch.float8_e4m3fn:
         raise ValueError("k and v must have the cache's dtype (float32, bfloat16 or float16 for a cache of float8_e4m3fn)")
-    if slots.dtype != torch.int64:
-        raise ValueError(f"slots must be int64, got {slots.dtype}")
-    _is_vector(slots, N, torch.int64, "slots")
+    if slots.dtype != torch.int64 or slots.dim() != 1 or slots.numel() != N or not slots.is_contiguous():
+        raise ValueError(f"slots must be a contiguous int64 vector of {N}, got {tuple(slots.shape)} {slots.dtype}")
     if (positions is None) != (freqs is None):
         raise ValueError("positions and freqs go together")
     turn = None if freqs is None else _turn(positions, freqs, N, d, interleaved, amplitude)
@@ -938,18 +952,18 @@ def kv_store(k, v, k_cache, v_cache, slots, *, q=None, q_out=None, positions=Non
     if q is not None:
         if turn is None:
             raise ValueError("q is passed to be turned: positions and freqs are missing")
-        (rows, H, q_d), sq = _packed_rows(q, "q")
+        q_shape, sq = _packed_rows(q, "q")
+        rows, H, q_d = q_shape
         if rows != N or q_d != d or q.dtype != dtype:
-            raise ValueError(f"q must have shape [{N}, heads, {d}] and the dtype of k, got {tuple(q.shape)} {q.dtype}")
-        q_out = _packed_out(q_out, q, "q_out")
-        so = q_out.stride()
+            raise ValueError(f"q must have shape [{N}, heads, {d}] and the dtype of k, got {tuple(q_shape)} {q.dtype}")
+        q_out, so = _packed_out(q_out, q, q_shape, "q_out")
     elif q_out is not None:
         raise ValueError("q_out needs q")
     _on_current_device(k, v, k_cache, v_cache, slots, q, q_out, positions, freqs)
     if N:
         _lib.check(_lib.load().lh_hip_kv_store(
             cache, k.data_ptr(), v.data_ptr(), sk[0], sk[1], sv[0], sv[1], slots.data_ptr(), q_out.data_ptr() if H else None,
-            q.data_ptr() if H else None, so[0], so[1], sq[0], sq[1], turn, N, H, lh_dtype(dtype), _stream()), "kv_store")
+            q.data_ptr() if H else None, so[0], so[1], sq[0], sq[1], turn, N, H, _LH_DTYPE[dtype], _stream()), "kv_store")
     return (k_cache, v_cache) if q is None else (q_out, k_cache, v_cache)
 
 
@@ -963,7 +977,8 @@ def paged_attention_chunk(q, k_cache, v_cache, block_table, lengths, starts, *, 
     What lies at positions that a row does not see does not matter to it.  Rows from starts[B] on stay as they were.  scale: 1 / sqrt(d) if None.
     `out` may be q.  `workspace` (uint8, see paged_attention_chunk_workspace_bytes): temporary memory, otherwise torch's allocator is asked; two
     calls that overlap in time need one each."""
-    (N, H, d), sq = _packed_rows(q, "q")
+    shape, sq = _packed_rows(q, "q")
+    N, H, d = shape
     dtype = q.dtype
     B = block_table.shape[0]
     cache, heads, cache_d, _ = _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale)
@@ -975,7 +990,7 @@ def paged_attention_chunk(q, k_cache, v_cache, block_table, lengths, starts, *, 
         raise ValueError("q must have the cache's dtype (bfloat16 or float16 for a cache of float8_e4m3fn)")
     _is_index(lengths, B, "lengths")
     _is_index(starts, B + 1, "starts")
-    out = _packed_out(out, q, "out")
+    out, so = _packed_out(out, q, shape, "out")
     _on_current_device(q, k_cache, v_cache, block_table, lengths, starts, out)
     if N == 0 or B == 0:
         return out
@@ -983,10 +998,9 @@ def paged_attention_chunk(q, k_cache, v_cache, block_table, lengths, starts, *, 
     need = lib.lh_hip_paged_attention_chunk_workspace_bytes(cache, N, B, H)
     if need:
         workspace = _vector_workspace(workspace, need, q)
-    so = out.stride()
     _lib.check(lib.lh_hip_paged_attention_chunk(
         cache, out.data_ptr(), q.data_ptr(), so[0], so[1], sq[0], sq[1], lengths.data_ptr(), starts.data_ptr(), N, B, H,
-        1.0 / math.sqrt(d) if scale is None else scale, lh_dtype(dtype), workspace.data_ptr() if need else None, need, _stream()),
+        1.0 / math.sqrt(d) if scale is None else scale, _LH_DTYPE[dtype], workspace.data_ptr() if need else None, need, _stream()),
         "paged_attention_chunk")
     return out
 
@@ -1004,30 +1018,34 @@ def rms_norm(x, gamma, eps=1e-5, *, residual=None, residual_out=None, out=None, 
     stays where `residual_out` (of its dtype) receives it.  out_dtype (default: that of x): float32, bfloat16, float16 or float8_e4m3fn; that one holds
     e4m3(y / scale), clamped to +-448: with `scale` given (a number: what gemm_fp8 takes as scale_a) the result is `out`; without, every row has
     the scale max |y| / 448 of its own (1 for a row of zeros) and the result is (out, row_scales), float32 [M]."""
-    if x.dim() != 2 or x.dtype not in _FLOATS or x.shape[1] < 1:
+    dtype, shape = x.dtype, x.shape
+    if len(shape) != 2 or dtype not in _FLOATS or shape[1] < 1:
         raise ValueError("rms_norm expects x of shape [M, C] in float32, bfloat16 or float16")
-    M, C = x.shape
+    M, C = shape
     _is_vector(gamma, C, torch.float32, "gamma")
     if out is None:
-        out = x.new_empty((M, C), dtype=out_dtype or x.dtype)
+        out = x.new_empty(shape) if out_dtype is None or out_dtype == dtype else x.new_empty(shape, dtype=out_dtype)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise ValueError(f"out must be {out_dtype}, got {out.dtype}")
-    if out.dtype not in _CACHE_DTYPES:
+    to = out.dtype
+    if to not in _CACHE_DTYPES:
         raise ValueError("out must be float32, bfloat16, float16 or float8_e4m3fn")
-    _is_matrix(out, M, C, "out")
-    _is_matrix(x, M, C, "x")
+    ld_out, ld_x = _row_stride(out, M, C, "out"), _row_stride(x, M, C, "x")
+    r, r_out, ld_r, ld_r_out, r_dtype = None, None, 0, 0, 0
     if residual is not None:
-        _is_matrix(residual, M, C, "residual")
-        if residual.dtype != x.dtype and residual.dtype != torch.float32:
+        ld_r = ld_r_out = _row_stride(residual, M, C, "residual")
+        if residual.dtype != dtype and residual.dtype != torch.float32:
             raise ValueError("residual must be float32 or have the dtype of x")
         if residual_out is None:
             residual_out = residual
         elif residual_out.dtype != residual.dtype:
             raise ValueError("residual_out must have the dtype of residual")
-        _is_matrix(residual_out, M, C, "residual_out")
+        else:
+            ld_r_out = _row_stride(residual_out, M, C, "residual_out")
+        r, r_out, r_dtype = residual.data_ptr(), residual_out.data_ptr(), _LH_DTYPE[residual.dtype]
     elif residual_out is not None:
         raise ValueError("residual_out needs residual")
-    coded = out.dtype == torch.float8_e4m3fn
+    coded = to == torch.float8_e4m3fn
     if scale is not None and not (coded and 0.0 < scale <= _F32_MAX):
         raise ValueError("scale belongs to a result of float8_e4m3fn, and must be a positive number")
     if coded and scale is None:
@@ -1039,14 +1057,6 @@ def rms_norm(x, gamma, eps=1e-5, *, residual=None, residual_out=None, out=None, 
     _on_current_device(x, gamma, residual, residual_out, out, row_scales)
     if M:
         _lib.check(_lib.load().lh_hip_rms_norm(
-            out.data_ptr(), x.data_ptr(), gamma.data_ptr(), residual.data_ptr() if residual is not None else None,
-            residual_out.data_ptr() if residual is not None else None, row_scales.data_ptr() if row_scales is not None else None,
-            scale or 1.0, M, C, out.stride(0), x.stride(0), residual.stride(0) if residual is not None else 0,
-            residual_out.stride(0) if residual is not None else 0, eps, lh_dtype(x.dtype),
-            lh_dtype(residual.dtype) if residual is not None else 0, lh_dtype(out.dtype), _stream()), "rms_norm")
+            out.data_ptr(), x.data_ptr(), gamma.data_ptr(), r, r_out, None if row_scales is None else row_scales.data_ptr(), scale or 1.0, M, C,
+            ld_out, ld_x, ld_r, ld_r_out, eps, _LH_DTYPE[dtype], r_dtype, _LH_DTYPE[to], _stream()), "rms_norm")
     return out if row_scales is None else (out, row_scales)
-
-
-def release_scratch() -> None:
-    """Free the library's pool of temporary buffers on the current device (waits for the device)."""
-    _lib.check(_lib.load().lh_hip_release_scratch(), "release_scratch")
