@@ -162,8 +162,14 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
     p.blocks = p.odd ? (blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8) : blocks <= 2 ? 2 : blocks <= 4 ? blocks : blocks <= 6 ? 6 : 8;
     p.width = 32 * p.blocks;
     // One share more than that would be a second round of workgroups for a few (a piece of 256 tokens after 16128 positions, 64 tiles: 6 shares
-    // 120 us, 8 104, 12 127).
-    p.share = chunk_share(c, 2 * num_cus() / (tiles * c.heads));
+    // 120 us, 8 104, 12 127; of wide rows, of which a CU holds one workgroup, after 7936 positions, 32 tiles: 8 shares 101, 16 118).  But in three
+    // shares each, tiles that leave a last round of workgroups mostly empty take a third of it, where a share is long against what its results cost (4
+    // pieces of 600 up to 8192, 300 tiles: 277 us, so 211; one of 2300 up to 16384, 568 tiles: 900, 731; 320 tiles of 64 columns up to 4096: 92, 71, up to
+    // 1024: 27, 38).
+    const int64_t at_once = (p.blocks > 4 ? 1 : 2) * (int64_t)num_cus(), workgroups = tiles * c.heads;
+    const int64_t whole = (workgroups + at_once - 1) / at_once, cut = (3 * workgroups + at_once - 1) / at_once;  // rounds, and thirds of rounds
+    const bool thirds = 2 * workgroups > at_once && whole <= 3 && 10 * cut <= 25 * whole && (int64_t)c.capacity() * p.width >= whole << 18;
+    p.share = chunk_share(c, thirds ? 3 : at_once / workgroups);
   }
   p.splits = (int)(((int64_t)c.capacity() + p.share - 1) / p.share);
   if (p.splits > 1) {

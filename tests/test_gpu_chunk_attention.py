@@ -165,6 +165,14 @@ def test_a_cache_behind_2_to_the_31_elements(d):
             assert ((out[i] - want).abs() <= allowed).all()
 
 
+@pytest.mark.parametrize("heads,counts,lengths,d", [(20, [700, 600, 500, 300], [4200, 700, 3000, 2100], 128), (9, [800, 700], [1100, 900], 256), (36, [700, 600, 800], [4100, 900, 3500], 64)])
+def test_tiles_that_nearly_fill_the_device(heads, counts, lengths, d):
+    """More tiles of 128 rows than half, or a little more than all, of the workgroups that run at once: in one share or in three."""
+    c = ref.Cache(lengths, heads, 64, d, bf16, seed=21)
+    q, out = run(c, counts, 2 * heads)
+    check(q, c, counts, out, rows=(0, 64, -1))
+
+
 def test_a_whole_prompt_is_what_attention_gives():
     c = ref.Cache([700, 300], 4, 16, 64, f32, seed=3)
     counts = [700, 300]
