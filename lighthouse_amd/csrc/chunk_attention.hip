@@ -125,6 +125,13 @@ static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
 enum ChunkPart { kAllFew, kAllMany, kTheFew, kTheMany };
 static ChunkPart chunk_part(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H) {
   const int64_t rows = N * (H / c.heads);
+  // Where there is little to do at all, tiles of 128 rows are longer chains.  Tiles of 16 rows times positions up to which the few are faster: f16 and bf16 160
+  // Ki (26 tokens up to 681, 6 heads of 256 with 3 queries: few 18, many 30; 100 up to 1000, 8 heads of 64: 11, 14; 4 of 64 up to 1000, 4 heads of 128
+  // with 2: 18, 21; 69 of 13 heads of 128 up to 1711: 23, 21), f32, whose matrix instructions take 16 times as long, 4 Mi (4 of 48 to 190, 4 heads of 128 with
+  // 3: 15, 42; 16 of 1 to 512 up to 2048, 4 heads of 64 with 4: 104, 114; 8 of 1024, 12 heads of 64: 157, 149), but for wide rows (7 of 70 to 278, 8 heads of
+  // 256 with 3: 156, 140).
+  const int64_t tiles = (rows + 15) / 16 * c.heads;
+  if (tiles * c.capacity() <= (cache_dtype == LH_F32 && c.d <= 128 ? 4 << 20 : 160 << 10)) return kAllFew;
   if (rows <= B * (cache_dtype == LH_F32 || c.d > 192 ? 64 : cache_dtype == LH_F8E4M3 ? 48 : 16)) return kAllFew;
   return rows < 128 * B || rows >= 4 * 128 * B || (rows / 128 + B) * c.heads > 2 * num_cus() ? kAllMany : kTheMany;
 }

@@ -14,6 +14,27 @@ pytestmark = pytest.mark.gpu
 bf16, f16, f32, e4m3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
 
 
+WIDE = [False]
+
+
+@pytest.fixture(autouse=True, params=[False, True], ids=["tight", "wide"])
+def wide(request):
+    """Every test with tables as wide as the sequences need, and with ones of 2^19 positions: which kernel a call is for goes by what it might have to do."""
+    WIDE[0] = request.param
+
+
+def widened(c, positions):
+    columns = positions // c.size
+    if columns > c.table.shape[1] and columns * c.table.shape[0] <= 1 << 24:
+        c.table = torch.nn.functional.pad(c.table, (0, columns - c.table.shape[1]), value=-1)
+    return c
+
+
+def cache(*args, **options):
+    c = ref.Cache(*args, **options)
+    return widened(c, 1 << 19) if WIDE[0] else c
+
+
 def starts_of(counts):
     return torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
 
@@ -61,7 +82,7 @@ SOME = (0, 1, 2, 15, 16, 31, 32, 63, 64, -1, -2)
 @pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
 @pytest.mark.parametrize("G", [1, 3])
 def test_lengths_around_every_border(dtype, d, G):
-    c = ref.Cache(RAGGED, 2, 16, d, dtype, seed=d, scales=(0.75, 1.5) if dtype == e4m3 else (1.0, 1.0))
+    c = cache(RAGGED, 2, 16, d, dtype, seed=d, scales=(0.75, 1.5) if dtype == e4m3 else (1.0, 1.0))
     q, out = run(c, COUNTS, 2 * G)
     check(q, c, COUNTS, out, rows=SOME)
 
@@ -70,7 +91,7 @@ def test_lengths_around_every_border(dtype, d, G):
 @pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
 @pytest.mark.parametrize("counts", [[0, 1, 1, 1, 1, 1, 1, 1], [0, 1, 4, 4, 3, 2, 1, 4], [0, 0, 0, 0, 0, 1, 0, 0]])
 def test_few_rows(dtype, d, counts):
-    c = ref.Cache(RAGGED, 2, 16, d, dtype, seed=d, scales=(0.75, 1.5) if dtype == e4m3 else (1.0, 1.0))
+    c = cache(RAGGED, 2, 16, d, dtype, seed=d, scales=(0.75, 1.5) if dtype == e4m3 else (1.0, 1.0))
     q, out = run(c, counts, 8)
     check(q, c, counts, out)
 
@@ -78,7 +99,7 @@ def test_few_rows(dtype, d, counts):
 @pytest.mark.parametrize("heads,G", [(1, 1), (12, 1), (3, 5), (2, 16), (1, 17), (2, 40), (1, 200)])
 def test_groups_of_heads(heads, G):
     for counts in ([9, 70], [1, 2]):
-        c = ref.Cache([70, 90], heads, 32, 64, bf16, seed=G)
+        c = cache([70, 90], heads, 32, 64, bf16, seed=G)
         q, out = run(c, counts, heads * G)
         check(q, c, counts, out, rows=SOME)
 
@@ -86,7 +107,7 @@ def test_groups_of_heads(heads, G):
 @pytest.mark.parametrize("size", [1, 7, 16, 24, 100, 1024])
 @pytest.mark.parametrize("layout", ["heads", "slots"])
 def test_page_sizes_and_layouts(size, layout):
-    c = ref.Cache([1, size, size + 1, 310], 3, size, 96, f16, seed=size, layout=layout, room=5)
+    c = cache([1, size, size + 1, 310], 3, size, 96, f16, seed=size, layout=layout, room=5)
     for counts in ([1, 1, 2, 140], [1, 1, 1, 1]):
         q, out = run(c, counts, 6)
         check(q, c, counts, out, rows=SOME)
@@ -97,17 +118,18 @@ def test_page_sizes_and_layouts(size, layout):
                                          (bf16, 8, 0), (bf16, 9, 0), (e4m3, 9, 1), (f32, 5, 0)])
 @pytest.mark.parametrize("counts", [[5, 90, 0, 129], [1, 4, 0, 3]])
 def test_odd_head_dimensions_and_row_strides(dtype, d, pad, counts):
-    c = ref.Cache([5, 130, 0, 257], 2, 16, d, dtype, seed=d, pad=pad, scales=(0.5, 2.0) if dtype == e4m3 else (1.0, 1.0))
+    c = cache([5, 130, 0, 257], 2, 16, d, dtype, seed=d, pad=pad, scales=(0.5, 2.0) if dtype == e4m3 else (1.0, 1.0))
     q, out = run(c, counts, 4)
     check(q, c, counts, out, rows=SOME)
 
 
 @pytest.mark.parametrize("dtype,d", [(bf16, 128), (f16, 64), (f32, 64), (e4m3, 128), (bf16, 256), (f16, 37)])
 @pytest.mark.parametrize("counts", [[140, 1, 0, 7], [2, 1, 0, 4], [1500, 1, 0, 60]])
-def test_long_caches_are_split_and_joined(dtype, d, counts):
-    c = ref.Cache([3000, 1, 0, 2222], 2, 64, d, dtype, seed=7)
+@pytest.mark.parametrize("positions", [3000, 20480])
+def test_long_caches_are_split_and_joined(dtype, d, counts, positions):
+    c = widened(cache([3000, 1, 0, 2222], 2, 64, d, dtype, seed=7), positions)
     q = queries(counts, 4, d, dtype, 7, size=3.0)
-    assert ops.paged_attention_chunk_workspace_bytes(q, c.k_cache, c.v_cache, c.table) > 0
+    assert positions == 3000 or ops.paged_attention_chunk_workspace_bytes(q, c.k_cache, c.v_cache, c.table) > 0
     out = ops.paged_attention_chunk(q, c.k_cache, c.v_cache, c.table, c.device_lengths, starts_of(counts))
     check(q, c, counts, out, rows=(0, 1, 63, 64, 65, 1000, -1))
 
@@ -119,7 +141,7 @@ def test_pieces_among_single_tokens(dtype, d, B):
     counts = [(1, 8, 9, 0, 300, 2, 33)[b % 7] if b < 14 else b % 2 for b in range(B)]
     counts[-1] = 140
     lengths = [n + (0, 1, 64, 250, 2700, 500)[b % 6] if b < 14 else n + b for b, n in enumerate(counts)]
-    c = ref.Cache(lengths, 2, 16, d, dtype, seed=B, scales=(0.75, 1.5) if dtype == e4m3 else (1.0, 1.0))
+    c = cache(lengths, 2, 16, d, dtype, seed=B, scales=(0.75, 1.5) if dtype == e4m3 else (1.0, 1.0))
     q, out = run(c, counts, 8, seed=B)
     check(q, c, counts, out, rows=(0, 31, 32, -1))
 
@@ -127,7 +149,7 @@ def test_pieces_among_single_tokens(dtype, d, B):
 @pytest.mark.parametrize("dtype", [bf16, f32, e4m3])
 def test_only_sequences_with_few_rows_are_cut(dtype):
     counts = [300, 2, 8, 10]
-    c = ref.Cache([300, 900, 1500, 700], 32, 16, 64, dtype, seed=18)
+    c = cache([300, 900, 1500, 700], 32, 16, 64, dtype, seed=18)
     q, out = run(c, counts, 128)
     check(q, c, counts, out, rows=(0, 3, 7, 255, -1))
 
@@ -138,7 +160,7 @@ def test_most_sequences_idle(B, dtype, some):
     counts, lengths = [0] * B, [0] * B
     for b, n in zip((0, 1, B // 2, B - 1), some):
         counts[b], lengths[b] = n, n + 1100 + b % 5
-    c = ref.Cache(lengths, 2, 16, 64, dtype, seed=20)
+    c = cache(lengths, 2, 16, 64, dtype, seed=20)
     q, out = run(c, counts, 8)
     check(q, c, counts, out, rows=(0, 1, -1))
     assert ops.paged_attention_chunk_workspace_bytes(q, c.k_cache, c.v_cache, c.table) < 16 << 20  # (256 rows, 8 shares: 1.1 MB)
@@ -168,13 +190,13 @@ def test_a_cache_behind_2_to_the_31_elements(d):
 @pytest.mark.parametrize("heads,counts,lengths,d", [(20, [700, 600, 500, 300], [4200, 700, 3000, 2100], 128), (9, [800, 700], [1100, 900], 256), (36, [700, 600, 800], [4100, 900, 3500], 64)])
 def test_tiles_that_nearly_fill_the_device(heads, counts, lengths, d):
     """More tiles of 128 rows than half, or a little more than all, of the workgroups that run at once: in one share or in three."""
-    c = ref.Cache(lengths, heads, 64, d, bf16, seed=21)
+    c = cache(lengths, heads, 64, d, bf16, seed=21)
     q, out = run(c, counts, 2 * heads)
     check(q, c, counts, out, rows=(0, 64, -1))
 
 
 def test_a_whole_prompt_is_what_attention_gives():
-    c = ref.Cache([700, 300], 4, 16, 64, f32, seed=3)
+    c = cache([700, 300], 4, 16, 64, f32, seed=3)
     counts = [700, 300]
     q, out = run(c, counts, 8)
     for b, n in enumerate(counts):
@@ -188,7 +210,7 @@ def test_a_whole_prompt_is_what_attention_gives():
 
 
 def test_chunks_give_what_the_whole_gives():
-    c = ref.Cache([517], 2, 16, 128, bf16, seed=4)
+    c = cache([517], 2, 16, 128, bf16, seed=4)
     q, whole = run(c, [517], 8)
     at = 0
     for n in (1, 100, 3, 256, 157):
@@ -200,7 +222,7 @@ def test_chunks_give_what_the_whole_gives():
 
 def test_rows_without_anything_to_see_and_rows_of_none():
     """More new tokens than the length counts: the first of them see nothing and become 0.  Rows behind the last sequence stay."""
-    c = ref.Cache([5, 0, 70], 2, 16, 64, bf16, seed=5)
+    c = cache([5, 0, 70], 2, 16, 64, bf16, seed=5)
     for counts in ([9, 4, 200], [3, 2, 4]):
         lengths = torch.tensor([5, -3, 2**30], dtype=torch.int32, device="cuda")  # (clamped to 0 and to the table)
         c.device_lengths = lengths
@@ -221,7 +243,7 @@ def test_rows_without_anything_to_see_and_rows_of_none():
 def test_pages_that_hold_nothing(dtype, G):
     """Positions on such pages are left out, wherever they lie."""
     for lengths, counts in (([200, 90], [150, 20]), ([200, 90], [2, 3])):
-        c = ref.Cache(lengths, 2, 16, 64, dtype, seed=6)
+        c = cache(lengths, 2, 16, 64, dtype, seed=6)
         q = queries(counts, 2 * G, 64, dtype, 6)
         keep = [torch.ones(n, dtype=torch.bool) for n in lengths]
         for b, page in ((0, 0), (0, 5), (0, 12), (1, 1), (1, 2)):
@@ -247,7 +269,7 @@ def test_what_a_row_does_not_see_does_not_reach_it(dtype, counts, bad):
     if dtype == e4m3:
         bad = math.nan
     lengths = [260, 45]
-    c = ref.Cache(lengths, 2, 16, 64, dtype, seed=8)
+    c = cache(lengths, 2, 16, 64, dtype, seed=8)
     q = queries(counts, 4, 64, dtype, 8)
     call = lambda: ops.paged_attention_chunk(q, c.k_cache, c.v_cache, c.table, c.device_lengths, starts_of(counts))  # noqa: E731
     clean = call()
@@ -275,7 +297,7 @@ def test_what_a_row_does_not_see_does_not_reach_it(dtype, counts, bad):
 @pytest.mark.parametrize("dtype", [bf16, f32, e4m3])
 def test_scales_of_any_sign(scale, dtype):
     for counts in ([20, 50], [1, 3]):
-        c = ref.Cache([90, 50], 2, 16, 64, dtype, seed=9, scales=(0.5, 3.0) if dtype == e4m3 else (1.0, 1.0))
+        c = cache([90, 50], 2, 16, 64, dtype, seed=9, scales=(0.5, 3.0) if dtype == e4m3 else (1.0, 1.0))
         q, out = run(c, counts, 4, scale=scale)
         check(q, c, counts, out, scale=scale, rows=SOME)
 
@@ -283,7 +305,7 @@ def test_scales_of_any_sign(scale, dtype):
 @pytest.mark.parametrize("dtype", [bf16, f16, f32])
 def test_scores_far_apart_and_long_flat_rows(dtype):
     """Maxima that grow by hundreds along the row, and rows whose many small weights add up."""
-    c = ref.Cache([1200], 1, 16, 64, dtype, seed=10)
+    c = cache([1200], 1, 16, 64, dtype, seed=10)
     grows = torch.linspace(0.0, 40.0, 1200)
     k = c.rows(c.k_cache, 0, 1200).clone()
     k[0, :, 0] = grows.to(dtype)
@@ -307,17 +329,17 @@ def test_a_table_much_wider_than_the_sequences():
 def test_many_sequences():
     lengths = [(7 * b) % 50 + 1 for b in range(300)]
     counts = [min(n, (3 * b) % 5) for b, n in enumerate(lengths)]
-    c = ref.Cache(lengths, 1, 8, 32, bf16, seed=11)
+    c = cache(lengths, 1, 8, 32, bf16, seed=11)
     q, out = run(c, counts, 2)
     check(q, c, counts, out)
-    c = ref.Cache([1] * 5000, 1, 1, 8, f32, seed=12)
+    c = cache([1] * 5000, 1, 1, 8, f32, seed=12)
     q, out = run(c, [1] * 5000, 1)
     want = c.v[:, 0, 0]  # p v / p: a rounding of each product and of the quotient
     assert ((out[:, 0].cpu() - want).abs() <= 4 * 2.0**-24 * want.abs()).all()
 
 
 def test_strided_queries_and_results():
-    c = ref.Cache([100, 33], 2, 16, 64, bf16, seed=13)
+    c = cache([100, 33], 2, 16, 64, bf16, seed=13)
     counts = [60, 5]
     qkv = queries(counts, 10, 64, bf16, 13)
     store = torch.full((65, 7, 70), 5.0, dtype=bf16, device="cuda")
@@ -330,14 +352,14 @@ def test_strided_queries_and_results():
 
 @pytest.mark.parametrize("counts", [[2000, 1, 40], [300, 1, 40], [4, 1, 2]])
 def test_the_result_may_take_the_place_of_the_queries(counts):
-    c = ref.Cache([2300, 700, 900], 2, 16, 64, bf16, seed=19)
+    c = cache([2300, 700, 900], 2, 16, 64, bf16, seed=19)
     q, want = run(c, counts, 8)
     got = ops.paged_attention_chunk(q, c.k_cache, c.v_cache, c.table, c.device_lengths, starts_of(counts), out=q)
     assert got is q and torch.equal(q, want)
 
 
 def test_starts_that_make_no_sense_stay_within_the_rows():
-    c = ref.Cache([100, 33, 50], 2, 16, 64, bf16, seed=14)
+    c = cache([100, 33, 50], 2, 16, 64, bf16, seed=14)
     q = queries([90], 4, 64, bf16, 14)
     for starts in ([5, 3, 2000, -7], [-5, 2**31 - 1, -(2**31), 90], [0, 0, 0, 0], [90, 90, 90, 90]):
         out = torch.empty_like(q)
@@ -346,7 +368,7 @@ def test_starts_that_make_no_sense_stay_within_the_rows():
 
 
 def test_results_repeat_themselves_and_graphs_have_workspaces_of_their_own():
-    cs = [ref.Cache([3000, 100], 2, 16, 128, bf16, seed=15 + i) for i in range(2)]
+    cs = [cache([3000, 100], 2, 16, 128, bf16, seed=15 + i) for i in range(2)]
     counts = [5, 3]
     qs = [queries(counts, 8, 128, bf16, 15 + i) for i in range(2)]
     starts = starts_of(counts)
@@ -378,7 +400,7 @@ def test_results_repeat_themselves_and_graphs_have_workspaces_of_their_own():
 
 
 def test_a_workspace_of_the_caller():
-    c = ref.Cache([3000], 2, 16, 64, f16, seed=17)
+    c = cache([3000], 2, 16, 64, f16, seed=17)
     q = queries([2], 4, 64, f16, 17)
     need = ops.paged_attention_chunk_workspace_bytes(q, c.k_cache, c.v_cache, c.table)
     store = torch.full((need + 256,), 77, dtype=torch.uint8, device="cuda")
