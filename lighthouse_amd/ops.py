@@ -1060,3 +1060,8 @@ def rms_norm(x, gamma, eps=1e-5, *, residual=None, residual_out=None, out=None, 
             out.data_ptr(), x.data_ptr(), gamma.data_ptr(), r, r_out, None if row_scales is None else row_scales.data_ptr(), scale or 1.0, M, C,
             ld_out, ld_x, ld_r, ld_r_out, eps, _LH_DTYPE[dtype], r_dtype, _LH_DTYPE[to], _stream()), "rms_norm")
     return out if row_scales is None else (out, row_scales)
+
+
+def release_scratch() -> None:
+    """Free the library's pool of temporary buffers on the current device (waits for the device)."""
+    _lib.check(_lib.load().lh_hip_release_scratch(), "release_scratch")
