@@ -13,15 +13,17 @@
 //    without LDS, in chunk_attention_few.hip.)
 //  * Long caches of few tiles are cut into shares of positions; a second launch joins them.
 //
-// The arithmetic bounds it: a step of a wave has 32 matrix instructions of 32 cycles at width 128 beside about 190 vector instructions, 32 of them
-// exponentials, and the two hardly overlap (2048 tokens after 14336, f16, 32 heads of 128: matrix unit 38 % of the cycles, vector unit 38 %).
-// So P is rounded to 16 bits once, as in attention over tensors, and the sum is that of the rounded values, so that the weights add up to 1; the
-// result's error against 64 bits is up to 1.4 times that of its own rounding.  Everything that was not needed in a step for which nothing has to be
-// masked is behind a uniform branch.
+// The arithmetic bounds it: a step of a wave has 48 matrix instructions of 32 cycles at width 128 beside about 330 vector instructions, 32 of them
+// exponentials, and the two hardly overlap (2048 tokens after 14336, f16, 32 heads of 128: matrix unit 45 % of the cycles, vector unit 43 %).
+// P is held in f32 and enters the second product as the sum of two 16-bit values, each nearest to what is left: off by 2^-16 of it at most in bf16,
+// 2^-18 in the mean, and by 2^-22 in f16.  One value would leave 2^-8 and make the result's error against 64 bits up to 1.4 times that of its own
+// rounding, 1.0 times with two, and the same row would differ from what the kernel for few rows makes of it (the same 2048 tokens 609 us with one,
+// 783 with two; 8 prompts of 1024, bf16, 12 heads of 64, 28.5 and 34.4).  A third of bf16 takes 964 and 40.1 us and changes neither of the
+// error's first two places.  Everything that was not needed in a step for which nothing has to be masked is behind a uniform branch.
 //
-// Measured: those 2048 tokens 600 us (859 TFLOP/s of the products that the mask leaves; 1180 is what a large f16 product reaches); 8 prompts of 1024,
-// bf16, 12 heads of 64, 28.4 us (454 TFLOP/s: steps of 16 matrix instructions, half of a tile's last two are masked); 512 tokens each of two sequences
-// of 4096 and 2458 positions, e4m3, 16 heads of 128, 57 us and 13 for the join, which moves 34 MB.
+// Measured: those 2048 tokens in f16 822 us (627 TFLOP/s of the products that the mask leaves; 1180 is what a large f16 product reaches, and half as
+// many products again are made); those prompts 34.5 us (374 TFLOP/s: steps of 24 matrix instructions, half of a tile's last two are masked); 512 tokens
+// each of two sequences of 4096 and 2458 positions, e4m3, 16 heads of 128, 68 us and 13 for the join, which moves 34 MB.
 #include "chunk_attention.h"
 
 #ifndef LH_CHUNK_CDT
@@ -37,11 +39,15 @@ constexpr int CES = CDT == LH_F8E4M3 ? 1 : F32 ? 4 : 2;  // bytes of an element 
 constexpr int QES = F32 ? 4 : 2;                         // of a query's, and in LDS
 constexpr int PE = F32 ? 4 : 8;                          // elements of a piece: 16 bytes in LDS
 constexpr int PW = PE * CES / 4;                         // its words in the cache
+// The 16-bit type of values and probabilities in the second product, of which a probability is the sum of two.  (Codes of e4m3 are exact in either
+// type; in f16 the sum has 22 places instead of 18.)
+constexpr int PDT = CDT == LH_F8E4M3 ? LH_F16 : QDT, PARTS = 2;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+template <int DT>
 __device__ __forceinline__ f32x16 mma(u32x4 x, u32x4 y, f32x16 c) {
-  if constexpr (QDT == LH_BF16)
+  if constexpr (DT == LH_BF16)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
@@ -121,25 +127,20 @@ __device__ __forceinline__ void settle_columns(uint32_t* w, int col, int d, uint
   for (int i = 0; i < W; ++i) w[i] &= keep;
 }
 
-// The sum of two values of the queries' type and of x.
-__device__ __forceinline__ float add_pair(uint32_t w, float x) {
-  if constexpr (QDT == LH_BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), bf16x2_t{(__bf16)1.0f, (__bf16)1.0f}, x, false);
-  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), f16x2_t{(_Float16)1.0f, (_Float16)1.0f}, x, false);
-}
-
-// Two e4m3 codes (the lower or upper two of a word) as two values of the queries' type: exact.
-template <bool HI>
+// Two e4m3 codes (the lower or upper two of a word) as two values of a 16-bit type: exact.
+template <int DT, bool HI>
 __device__ __forceinline__ uint32_t of_e4m3(uint32_t w) {
-  if constexpr (QDT == LH_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+  if constexpr (DT == LH_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
 }
+template <int DT>
 __device__ __forceinline__ u32x4 in_lds(const uint32_t* w) {
-  if constexpr (CDT == LH_F8E4M3) return u32x4{of_e4m3<false>(w[0]), of_e4m3<true>(w[0]), of_e4m3<false>(w[1]), of_e4m3<true>(w[1])};
+  if constexpr (CDT == LH_F8E4M3) return u32x4{of_e4m3<DT, false>(w[0]), of_e4m3<DT, true>(w[0]), of_e4m3<DT, false>(w[1]), of_e4m3<DT, true>(w[1])};
   else return u32x4{w[0], w[1], w[2], w[3]};
 }
-// Not 0 where a piece in LDS holds an infinity or a NaN: an exponent of ones carries into the sign's place.
+// Not 0 where a piece of values in LDS holds an infinity or a NaN: an exponent of ones carries into the sign's place.
 __device__ __forceinline__ uint32_t wild_bits(u32x4 w) {
-  constexpr uint32_t top = F32 ? 0x7f800000u : QDT == LH_BF16 ? 0x7f807f80u : 0x7c007c00u, one = F32 ? 0x00800000u : QDT == LH_BF16 ? 0x00800080u : 0x04000400u;
+  constexpr uint32_t top = F32 ? 0x7f800000u : PDT == LH_BF16 ? 0x7f807f80u : 0x7c007c00u, one = F32 ? 0x00800000u : PDT == LH_BF16 ? 0x00800080u : 0x04000400u;
   uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) bits |= (w[i] & top) + one;
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
     for (int v = 0; v < 16; ++v) acc[j][v] = 0.0f;
   // What p is relative to: the maximum, or, in f16, 2^12 below it, so that small probabilities keep their part in a long row (the
   // smallest number of f16 is 2^-24).  It moves only when a p would pass 2^slack.
-  constexpr float below = QDT == LH_F16 ? 12.0f : 0.0f, slack = QDT == LH_F16 ? 14.0f : 10.0f;
+  constexpr float below = PDT == LH_F16 ? 12.0f : 0.0f, slack = PDT == LH_F16 ? 14.0f : 10.0f;
   float m_run = row_live ? -INFINITY : 0.0f, l_run = 0.0f;  // (a row that is none waits for no maximum)
 
   const int steps = (k1 - k0 + KEYS - 1) / KEYS;
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
       settle_columns<CES, ODD, SHORT>(k, col, d, there);
       settle_columns<CES, ODD, SHORT>(v, col, d, there);
     }
-    const u32x4 kw = in_lds(k), vw = in_lds(v);
+    const u32x4 kw = in_lds<QDT>(k), vw = in_lds<PDT>(v);
     *reinterpret_cast<u32x4*>(Ks + key * KROW + col) = kw;
     *reinterpret_cast<u32x4*>(Ks + KEYS * KROW + key * VROW + col) = vw;
     return look ? wild_bits(vw) : 0u;
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
 #pragma unroll 1
       for (int c = tid; c < KEYS * D; c += 256) {
         elem* const x = Vs + c / D * VROW + c % D;
-        const uint32_t bits = F32 ? __builtin_bit_cast(uint32_t, (float)*x) : (uint32_t)*x, top = F32 ? 0x7f800000u : QDT == LH_BF16 ? 0x7f80u : 0x7c00u;
+        const uint32_t bits = F32 ? __builtin_bit_cast(uint32_t, (float)*x) : (uint32_t)*x, top = F32 ? 0x7f800000u : PDT == LH_BF16 ? 0x7f80u : 0x7c00u;
         if ((bits & top) == top) {
           *x = 0;
           atomicMin(&first_wild[c % D], c / D);
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
             for (int t = 0; t < 4; ++t)
               s[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(f32_of(kf[t]), f32_of(qe[t]), s[i], 0, 0, 0);
           } else {
-            s[i] = mma(kf, qe, s[i]);
+            s[i] = mma<QDT>(kf, qe, s[i]);
           }
         }
       }
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           s[i][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][v], a.scale_log2e, -off));
-          if constexpr (F32) l_run += s[i][v];
+          l_run += s[i][v];
         }
       if constexpr (F32) {
 #pragma unroll
@@ -460,11 +461,15 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
         for (int i = 0; i < NI; ++i)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            u32x4 pf;
+            u32x4 part[PARTS];  // each nearest to what the ones before leave
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              pf[e] = pack2<QDT>(s[i][8 * u + 2 * e], s[i][8 * u + 2 * e + 1]);
-              l_run = add_pair(pf[e], l_run);  // (what the values are weighted with)
+              float p0 = s[i][8 * u + 2 * e], p1 = s[i][8 * u + 2 * e + 1];
+#pragma unroll
+              for (int n = 0; n < PARTS; ++n) {
+                part[n][e] = pack2<PDT>(p0, p1);
+                p0 -= unpack_lo<PDT>(part[n][e]), p1 -= unpack_hi<PDT>(part[n][e]);
+              }
             }
 #pragma unroll
             for (int j = 0; j < DB; ++j) {
@@ -472,7 +477,8 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
               const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p0);
               const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p0 + 8 * VROW));
               const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
-              acc[j] = mma(u32x4{l2[0], l2[1], h2[0], h2[1]}, pf, acc[j]);
+#pragma unroll
+              for (int n = 0; n < PARTS; ++n) acc[j] = mma<PDT>(u32x4{l2[0], l2[1], h2[0], h2[1]}, part[n], acc[j]);
             }
           }
       }
