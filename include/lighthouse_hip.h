@@ -482,7 +482,7 @@ int lh_hip_sample(int64_t* tokens, const void* logits, const float* uniform, int
  * [n_pages] begins with the *n_free pages that no sequence has, the last of them taken first.  With size = page_size, of sequence b:
  *   counts[b] >= 0: it gets counts[b] tokens, behind its first lengths[b] (clamped to 0 .. max_pages * size) positions;
  *   counts[b] < 0: it has ended, its length becomes 0.
- * A sequence is refused if the new length passes max_pages * size or its tokens pass N.  Of the others the pages behind
+ * A sequence is refused if the new length passes max_pages * size or its tokens, if it gets any, pass N.  Of the others the pages behind
  * ceil(new length / size) go back to the end of free_pages, in the order of sequences and positions, their entries become -1.  Then,
  * sequence after sequence, missing pages are taken from the end of the list; a sequence that misses more than there are, with
  * all that the ones before it missed, is refused, too.  A refused one keeps its pages and length, and its tokens have no place.

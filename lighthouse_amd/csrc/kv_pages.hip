@@ -66,7 +66,7 @@ struct PagesSequence {
   int32_t length, held, need;
   int32_t start;  // its first token
   int64_t count;
-  bool fits;  // in the table, and its tokens among the N
+  bool fits;  // in the table, and its tokens, if it gets any, among the N
 };
 
 __device__ __forceinline__ int pages_for(const PagesArgs& a, int64_t length) {  // (0 <= length <= P size)
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(THREADS) kv_pages_kernel(PagesArgs a) {
     }
     const uint64_t end = tokens + pages_scan<THREADS / 64>((uint64_t)max(s.count, (int64_t)0), scan, round_tokens);
     const int64_t length = s.count < 0 ? 0 : s.length + s.count;
-    s.fits = b < a.B && length <= (int64_t)a.P * a.size && end <= (uint64_t)a.N;
+    s.fits = b < a.B && length <= (int64_t)a.P * a.size && (s.count <= 0 || end <= (uint64_t)a.N);
     s.need = s.fits ? pages_for(a, length) : s.held;
     s.start = (int32_t)min(end - (uint64_t)max(s.count, (int64_t)0), (uint64_t)a.N);
     ends[tid] = (int32_t)min(end, (uint64_t)a.N);
