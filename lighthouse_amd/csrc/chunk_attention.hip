@@ -1,5 +1,8 @@
 // Attention of packed chunks of new tokens over a paged cache: how a call is cut into workgroups, the join of shares of positions, the
 // entry points.  The kernel is in chunk_attention_kernel.hip.
+#include <algorithm>
+#include <utility>
+
 #include "paged_rows.h"
 
 namespace lh {
@@ -136,10 +139,14 @@ static ChunkPart chunk_part(const Paged& c, int cache_dtype, int64_t N, int64_t 
   return rows < 128 * B || rows >= 4 * 128 * B || (rows / 128 + B) * c.heads > 2 * num_cus() ? kAllMany : kTheMany;
 }
 
-// Positions of each of `splits` shares of a sequence's, which have no fewer than 256.
-static int chunk_share(const Paged& c, int64_t splits) {
-  const int64_t most = (c.capacity() + 255) / 256;
-  splits = splits < 1 ? 1 : splits > most ? most : splits;
+// A launch has fewer than 2^32 threads.
+constexpr int64_t kMostWorkgroups = (1ll << 32) / 256 - 1;
+
+// Positions of each of `splits` shares of a sequence's, which have no fewer than 256; `items` workgroups take a share each.
+static int chunk_share(const Paged& c, int64_t splits, int64_t items) {
+  const int64_t most = std::min<int64_t>((c.capacity() + 255) / 256, kMostWorkgroups / items);
+  splits = splits > most ? most : splits;
+  splits = splits < 1 ? 1 : splits;
   return (int)(((c.capacity() + splits - 1) / splits + kPagedShare - 1) / kPagedShare * kPagedShare);
 }
 
@@ -155,14 +162,14 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
   // may not be full: `tiles` is how many there probably are.
   const int64_t live = B < N ? B : N, full = N * G / p.tile_rows, some = part == kTheMany ? 1 : live;
   p.slots = (int)(part == kTheFew ? 2 * live : full + (B <= kChunkSums ? live : B));
-  const int64_t tiles = part == kTheFew || full < some ? some : full;
+  const int64_t tiles = part == kTheFew || full < some ? some : full, items = (int64_t)p.slots * c.heads;
   if (p.few) {
     p.mode = paged_mode(c, es, aligned);
     p.width = paged_width(c.d);
     // As many shares of positions as the workgroups that run at once allow for (4 drafted tokens of 8 sequences of up to 4096 positions, 64 tiles:
     // 4 shares 36.3 us, 8 34.0, 12 31.9, 16 36.9; 128 tiles: 4 53.5, 6 48.9, 8 50.8), of no fewer than 256 positions.
     const int per_cu = paged_occupancy(cache_dtype, p.width, p.mode, true);
-    p.share = chunk_share(c, (per_cu < 3 ? per_cu : 3) * (int64_t)num_cus() / (tiles * c.heads));
+    p.share = chunk_share(c, (per_cu < 3 ? per_cu : 3) * (int64_t)num_cus() / (tiles * c.heads), items);
   } else {
     p.odd = c.d % (cache_dtype == LH_F32 ? 4 : 8) != 0;
     const int blocks = (c.d + 31) / 32;
@@ -176,7 +183,7 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
     const int64_t at_once = (p.blocks > 4 ? 1 : 2) * (int64_t)num_cus(), workgroups = tiles * c.heads;
     const int64_t whole = (workgroups + at_once - 1) / at_once, cut = (3 * workgroups + at_once - 1) / at_once;  // rounds, and thirds of rounds
     const bool thirds = 2 * workgroups > at_once && whole <= 3 && 10 * cut <= 25 * whole && (int64_t)c.capacity() * p.width >= whole << 18;
-    p.share = chunk_share(c, thirds ? 3 : at_once / workgroups);
+    p.share = chunk_share(c, thirds ? 3 : at_once / workgroups, items);
   }
   p.splits = (int)(((int64_t)c.capacity() + p.share - 1) / p.share);
   if (p.splits > 1) {
@@ -229,6 +236,9 @@ int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const v
   const ChunkPlan p = chunk_plan(a.c, cache->dtype, N, B, H, aligned, part);
   ChunkPlan f = {};
   if (part == kTheMany) f = chunk_plan(a.c, cache->dtype, N, B, H, aligned, kTheFew);
+  for (const ChunkPlan* plan : {&std::as_const(p), &std::as_const(f)})
+    LH_REQUIRE((int64_t)plan->slots * a.c.heads <= kMostWorkgroups / (plan->splits > 1 ? plan->splits : 1),
+               "%s: too many rows and heads for one launch (%lld workgroups, at most 2^24 - 1)", what, (long long)plan->slots * a.c.heads);
   const size_t need = p.total() + f.total();
   LH_REQUIRE(need == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= need),
              "%s: workspace too small or not 256-byte aligned: %zu of %zu bytes", what, workspace_bytes, need);

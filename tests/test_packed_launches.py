@@ -1,0 +1,83 @@
+"""What the operators on packed tokens launch at the limits of their sizes, on any machine: launches within what a device takes (fewer than 2^32
+threads), or a refusal.  The calls run on a recorder in the place of the HIP runtime, in a process of its own."""
+
+import math
+import multiprocessing
+import random
+import struct
+
+import pytest
+
+from tests import recorded_launches as rec
+
+BF16, F32, E4M3 = rec._lib.BF16, rec._lib.F32, rec._lib.F8E4M3
+K, V, TABLE, Q, OUT, LENGTHS, STARTS, WORKSPACE = (n << 50 for n in range(1, 9))  # far apart, aligned
+
+
+@pytest.fixture(scope="module")
+def recorded(tmp_path_factory):
+    """recorded(check, *args): check(recorder, *args) in a process whose library launches nothing."""
+    so = rec.build(tmp_path_factory.mktemp("recorder"))
+    with multiprocessing.get_context("spawn").Pool(1) as pool:
+        yield lambda check, *args: pool.apply(_on_recorder, (so, check, args))
+
+
+_recorder = None
+
+
+def _on_recorder(so, check, args):
+    global _recorder
+    _recorder = _recorder or rec.Recorder(so)
+    return check(_recorder, *args)
+
+
+def _cache(heads, d, positions, size=16, dtype=BF16, pad=0, pages=64):
+    row, columns = d + pad, -(-positions // size)
+    strides = (heads * size * row, size * row, row)
+    return struct.pack(rec._lib.PAGED_CACHE_FORMAT, K, V, TABLE, columns, *strides, *strides, pages, columns, size, heads, d, dtype, 1.0, 1.0)
+
+
+def _within(launches):
+    return all(launch.grid > 0 and launch.grid * launch.block < 2**32 for launch in launches)
+
+
+def _chunk(r, cache, N, B, H, d, dtype=BF16):
+    need = r.lib.lh_hip_paged_attention_chunk_workspace_bytes(cache, N, B, H)
+    rc, launches = r.calls("lh_hip_paged_attention_chunk", cache, OUT, Q, H * d, d, H * d, d, LENGTHS, STARTS, N, B, H, 0.1, dtype, WORKSPACE if need else None,
+                           need, None)
+    return rc, launches, r.lib.lh_hip_last_error().decode()
+
+
+def _few_tokens_among_many_sequences(r):
+    for B in (2**12, 2**12 + 1, 2**16, 2**18, 2**20 - 1):
+        for N in (1, 8, 300):
+            for positions in (16, 16384, 2**20, 2**30):
+                rc, launches, said = _chunk(r, _cache(8, 128, positions), N, B, 8, 128)
+                assert rc == 0 and launches and _within(launches), (B, N, positions, said, [(x.grid, x.block) for x in launches])
+
+
+def test_few_tokens_among_many_sequences(recorded):
+    """Above 4096 sequences idle ones have workgroups, too: the shares of positions are as many as a launch has room for."""
+    recorded(_few_tokens_among_many_sequences)
+
+
+def _attention_of_any_size(r):
+    rng = random.Random(3)
+    log = lambda lo, hi: int(math.exp(rng.uniform(math.log(lo), math.log(hi))))  # noqa: E731
+    refused = 0
+    for _ in range(20000):
+        heads, G, B, N = log(1, 300), log(1, 64), log(1, 2**20), log(1, 2**29)
+        dtype, d = rng.choice([BF16, F32, E4M3]), rng.choice([64, 96, 128, 200, 256])
+        rc, launches, said = _chunk(r, _cache(heads, d, log(1, 2**24), dtype=dtype), N, B, heads * G, d, BF16 if dtype == E4M3 else dtype)
+        case = (heads, G, B, N, dtype, d, said)
+        if rc == 0:
+            assert launches and _within(launches), case
+        else:
+            refused += 1
+            sizes = N * heads * G >= 2**32 or N * G >= 2**31 - 256
+            assert "bad sizes" in said if sizes else ("too many rows" in said or "bad sizes" in said) and (N * G / 16 + B) * heads >= 2**24, case
+    assert 1000 < refused < 15000
+
+
+def test_attention_of_any_size_is_launched_or_refused(recorded):
+    recorded(_attention_of_any_size)
