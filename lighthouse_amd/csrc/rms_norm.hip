@@ -4,6 +4,8 @@
 // columns) or of a workgroup (up to 16384) between its sums, so that nothing is read twice; longer rows are read again, from the caches.
 // 8192 rows of 8192, bf16 with a residual, into e4m3 with a scale a row: 90.7 us (5.2 TB/s, what a copy reaches); 64 rows of 768: 4.5 us, a launch and
 // one round trip to memory.
+#include <algorithm>
+
 #include "elements.h"
 
 namespace lh {
@@ -218,7 +220,7 @@ __global__ void __launch_bounds__(1024) rms_norm_long(RmsArgs a) {
 }
 
 template <int XDT, int RES>
-static int launch_rms(const RmsArgs& a, hipStream_t s) {
+static int launch_rms_rows(const RmsArgs& a, hipStream_t s) {
   const int pieces = (a.C + kPiece - 1) / kPiece;
   const dim3 four((unsigned)((a.M + 3) / 4)), one((unsigned)a.M);
   if (pieces <= 64) LH_LAUNCH((rms_norm_kernel<XDT, RES, 1, 1>), four, dim3(256), 0, s, a);
@@ -229,6 +231,26 @@ static int launch_rms(const RmsArgs& a, hipStream_t s) {
   else if (pieces <= 2048) LH_LAUNCH((rms_norm_kernel<XDT, RES, 16, 2>), one, dim3(1024), 0, s, a);
   else LH_LAUNCH((rms_norm_long<XDT, RES>), one, dim3(1024), 0, s, a);
   return check_launch("rms_norm");
+}
+
+// A launch has fewer than 2^32 threads, which is 2^26 rows of a wave each, 2^24 of four: more rows are more launches.
+template <int XDT, int RES>
+static int launch_rms(const RmsArgs& all, hipStream_t s) {
+  constexpr int RDT = RES == kF32Residual ? LH_F32 : XDT;
+  const int64_t most = (1ll << 32) / (all.C <= 128 * kPiece ? 64 : all.C <= 1024 * kPiece ? 256 : 1024) - 4;
+  for (int64_t row = 0; row < all.M; row += most) {
+    RmsArgs a = all;
+    a.M = (int32_t)std::min<int64_t>(all.M - row, most);
+    a.x = static_cast<const uint8_t*>(all.x) + row * all.ld_x * elem_bytes<XDT>();
+    a.out = static_cast<uint8_t*>(all.out) + row * all.ld_out * (int64_t)dtype_size(all.out_dtype);
+    if (RES != kNoResidual) {
+      a.residual = static_cast<const uint8_t*>(all.residual) + row * all.ld_residual * elem_bytes<RDT>();
+      a.sum = static_cast<uint8_t*>(all.sum) + row * all.ld_sum * elem_bytes<RDT>();
+    }
+    if (all.scales != nullptr) a.scales = all.scales + row;
+    if (const int rc = launch_rms_rows<XDT, RES>(a, s)) return rc;
+  }
+  return LH_OK;
 }
 
 template <int XDT>

@@ -177,3 +177,19 @@ def test_captured_and_replayed():
         want = run()
         torch.cuda.synchronize()
         assert torch.equal(got[0], as_bits(want[0])) and torch.equal(got[1], want[1]) and torch.equal(got[2], after)
+
+
+@pytest.mark.parametrize("out_dtype", [bf16, f32, e4m3])
+def test_more_rows_than_a_launch_has(out_dtype):
+    """2^26 rows of a wave each are 2^32 threads: around where the second launch begins and at the end every row is what it is by itself."""
+    M = 2**26 + 9
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x, residual = (torch.randn(M, 2, device="cuda", generator=g).to(bf16) for _ in range(2))
+    gamma, after = torch.tensor([1.5, -0.25], device="cuda"), torch.empty_like(residual)
+    got = ops.rms_norm(x, gamma, residual=residual, residual_out=after, out_dtype=out_dtype)
+    for some in (slice(0, 64), slice(2**26 - 64, 2**26 + 9)):
+        part_after = torch.empty_like(residual[some])
+        part = ops.rms_norm(x[some], gamma, residual=residual[some], residual_out=part_after, out_dtype=out_dtype)
+        assert torch.equal(after[some], part_after)
+        for whole, piece in zip(got, part) if out_dtype == e4m3 else [(got, part)]:
+            assert torch.equal(as_bits(whole[some]), as_bits(piece))

@@ -81,3 +81,38 @@ def _attention_of_any_size(r):
 
 def test_attention_of_any_size_is_launched_or_refused(recorded):
     recorded(_attention_of_any_size)
+
+
+def _norms_of_any_size(r):
+    """Rows of up to 512 and 1024 columns are four a workgroup, others one."""
+    for C in (1, 512, 513, 1024, 1025, 2048, 2049, 4096, 8192, 8193, 16384, 16385, 2**29):
+        for M in (1, 5, 2**22 - 5, 2**22, 2**24 - 1, 2**24 + 3, 2**26 - 1, 2**26, 2**26 + 1, 2**31 - 1):
+            for x_dtype, residual, out_dtype, scales in ((BF16, None, BF16, None), (F32, Q, F32, None), (BF16, Q, E4M3, STARTS)):
+                rc, launches = r.calls("lh_hip_rms_norm", OUT, K, V, residual, residual, scales, 1.0, M, C, C, C, C, C, 1e-5, x_dtype, x_dtype, out_dtype, None)
+                case = (C, M, x_dtype, out_dtype, r.lib.lh_hip_last_error(), [(x.grid, x.block) for x in launches])
+                assert rc == 0 and _within(launches), case
+                rows = 4 if C <= 1024 else 1
+                assert sum(x.grid for x in launches) == -(-M // rows) and len(launches) == 1 + (M - 1) // (2**32 * rows // launches[0].block - 4), case
+
+
+def test_norms_of_any_size(recorded):
+    recorded(_norms_of_any_size)
+
+
+def _turns_and_pages_of_any_size(r):
+    rng = random.Random(4)
+    log = lambda lo, hi: int(math.exp(rng.uniform(math.log(lo), math.log(hi))))  # noqa: E731
+    turn = struct.pack(rec._lib.ROTARY_FORMAT, LENGTHS, STARTS, 2, 0, 1.0)
+    for _ in range(5000):
+        N, H, d = log(1, 2**31 - 1), log(1, 2**20 - 1), rng.randint(2, 256)
+        rc, launches = r.calls("lh_hip_rotary", OUT, Q, H * d, d, H * d, d, turn, N, H, d, BF16, None)
+        assert (rc == 0 and launches and _within(launches)) or N * H * (d + 30) >= 2**34, (N, H, d)
+        rc, launches = r.calls("lh_hip_kv_store", _cache(8, d, 16), Q, Q, 8 * d, d, 8 * d, d, LENGTHS, OUT, Q, H * d, d, H * d, d, turn, N, H, BF16, None)
+        assert (rc == 0 and launches and _within(launches)) or N * (H + 16) * (d + 30) >= 2**34, (N, H, d)
+        B, N = log(1, 2**20 - 1), log(1, 2**30 - 1)
+        rc, launches = r.calls("lh_hip_kv_pages", TABLE, 4, LENGTHS, LENGTHS, LENGTHS, K, V, STARTS, OUT, Q, B, 4, 1000, 16, N, None)
+        assert rc == 0 and launches and _within(launches), (B, N)
+
+
+def test_turns_and_pages_of_any_size(recorded):
+    recorded(_turns_and_pages_of_any_size)
