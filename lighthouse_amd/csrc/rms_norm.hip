@@ -115,8 +115,12 @@ __device__ __forceinline__ void rms_store(const RmsArgs& a, int64_t row, int col
   }
 }
 
-// The scale of a row whose largest |y| has the bits m: 448 stands for it; 1 for a row of zeros.
-__device__ __forceinline__ float rms_row_scale(uint32_t m) { return m == 0 ? 1.0f : __builtin_bit_cast(float, m) / 448.0f; }
+// The scale of a row whose largest |y| has the bits m: 448 stands for it; 1 for a row of zeros.  No less than the smallest number, which a
+// quotient below half of it would make a 0, and zeros of the row 0 / 0.
+__device__ __forceinline__ float rms_row_scale(uint32_t m) {
+  const float scale = __builtin_bit_cast(float, m) / 448.0f;
+  return m == 0 ? 1.0f : scale == 0.0f ? 0x1p-149f : scale;
+}
 
 // WAVES of a row, VPT pieces a thread; a workgroup of one-wave rows has four.
 template <int XDT, int RES, int WAVES, int VPT>

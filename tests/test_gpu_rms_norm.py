@@ -193,3 +193,18 @@ def test_more_rows_than_a_launch_has(out_dtype):
         assert torch.equal(after[some], part_after)
         for whole, piece in zip(got, part) if out_dtype == e4m3 else [(got, part)]:
             assert torch.equal(as_bits(whole[some]), as_bits(piece))
+
+
+@pytest.mark.parametrize("C", [16, 2000, 20000])
+def test_rows_whose_scale_would_be_no_number(C):
+    """Results of a few times 2^-149, the smallest number: it is the row's scale, and their codes are those whole numbers; zeros stay zeros."""
+    x = torch.zeros(3, C, device="cuda")
+    x[0, ::2], x[0, 1], x[2, 3] = 1.0, -1.0, 4.0
+    gamma = torch.full((C,), 2.0**-147, device="cuda")
+    out, scales = ops.rms_norm(x, gamma, out_dtype=e4m3)
+    whole = ops.rms_norm(x, gamma).cpu().double() / 2.0**-149
+    assert (whole[0].abs() <= 8).all() and whole[0].abs().max() >= 1 and (whole[1] == 0).all()
+    assert scales[:2].tolist() == [2.0**-149, 1.0]
+    assert torch.equal(out[:2].cpu().double(), whole[:2])
+    top = float(whole[2].abs().max())  # (4 sqrt(C): above 224 the quotient by 448 is a number again)
+    assert float(scales[2].double()) / 2.0**-149 == max(1.0, round(top / 448)) and torch.isfinite(out.float()).all()
