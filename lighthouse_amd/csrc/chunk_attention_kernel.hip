@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
             s[i][v] = f32_of((bits_of(s[i][v]) & keep) | (0xff800000u & ~keep));
           }
       }
-      // The maximum is followed with a delay: nothing moves until a p would pass 2^10, which is as accurate as one of 1, and then for all lanes.
+      // The maximum is followed with a delay: nothing moves until a p would pass 2^10, which is as accurate as one of 1.  (Row by row, so that what
+      // others see does not reach a row's roundings.)
       float mx = s[0][0];
 #pragma unroll
       for (int i = 0; i < NI; ++i)
@@ -426,7 +427,7 @@ __global__ void __launch_bounds__(256, occupancy(DB, ODD)) chunk_attention_kerne
       mx *= a.scale_log2e;
       if (__any(mx > m_run + slack)) {
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float m_new = fmaxf(m_run, mx - below);
+        const float m_new = mx > m_run + slack ? mx - below : m_run;
         const float safe = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = __builtin_amdgcn_exp2f(m_run - safe);
         l_run *= alpha;

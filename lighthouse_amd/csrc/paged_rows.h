@@ -407,10 +407,12 @@ __global__ void __launch_bounds__(NW * 64, paged_occupancy(CDT, DP, MODE, std::i
     // What p is relative to follows the true maximum with a delay: nothing is done until a p would be above 2^10 (which is as
     // accurate as one of 1), or 2^14 in f16, and then by all lanes together.  In f16 it lies 2^12 below the maximum: thousands of positions
     // with 2^-25 of the largest weight, which f16 has no numbers for, have their part in a long row.
-    if (__any(mx > m_run + (QDT == LH_F16 ? 14.0f : 10.0f))) {
+    constexpr float slack = QDT == LH_F16 ? 14.0f : 10.0f;
+    if (__any(mx > m_run + slack)) {
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float m_new = fmaxf(m_run, QDT == LH_F16 ? mx - 12.0f : mx);
+      float m_new = fmaxf(m_run, QDT == LH_F16 ? mx - 12.0f : mx);
+      if constexpr (CHUNK) m_new = mx > m_run + slack ? m_new : m_run;  // (what other rows see does not reach a row's roundings)
       const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
