@@ -532,7 +532,8 @@ int lh_hip_kv_store(const lh_paged_cache* cache, const void* k, const void* v, i
  * it (and, in f16, 2^-37 of the largest).  An infinite value makes an infinity or a NaN of the rows that see it.  out may be q.  dtype (of q and
  * out) is the cache's, or BF16 or F16 for a cache of e4m3.  B < 2^20, N < 2^30, N H < 2^32, N H / n_kv_heads < 2^31 - 256, and fewer workgroups
  * than a launch may have: (N H / n_kv_heads / 16 + B) n_kv_heads < 2^24, or / 128 where sequences have many rows.
- * `workspace` as for lh_hip_paged_attention, of lh_hip_paged_attention_chunk_workspace_bytes(...), which goes by sizes and types.
+ * `workspace` as for lh_hip_paged_attention, of lh_hip_paged_attention_chunk_workspace_bytes(...), which goes by sizes and types, not by strides.
+ * Fewer rows or sequences may take more of it (their positions are cut into more shares): one for several calls is the largest of theirs.
  */
 size_t lh_hip_paged_attention_chunk_workspace_bytes(const lh_paged_cache* cache, int64_t N, int64_t B, int64_t H);
 int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const void* q, int64_t out_stride_n, int64_t out_stride_h,

@@ -150,11 +150,10 @@ static int chunk_share(const Paged& c, int64_t splits, int64_t items) {
   return (int)(((c.capacity() + splits - 1) / splits + kPagedShare - 1) / kPagedShare * kPagedShare);
 }
 
-// `aligned`: keys and values begin at multiples of 16 bytes.
-static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H, bool aligned, ChunkPart part) {
+// `mode`: how the kernel of the few loads rows.
+static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H, PagedMode mode, ChunkPart part) {
   ChunkPlan p = {};
   const int64_t G = H / c.heads;
-  const int es = (int)dtype_size(cache_dtype);
   p.few = part == kAllFew || part == kTheFew;
   p.least = part == kTheMany ? kChunkFew + 1 : 0, p.most = part == kTheFew ? kChunkFew : 0x7fffffff;
   p.tile_rows = p.few ? 16 : 128;
@@ -164,7 +163,7 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
   p.slots = (int)(part == kTheFew ? 2 * live : full + (B <= kChunkSums ? live : B));
   const int64_t tiles = part == kTheFew || full < some ? some : full, items = (int64_t)p.slots * c.heads;
   if (p.few) {
-    p.mode = paged_mode(c, es, aligned);
+    p.mode = mode;
     p.width = paged_width(c.d);
     // As many shares of positions as the workgroups that run at once allow for (4 drafted tokens of 8 sequences of up to 4096 positions, 64 tiles:
     // 4 shares 36.3 us, 8 34.0, 12 31.9, 16 36.9; 128 tiles: 4 53.5, 6 48.9, 8 50.8), of no fewer than 256 positions.
@@ -208,12 +207,12 @@ extern "C" {
 size_t lh_hip_paged_attention_chunk_workspace_bytes(const lh_paged_cache* cache, int64_t N, int64_t B, int64_t H) {
   Paged c;
   if (paged_cache(cache, "lh_hip_paged_attention_chunk_workspace_bytes", &c) != LH_OK || !chunk_sizes(c, N, B, H)) return 0;
-  // (Room for either alignment: a caller may size it with one cache and pass a view of another.)
+  // (Room for every way to load rows: a caller may size it with one cache and pass a view of another, of other strides or alignment.)
   const ChunkPart part = chunk_part(c, cache->dtype, N, B, H);
   size_t bytes = 0;
-  for (int aligned = 0; aligned < 2; ++aligned) {
-    size_t sum = chunk_plan(c, cache->dtype, N, B, H, aligned, part).total();
-    if (part == kTheMany) sum += chunk_plan(c, cache->dtype, N, B, H, aligned, kTheFew).total();
+  for (PagedMode mode : {kTiles, kWholeRows, kOddRows}) {
+    size_t sum = chunk_plan(c, cache->dtype, N, B, H, mode, part).total();
+    if (part == kTheMany) sum += chunk_plan(c, cache->dtype, N, B, H, mode, kTheFew).total();
     bytes = sum > bytes ? sum : bytes;
   }
   return bytes;
@@ -231,11 +230,11 @@ int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const v
   LH_REQUIRE(out && q && lengths && starts, "%s: null pointer", what);
   LH_REQUIRE(dtype == cache->dtype || (cache->dtype == LH_F8E4M3 && (dtype == LH_BF16 || dtype == LH_F16)),
              "%s: queries must have the cache's dtype (bf16 or f16 for a cache of e4m3)", what);
-  const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
+  const PagedMode mode = (PagedMode)paged_mode(a.c, (int)dtype_size(cache->dtype), aligned16(a.c.k) && aligned16(a.c.v));
   const ChunkPart part = chunk_part(a.c, cache->dtype, N, B, H);
-  const ChunkPlan p = chunk_plan(a.c, cache->dtype, N, B, H, aligned, part);
+  const ChunkPlan p = chunk_plan(a.c, cache->dtype, N, B, H, mode, part);
   ChunkPlan f = {};
-  if (part == kTheMany) f = chunk_plan(a.c, cache->dtype, N, B, H, aligned, kTheFew);
+  if (part == kTheMany) f = chunk_plan(a.c, cache->dtype, N, B, H, mode, kTheFew);
   for (const ChunkPlan* plan : {&std::as_const(p), &std::as_const(f)})
     LH_REQUIRE((int64_t)plan->slots * a.c.heads <= kMostWorkgroups / (plan->splits > 1 ? plan->splits : 1),
                "%s: too many rows and heads for one launch (%lld workgroups, at most 2^24 - 1)", what, (long long)plan->slots * a.c.heads);

@@ -1006,7 +1006,8 @@ def paged_attention_chunk(q, k_cache, v_cache, block_table, lengths, starts, *, 
 
 
 def paged_attention_chunk_workspace_bytes(q, k_cache, v_cache, block_table) -> int:
-    """Bytes of temporary memory that paged_attention_chunk takes for these tensors (only their shapes and types matter)."""
+    """Bytes of temporary memory that paged_attention_chunk takes for these tensors (only their shapes and types matter).  Fewer tokens or sequences
+    may take more: a workspace for several calls is the largest of theirs."""
     cache = _paged_cache(k_cache, v_cache, block_table, block_table.shape[0], 1.0, 1.0)[0]
     return int(_lib.load().lh_hip_paged_attention_chunk_workspace_bytes(cache, q.shape[0], block_table.shape[0], q.shape[1]))
 

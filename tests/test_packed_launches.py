@@ -83,6 +83,29 @@ def test_attention_of_any_size_is_launched_or_refused(recorded):
     recorded(_attention_of_any_size)
 
 
+def _one_workspace_for_caches_of_any_strides(r):
+    """Sized with rows that are padded and pages of any size, for calls on contiguous ones, and the other way round."""
+    rng = random.Random(6)
+    log = lambda lo, hi: int(math.exp(rng.uniform(math.log(lo), math.log(hi))))  # noqa: E731
+    for _ in range(10000):
+        heads, G, B, N = log(1, 32), log(1, 16), log(1, 200), log(1, 4096)
+        dtype, d = rng.choice([BF16, F32, E4M3]), rng.choice([64, 96, 128, 200, 256, 100, 37])
+        size = rng.choice([16, 48, 128])
+        positions = size * log(1, 2**17 // size)
+        caches = [_cache(heads, d, positions, size=size, dtype=dtype, pad=pad) for pad in (0, 1, 8)]
+        needs = {r.lib.lh_hip_paged_attention_chunk_workspace_bytes(cache, N, B, heads * G) for cache in caches}
+        assert len(needs) == 1, (heads, G, B, N, dtype, d, size, positions, needs)
+        need = needs.pop()
+        for cache in caches:
+            rc, _ = r.calls("lh_hip_paged_attention_chunk", cache, OUT, Q, heads * G * d, d, heads * G * d, d, LENGTHS, STARTS, N, B, heads * G, 0.1,
+                            BF16 if dtype == E4M3 else dtype, WORKSPACE if need else None, need, None)
+            assert rc == 0, (heads, G, B, N, dtype, d, size, positions, need, r.lib.lh_hip_last_error())
+
+
+def test_one_workspace_for_caches_of_any_strides(recorded):
+    recorded(_one_workspace_for_caches_of_any_strides)
+
+
 def _norms_of_any_size(r):
     """Rows of up to 512 and 1024 columns are four a workgroup, others one."""
     for C in (1, 512, 513, 1024, 1025, 2048, 2049, 4096, 8192, 8193, 16384, 16385, 2**29):
