@@ -514,7 +514,8 @@ int lh_hip_rotary(void* out, const void* x, int64_t out_stride_n, int64_t out_st
 /*
  * Keys and values of packed tokens into their slots: k, v [N, n_kv_heads, d] (element strides of token and head) in the cache's dtype,
  * or F32, BF16 or F16 for a cache of e4m3, which holds e4m3(clamp(x / scale, +-448)), rounded to nearest even.  slots[n] = page * page_size + slot;
- * a token with a slot outside 0 .. n_pages * page_size - 1 is dropped; two for one slot leave either.  The cache's table is not read.
+ * a token with a slot outside 0 .. n_pages * page_size - 1 is dropped; two for one slot leave either.  The cache's table is not read (block_table
+ * may be NULL, table_stride and max_pages 0).
  * With `turn` the keys turn on their way (one rounding), and so do q [N, H, d] to q_out (which may be q), in the dtype of k, of every row, where H > 0.
  */
 int lh_hip_kv_store(const lh_paged_cache* cache, const void* k, const void* v, int64_t k_stride_n, int64_t k_stride_h, int64_t v_stride_n,

@@ -7,18 +7,18 @@
 
 namespace lh {
 
-int paged_cache(const lh_paged_cache* c, const char* what, Paged* out) {
+int paged_cache(const lh_paged_cache* c, const char* what, Paged* out, bool reads_table) {
   LH_REQUIRE(c != nullptr, "%s: cache is null", what);
-  LH_REQUIRE(c->k && c->v && c->block_table, "%s: null pointer in the cache", what);
+  LH_REQUIRE(c->k && c->v && (c->block_table || !reads_table), "%s: null pointer in the cache", what);
   LH_REQUIRE(c->dtype == LH_F32 || c->dtype == LH_BF16 || c->dtype == LH_F16 || c->dtype == LH_F8E4M3,
              "%s: unsupported cache dtype %d", what, c->dtype);
   LH_REQUIRE(c->n_pages > 0 && c->n_pages < (1ll << 31) && c->page_size > 0 && c->page_size < (1ll << 31) &&
-                 c->max_pages > 0 && c->max_pages < (1ll << 31) && c->max_pages * c->page_size < (1ll << 31) - 65536,
+                 (!reads_table || (c->max_pages > 0 && c->max_pages < (1ll << 31) && c->max_pages * c->page_size < (1ll << 31) - 65536)),
              "%s: bad page counts (%lld pages of %lld, table of %lld)", what, (long long)c->n_pages,
              (long long)c->page_size, (long long)c->max_pages);
   LH_REQUIRE(c->n_kv_heads > 0 && c->n_kv_heads < 65536 && c->d >= 1 && c->d <= 256, "%s: bad head count %lld or head dimension %lld (1 to 256)",
              what, (long long)c->n_kv_heads, (long long)c->d);
-  LH_REQUIRE(c->table_stride >= c->max_pages, "%s: rows of the block table overlap", what);
+  LH_REQUIRE(!reads_table || c->table_stride >= c->max_pages, "%s: rows of the block table overlap", what);
   for (const lh_strides3* s : {&c->sk, &c->sv})
     LH_REQUIRE((c->page_size == 1 || s->t >= c->d) && (c->n_kv_heads == 1 || s->h >= c->d) && (c->n_pages == 1 || s->z >= c->d),
                "%s: rows of the cache overlap", what);

@@ -45,7 +45,7 @@ struct Paged {
   __host__ __device__ int capacity() const { return max_pages * size; }
 };
 
-// Checks what every entry point asks of a cache and fills `out`.
-int paged_cache(const lh_paged_cache* c, const char* what, Paged* out);
+// Checks what every entry point asks of a cache (of its table only if that is read) and fills `out`.
+int paged_cache(const lh_paged_cache* c, const char* what, Paged* out, bool reads_table = true);
 
 }  // namespace lh

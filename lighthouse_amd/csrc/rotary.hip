@@ -241,7 +241,7 @@ int lh_hip_kv_store(const lh_paged_cache* cache, const void* k, const void* v, i
                     int64_t q_stride_n, int64_t q_stride_h, const lh_rotary* turn, int64_t N, int64_t H, int32_t dtype, void* stream) {
   const char* what = "lh_hip_kv_store";
   Paged c;
-  if (const int rc = paged_cache(cache, what, &c)) return rc;
+  if (const int rc = paged_cache(cache, what, &c, false)) return rc;
   RotaryArgs a = {};
   LH_REQUIRE(N >= 0 && N < (1ll << 31) && H >= 0 && H < (1ll << 20), "%s: bad sizes", what);
   LH_REQUIRE(dtype == cache->dtype || (cache->dtype == LH_F8E4M3 && (dtype == LH_F32 || dtype == LH_BF16 || dtype == LH_F16)),

@@ -576,7 +576,7 @@ def _paged_cache(k_cache, v_cache, block_table, B, k_scale, v_scale):
         if (st[0] < d and pages > 1) or (st[1] < d and heads > 1) or (st[2] < d and size > 1):
             raise ValueError("k_cache and v_cache: rows overlap")
     if block_table is None:  # (for calls that name slots, which read none)
-        rows, step, table = (B, 1), 1, k_cache.data_ptr()
+        rows, step, table = (B, 0), 0, 0
     else:
         table = block_table.data_ptr()
         rows = block_table.shape

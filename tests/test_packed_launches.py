@@ -139,3 +139,16 @@ def _turns_and_pages_of_any_size(r):
 
 def test_turns_and_pages_of_any_size(recorded):
     recorded(_turns_and_pages_of_any_size)
+
+
+def _stores_without_a_table(r):
+    for table, stride, columns in ((0, 0, 0), (0, 0, 2**31), (TABLE, 1, 4)):
+        cache = struct.pack(rec._lib.PAGED_CACHE_FORMAT, K, V, table, stride, *(2048, 1024, 64), *(2048, 1024, 64), 9, columns, 16, 2, 64, BF16, 1.0, 1.0)
+        rc, launches = r.calls("lh_hip_kv_store", cache, Q, Q, 128, 64, 128, 64, LENGTHS, None, None, 0, 0, 0, 0, None, 5, 0, BF16, None)
+        assert rc == 0 and len(launches) == 1, (table, columns, r.lib.lh_hip_last_error())
+        if not table:  # (what reads one still asks for it)
+            assert r.calls("lh_hip_paged_attention_chunk", cache, OUT, Q, 128, 64, 128, 64, LENGTHS, STARTS, 5, 1, 2, 0.1, BF16, None, 0, None)[0] != 0
+
+
+def test_stores_read_no_table(recorded):
+    recorded(_stores_without_a_table)
