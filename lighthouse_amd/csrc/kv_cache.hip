@@ -1,7 +1,6 @@
 // Filling a paged key / value cache and dropping from it the positions that got least attention.  Both move bytes: what
 // bounds them is memory, or, for a step of one token per sequence, the launch.
-#include <cstring>
-
+#include "elements.h"
 #include "paged.h"
 #include "wave_scan.h"
 
@@ -50,35 +49,6 @@ struct AppendArgs {
   FastDiv by_chunks;
   float k_inv, v_inv;     // 1 / scale, rounded, or 0 where the short division does not apply
 };
-
-// Two floats, no larger than 448, -> two e4m3 codes in the low half of a word, rounded to nearest even; a NaN stays one.
-__device__ __forceinline__ uint32_t e4m3_pack2(float a, float b) { return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu; }
-// (Comparisons keep a NaN, fmin and fmax would not.)
-__device__ __forceinline__ float e4m3_clamp(float x) {
-  x = x > 448.0f ? 448.0f : x;
-  return x < -448.0f ? -448.0f : x;
-}
-// Eight numbers x -> x / scale, clamped to +-448: the quotient that a division rounds, so that the codes are those of the formula and
-// not of a rounded reciprocal.  With inv = 1 / scale rounded, q = x inv and r = q scale - x (exact), q - r inv is that quotient
-// (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990), but for a
-// scale whose mantissa is all ones, and where x or r leaves the normal range: the host passes inv = 0 for scales
-// that are not between 2^-60 and 2^60, whose quotients that are not 0 in e4m3 are far from it, and numbers that are not finite
-// or far above 448 take the division.  (3 instructions instead of 11: 8 prompts of 1024 tokens, 12 heads of 64, 15.9 -> 11.4 us.)
-__device__ __forceinline__ void e4m3_divide(float* x, float scale, float inv) {
-  float size = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) size += fabsf(x[e]);
-  if (inv != 0.0f && size <= 4096.0f * scale) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float q = x[e] * inv, r = __builtin_fmaf(q, scale, -x[e]);
-      x[e] = __builtin_amdgcn_fmed3f(__builtin_fmaf(-r, inv, q), -448.0f, 448.0f);
-    }
-  } else {
-#pragma unroll 1
-    for (int e = 0; e < 8; ++e) x[e] = e4m3_clamp(x[e] / scale);
-  }
-}
 
 // A thread takes one chunk (16 bytes of the source; 8 elements for a cache of 8 bits) of one head's key or value, of several
 // tokens of a sequence one after the other, four at a time; a token's chunks are neighbours, so that both sides are read and
@@ -138,10 +108,10 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
               else x[4 * l + e] = bits_to_f32(w[u][l][e]);
             }
           typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
-          e4m3_divide(x, scale, inv);
+          e4m3_quotients(x, scale, inv);
           u32x2_any o;
 #pragma unroll
-          for (int p = 0; p < 2; ++p) o[p] = e4m3_pack2(x[4 * p], x[4 * p + 1]) | e4m3_pack2(x[4 * p + 2], x[4 * p + 3]) << 16;
+          for (int p = 0; p < 2; ++p) o[p] = e4m3_codes(x[4 * p], x[4 * p + 1]) | e4m3_codes(x[4 * p + 2], x[4 * p + 3]) << 16;
           *reinterpret_cast<u32x2_any*>(to) = o;
         }
       }
@@ -152,7 +122,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
         const uint8_t* from = src + (int64_t)(t1 + u) * ss.t * SES;
         uint8_t* to = dst + (page[u] * cs.z + slot[u] * cs.t) * CES;
         for (int e = 0; e < n; ++e) {
-          if constexpr (CDT == LH_F8E4M3) to[e] = (uint8_t)e4m3_pack2(e4m3_clamp(load_as_f32<SDT>(from, e) / scale), 0.0f);
+          if constexpr (CDT == LH_F8E4M3) to[e] = (uint8_t)e4m3_codes(e4m3_clamp(load_as_f32<SDT>(from, e) / scale), 0.0f);
           else if constexpr (SES == 4) reinterpret_cast<uint32_t*>(to)[e] = reinterpret_cast<const uint32_t*>(from)[e];
           else reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(from)[e];
         }
@@ -551,12 +521,7 @@ int lh_hip_kv_append(const lh_paged_cache* cache, const void* k, const void* v, 
   a.token_blocks = (int32_t)((T + a.tokens - 1) / a.tokens);
   LH_REQUIRE(B * a.token_blocks * a.parts < (1ll << 24), "lh_hip_kv_append: too many tokens");
   const unsigned blocks = (unsigned)(B * a.token_blocks * a.parts);
-  auto short_division = [](float scale) {
-    uint32_t bits;
-    std::memcpy(&bits, &scale, 4);
-    return scale >= 0x1p-60f && scale <= 0x1p60f && (bits & 0x7fffffu) != 0x7fffffu ? 1.0f / scale : 0.0f;
-  };
-  a.k_inv = short_division(a.c.k_scale), a.v_inv = short_division(a.c.v_scale);
+  a.k_inv = e4m3_inverse(a.c.k_scale), a.v_inv = e4m3_inverse(a.c.v_scale);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (cache->dtype == LH_F8E4M3) {
     if (dtype == LH_BF16) return append_launch<LH_BF16, LH_F8E4M3>(a, blocks, threads, s);
