@@ -544,7 +544,7 @@ int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const v
 
 /*
  * Root-mean-square norm of rows: s = x + residual (f32; without residual: x), out = s / sqrt(mean(s^2) + eps) * gamma, and
- * residual_out = s, rounded to residual_dtype (residual_out may be residual).  x, out, residual [M, C] with row strides, gamma [C] f32.
+ * residual_out = s, rounded to residual_dtype (residual_out may be residual).  x, out, residual [M, C] with row strides of at least C, gamma [C] f32.
  * x_dtype F32, BF16 or F16, residual_dtype F32 or x_dtype; out_dtype F32, BF16, F16 or F8E4M3.  A result of e4m3 is e4m3(clamp(y / scale,
  * +-448)), with `scale`, or, where row_scales is not NULL, row_scales[m] = max |y| / 448 of its row (1 for a row of zeros, otherwise 2^-149 at
  * least).

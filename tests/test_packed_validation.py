@@ -222,3 +222,17 @@ def test_the_entry_points_check_for_themselves():
     says("positive scale", norm(od=_lib.F8E4M3, scale=0.0))
     says("positive scale", norm(od=_lib.F8E4M3, scale=math.nan))
     says("positive scale", norm(scales=at))
+
+
+def test_the_entry_point_of_the_norm_checks_its_row_strides():
+    lib = _lib.load()
+    p = ctypes.create_string_buffer(4096)
+    at = ctypes.addressof(p)
+    norm = lambda M=4, strides=(16, 16, 16, 16), residual=at: lib.lh_hip_rms_norm(  # noqa: E731
+        at, at, at, residual, residual, None, 1.0, M, 16, *strides, 1e-5, _lib.BF16, _lib.F32, _lib.BF16, None)
+    for i in range(4):
+        strides = [16] * 4
+        strides[i] = 15
+        for M in (4, 2):
+            assert norm(M, strides) == _lib.LH_ERR_INVALID and "rows overlap" in lib.lh_hip_last_error().decode()
+    assert norm(0, (0, 0, 0, 0)) == 0
