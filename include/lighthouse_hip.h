@@ -499,7 +499,7 @@ int lh_hip_kv_pages(int32_t* block_table, int64_t table_stride, const int32_t* l
  * by positions[n] * freqs[i] (radians, in 64 bits), times `amplitude`:
  *   a' = amplitude (a cos - b sin),  b' = amplitude (b cos + a sin);  the other columns stay.
  * Sines, cosines and sums are f32.  x, out [N, H, d] in F32, BF16 or F16 (element strides of token and head, unit stride along d); out
- * may be x, but not another view of its memory.  Negated freqs turn back (and take the gradient back, at amplitude 1).  N H (d + 30) < 2^34.
+ * may be x, but not another view of its memory.  Negated freqs take a gradient back (at the same amplitude), and at amplitude 1 turn back.  N H (d + 30) < 2^34.
  */
 typedef struct lh_rotary {
   const int32_t* positions; /* [N] */

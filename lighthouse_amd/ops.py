@@ -909,7 +909,7 @@ def rotary(x, positions, freqs, *, interleaved=False, amplitude=1.0, out=None):
     """Rotary positions: of every head of x [N, heads, d] (any strides with unit stride along d) the column pairs (i, i + R / 2), or (2 i, 2 i + 1)
     if `interleaved`, turn by positions[n] * freqs[i]: (a cos - b sin, b cos + a sin), times `amplitude`.  freqs: float64 [R / 2] (see
     rotary_frequencies), radians a position; columns from R on stay.  positions: int32 [N].  `out` may be x.
-    Turning by -freqs takes it back, and takes a gradient from the result to x."""
+    Turning by -freqs takes a gradient from the result to x (at the same amplitude), and at amplitude 1 the result back to x."""
     shape, sx = _packed_rows(x, "x")
     N, heads, d = shape
     turn = _turn(positions, freqs, N, d, interleaved, amplitude)

@@ -267,3 +267,20 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
         assert torch.equal(as_bits(k_cache), as_bits(other[0])) and torch.equal(as_bits(v_cache), as_bits(other[1]))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("amplitude", [0.25, 1.3])
+def test_the_gradient_at_an_amplitude(interleaved, amplitude):
+    """Turning by -freqs at the same amplitude: against the formula's gradient, whose matrix is the transposed one."""
+    g, positions = case(50, 4, 96, f32, seed=9)
+    freqs = ops.rotary_frequencies(64)
+    grad = ops.rotary(g, positions, -freqs, interleaved=interleaved, amplitude=amplitude)
+    xx = torch.randn(g.shape, generator=torch.Generator().manual_seed(10), dtype=torch.float64).requires_grad_()
+    angle = positions.cpu().double()[:, None, None] * freqs.cpu()
+    a, b = (xx[..., 0:64:2], xx[..., 1:64:2]) if interleaved else (xx[..., :32], xx[..., 32:64])
+    turned = [amplitude * (a * angle.cos() - b * angle.sin()), amplitude * (b * angle.cos() + a * angle.sin())]
+    turned = torch.stack(turned, -1).flatten(-2) if interleaved else torch.cat(turned, -1)
+    (torch.cat([turned, xx[..., 64:]], -1) * g.cpu().double()).sum().backward()
+    _, allowed = ref.rotary(g.cpu(), positions.cpu(), -freqs.cpu(), interleaved, amplitude)
+    close(grad, xx.grad, allowed, f32)
