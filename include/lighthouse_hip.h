@@ -530,7 +530,8 @@ int lh_hip_kv_store(const lh_paged_cache* cache, const void* k, const void* v, i
  * Positions on pages that hold nothing are left out; 0 where nothing is left; what lies at positions that a row does not see does not matter to it.
  * Rows from starts[B] on stay as they were.  starts are taken as clamped to 0 .. N, a sequence whose end is not behind its beginning has no rows.
  * Scores, softmax and sums are f32.  With 16-bit queries w_t in front of v_t is the sum of at least two 16-bit values, off by no more than 2^-16 of
- * it (and, in f16, 2^-37 of the largest).  An infinite value makes an infinity or a NaN of the rows that see it.  out may be q.  dtype (of q and
+ * it (and, in f16, 2^-37 of the largest).  An infinite value makes an infinity or a NaN of the rows that see it.  out may be q, but not
+ * another view of its memory.  dtype (of q and
  * out) is the cache's, or BF16 or F16 for a cache of e4m3.  B < 2^20, N < 2^30, N H < 2^32, N H / n_kv_heads < 2^31 - 256, and fewer workgroups
  * than a launch may have: (N H / n_kv_heads / 16 + B) n_kv_heads < 2^24, or / 128 where sequences have many rows.
  * `workspace` as for lh_hip_paged_attention, of lh_hip_paged_attention_chunk_workspace_bytes(...), which goes by sizes and types, not by strides.

@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
 
 template <int SDT, int CDT, bool INTERLEAVED>
 static int launch_rotary(RotaryArgs& a, int64_t N, int heads_all, int chunks, hipStream_t s) {
-  // Two heads a thread, which share their angles, where half as many threads still fill half of the chip: prompts of 8192 tokens, 24 heads of 64,
+  // Two heads a thread, which share their angles, where one head a thread would fill half of the chip: prompts of 8192 tokens, 24 heads of 64,
   // into e4m3 13.9 us (one head 16.4, four 13.7); 64 tokens of 24 heads 4.4 us (one head 3.8).  (Stores past the
   // caches cost their reader more than they save: 8192 tokens of 40 heads of 128, f16, into one buffer that is read after, 92.5 us; 81.1 kept.)
   const int64_t values = N * heads_all * chunks, at_once = (int64_t)num_cus() * 2048;

@@ -975,7 +975,7 @@ def paged_attention_chunk(q, k_cache, v_cache, block_table, lengths, starts, *, 
     starts[b] .. starts[b + 1] - 1 (int32 [B + 1], from 0 up); the last one is at position lengths[b] - 1 (int32 [B]: the new tokens count, and
     have been stored), the others right before it, and each sees the positions up to its own: softmax(scale q . k_t) v_t, 0 where it sees none.
     What lies at positions that a row does not see does not matter to it.  Rows from starts[B] on stay as they were.  scale: 1 / sqrt(d) if None.
-    `out` may be q.  `workspace` (uint8, see paged_attention_chunk_workspace_bytes): temporary memory, otherwise torch's allocator is asked; two
+    `out` may be q, but not another view of its memory.  `workspace` (uint8, see paged_attention_chunk_workspace_bytes): temporary memory, otherwise torch's allocator is asked; two
     calls that overlap in time need one each."""
     shape, sq = _packed_rows(q, "q")
     N, H, d = shape
