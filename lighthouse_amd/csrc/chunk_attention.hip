@@ -117,25 +117,25 @@ static size_t granules(size_t b) { return (b + 255) / 256 * 256; }
 
 // Which kernel a call is for.  The few read every position once for 16 rows; the many have more to do for a tile of 128, however few rows it has.
 // Rows of a sequence up to which the few are faster, all alike (few against many, us): 16-bit types 16 (64 sequences of up to 1024, 12 heads of 64: 16
-// rows 33.3, 37.3; 17 rows 47.2, 37.4), e4m3 48 (16 of up to 4096, 4 heads of 128: 48 rows 31.7, 34.6; 64 rows 37.3, 35.0), f32 and wide rows 64
-// and more (8 of up to 2048, 4 heads of 128, f32: 34, 91; 32 of them, 4 heads of 256, bf16: 106, 136).
+// rows 32.7, 38.0; 17 rows 46.8, 38.3), e4m3, whose codes are half of the bytes, 64 (16 of up to 4096, 4 heads of 128: 64 rows 35.6, 39.1; 80 rows 45.8,
+// 41.8), f32 and wide rows 64 and more (8 of up to 2048, 4 heads of 128, f32: 33, 92; 32 of them, 4 heads of 256, bf16: 105, 136).
 //
 // Of unlike sequences, those with up to 32 rows are for the few, those with more for the many, in two launches: two pieces of 512 among 14 tokens of 16
-// heads take 98 us in the kernel of the many, 82 so; of 32 heads 163 and 146.  But all are for the many where there are fewer than 128 rows a
-// sequence, so that they may be alike (8 of 20 rows 30.5 us, 38 in two launches), where a tile of 128 for each would add less than a quarter to the
+// heads take 104 us in the kernel of the many, 87 so; of 32 heads 178 and 142.  But all are for the many where there are fewer than 128 rows a
+// sequence, so that they may be alike (8 of 20 rows 31 us, 36 in two launches), where a tile of 128 for each would add less than a quarter to the
 // rows that there are, and where there are more tiles than workgroups run at once: single tokens, bound by memory, then run beside the others (8
-// pieces of 512 among 56 tokens of 32 heads: 176 us, 188 in two launches; 32 of 256 among 224: 236, 256).
+// pieces of 512 among 56 tokens of 32 heads, up to 4096: 392 us, 410 in two launches; 32 of 256 among 224, up to 1024: 257, 270).
 enum ChunkPart { kAllFew, kAllMany, kTheFew, kTheMany };
 static ChunkPart chunk_part(const Paged& c, int cache_dtype, int64_t N, int64_t B, int64_t H) {
   const int64_t rows = N * (H / c.heads);
   // Where there is little to do at all, tiles of 128 rows are longer chains.  Tiles of 16 rows times positions up to which the few are faster: f16 and bf16 160
-  // Ki (26 tokens up to 681, 6 heads of 256 with 3 queries: few 18, many 30; 100 up to 1000, 8 heads of 64: 11, 14; 4 of 64 up to 1000, 4 heads of 128
-  // with 2: 18, 21; 69 of 13 heads of 128 up to 1711: 23, 21), f32, whose matrix instructions take 16 times as long, 4 Mi (4 of 48 to 190, 4 heads of 128 with
+  // Ki (26 tokens up to 681, 6 heads of 256 with 3 queries: few 17, many 31; 100 up to 1000, 8 heads of 64: 10, 15; 4 of 64 up to 1000, 4 heads of 128
+  // with 2: 18, 20; 69 of 13 heads of 128 up to 1711: 21, 21), f32, whose matrix instructions take 16 times as long, 4 Mi (4 of 48 to 190, 4 heads of 128 with
   // 3: 15, 42; 16 of 1 to 512 up to 2048, 4 heads of 64 with 4: 104, 114; 8 of 1024, 12 heads of 64: 157, 149), but for wide rows (7 of 70 to 278, 8 heads of
   // 256 with 3: 156, 140).
   const int64_t tiles = (rows + 15) / 16 * c.heads;
   if (tiles * c.capacity() <= (cache_dtype == LH_F32 && c.d <= 128 ? 4 << 20 : 160 << 10)) return kAllFew;
-  if (rows <= B * (cache_dtype == LH_F32 || c.d > 192 ? 64 : cache_dtype == LH_F8E4M3 ? 48 : 16)) return kAllFew;
+  if (rows <= B * (cache_dtype == LH_F32 || cache_dtype == LH_F8E4M3 || c.d > 192 ? 64 : 16)) return kAllFew;
   return rows < 128 * B || rows >= 4 * 128 * B || (rows / 128 + B) * c.heads > 2 * num_cus() ? kAllMany : kTheMany;
 }
 
@@ -175,10 +175,10 @@ static ChunkPlan chunk_plan(const Paged& c, int cache_dtype, int64_t N, int64_t 
     p.blocks = p.odd ? (blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8) : blocks <= 2 ? 2 : blocks <= 4 ? blocks : blocks <= 6 ? 6 : 8;
     p.width = 32 * p.blocks;
     // One share more than that would be a second round of workgroups for a few (a piece of 256 tokens after 16128 positions, 64 tiles: 6 shares
-    // 120 us, 8 104, 12 127; of wide rows, of which a CU holds one workgroup, after 7936 positions, 32 tiles: 8 shares 101, 16 118).  But in three
+    // 138 us, 8 118, 12 127; of wide rows, of which a CU holds one workgroup, after 7936 positions, 32 tiles: 8 shares 112, 16 127).  But in three
     // shares each, tiles that leave a last round of workgroups mostly empty take a third of it, where a share is long against what its results cost (4
-    // pieces of 600 up to 8192, 300 tiles: 277 us, so 211; one of 2300 up to 16384, 568 tiles: 900, 731; 320 tiles of 64 columns up to 4096: 92, 71, up to
-    // 1024: 27, 38).
+    // pieces of 600 up to 8192, 300 tiles: 323 us, so 238; one of 2300 up to 16384, 568 tiles: 1111, 910; 320 tiles of 64 columns up to 4096: 111, 81, up
+    // to 1024: 30, 41).
     const int64_t at_once = (p.blocks > 4 ? 1 : 2) * (int64_t)num_cus(), workgroups = tiles * c.heads;
     const int64_t whole = (workgroups + at_once - 1) / at_once, cut = (3 * workgroups + at_once - 1) / at_once;  // rounds, and thirds of rounds
     const bool thirds = 2 * workgroups > at_once && whole <= 3 && 10 * cut <= 25 * whole && (int64_t)c.capacity() * p.width >= whole << 18;

@@ -1,7 +1,7 @@
 // Attention of packed chunks with few rows a sequence over a paged cache (a token each, a few drafted ones), for one pair of types: the kernel of
 // one token of every sequence, with 16 neighbouring rows of (token, query of the group) where that has the queries of a group.  Like it, it is
 // bound by memory, and P is the sum of three values of bf16 or two of f16.  4 tokens each of 8 sequences of 1024 to 4096 positions, bf16, 32 heads
-// of 128 over 8: 24.9 us with the join (3.4 TB/s; in tiles of 128 rows 38.5).
+// of 128 over 8: 24.9 us with the join (3.4 TB/s; in tiles of 128 rows 31.2).
 #include "paged_rows.h"
 
 #ifndef LH_CHUNK_CDT

@@ -13,7 +13,7 @@
 //    without LDS, in chunk_attention_few.hip.)
 //  * Long caches of few tiles are cut into shares of positions; a second launch joins them.
 //
-// The arithmetic bounds it: a step of a wave has 48 matrix instructions of 32 cycles at width 128 beside about 330 vector instructions, 32 of them
+// The arithmetic bounds it: a step of a wave has 48 matrix instructions of 32 cycles at width 128 beside about 290 vector instructions, 32 of them
 // exponentials, and the two hardly overlap (2048 tokens after 14336, f16, 32 heads of 128: matrix unit 45 % of the cycles, vector unit 43 %).
 // P is held in f32 and enters the second product as the sum of two 16-bit values, each nearest to what is left: off by 2^-16 of it at most in bf16,
 // 2^-18 in the mean, and by 2^-22 in f16.  One value would leave 2^-8 and make the result's error against 64 bits up to 1.4 times that of its own
@@ -23,7 +23,7 @@
 //
 // Measured: those 2048 tokens in f16 822 us (627 TFLOP/s of the products that the mask leaves; 1180 is what a large f16 product reaches, and half as
 // many products again are made); those prompts 34.5 us (374 TFLOP/s: steps of 24 matrix instructions, half of a tile's last two are masked); 512 tokens
-// each of two sequences of 4096 and 2458 positions, e4m3, 16 heads of 128, 68 us and 13 for the join, which moves 34 MB.
+// each of two sequences of 4096 and 2458 positions, e4m3, 16 heads of 128, 70 us and 13 for the join, which moves 34 MB.
 #include "chunk_attention.h"
 
 #ifndef LH_CHUNK_CDT
