@@ -17,13 +17,13 @@
 // exponentials, and the two hardly overlap (2048 tokens after 14336, f16, 32 heads of 128: matrix unit 45 % of the cycles, vector unit 43 %).
 // P is held in f32 and enters the second product as the sum of two 16-bit values, each nearest to what is left: off by 2^-16 of it at most in bf16,
 // 2^-18 in the mean, and by 2^-22 in f16.  One value would leave 2^-8 and make the result's error against 64 bits up to 1.4 times that of its own
-// rounding, 1.0 times with two, and the same row would differ from what the kernel for few rows makes of it (the same 2048 tokens 609 us with one,
-// 783 with two; 8 prompts of 1024, bf16, 12 heads of 64, 28.5 and 34.4).  A third of bf16 takes 964 and 40.1 us and changes neither of the
+// rounding, 1.0 times with two, and the same row would differ from what the kernel for few rows makes of it (the same 2048 tokens in bf16 609 us with
+// one, 783 with two; 8 prompts of 1024, bf16, 12 heads of 64, 28.6 and 34.0).  A third of bf16 takes 964 and 40.1 us and changes neither of the
 // error's first two places.  Everything that was not needed in a step for which nothing has to be masked is behind a uniform branch.
 //
-// Measured: those 2048 tokens in f16 822 us (627 TFLOP/s of the products that the mask leaves; 1180 is what a large f16 product reaches, and half as
-// many products again are made); those prompts 34.5 us (374 TFLOP/s: steps of 24 matrix instructions, half of a tile's last two are masked); 512 tokens
-// each of two sequences of 4096 and 2458 positions, e4m3, 16 heads of 128, 70 us and 13 for the join, which moves 34 MB.
+// Measured: those 2048 tokens in f16 810 us (636 TFLOP/s of the products that the mask leaves, with half as many again made; 1180 is what a large f16
+// product reaches); those prompts 34.0 us (380 TFLOP/s: steps of 24 matrix instructions, half of a tile's last two are masked); 512 tokens each of two
+// sequences of 4096 and 2458 positions, e4m3, 16 heads of 128, 70 us and 13 for the join, which moves 34 MB.
 #include "chunk_attention.h"
 
 #ifndef LH_CHUNK_CDT
