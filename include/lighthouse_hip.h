@@ -530,10 +530,10 @@ int lh_hip_kv_store(const lh_paged_cache* cache, const void* k, const void* v, i
  * Positions on pages that hold nothing are left out; 0 where nothing is left; what lies at positions that a row does not see does not matter to it.
  * Rows from starts[B] on stay as they were.  starts are taken as clamped to 0 .. N, a sequence whose end is not behind its beginning has no rows.
  * Scores, softmax and sums are f32.  With 16-bit queries w_t in front of v_t is the sum of at least two 16-bit values, off by no more than 2^-16 of
- * it (and, in f16, 2^-37 of the largest).  An infinite value makes an infinity or a NaN of the rows that see it.  out may be q, but not
- * another view of its memory.  dtype (of q and
- * out) is the cache's, or BF16 or F16 for a cache of e4m3.  B < 2^20, N < 2^30, N H < 2^32, N H / n_kv_heads < 2^31 - 256, and fewer workgroups
- * than a launch may have: (N H / n_kv_heads / 16 + B) n_kv_heads < 2^24, or / 128 where sequences have many rows.
+ * it (and, in f16, 2^-37 of the largest).  An infinite value makes an infinity or a NaN of the rows that see it.  out may be q, but not another
+ * view of its memory.  dtype (of q and out) is the cache's, or BF16 or F16 for a cache of e4m3.  B < 2^20, N < 2^30, N H < 2^32,
+ * N H / n_kv_heads < 2^31 - 256, and fewer workgroups than a launch may have: (N H / n_kv_heads / 16 + B) n_kv_heads < 2^24, or / 128 where sequences
+ * have many rows.
  * `workspace` as for lh_hip_paged_attention, of lh_hip_paged_attention_chunk_workspace_bytes(...), which goes by sizes and types, not by strides.
  * Fewer rows or sequences may take more of it (their positions are cut into more shares): one for several calls is the largest of theirs.
  */
@@ -545,7 +545,7 @@ int lh_hip_paged_attention_chunk(const lh_paged_cache* cache, void* out, const v
 
 /*
  * Root-mean-square norm of rows: s = x + residual (f32; without residual: x), out = s / sqrt(mean(s^2) + eps) * gamma, and
- * residual_out = s, rounded to residual_dtype (residual_out may be residual).  x, out, residual [M, C] with row strides of at least C, gamma [C] f32.
+ * residual_out = s, rounded to residual_dtype (residual_out may be residual).  x, out, residual [M, C] with row strides (of results: C at least), gamma [C] f32.
  * x_dtype F32, BF16 or F16, residual_dtype F32 or x_dtype; out_dtype F32, BF16, F16 or F8E4M3.  A result of e4m3 is e4m3(clamp(y / scale,
  * +-448)), with `scale`, or, where row_scales is not NULL, row_scales[m] = max |y| / 448 of its row (1 for a row of zeros, otherwise 2^-149 at
  * least).

@@ -279,7 +279,7 @@ extern "C" int lh_hip_rms_norm(void* out, const void* x, const float* gamma, con
   LH_REQUIRE((residual == nullptr) == (residual_out == nullptr), "%s: a residual needs a place for its sum", what);
   LH_REQUIRE(out_dtype == LH_F8E4M3 ? row_scales != nullptr || (scale > 0.0f && scale < INFINITY) : row_scales == nullptr,
              "%s: a result of e4m3 needs a positive scale or room for one per row, others take none", what);
-  LH_REQUIRE(M <= 1 || (ld_out >= C && ld_x >= C && (residual == nullptr || (ld_residual >= C && ld_residual_out >= C))), "%s: rows overlap", what);
+  LH_REQUIRE(M <= 1 || (ld_out >= C && (residual == nullptr || ld_residual_out >= C)), "%s: rows of a result overlap", what);
   if (M == 0) return LH_OK;
   LH_REQUIRE(out && x && gamma, "%s: null pointer", what);
   // A sum that the L2 caches (32 MiB) do not hold goes past them: who reads it next comes after the product that reads the result.  (8192 rows of

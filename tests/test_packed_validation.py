@@ -230,9 +230,7 @@ def test_the_entry_point_of_the_norm_checks_its_row_strides():
     at = ctypes.addressof(p)
     norm = lambda M=4, strides=(16, 16, 16, 16), residual=at: lib.lh_hip_rms_norm(  # noqa: E731
         at, at, at, residual, residual, None, 1.0, M, 16, *strides, 1e-5, _lib.BF16, _lib.F32, _lib.BF16, None)
-    for i in range(4):
-        strides = [16] * 4
-        strides[i] = 15
+    for strides in ((15, 16, 16, 16), (16, 16, 16, 15)):  # (of out and residual_out)
         for M in (4, 2):
-            assert norm(M, strides) == _lib.LH_ERR_INVALID and "rows overlap" in lib.lh_hip_last_error().decode()
+            assert norm(M, strides) == _lib.LH_ERR_INVALID and "rows of a result overlap" in lib.lh_hip_last_error().decode()
     assert norm(0, (0, 0, 0, 0)) == 0
