@@ -104,7 +104,7 @@ template <int QDT>
 static void chunk_join_launch(const ChunkArgs& a, const ChunkArgs& few, hipStream_t s) {
   const int64_t rows = (int64_t)a.N * a.H, few_rows = (int64_t)a.B * a.c.heads * kChunkFew;
   // A wave for up to 8 shares, and where the rows are enough to fill the device (4 drafted tokens after 8188 positions, 32 shares: 24.3 us, with
-  // four waves 17.7; 1038 tokens of 16 heads, few of them of 12 shares: 76 us, with four 93).  (Where only the
+  // four waves 17.7; 1038 tokens of 16 heads, few of them of 12 shares: 88 us, with four 103).  (Where only the
   // sequences with few rows are cut, their rows are that many, or their shares that few.)
   if (a.splits == 1) LH_LAUNCH((chunk_join_kernel<QDT, 1, false>), dim3((unsigned)((few_rows + 3) / 4)), dim3(256), 0, s, a, few);
   else if ((a.splits <= 8 && few.splits <= 8) || rows > 8 * num_cus()) LH_LAUNCH((chunk_join_kernel<QDT, 1, true>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, few);

@@ -4,9 +4,9 @@
 // workgroup takes a tile of them and walks over the positions up to the last one that any of them sees:
 //
 //  * Both products are transposed, S^T = K Q^T and O^T = V^T P^T on 32-wide matrix instructions: a lane has one row, its softmax state
-//    is a scalar per lane, and the accumulators of S^T are, rounded, the second operand of O^T.
+//    is a scalar per lane, and the accumulators of S^T are, as sums of 16-bit values, the second operand of O^T.
 //  * Keys and values of a step go through registers into LDS, two steps of which are there where that costs a CU no workgroup (the next one's are
-//    put there between the two products: 2.1 % of a long step's time, 7.5 % of a short one's); they are asked for up to two steps ahead, as far as
+//    put there between the two products: 2 % of a short step's time, less of a long one's); they are asked for up to two steps ahead, as far as
 //    registers suffice.  Where each position's row lies is looked up before that, one position a thread, so
 //    that any page size and any strides cost the same.
 //  * 128 rows a workgroup, 32 for each of four waves, 64 positions a step, which all waves read.  (Sequences with few rows have a kernel
@@ -18,7 +18,7 @@
 // P is held in f32 and enters the second product as the sum of two 16-bit values, each nearest to what is left: off by 2^-16 of it at most in bf16,
 // 2^-18 in the mean, and by 2^-22 in f16.  One value would leave 2^-8 and make the result's error against 64 bits up to 1.4 times that of its own
 // rounding, 1.0 times with two, and the same row would differ from what the kernel for few rows makes of it (the same 2048 tokens in bf16 609 us with
-// one, 783 with two; 8 prompts of 1024, bf16, 12 heads of 64, 28.6 and 34.0).  A third of bf16 takes 964 and 40.1 us and changes neither of the
+// one, 757 to 783 with two; 8 prompts of 1024, bf16, 12 heads of 64, 28.6 and 34.0).  A third of bf16 takes 964 and 40.1 us and changes neither of the
 // error's first two places.  Everything that was not needed in a step for which nothing has to be masked is behind a uniform branch.
 //
 // Measured: those 2048 tokens in f16 810 us (636 TFLOP/s of the products that the mask leaves, with half as many again made; 1180 is what a large f16
